@@ -2557,3 +2557,379 @@ emel_status emel_op_l2_norm(const emel_tensor_view *in, const emel_tensor_view_m
     if (!(sum > 0.0f)) return fail(EMEL_ERR_ZERO_NORM, "l2_norm: the sum of squares is not positive");
     return launched(emel::launch_generic_l2_apply(x, y, ws, hs));
 }
+
+// ---- products with packed 4-bit weights, the paged cache, logits adjustment ---------
+//
+// The guards of a call that has no reference event: NULL or misaligned
+// pointers, then extents, views, shapes, parameters and overlaps.
+
+namespace {
+
+constexpr uint64_t kMaxExtent = 0x7fffffffull;
+
+// A C entry reports what it cannot allocate as a status, never as an
+// exception that its caller's language does not know.
+template <class F>
+emel_status entry(F &&body)
+{
+    try {
+        return body();
+    } catch (...) {
+        return EMEL_ERR_INTERNAL;
+    }
+}
+
+template <class V>
+bool data_ok(const V *v, uint64_t align)
+{
+    return v && v->data && reinterpret_cast<uintptr_t>(v->data) % align == 0;
+}
+
+// Extents within what the kernels count in 32 bits (which also keeps a
+// span's products within 128 bits).
+template <class... V>
+bool extents_ok(const V &...views)
+{
+    auto one = [](const auto &v) {
+        for (int d = 0; d < 4; ++d)
+            if (v.ne[d] > kMaxExtent) return false;
+        return true;
+    };
+    return (one(views) && ...);
+}
+
+struct Span {
+    uintptr_t lo, hi;
+};
+template <class V>
+Span span_of(const V &v, uint64_t elem)
+{
+    const auto r = byte_range(v, elem);
+    return {r.first, r.second};
+}
+bool apart(Span a, Span b) { return a.hi <= b.lo || b.hi <= a.lo; }
+
+bool ne_is(const uint64_t ne[4], uint64_t a, uint64_t b, uint64_t c = 1, uint64_t d = 1)
+{
+    return ne[0] == a && ne[1] == b && ne[2] == c && ne[3] == d;
+}
+
+emel_status mul_mat_q4(bool q4k, const emel_tensor_view *w, const emel_tensor_view *x, const emel_tensor_view_mut *y,
+                       emel_stream stream)
+{
+    if (!data_ok(w, 1) || !data_ok(x, 4) || !data_ok(y, 4))
+        return fail(EMEL_ERR_INVALID_ARGUMENT, "null view or data, or a misaligned pointer");
+    if (!extents_ok(*w, *x, *y)) return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent is past 2^31 - 1");
+    if (w->reserved != 0 || !(q4k ? packed_view_valid(*w, EMEL_DTYPE_Q4_K, 256, 144)
+                                  : packed_view_valid(*w, EMEL_DTYPE_Q4_0, 32, 18)) ||
+        !valid_f32(*x, true) || !valid_f32(*y, true))
+        return fail(EMEL_ERR_INVALID_VIEW, "mul_mat view failed validation");
+    if (w->ne[2] != 1 || w->ne[3] != 1 || !ne_is(x->ne, w->ne[0], x->ne[1]) || !ne_is(y->ne, w->ne[1], x->ne[1]))
+        return fail(EMEL_ERR_SHAPE_MISMATCH, "mul_mat takes [k, m], [k, n] and [m, n]");
+    const uintptr_t wp = reinterpret_cast<uintptr_t>(w->data);
+    const Span ys = span_of(*y, 4);
+    if (!apart(ys, span_of(*x, 4)) || !apart(ys, {wp, wp + w->nb[1] * w->ne[1]}))
+        return fail(EMEL_ERR_INVALID_VIEW, "dst overlaps a source");
+    if (!elements_disjoint(*y, 4)) return fail(EMEL_ERR_INVALID_VIEW, "dst elements overlap one another");
+    emel_status s = ensure_device();
+    if (s != EMEL_OK) return s;
+    const Operand xo = operand(*x, 4), yo = operand(*y, 4);
+    emel::QMatArgs a{};
+    a.q4k = q4k;
+    a.w = w->data;
+    a.k = static_cast<uint32_t>(w->ne[0]);
+    a.m = static_cast<uint32_t>(w->ne[1]);
+    a.n = static_cast<uint32_t>(x->ne[1]);
+    a.x = static_cast<const float *>(xo.data);
+    a.y = static_cast<float *>(yo.data);
+    for (int d = 0; d < 2; ++d) {
+        a.x_st[d] = xo.st[d];
+        a.y_st[d] = yo.st[d];
+    }
+    StreamLease lease;
+    if (const uint64_t bytes = emel::quant_mat_workspace_bytes(a)) {
+        s = lease.acquire(as_stream(stream));
+        if (s == EMEL_OK) s = lease.work(bytes, &a.workspace);
+        if (s != EMEL_OK) return s;
+    }
+    return launched(emel::launch_quant_mat(a, as_stream(stream)));
+}
+
+// A pool of pages: halves with unit stride along dim.
+template <class V>
+bool pages_valid(const V &v)
+{
+    uint64_t count;
+    if ((v.dtype != EMEL_DTYPE_F16 && v.dtype != EMEL_DTYPE_BF16) || v.reserved != 0) return false;
+    if (!element_count(v, count) || v.nb[0] != 2) return false;
+    for (int d = 1; d < 4; ++d)
+        if (v.ne[d] > 1 && (v.nb[d] < 2 || v.nb[d] % 2 != 0)) return false;
+    uint64_t st[4];
+    for (int d = 0; d < 4; ++d) st[d] = v.ne[d] > 1 ? v.nb[d] : 0;
+    return span_fits(v, st, 2);
+}
+
+template <class V>
+Span pages_span(const V &v)
+{
+    uintptr_t bytes = 2;
+    for (int d = 0; d < 4; ++d) bytes += (v.ne[d] - 1) * (v.ne[d] > 1 ? v.nb[d] : 0);
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(v.data);
+    return {lo, lo + bytes};
+}
+
+template <class V>
+emel::PagePool pool_of(const V &v)
+{
+    auto st = [&](int d) { return static_cast<int64_t>(v.ne[d] > 1 ? v.nb[d] / 2 : 0); };
+    return {static_cast<uint16_t *>(const_cast<void *>(static_cast<const void *>(v.data))), st(1), st(2), st(3)};
+}
+
+// Whether no slot of either pool shares a byte with another, by the rule of
+// elements_disjoint.  Pools of one layout that lie inside one another's span
+// (keys and values side by side in each page) count as one tensor with a
+// dimension of two more.
+bool pools_disjoint(const emel_tensor_view_mut &k, const emel_tensor_view_mut &v)
+{
+    struct Dim {
+        uint64_t ne, st;
+    };
+    auto rule = [](Dim *d, int n) {
+        for (int i = 1; i < n; ++i)
+            for (int j = i; j > 0 && d[j].st < d[j - 1].st; --j) std::swap(d[j], d[j - 1]);
+        u128 span = 2;
+        for (int i = 0; i < n; ++i) {
+            if (d[i].st < span) return false;
+            span += static_cast<u128>(d[i].ne - 1) * d[i].st;
+        }
+        return true;
+    };
+    auto dims = [](const emel_tensor_view_mut &t, Dim *d) {
+        int n = 0;
+        for (int i = 0; i < 4; ++i)
+            if (t.ne[i] > 1) d[n++] = {t.ne[i], t.nb[i]};
+        return n;
+    };
+    Dim d[5];
+    if (!rule(d, dims(k, d)) || !rule(d, dims(v, d))) return false;
+    const Span ks = pages_span(k), vs = pages_span(v);
+    if (apart(ks, vs)) return true;
+    for (int i = 0; i < 4; ++i)
+        if (k.ne[i] > 1 && k.nb[i] != v.nb[i]) return false;
+    const int n = dims(k, d);
+    d[n] = {2, ks.lo < vs.lo ? vs.lo - ks.lo : ks.lo - vs.lo};
+    return rule(d, n + 1);
+}
+
+template <class A, class B>
+bool pools_alike(const A &k, const B &v)
+{
+    return k.dtype == v.dtype && same_ne(k, v);
+}
+
+emel_status paged_append(const emel_tensor_view *k, const emel_tensor_view *v, const emel_tensor_view *slots,
+                         const emel_tensor_view_mut *kp, const emel_tensor_view_mut *vp, emel_stream stream)
+{
+    if (!data_ok(k, 4) || !data_ok(v, 4) || !data_ok(slots, 4) || !data_ok(kp, 2) || !data_ok(vp, 2))
+        return fail(EMEL_ERR_INVALID_ARGUMENT, "null view or data, or a misaligned pointer");
+    if (!extents_ok(*k, *v, *slots, *kp, *vp)) return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent is past 2^31 - 1");
+    if (!valid_f32(*k, true) || !valid_f32(*v, true) || !valid_i32(*slots) || !pages_valid(*kp) || !pages_valid(*vp))
+        return fail(EMEL_ERR_INVALID_VIEW, "paged append view failed validation");
+    if (!pools_alike(*kp, *vp) || !ne_is(k->ne, kp->ne[0], kp->ne[2], k->ne[2]) || !same_ne(*k, *v) ||
+        !ne_is(slots->ne, k->ne[2], 1))
+        return fail(EMEL_ERR_SHAPE_MISMATCH, "paged append takes [dim, heads, tokens], [tokens] and two pools alike");
+    const Span ks = pages_span(*kp), vs = pages_span(*vp);
+    for (const Span s : {span_of(*k, 4), span_of(*v, 4), span_of(*slots, 4)})
+        if (!apart(s, ks) || !apart(s, vs)) return fail(EMEL_ERR_INVALID_VIEW, "the pages overlap a source");
+    if (!pools_disjoint(*kp, *vp)) return fail(EMEL_ERR_INVALID_VIEW, "slots of the pools overlap one another");
+    emel_status s = ensure_device();
+    if (s != EMEL_OK) return s;
+    const Operand ko = operand(*k, 4), vo = operand(*v, 4);
+    emel::PagedAppendArgs a{};
+    a.bf16 = kp->dtype == EMEL_DTYPE_BF16;
+    a.dim = static_cast<uint32_t>(kp->ne[0]);
+    a.page = static_cast<uint32_t>(kp->ne[1]);
+    a.kv_heads = static_cast<uint32_t>(kp->ne[2]);
+    a.pages = static_cast<uint32_t>(kp->ne[3]);
+    a.tokens = static_cast<uint32_t>(k->ne[2]);
+    a.k = static_cast<const float *>(ko.data);
+    a.v = static_cast<const float *>(vo.data);
+    for (int d = 0; d < 3; ++d) {
+        a.k_st[d] = ko.st[d];
+        a.v_st[d] = vo.st[d];
+    }
+    a.slots = static_cast<const int32_t *>(slots->data);
+    a.slots_st = static_cast<int64_t>(slots->nb[0] / 4);
+    a.k_pool = pool_of(*kp);
+    a.v_pool = pool_of(*vp);
+    return launched(emel::launch_paged_append(a, as_stream(stream)));
+}
+
+emel_status paged_attention(const emel_tensor_view *q, const emel_tensor_view *kp, const emel_tensor_view *vp,
+                            const emel_tensor_view *table, const emel_tensor_view *lengths, float scale,
+                            uint64_t window, float soft_cap, const emel_tensor_view_mut *y, emel_stream stream)
+{
+    if (!data_ok(q, 4) || !data_ok(kp, 2) || !data_ok(vp, 2) || !data_ok(table, 4) || !data_ok(lengths, 4) ||
+        !data_ok(y, 4))
+        return fail(EMEL_ERR_INVALID_ARGUMENT, "null view or data, or a misaligned pointer");
+    if (!extents_ok(*q, *kp, *vp, *table, *lengths, *y))
+        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent is past 2^31 - 1");
+    if (!valid_f32(*q, true) || !valid_f32(*y, true) || !pages_valid(*kp) || !pages_valid(*vp) || !valid_i32(*table) ||
+        !valid_i32(*lengths))
+        return fail(EMEL_ERR_INVALID_VIEW, "paged attention view failed validation");
+    const uint64_t seqs = q->ne[2];
+    if (!pools_alike(*kp, *vp) || !ne_is(q->ne, kp->ne[0], q->ne[1], seqs) || q->ne[1] % kp->ne[2] != 0 ||
+        !same_ne(*q, *y) || !ne_is(table->ne, table->ne[0], seqs) || !ne_is(lengths->ne, seqs, 1))
+        return fail(EMEL_ERR_SHAPE_MISMATCH,
+                    "paged attention takes [dim, heads, seqs], two pools alike, [max pages, seqs] and [seqs]");
+    if (!std::isfinite(scale) || !std::isfinite(soft_cap) || soft_cap < 0.0f)
+        return fail(EMEL_ERR_INVALID_PARAMETERS, "scale and soft_cap are finite, soft_cap >= 0");
+    if (kp->ne[0] % 8 != 0 || kp->ne[0] > 256 || table->ne[0] * kp->ne[1] > kMaxExtent)
+        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "dim is a multiple of 8 up to 256, max pages * page below 2^31");
+    const Span ys = span_of(*y, 4);
+    for (const Span s : {span_of(*q, 4), pages_span(*kp), pages_span(*vp), span_of(*table, 4), span_of(*lengths, 4)})
+        if (!apart(s, ys)) return fail(EMEL_ERR_INVALID_VIEW, "dst overlaps a source");
+    if (!elements_disjoint(*y, 4)) return fail(EMEL_ERR_INVALID_VIEW, "dst elements overlap one another");
+    emel_status s = ensure_device();
+    if (s != EMEL_OK) return s;
+    const Operand qo = operand(*q, 4), yo = operand(*y, 4);
+    emel::PagedAttnArgs a{};
+    a.bf16 = kp->dtype == EMEL_DTYPE_BF16;
+    a.dim = static_cast<uint32_t>(kp->ne[0]);
+    a.page = static_cast<uint32_t>(kp->ne[1]);
+    a.kv_heads = static_cast<uint32_t>(kp->ne[2]);
+    a.pages = static_cast<uint32_t>(kp->ne[3]);
+    a.heads = static_cast<uint32_t>(q->ne[1]);
+    a.seqs = static_cast<uint32_t>(seqs);
+    a.max_pages = static_cast<uint32_t>(table->ne[0]);
+    a.q = static_cast<const float *>(qo.data);
+    a.y = static_cast<float *>(yo.data);
+    for (int d = 0; d < 3; ++d) {
+        a.q_st[d] = qo.st[d];
+        a.y_st[d] = yo.st[d];
+    }
+    a.k_pool = pool_of(*kp);
+    a.v_pool = pool_of(*vp);
+    a.table = static_cast<const int32_t *>(table->data);
+    a.table_st[0] = static_cast<int64_t>(table->nb[0] / 4);
+    a.table_st[1] = static_cast<int64_t>(table->nb[1] / 4);
+    a.lengths = static_cast<const int32_t *>(lengths->data);
+    a.lengths_st = static_cast<int64_t>(lengths->nb[0] / 4);
+    a.scale = scale;
+    a.soft_cap = soft_cap;
+    a.window = static_cast<uint32_t>(window > kMaxExtent ? 0 : window); // longer than any sequence: none
+    StreamLease lease;
+    if (const uint64_t bytes = emel::paged_attn_workspace_bytes(a)) {
+        s = lease.acquire(as_stream(stream));
+        if (s == EMEL_OK) s = lease.work(bytes, &a.workspace);
+        if (s != EMEL_OK) return s;
+    }
+    return launched(emel::launch_paged_attn(a, as_stream(stream)));
+}
+
+emel_status logits_adjust(const emel_logits_adjust_request *r, emel_stream stream)
+{
+    if (!r || !data_ok(r->logits, 4) || !data_ok(r->adjusted, 4))
+        return fail(EMEL_ERR_INVALID_ARGUMENT, "null request, view or data, or a misaligned pointer");
+    const emel_tensor_view *parts[] = {r->history, r->history_len, r->repeat, r->frequency,
+                                       r->presence, r->bias_ids,   r->bias,   r->allowed};
+    for (const emel_tensor_view *p : parts)
+        if (p && !data_ok(p, 4)) return fail(EMEL_ERR_INVALID_ARGUMENT, "null data or a misaligned pointer");
+    if (r->reserved != 0 || (!r->bias_ids) != (!r->bias) ||
+        (!r->history && (r->history_len || r->repeat || r->frequency || r->presence)))
+        return fail(EMEL_ERR_INVALID_REQUEST, "bias_ids goes with bias, lengths and penalties with a history");
+    const emel_tensor_view &x = *r->logits;
+    const emel_tensor_view_mut &y = *r->adjusted;
+    bool extents = extents_ok(x, y), views = valid_f32(x, true) && valid_f32(y, true);
+    for (const emel_tensor_view *p : parts) {
+        if (!p) continue;
+        const bool f32 = p == r->repeat || p == r->frequency || p == r->presence || p == r->bias;
+        extents = extents && extents_ok(*p);
+        views = views && extents && (f32 ? valid_f32(*p, true) : valid_i32(*p));
+    }
+    if (!extents) return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent is past 2^31 - 1");
+    if (!views) return fail(EMEL_ERR_INVALID_VIEW, "logits adjustment view failed validation");
+    const uint64_t card = x.ne[0], rows = x.ne[1];
+    bool shapes = same_ne(x, y) && x.ne[2] == 1 && x.ne[3] == 1;
+    auto rows_fit = [&](uint64_t n) { return n == rows || n == 1; };
+    for (const emel_tensor_view *p : {r->history, r->bias_ids, r->bias, r->allowed})
+        if (p) shapes = shapes && rows_fit(p->ne[1]) && p->ne[2] == 1 && p->ne[3] == 1;
+    for (const emel_tensor_view *p : {r->history_len, r->repeat, r->frequency, r->presence})
+        if (p) shapes = shapes && rows_fit(p->ne[0]) && p->ne[1] == 1 && p->ne[2] == 1 && p->ne[3] == 1;
+    if (r->bias) shapes = shapes && same_ne(*r->bias, *r->bias_ids);
+    if (r->allowed) shapes = shapes && r->allowed->ne[0] == (card + 31) / 32;
+    if (!shapes) return fail(EMEL_ERR_SHAPE_MISMATCH, "logits adjustment extents do not match");
+    const Span ys = span_of(y, 4);
+    for (const emel_tensor_view *p : parts)
+        if (p && !apart(ys, span_of(*p, 4))) return fail(EMEL_ERR_INVALID_VIEW, "adjusted overlaps an operand");
+    if (!overlap_ok(y, 4, x, 4)) return fail(EMEL_ERR_INVALID_VIEW, "adjusted partially overlaps logits");
+    if (!elements_disjoint(y, 4)) return fail(EMEL_ERR_INVALID_VIEW, "adjusted elements overlap one another");
+    emel_status s = ensure_device();
+    if (s != EMEL_OK) return s;
+    const Operand xo = operand(x, 4), yo = operand(y, 4);
+    emel::LogitsAdjustArgs a{};
+    a.card = static_cast<uint32_t>(card);
+    a.rows = static_cast<uint32_t>(rows);
+    a.x = static_cast<const float *>(xo.data);
+    a.x_st = xo.st[0];
+    a.x_row = xo.st[1];
+    a.y = static_cast<float *>(yo.data);
+    a.y_st = yo.st[0];
+    a.y_row = yo.st[1];
+    auto table = [](const emel_tensor_view *v, bool per_row) {
+        emel::RowTable t{};
+        if (!v) return t;
+        const Operand o = operand(*v, 4);
+        t.data = v->data;
+        t.entries = per_row ? 1u : static_cast<uint32_t>(v->ne[0]);
+        t.st = per_row ? 0 : o.st[0];
+        const int d = per_row ? 0 : 1;
+        t.row_st = v->ne[d] > 1 ? o.st[d] : 0;
+        return t;
+    };
+    a.history = table(r->history, false);
+    a.history_len = table(r->history_len, true);
+    a.repeat = table(r->repeat, true);
+    a.frequency = table(r->frequency, true);
+    a.presence = table(r->presence, true);
+    a.bias_ids = table(r->bias_ids, false);
+    a.bias = table(r->bias, false);
+    a.allowed = table(r->allowed, false);
+    return launched(emel::launch_logits_adjust(a, as_stream(stream)));
+}
+
+} // namespace
+
+emel_status emel_op_mul_mat_q4_0(const emel_tensor_view *weights, const emel_tensor_view *x,
+                                 const emel_tensor_view_mut *dst, emel_stream stream)
+{
+    return entry([&] { return mul_mat_q4(false, weights, x, dst, stream); });
+}
+
+emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_tensor_view *x,
+                                 const emel_tensor_view_mut *dst, emel_stream stream)
+{
+    return entry([&] { return mul_mat_q4(true, weights, x, dst, stream); });
+}
+
+emel_status emel_op_paged_kv_append(const emel_tensor_view *k, const emel_tensor_view *v,
+                                    const emel_tensor_view *slots, const emel_tensor_view_mut *k_pages,
+                                    const emel_tensor_view_mut *v_pages, emel_stream stream)
+{
+    return entry([&] { return paged_append(k, v, slots, k_pages, v_pages, stream); });
+}
+
+emel_status emel_op_paged_attention(const emel_tensor_view *q, const emel_tensor_view *k_pages,
+                                    const emel_tensor_view *v_pages, const emel_tensor_view *page_table,
+                                    const emel_tensor_view *lengths, float scale, uint64_t window, float soft_cap,
+                                    const emel_tensor_view_mut *dst, emel_stream stream)
+{
+    return entry([&] {
+        return paged_attention(q, k_pages, v_pages, page_table, lengths, scale, window, soft_cap, dst, stream);
+    });
+}
+
+emel_status emel_logits_adjust(const emel_logits_adjust_request *request, emel_stream stream)
+{
+    return entry([&] { return logits_adjust(request, stream); });
+}

@@ -233,6 +233,83 @@ bool get_rows_row_kernels(const GetRowsArgs &args);
 // inline_idx: NULL reads args.idx from device memory.
 hipError_t launch_get_rows(const GetRowsArgs &args, const IdxInline *inline_idx, hipStream_t stream);
 
+// ---- products with packed 4-bit weights (quantmat.hip) --------------------------
+
+struct QMatArgs {
+    bool q4k;            // Q4_K blocks of 256 values, else Q4_0 blocks of 32
+    const void *w;       // m packed rows of k values, row after row
+    uint32_t k, m, n;
+    const float *x;      // [k, n]
+    int64_t x_st[2];     // element strides
+    float *y;            // [m, n]
+    int64_t y_st[2];
+    void *workspace;     // quant_mat_workspace_bytes
+};
+
+uint64_t quant_mat_workspace_bytes(const QMatArgs &args);
+hipError_t launch_quant_mat(const QMatArgs &args, hipStream_t stream);
+
+// ---- paged key-value cache (paged.hip) --------------------------------------------
+
+// One pool of pages of halves, [dim, page, kv_heads, pages]; strides in halves.
+struct PagePool {
+    uint16_t *data;
+    int64_t st_tok, st_head, st_page;
+};
+
+struct PagedAppendArgs {
+    bool bf16;
+    uint32_t dim, page, kv_heads, pages, tokens;
+    const float *k, *v;  // [dim, kv_heads, tokens]
+    int64_t k_st[3], v_st[3];
+    const int32_t *slots;
+    int64_t slots_st;
+    PagePool k_pool, v_pool;
+};
+
+hipError_t launch_paged_append(const PagedAppendArgs &args, hipStream_t stream);
+
+struct PagedAttnArgs {
+    bool bf16;
+    uint32_t dim, page, kv_heads, pages, heads, seqs, max_pages;
+    const float *q;      // [dim, heads, seqs]
+    int64_t q_st[3];
+    PagePool k_pool, v_pool;
+    const int32_t *table; // [max_pages, seqs]
+    int64_t table_st[2];
+    const int32_t *lengths;
+    int64_t lengths_st;
+    float scale, soft_cap;
+    uint32_t window;     // 0: none
+    float *y;            // [dim, heads, seqs]
+    int64_t y_st[3];
+    void *workspace;     // paged_attn_workspace_bytes
+};
+
+uint64_t paged_attn_workspace_bytes(const PagedAttnArgs &args);
+hipError_t launch_paged_attn(const PagedAttnArgs &args, hipStream_t stream);
+
+// ---- logits penalties, biases and masks (logits.hip) --------------------------------
+
+// A [entries, rows] operand; data is null when absent, row stride 0 for one
+// row that serves all.
+struct RowTable {
+    const void *data;
+    uint32_t entries;
+    int64_t st, row_st; // element strides
+};
+
+struct LogitsAdjustArgs {
+    uint32_t card, rows;
+    const float *x;
+    int64_t x_st, x_row;
+    float *y;
+    int64_t y_st, y_row;
+    RowTable history, history_len, repeat, frequency, presence, bias_ids, bias, allowed;
+};
+
+hipError_t launch_logits_adjust(const LogitsAdjustArgs &args, hipStream_t stream);
+
 // ---- logits sampler and validator (sampler.hip) -------------------------------
 
 // rows independent SampleTemperatureTopK requests over row-strided buffers

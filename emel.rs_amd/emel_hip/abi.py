@@ -274,6 +274,14 @@ class CSampleRows(ctypes.Structure):
     ]
 
 
+class CLogitsAdjustRequest(ctypes.Structure):
+    """emel_logits_adjust_request: operands by pointer, absent ones NULL."""
+
+    _fields_ = [(name, ctypes.POINTER(CView)) for name in (
+        "logits", "adjusted", "history", "history_len", "repeat", "frequency", "presence", "bias_ids", "bias",
+        "allowed")] + [("reserved", ctypes.c_uint64)]
+
+
 _V = ctypes.POINTER(CView)
 _S = ctypes.c_void_p
 _ST = ctypes.c_int
@@ -341,6 +349,11 @@ SIGNATURES = {
     "emel_stream_workspace": [_S, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)],
     "emel_device_prepare": [_S],
     "emel_stream_copy": [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, _S],
+    "emel_op_mul_mat_q4_0": [_V, _V, _V, _S],
+    "emel_op_mul_mat_q4_k": [_V, _V, _V, _S],
+    "emel_op_paged_kv_append": [_V, _V, _V, _V, _V, _S],
+    "emel_op_paged_attention": [_V, _V, _V, _V, _V, ctypes.c_float, ctypes.c_uint64, ctypes.c_float, _V, _S],
+    "emel_logits_adjust": [ctypes.POINTER(CLogitsAdjustRequest), _S],
     "emel_generic_dispatch": [ctypes.POINTER(CGenericRequest), _S],
     **{f"emel_op_get_rows{suffix}": [_V, ctypes.POINTER(CIndexView), _V, _S]
        for suffix in ("", "_f32_bytes", "_f16", "_bf16", "_q4_0", "_q8_0", "_q4_k")},

@@ -286,6 +286,23 @@ pub struct EmelSampleRows {
     pub top_stride: u64,
 }
 
+/// `emel_logits_adjust_request`: absent operands are null.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct EmelLogitsAdjustRequest {
+    pub logits: *const EmelTensorView,
+    pub adjusted: *const EmelTensorViewMut,
+    pub history: *const EmelTensorView,
+    pub history_len: *const EmelTensorView,
+    pub repeat: *const EmelTensorView,
+    pub frequency: *const EmelTensorView,
+    pub presence: *const EmelTensorView,
+    pub bias_ids: *const EmelTensorView,
+    pub bias: *const EmelTensorView,
+    pub allowed: *const EmelTensorView,
+    pub reserved: u64,
+}
+
 // Linked by build.rs (`cargo:rustc-link-lib=dylib=emel_hip`).
 unsafe extern "C" {
     pub fn emel_abi_version() -> u32;
@@ -361,9 +378,14 @@ unsafe extern "C" {
     pub fn emel_op_get_rows_q4_0(src: *const EmelTensorView, indices: *const EmelIndexView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_op_get_rows_q8_0(src: *const EmelTensorView, indices: *const EmelIndexView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_op_get_rows_q4_k(src: *const EmelTensorView, indices: *const EmelIndexView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
+    pub fn emel_op_mul_mat_q4_0(weights: *const EmelTensorView, x: *const EmelTensorView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
+    pub fn emel_op_mul_mat_q4_k(weights: *const EmelTensorView, x: *const EmelTensorView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
+    pub fn emel_op_paged_kv_append(k: *const EmelTensorView, v: *const EmelTensorView, slots: *const EmelTensorView, k_pages: *const EmelTensorViewMut, v_pages: *const EmelTensorViewMut, stream: Stream) -> Status;
+    pub fn emel_op_paged_attention(q: *const EmelTensorView, k_pages: *const EmelTensorView, v_pages: *const EmelTensorView, page_table: *const EmelTensorView, lengths: *const EmelTensorView, scale: f32, window: u64, soft_cap: f32, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_generic_dispatch(request: *const EmelGenericRequest, stream: Stream) -> Status;
     pub fn emel_sample_temperature_top_k(request: *const EmelSampleTemperatureTopKRequest, stream: Stream) -> Status;
     pub fn emel_sample_temperature_top_k_rows(request: *const EmelSampleTemperatureTopKRequest, rows: *const EmelSampleRows, stream: Stream) -> Status;
     pub fn emel_sample_preselected(vocab_size: u64, selected_token: i32, token_out: *mut i32) -> Status;
+    pub fn emel_logits_adjust(request: *const EmelLogitsAdjustRequest, stream: Stream) -> Status;
     pub fn emel_logits_validator_build(logits: *const f32, logits_len: u64, vocab_size: i32, candidate_ids: *mut i32, candidate_ids_len: u64, candidate_scores: *mut f32, candidate_scores_len: u64, candidate_capacity: i32, candidate_count_out: *mut i32, error_out: *mut i32, stream: Stream) -> Status;
 }

@@ -23,6 +23,7 @@
 
 #![allow(unsafe_code)] // an FFI crate: every unsafe block carries its SAFETY note
 
+pub mod decode;
 mod device;
 pub mod event;
 pub mod ffi;

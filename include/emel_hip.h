@@ -497,6 +497,71 @@ emel_status emel_op_get_rows_q8_0(const emel_tensor_view *src, const emel_index_
 emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_view *indices,
                                   const emel_tensor_view_mut *dst, emel_stream stream);
 
+/* ---- products with packed 4-bit weights ------------------------------------------
+ * No counterpart in the pinned path: the product that goes with the Q4_0 and
+ * Q4_K rows get_rows decodes, for a decoder's projections and output head.
+ *   dst[r, c] = sum over k of W[r, k] x[k, c]
+ * weights is a packed view [k, m, 1, 1] (the rules of get_rows' packed
+ * sources: nb = [1, row bytes, ...], k a multiple of 32 resp. 256), x is F32
+ * [k, n, 1, 1], dst F32 [m, n, 1, 1]; x and dst may have any strides, dst's
+ * elements disjoint and apart from both sources.  W[r, k] is the value that
+ * get_rows gives: (q - 8) d for Q4_0, d sc q - dmin m for Q4_K.  Each x is
+ * read to 22 bits below its leading one (values under 2^-16 of their
+ * column's largest lose further low bits), products are exact and sums are
+ * f32, in an order that depends on the sizes alone; infinities and NaN go
+ * through as in the formula.  Wants the stream's workspace for n > 4 or a
+ * long k, which grows as the reductions' does.  Guards: a NULL view or data,
+ * or an unaligned F32 pointer, is INVALID_ARGUMENT; a view that fails its
+ * rules, or an overlap, INVALID_VIEW; extents that do not match,
+ * SHAPE_MISMATCH; an extent past 2^31 - 1, UNSUPPORTED_OPERATION. */
+emel_status emel_op_mul_mat_q4_0(const emel_tensor_view *weights, const emel_tensor_view *x,
+                                 const emel_tensor_view_mut *dst, emel_stream stream);
+emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_tensor_view *x,
+                                 const emel_tensor_view_mut *dst, emel_stream stream);
+
+/* ---- paged key-value cache ---------------------------------------------------------
+ * No counterpart in the pinned path.  The cache is two pools of pages, one for
+ * keys and one for values: F16 or BF16 views [dim, page, kv_heads, pages]
+ * with nb[0] == 2 and any other strides (a token's heads side by side, or a
+ * head's tokens, or both pools interleaved in one allocation), the same type
+ * and extents for both.  Slot p * page + t is token t of page p.
+ *
+ * emel_op_paged_kv_append writes token t's keys k[:, :, t] and values
+ * v[:, :, t] (F32 [dim, kv_heads, tokens, 1]), rounded to the nearest half,
+ * into slot slots[t] (I32 [tokens, 1, 1, 1], device memory).  A slot that is
+ * negative or past the pool skips its token; of tokens with the same slot
+ * the last one is stored.
+ *
+ * emel_op_paged_attention attends from one new token of each sequence:
+ *   dst[:, h, s] = sum over j of softmax_j(f(scale q[:, h, s] . k_j)) v_j
+ * over positions j in [max(0, len - window), len), len = lengths[s] (window 0:
+ * all of them; the new token's own key is in the cache by then), f(z) =
+ * soft_cap tanh(z / soft_cap) where soft_cap > 0 and z where it is 0.  q and
+ * dst are F32 [dim, heads, seqs, 1]; heads is a multiple of kv_heads, and
+ * head h reads cache head h / (heads / kv_heads).  Position j of sequence s
+ * is token j % page of page page_table[j / page, s] (I32 [max pages, seqs, 1,
+ * 1]); lengths is I32 [seqs, 1, 1, 1].  dim is a multiple of 8, at most 256
+ * (else UNSUPPORTED_OPERATION).  Both index tensors are device memory, read
+ * when the kernel runs, so a captured call follows them.  A sequence of
+ * length 0 gets zeros.  One whose length is negative or past max pages * page, or that
+ * reaches a page id outside the pool, gets NaN, and nothing outside the pool
+ * is read.  What lies behind a sequence's length, and before its window, is
+ * never read.  Scores, softmax and sums are f32; q and the softmax weights
+ * keep 22 bits (F16 pools) or 24 (BF16) in products with the cached halves.
+ * Wants the stream's workspace, which grows as the reductions' does: graphs
+ * captured from one stream share it, and run one after the other, or are
+ * captured from streams of their own.
+ *
+ * Guards of both: as mul_mat_q4_0; parameters that are not finite, or a
+ * negative soft_cap, are INVALID_PARAMETERS. */
+emel_status emel_op_paged_kv_append(const emel_tensor_view *k, const emel_tensor_view *v,
+                                    const emel_tensor_view *slots, const emel_tensor_view_mut *k_pages,
+                                    const emel_tensor_view_mut *v_pages, emel_stream stream);
+emel_status emel_op_paged_attention(const emel_tensor_view *q, const emel_tensor_view *k_pages,
+                                    const emel_tensor_view *v_pages, const emel_tensor_view *page_table,
+                                    const emel_tensor_view *lengths, float scale, uint64_t window, float soft_cap,
+                                    const emel_tensor_view_mut *dst, emel_stream stream);
+
 /* ---- generic wire envelope ----------------------------------------------------
  * event::GenericEvent::new(GenericRequest::new(operation, src0, src1, src2,
  * dst, OpParams).with_unary(..).with_index_out(..)) (generic.rs:634-797):
@@ -652,6 +717,40 @@ emel_status emel_sample_temperature_top_k_rows(const emel_sample_temperature_top
  * selected_token)) (sampler/sm.rs:129-146, :366-378, guard :685-695):
  * host-only; writes *token_out (HOST) on success. */
 emel_status emel_sample_preselected(uint64_t vocab_size, int32_t selected_token, int32_t *token_out);
+
+/* Penalties, biases and a token mask on logits ahead of the sampler; no
+ * counterpart in the pinned path.  adjusted (F32 [card, rows, 1, 1]) may be
+ * exactly logits (in place: only what changes is written) or apart from it.
+ * In this order, each step rounded to f32, for token i of row r:
+ *   seen n > 0 times in the row's history:
+ *     l = l > 0 ? l / repeat[r] : l * repeat[r];
+ *     l = (l - n * frequency[r]) - presence[r];
+ *   named by a bias entry: l = l + bias (of entries with the same id the last);
+ *   its bit clear in the row's mask: l = -inf.
+ * history is I32 [entries, rows, 1, 1], of which the first history_len[r] (I32
+ * [rows, 1, 1, 1], clamped to [0, entries]; NULL: all) count; ids outside
+ * [0, card) are ignored, in bias_ids too.  repeat, frequency and presence
+ * (F32 [rows, 1, 1, 1], used as they are; NULL: 1, 0, 0) go with a history.
+ * bias_ids (I32) and bias (F32) are [entries, rows, 1, 1], both or neither.
+ * allowed is I32 [ceil(card / 32), rows, 1, 1], bit i % 32 of word i / 32.
+ * An operand whose rows extent is 1 serves every row.  All views are device
+ * memory; absent ones are NULL.  Guards: as emel_op_mul_mat_q4_0, reserved !=
+ * 0 or a part without its other half is INVALID_REQUEST. */
+typedef struct emel_logits_adjust_request {
+    const emel_tensor_view *logits;
+    const emel_tensor_view_mut *adjusted;
+    const emel_tensor_view *history;
+    const emel_tensor_view *history_len;
+    const emel_tensor_view *repeat;
+    const emel_tensor_view *frequency;
+    const emel_tensor_view *presence;
+    const emel_tensor_view *bias_ids;
+    const emel_tensor_view *bias;
+    const emel_tensor_view *allowed;
+    uint64_t reserved; /* must be 0 */
+} emel_logits_adjust_request;
+
+emel_status emel_logits_adjust(const emel_logits_adjust_request *request, emel_stream stream);
 
 /* ValidatorError (validator/sm.rs:15-21) discriminants, as *error_out. */
 typedef enum emel_validator_error {
