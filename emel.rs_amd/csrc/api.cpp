@@ -2819,11 +2819,11 @@ emel_status paged_attention(const emel_tensor_view *q, const emel_tensor_view *k
     a.soft_cap = soft_cap;
     a.window = static_cast<uint32_t>(window > kMaxExtent ? 0 : window); // longer than any sequence: none
     StreamLease lease;
-    if (const uint64_t bytes = emel::paged_attn_workspace_bytes(a)) {
-        s = lease.acquire(as_stream(stream));
-        if (s == EMEL_OK) s = lease.work(bytes, &a.workspace);
-        if (s != EMEL_OK) return s;
-    }
+    const emel::PagedScratch need = emel::paged_attn_scratch(a);
+    s = lease.acquire(as_stream(stream));
+    if (s == EMEL_OK) s = lease.work(need.work, &a.workspace);
+    if (s == EMEL_OK) s = lease.counters(need.counters, &a.counters);
+    if (s != EMEL_OK) return s;
     return launched(emel::launch_paged_attn(a, as_stream(stream)));
 }
 

@@ -283,10 +283,14 @@ struct PagedAttnArgs {
     uint32_t window;     // 0: none
     float *y;            // [dim, heads, seqs]
     int64_t y_st[3];
-    void *workspace;     // paged_attn_workspace_bytes
+    void *workspace;     // at least scratch.work bytes
+    void *counters;      // at least scratch.counters bytes, zero at rest
 };
 
-uint64_t paged_attn_workspace_bytes(const PagedAttnArgs &args);
+struct PagedScratch {
+    uint64_t work, counters;
+};
+PagedScratch paged_attn_scratch(const PagedAttnArgs &args);
 hipError_t launch_paged_attn(const PagedAttnArgs &args, hipStream_t stream);
 
 // ---- logits penalties, biases and masks (logits.hip) --------------------------------
