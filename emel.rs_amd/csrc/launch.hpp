@@ -291,6 +291,8 @@ struct PagedScratch {
     uint64_t work, counters;
 };
 PagedScratch paged_attn_scratch(const PagedAttnArgs &args);
+// Sequences of these extents that one launch takes; 0: not even one.
+uint32_t paged_attn_seqs(const PagedAttnArgs &args);
 hipError_t launch_paged_attn(const PagedAttnArgs &args, hipStream_t stream);
 
 // ---- logits penalties, biases and masks (logits.hip) --------------------------------

@@ -76,7 +76,10 @@ __global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a)
 
 constexpr uint32_t kPaUnit = 128;  // tokens of a unit, 32 a wave
 constexpr uint32_t kPaLine = 64;   // words between arrival counters (a cache line each)
-constexpr uint32_t kPaPerCu = 3;   // workgroups per compute unit
+
+// Workgroups that a compute unit holds at once: the registers that their
+// launch bounds leave them.
+constexpr uint32_t pa_per_cu(int ks) { return 2; }
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
@@ -85,6 +88,7 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 // pools may start at any half
 typedef u4 u4_any __attribute__((aligned(2)));
 typedef u2 u2_any __attribute__((aligned(2)));
+typedef v4f v4f_any __attribute__((aligned(4)));
 
 template <bool BF16>
 __device__ __forceinline__ v4f mfma32(u4 a, u4 b, v4f c)
@@ -129,11 +133,29 @@ __device__ __forceinline__ float rows16(float v, F f)
     return f(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
 }
 
+// Inclusive sum over the lanes up to each: within rows of 16 by shifts, then
+// each row's last lane to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t v)
+{
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v)
+{
+    v += dpp_or_zero<0x111, 0xF>(v); // row_shr 1, 2, 4, 8
+    v += dpp_or_zero<0x112, 0xF>(v);
+    v += dpp_or_zero<0x114, 0xF>(v);
+    v += dpp_or_zero<0x118, 0xF>(v);
+    v += dpp_or_zero<0x142, 0xA>(v); // row_bcast 15 into rows 1 and 3
+    v += dpp_or_zero<0x143, 0xC>(v); // row_bcast 31 into rows 2 and 3
+    return v;
+}
+
 // What a launch derives on the host.
 struct PaPlan {
     FastDiv page;       // tokens per page
+    FastDiv dim, grid, hgroups;
     uint32_t group;     // query heads of a cache head
-    uint32_t hgroups;   // 16s of them
     uint32_t rows;      // rows of a sequence: kv_heads * hgroups
     uint32_t slot;      // floats of a workspace slot
     float *parts;       // 2 slots a workgroup
@@ -145,9 +167,13 @@ struct PaSeq {
     bool bad;
 };
 
-__device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs &a, uint32_t s)
+__device__ __forceinline__ int32_t pa_len(const PagedAttnArgs &a, uint32_t s)
 {
-    const int32_t len = a.lengths[static_cast<int64_t>(s) * a.lengths_st];
+    return a.lengths[static_cast<int64_t>(s) * a.lengths_st];
+}
+
+__device__ __forceinline__ PaSeq pa_seq(const PagedAttnArgs &a, int32_t len)
+{
     PaSeq q;
     q.bad = len < 0 || static_cast<uint64_t>(len) > static_cast<uint64_t>(a.max_pages) * a.page;
     const uint32_t n = q.bad ? 0u : static_cast<uint32_t>(len);
@@ -165,6 +191,26 @@ __device__ __forceinline__ float pa_load(const float *p)
 {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ void pa_store2(float *p, float x, float y)
+{
+    const uint64_t v = __builtin_bit_cast(uint32_t, x) | static_cast<uint64_t>(__builtin_bit_cast(uint32_t, y)) << 32;
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 pa_load2(const float *p)
+{
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return __builtin_bit_cast(float2, v);
+}
+
+// tanh to a few units in the last place: its series to x^9 below 1/4 (the next term is
+// 2^-27 of x), 1 - 2 / (e^2x + 1) above.
+__device__ __forceinline__ float pa_tanh(float x)
+{
+    const float s = x * x;
+    const float p = x - x * s * (0.333333343f - s * (0.133333340f - s * (0.0539682545f - s * 0.0218694881f)));
+    const float e = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.88539008177792681472f) + 1.0f);
+    return __builtin_fabsf(x) < 0.25f ? p : e;
+}
 
 // 2^(m - ref) of a part whose maximum is m, in a whole whose maximum is ref.
 __device__ __forceinline__ float pa_weight(float m, float ref)
@@ -174,103 +220,93 @@ __device__ __forceinline__ float pa_weight(float m, float ref)
 
 // KS: 32-dim steps of a score; VW: dims of a lane's values (4, 8, 12 or 16).
 template <bool BF16, int KS, int VW>
-__global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
+__global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
 {
     constexpr int P = kParts<BF16>;
     constexpr int kWaves = kBlock / kWave;
     constexpr float kLift = BF16 ? 0.0f : 14.0f;
-    extern __shared__ float joined[];            // [wave][head of the group][dim]
+    extern __shared__ __attribute__((aligned(16))) float joined[];            // [wave][head of the group][dim]
     __shared__ u4 qop[KS * P * kWave];           // score operands, lane after lane
-    __shared__ float qinv[16];
     __shared__ int64_t off[kWaves][2][32];       // a step's tokens in the key and value pools
-    __shared__ float wm[kWaves][16], wl[kWaves][16], jm[16], jl[16];
-    __shared__ uint64_t scan[kWaves], found[2];
+    __shared__ float wm[kWaves][16], wl[kWaves][16], jl[16];
+    __shared__ uint32_t scan[kWaves], found[2];
     __shared__ uint32_t last;
     const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     const uint32_t col = lane % 16, g = lane / 16;
-    const uint32_t dim = a.dim;
+    const uint32_t dim = a.dim, pitch = dim + 4; // of a head in joined
 
-    // this workgroup's run of units, and the sequence it starts in
-    const uint32_t per = (a.seqs + kBlock - 1) / kBlock;
-    const uint32_t s0 = tid * per < a.seqs ? tid * per : a.seqs, s1 = s0 + per < a.seqs ? s0 + per : a.seqs;
-    uint64_t mine = 0;
-    for (uint32_t s = s0; s < s1; ++s) mine += pa_seq(a, s).units;
-    uint64_t pre = mine;
-    for (int d = 1; d < kWave; d <<= 1) {
-        const uint64_t up = __shfl_up(pre, d, kWave);
-        if (lane >= static_cast<uint32_t>(d)) pre += up;
-    }
-    if (lane == kWave - 1) scan[wave] = pre;
-    __syncthreads();
-    uint64_t all = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (static_cast<uint32_t>(w) < wave) pre += scan[w];
-        all += scan[w];
-    }
-    pre -= mine;
-    const uint64_t total = all * pl.rows;
-    const uint64_t run = (total + gridDim.x - 1) / gridDim.x;
-    uint64_t cur = blockIdx.x * run;
-    if (cur >= total) return;
-    const uint64_t end = cur + run < total ? cur + run : total;
-    if (mine && pre * pl.rows <= cur && cur < (pre + mine) * pl.rows) {
-        uint32_t s = s0;
-        uint64_t at = pre;
-        for (uint32_t u = pa_seq(a, s).units; (at + u) * pl.rows <= cur; u = pa_seq(a, s).units) {
-            at += u;
-            ++s;
+    // This workgroup's run of units, and the sequence it starts in.  A row's
+    // set-up and end cost about a unit: it counts as one more, but where there
+    // is no more than a unit to a workgroup (that would only part the rows).
+    uint32_t total, run, cur, base; // base: the sequence's first unit
+    uint32_t s, setup;
+    int32_t s_len;
+    if (__builtin_expect(a.seqs <= kWave, 1)) { // every wave for itself: a sequence per lane
+        const int32_t len = lane < a.seqs ? pa_len(a, lane) : 0;
+        const uint32_t mine = lane < a.seqs ? pa_seq(a, len).units : 0;
+        uint32_t pre = wave_scan(mine);
+        const uint32_t all = lane_u32(pre, kWave - 1);
+        setup = all * pl.rows > gridDim.x;
+        total = (all + setup * a.seqs) * pl.rows;
+        pre += setup * (lane + 1);
+        run = pl.grid.div(total + gridDim.x - 1);
+        cur = blockIdx.x * run;
+        if (cur >= total) return;
+        s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__popcll(__ballot(lane < a.seqs && pre * pl.rows <= cur))));
+        base = lane_u32(pre - mine - setup, s) * pl.rows;
+        s_len = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len), s));
+    } else {
+        const uint32_t per = (a.seqs + kBlock - 1) / kBlock;
+        const uint32_t s0 = tid * per < a.seqs ? tid * per : a.seqs, s1 = s0 + per < a.seqs ? s0 + per : a.seqs;
+        uint32_t mine = 0;
+#pragma unroll 1
+        for (uint32_t i = s0; i < s1; ++i) mine += pa_seq(a, pa_len(a, i)).units;
+        uint32_t pre = wave_scan(mine);
+        if (lane == kWave - 1) scan[wave] = pre;
+        __syncthreads();
+        uint32_t all = 0;
+        for (int w = 0; w < kWaves; ++w) {
+            if (static_cast<uint32_t>(w) < wave) pre += scan[w];
+            all += scan[w];
         }
-        found[0] = s;
-        found[1] = at;
-    }
-    __syncthreads();
-    uint32_t s = static_cast<uint32_t>(found[0]);
-    uint64_t base = found[1] * pl.rows; // the sequence's first unit
-
-    while (cur < end) {
-        const PaSeq sq = pa_seq(a, s);
-        const uint32_t row = static_cast<uint32_t>((cur - base) / sq.units);
-        const uint64_t row_at = base + static_cast<uint64_t>(row) * sq.units;
-        const uint32_t u0 = static_cast<uint32_t>(cur - row_at);
-        const uint32_t u1 = end - row_at < sq.units ? static_cast<uint32_t>(end - row_at) : sq.units;
-        const uint32_t kh = row / pl.hgroups, h0 = kh * pl.group + (row % pl.hgroups) * 16;
-        const uint32_t heads = (kh + 1) * pl.group - h0 < 16 ? (kh + 1) * pl.group - h0 : 16;
-
-        // score operands: thread (head, i) takes dims i, i + 16, ... of its head
-        {
-            const uint32_t h = tid / 16, i = tid % 16;
-            const float *q = a.q + static_cast<int64_t>(h0 + h) * a.q_st[1] + static_cast<int64_t>(s) * a.q_st[2];
-            const float c = a.soft_cap > 0.0f ? a.scale / a.soft_cap : a.scale * 1.44269504088896340736f;
-            float v[2 * KS], top = 0.0f;
-            for (int e = 0; e < 2 * KS; ++e) {
-                const uint32_t d = 16 * e + i;
-                v[e] = h < heads && d < dim ? q[static_cast<int64_t>(d) * a.q_st[0]] * c : 0.0f;
-                const float m = __builtin_fabsf(v[e]);
-                top = m > top && m < __builtin_inff() ? m : top;
+        setup = all * pl.rows > gridDim.x;
+        pre += setup * s0 - mine;
+        mine += setup * (s1 - s0);
+        total = (all + setup * a.seqs) * pl.rows;
+        run = pl.grid.div(total + gridDim.x - 1);
+        cur = blockIdx.x * run;
+        if (cur >= total) return;
+        if (mine && pre * pl.rows <= cur && cur < (pre + mine) * pl.rows) {
+            uint32_t i = s0;
+#pragma unroll 1
+            for (uint32_t u = pa_seq(a, pa_len(a, i)).units + setup; (pre + u) * pl.rows <= cur; u = pa_seq(a, pa_len(a, i)).units + setup) {
+                pre += u;
+                ++i;
             }
-            float up = 1.0f;
-            if constexpr (!BF16) {
-                for (int d = 8; d > 0; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 16));
-                int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
-                e = top == 0.0f ? 0 : e < -110 ? -110 : e;
-                up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 14 - e) << 23);
-                if (i == 0) qinv[h] = __builtin_bit_cast(float, static_cast<uint32_t>(127 - 14 + e) << 23);
-            }
-            uint16_t *halves = reinterpret_cast<uint16_t *>(qop);
-            for (int e = 0; e < 2 * KS; ++e) {
-                const uint32_t d = 16 * e + i;
-                uint32_t part[3];
-                split<BF16>(v[e] * up, part);
-                for (int p = 0; p < P; ++p)
-                    halves[(((d / 32) * P + p) * kWave + (d % 32) / 8 * 16 + h) * 8 + d % 8] = static_cast<uint16_t>(part[p]);
-            }
+            found[0] = i;
+            found[1] = pre;
         }
         __syncthreads();
+        s = found[0];
+        base = found[1] * pl.rows;
+        s_len = pa_len(a, s);
+    }
+    const uint32_t end = cur + run < total ? cur + run : total;
+
+    PaSeq sq = pa_seq(a, s_len);
+    uint32_t units = sq.units + setup;
+    uint32_t row = (cur - base) / units;
+    uint32_t row_at = base + row * units;
+
+    while (cur < end) {
+        const uint32_t n0 = cur - row_at, n1 = end - row_at < units ? end - row_at : units;
+        const uint32_t u0 = n0 > setup ? n0 - setup : 0, u1 = n1 - setup;
+        const uint32_t kh = pl.hgroups.div(row), h0 = kh * pl.group + (row - kh * pl.hgroups.d) * 16;
+        const uint32_t heads = (kh + 1) * pl.group - h0 < 16 ? (kh + 1) * pl.group - h0 : 16;
 
         const uint16_t *kbase = a.k_pool.data + static_cast<int64_t>(kh) * a.k_pool.st_head;
         const uint16_t *vbase = a.v_pool.data + static_cast<int64_t>(kh) * a.v_pool.st_head;
         const int32_t *table = a.table + static_cast<int64_t>(s) * a.table_st[1];
-        const float inv = BF16 ? 1.0f : qinv[col];
         float m = -__builtin_inff(), l = 0.0f;
         v4f acc[VW];
         for (int j = 0; j < VW; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -283,6 +319,68 @@ __global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
             return t < t_end ? table[static_cast<int64_t>(pl.page.div(sq.first + t)) * a.table_st[0]] : 0;
         };
         int32_t next = page_of(t0 + lane % 32);
+
+        // score operands, lane (col, g): dims 32 e + 8 g .. + 7 of head col;
+        // each wave lays out every fourth e
+        float inv = 1.0f;
+        {
+            const float *q = a.q + static_cast<int64_t>(h0 + col) * a.q_st[1] + static_cast<int64_t>(s) * a.q_st[2];
+            const float c = a.soft_cap > 0.0f ? a.scale / a.soft_cap : a.scale * 1.44269504088896340736f;
+            auto eight = [&](uint32_t e, float x[8]) {
+                const uint32_t d = 32 * e + 8 * g;
+                if (col < heads && d < dim) {
+                    if (__builtin_expect(a.q_st[0] == 1, 1)) {
+                        const v4f lo = *reinterpret_cast<const v4f_any *>(q + d), hi = *reinterpret_cast<const v4f_any *>(q + d + 4);
+                        for (int i = 0; i < 4; ++i) {
+                            x[i] = lo[i] * c;
+                            x[4 + i] = hi[i] * c;
+                        }
+                    } else {
+                        for (int i = 0; i < 8; ++i) x[i] = q[static_cast<int64_t>(d + i) * a.q_st[0]] * c;
+                    }
+                } else {
+                    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+                }
+            };
+            float up = 1.0f;
+            if constexpr (!BF16) { // the head's largest value to [2^14, 2^15)
+                float top = 0.0f;
+                auto fold = [&](const float x[8]) {
+                    for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(x[i]));
+                };
+                if constexpr (KS <= 4) { // all loads at once
+                    float x[KS][8];
+                    for (int e = 0; e < KS; ++e) eight(e, x[e]);
+                    for (int e = 0; e < KS; ++e) fold(x[e]);
+                } else {
+#pragma unroll 2
+                    for (int e = 0; e < KS; ++e) {
+                        float x[8];
+                        eight(e, x);
+                        fold(x);
+                    }
+                }
+                top = rows16(top, [](float u, float v) { return __builtin_fmaxf(u, v); });
+                int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
+                e = top == 0.0f || e == 128 ? 0 : e < -110 ? -110 : e; // infinite: the wave walks below
+                up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 14 - e) << 23);
+                inv = __builtin_bit_cast(float, static_cast<uint32_t>(127 - 14 + e) << 23);
+            }
+#pragma unroll 1
+            for (uint32_t e = wave; e < KS; e += kWaves) {
+                float x[8];
+                eight(e, x);
+                u4 w[P];
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t even[3], odd[3];
+                    split<BF16>(x[2 * i] * up, even);
+                    split<BF16>(x[2 * i + 1] * up, odd);
+                    for (int p = 0; p < P; ++p) w[p][i] = even[p] | (odd[p] << 16);
+                }
+                for (int p = 0; p < P; ++p) qop[(e * P + p) * kWave + lane] = w[p];
+            }
+        }
+        __syncthreads();
         for (; t0 < t_end; t0 += kPaUnit) {
             {
                 const uint32_t t = t0 + lane % 32;
@@ -327,8 +425,8 @@ __global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
                     for (int p = P - 1; p >= 0; --p) c = mfma32<BF16>(k[b][e], qop[(e * P + p) * kWave + lane], c);
                 for (int i = 0; i < 4; ++i) z[4 * b + i] = BF16 ? c[i] : c[i] * inv;
             }
-            if (a.soft_cap > 0.0f)
-                for (int i = 0; i < 8; ++i) z[i] = tanhf(z[i]) * (a.soft_cap * 1.44269504088896340736f);
+            if (__builtin_expect(a.soft_cap > 0.0f, 0))
+                for (int i = 0; i < 8; ++i) z[i] = pa_tanh(z[i]) * (a.soft_cap * 1.44269504088896340736f);
             if (t0 + 32 > t_end) { // the sequence ends in this step: nothing of what lies behind it counts
                 for (int b = 0; b < 8; ++b) {
                     if (t0 + 16 * (b / 4) + 4 * g + b % 4 < t_end) continue;
@@ -365,13 +463,14 @@ __global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
         }
 
         // the wave's part: [head][dim], dims of lane row c = 4 g + i
-        float *own = joined + static_cast<size_t>(wave) * heads * dim;
+        float *own = joined + wave * heads * pitch;
         l = rows16(l, [](float x, float y) { return x + y; });
-        bool odd = !(__builtin_fabsf(l) < __builtin_inff());
+        v4f zero = {l * 0.0f, 0.0f, 0.0f, 0.0f}; // stays zero while all is finite
         for (int j = 0; j < VW; ++j)
-            for (int i = 0; i < 4; ++i) odd |= !(__builtin_fabsf(acc[j][i]) < __builtin_inff());
+            for (int i = 0; i < 4; ++i) zero[i] = __builtin_fmaf(acc[j][i], 0.0f, zero[i]);
+        const bool odd = !((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f);
         bad = __any(bad);
-        if (__any(odd && col < heads) && !bad) {
+        if (__builtin_expect(__any(odd && col < heads) && !bad, 0)) {
             // as the formula stands: a head and a token at a time, a lane four dims
             for (uint32_t h = 0; h < heads; ++h) {
                 const float *q = a.q + static_cast<int64_t>(h0 + h) * a.q_st[1] + static_cast<int64_t>(s) * a.q_st[2];
@@ -390,7 +489,7 @@ __global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
                         for (uint32_t i = 0; i < 4; ++i)
                             if (4 * lane + i < dim) zz += qv[i] * from_half<BF16>(kp[4 * lane + i]);
                         zz = wave_sum(zz) * a.scale;
-                        if (a.soft_cap > 0.0f) zz = a.soft_cap * tanhf(zz / a.soft_cap);
+                        if (a.soft_cap > 0.0f) zz = a.soft_cap * pa_tanh(zz / a.soft_cap);
                         zz *= 1.44269504088896340736f;
                         const float m1 = __builtin_fmaxf(mm, zz);
                         const float ref = m1 == -__builtin_inff() ? 0.0f : m1;
@@ -404,7 +503,7 @@ __global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
                 }
                 const float lift = BF16 ? 1.0f : 16384.0f;
                 for (uint32_t i = 0; i < 4; ++i)
-                    if (4 * lane + i < dim) own[h * dim + 4 * lane + i] = av[i] * lift;
+                    if (4 * lane + i < dim) own[h * pitch + 4 * lane + i] = av[i] * lift;
                 if (lane == 0) {
                     wm[wave][h] = mm;
                     wl[wave][h] = ll * lift;
@@ -419,46 +518,59 @@ __global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
                 const uint32_t c = 4 * g + i;
                 for (int e = 0; e < VW / 8; ++e)
                     if (128 * e + 8 * c < dim)
-                        for (int j = 0; j < 8; ++j) own[col * dim + 128 * e + 8 * c + j] = acc[8 * e + j][i];
+                        for (int j = 0; j < 8; j += 4)
+                            *reinterpret_cast<v4f *>(own + col * pitch + 128 * e + 8 * c + j) =
+                                v4f{acc[8 * e + j][i], acc[8 * e + j + 1][i], acc[8 * e + j + 2][i], acc[8 * e + j + 3][i]};
                 if constexpr (VW % 8) {
                     const uint32_t d = VW / 8 * 128 + 4 * c;
                     if (d < dim)
-                        for (int j = 0; j < 4; ++j) own[col * dim + d + j] = acc[VW - 4 + j][i];
+                        *reinterpret_cast<v4f *>(own + col * pitch + d) = v4f{acc[VW - 4][i], acc[VW - 3][i], acc[VW - 2][i], acc[VW - 1][i]};
                 }
             }
         }
         __syncthreads();
-        if (tid < heads) {
-            float top = wm[0][tid], sum = 0.0f;
-            for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, wm[w][tid]);
-            for (int w = 0; w < kWaves; ++w) sum += wl[w][tid] * pa_weight(wm[w][tid], top);
-            jm[tid] = top;
-            jl[tid] = sum;
+        const bool whole = n0 == 0 && n1 == units;
+        const uint32_t w0 = n0 == 0 ? blockIdx.x : row_at / run; // the row's first workgroup
+        float *slot = pl.parts + static_cast<size_t>(2 * blockIdx.x + (n0 == 0 ? 1 : 0)) * pl.slot;
+        // the waves' maximum and sum of a head, and each wave's weight
+        auto join = [&](uint32_t h, float f[kWaves], float &sum) {
+            float top = wm[0][h];
+            for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, wm[w][h]);
+            sum = 0.0f;
+            for (int w = 0; w < kWaves; ++w) {
+                f[w] = pa_weight(wm[w][h], top);
+                sum += wl[w][h] * f[w];
+            }
+            return top;
+        };
+        const uint32_t cells = heads * dim; // dim is even: pairs do not cross heads
+        float *out = a.y + static_cast<int64_t>(h0) * a.y_st[1] + static_cast<int64_t>(s) * a.y_st[2];
+        auto put = [&](uint32_t h, uint32_t d, float x, float y) {
+            float *o = out + static_cast<int64_t>(d) * a.y_st[0] + static_cast<int64_t>(h) * a.y_st[1];
+            o[0] = x;
+            o[a.y_st[0]] = y;
+        };
+        for (uint32_t e = 2 * tid; e < cells; e += 2 * kBlock) {
+            const uint32_t h = pl.dim.div(e), d = e - h * dim;
+            float f[kWaves], sum, x = 0.0f, y = 0.0f;
+            join(h, f, sum);
+            for (int w = 0; w < kWaves; ++w) {
+                x += joined[(w * heads + h) * pitch + d] * f[w];
+                y += joined[(w * heads + h) * pitch + d + 1] * f[w];
+            }
+            if (!whole) pa_store2(slot + 32 + e, x, y);
+            else if (sq.tokens == 0 && !sq.bad) put(h, d, 0.0f, 0.0f);
+            else put(h, d, x * (1.0f / sum), y * (1.0f / sum));
         }
-        __syncthreads();
-        const bool whole = u0 == 0 && u1 == sq.units;
-        const uint32_t w0 = static_cast<uint32_t>(row_at / run); // the row's first workgroup
-        float *slot = pl.parts + static_cast<size_t>(2 * blockIdx.x + (blockIdx.x == w0 ? 1 : 0)) * pl.slot;
-        const uint32_t cells = heads * dim;
-        for (uint32_t e = tid; e < cells; e += kBlock) {
-            const uint32_t h = e / dim, d = e % dim;
-            float v = 0.0f;
-            for (int w = 0; w < kWaves; ++w)
-                v += joined[static_cast<size_t>(w) * cells + e] * pa_weight(wm[w][h], jm[h]);
-            if (whole)
-                a.y[static_cast<int64_t>(d) * a.y_st[0] + static_cast<int64_t>(h0 + h) * a.y_st[1] + static_cast<int64_t>(s) * a.y_st[2]] =
-                    sq.tokens == 0 && !sq.bad ? 0.0f : v / jl[h];
-            else
-                pa_store(slot + 32 + e, v);
-        }
-        if (!whole) {
+        if (__builtin_expect(!whole, 0)) {
             if (tid < heads) {
-                pa_store(slot + tid, jm[tid]);
-                pa_store(slot + 16 + tid, jl[tid]);
+                float f[kWaves], sum;
+                pa_store(slot + tid, join(tid, f, sum));
+                pa_store(slot + 16 + tid, sum);
             }
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
-            const uint32_t w1 = static_cast<uint32_t>((row_at + sq.units - 1) / run), pieces = w1 - w0 + 1;
+            const uint32_t pieces = (row_at + units - 1) / run - w0 + 1;
             if (tid == 0) {
                 uint32_t *arrived = pl.arrived + static_cast<size_t>(w0) * kPaLine;
                 last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == pieces - 1;
@@ -467,33 +579,76 @@ __global__ __launch_bounds__(kBlock) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
             __syncthreads();
             if (last) {
                 auto piece = [&](uint32_t p) { return pl.parts + static_cast<size_t>(2 * (w0 + p) + (p == 0 ? 1 : 0)) * pl.slot; };
-                if (tid / 16 < heads) { // 16 threads a head
-                    const uint32_t h = tid / 16;
-                    float top = -__builtin_inff(), sum = 0.0f;
-                    for (uint32_t p = tid % 16; p < pieces; p += 16) top = __builtin_fmaxf(top, pa_load(piece(p) + h));
-                    for (int d = 8; d > 0; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 16));
-                    for (uint32_t p = tid % 16; p < pieces; p += 16) sum += pa_load(piece(p) + 16 + h) * pa_weight(pa_load(piece(p) + h), top);
-                    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 16);
-                    if (tid % 16 == 0) {
-                        jm[h] = top;
-                        jl[h] = sum;
+                float *weight = joined; // [piece][head]
+                // The first loads of everything go out together: maxima and
+                // sums (16 threads a head), then the thread's first pair.
+                const uint32_t hh = tid / 16 < heads ? tid / 16 : 0, i0 = tid % 16;
+                float pm[4], ps[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t p = i0 + 16 * i;
+                    const float *from = piece(p < pieces ? p : pieces - 1) + hh;
+                    pm[i] = pa_load(from);
+                    ps[i] = pa_load(from + 16);
+                }
+                float2 v[16];
+                auto sixteen = [&](uint32_t p0, uint32_t e) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) v[i] = pa_load2(piece(p0 + i < pieces ? p0 + i : pieces - 1) + 32 + e);
+                };
+                sixteen(0, 2 * tid < cells ? 2 * tid : 0);
+                float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) top = __builtin_fmaxf(top, pm[i]); // a repeated last piece changes nothing
+                const uint32_t more = tid / 16 < heads ? pieces : 0; // past 64, of the threads with a head
+                for (uint32_t p = i0 + 64; p < more; p += 16) {
+                    const float m1 = pa_load(piece(p) + hh);
+                    weight[p * heads + hh] = m1;
+                    top = __builtin_fmaxf(top, m1);
+                }
+                for (int d = 8; d > 0; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 16));
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t p = i0 + 16 * i;
+                    const float f = pa_weight(pm[i], top);
+                    if (p < pieces) {
+                        sum += ps[i] * f;
+                        if (tid / 16 < heads) weight[p * heads + hh] = f;
                     }
                 }
+                for (uint32_t p = i0 + 64; p < more; p += 16) {
+                    const float f = pa_weight(weight[p * heads + hh], top);
+                    sum += pa_load(piece(p) + 16 + hh) * f;
+                    weight[p * heads + hh] = f;
+                }
+                for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 16);
+                if (i0 == 0 && tid / 16 < heads) jl[hh] = sum;
                 __syncthreads();
-                for (uint32_t e = tid; e < cells; e += kBlock) {
-                    const uint32_t h = e / dim, d = e % dim;
-                    float v = 0.0f;
-#pragma unroll 4
-                    for (uint32_t p = 0; p < pieces; ++p) v += pa_load(piece(p) + 32 + e) * pa_weight(pa_load(piece(p) + h), jm[h]);
-                    a.y[static_cast<int64_t>(d) * a.y_st[0] + static_cast<int64_t>(h0 + h) * a.y_st[1] + static_cast<int64_t>(s) * a.y_st[2]] = v / jl[h];
+                for (uint32_t e = 2 * tid; e < cells; e += 2 * kBlock) {
+                    const uint32_t h = pl.dim.div(e), d = e - h * dim;
+                    float x = 0.0f, y = 0.0f;
+                    for (uint32_t p0 = 0; p0 < pieces; p0 += 16) {
+                        if (p0 > 0 || e != 2 * tid) sixteen(p0, e);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i)
+                            if (p0 + i < pieces) {
+                                const float f = weight[(p0 + i) * heads + h];
+                                x += v[i].x * f;
+                                y += v[i].y * f;
+                            }
+                    }
+                    if (sq.tokens == 0 && !sq.bad) put(h, d, 0.0f, 0.0f);
+                    else put(h, d, x * (1.0f / jl[h]), y * (1.0f / jl[h]));
                 }
             }
         }
         __syncthreads(); // the next segment reuses the shared arrays
-        cur = row_at + u1;
-        if (u1 == sq.units && row + 1 == pl.rows) {
-            ++s;
-            base += static_cast<uint64_t>(sq.units) * pl.rows;
+        cur = row_at + n1;
+        row_at += units;
+        if (++row == pl.rows && cur < end) {
+            row = 0;
+            sq = pa_seq(a, pa_len(a, ++s));
+            units = sq.units + setup;
         }
     }
 }
@@ -510,29 +665,39 @@ hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t stream)
 
 namespace {
 
-uint32_t pa_workgroups()
-{
-    static const uint32_t n = [] {
-        int dev = 0, cus = 0;
-        if (hipGetDevice(&dev) != hipSuccess ||
-            hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
-            cus = 256;
-        return static_cast<uint32_t>(cus) * kPaPerCu;
-    }();
-    return n;
-}
-
 uint32_t pa_heads(const PagedAttnArgs &a) // of a row
 {
     const uint32_t group = a.heads / a.kv_heads;
     return group < 16 ? group : 16;
 }
 
+// Workgroups that run at once, by registers and LDS, and their LDS: more would
+// wait for a second round with as large a run each.
+struct PaGrid {
+    uint32_t workgroups, lds;
+};
+PaGrid pa_grid(const PagedAttnArgs &a)
+{
+    static const uint32_t cus = [] {
+        int dev = 0, n = 0;
+        if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
+            n = 256;
+        return static_cast<uint32_t>(n);
+    }();
+    const uint32_t ks = (a.dim + 31) / 32, fixed = 4096 + ks * 3 * 1024;
+    uint32_t per = pa_per_cu(static_cast<int>(ks));
+    for (;; --per) {
+        const uint32_t joined = 4 * pa_heads(a) * (a.dim + 4), weights = pa_heads(a) * cus * per;
+        const uint32_t lds = 4 * (joined > weights ? joined : weights);
+        if (per == 1 || per * (fixed + lds) <= 160 * 1024) return {cus * per, lds};
+    }
+}
+
 template <bool BF16>
 hipError_t pa_launch(const PagedAttnArgs &a, const PaPlan &pl, hipStream_t stream)
 {
-    const uint32_t lds = 4 * pa_heads(a) * a.dim * sizeof(float);
-    const dim3 grid(pa_workgroups());
+    const PaGrid g = pa_grid(a);
+    const uint32_t grid = g.workgroups, lds = g.lds;
     switch ((a.dim + 31) / 32) {
     case 1: k_pa_attn<BF16, 1, 4><<<grid, kBlock, lds, stream>>>(a, pl); break;
     case 2: k_pa_attn<BF16, 2, 4><<<grid, kBlock, lds, stream>>>(a, pl); break;
@@ -550,21 +715,43 @@ hipError_t pa_launch(const PagedAttnArgs &a, const PaPlan &pl, hipStream_t strea
 
 PagedScratch paged_attn_scratch(const PagedAttnArgs &a)
 {
-    const uint64_t n = pa_workgroups();
+    const uint64_t n = pa_grid(a).workgroups;
     return {n * 2 * (32 + static_cast<uint64_t>(pa_heads(a)) * a.dim) * sizeof(float), n * kPaLine * sizeof(uint32_t)};
+}
+
+uint32_t paged_attn_seqs(const PagedAttnArgs &a)
+{
+    const uint64_t group = a.heads / a.kv_heads, rows = a.kv_heads * ((group + 15) / 16);
+    const uint64_t units = (static_cast<uint64_t>(a.max_pages) * a.page + kPaUnit - 1) / kPaUnit + 1;
+    const uint64_t n = 0x7fff0000ull / rows / units; // both factors are below 2^32
+    return static_cast<uint32_t>(n < a.seqs ? n : a.seqs);
 }
 
 hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream)
 {
     PaPlan pl;
     pl.page = FastDiv(a.page);
+    pl.dim = FastDiv(a.dim);
     pl.group = a.heads / a.kv_heads;
-    pl.hgroups = (pl.group + 15) / 16;
-    pl.rows = a.kv_heads * pl.hgroups;
+    pl.hgroups = FastDiv((pl.group + 15) / 16);
+    pl.rows = a.kv_heads * pl.hgroups.d;
+    pl.grid = FastDiv(pa_grid(a).workgroups);
     pl.slot = 32 + pa_heads(a) * a.dim;
     pl.parts = static_cast<float *>(a.workspace);
     pl.arrived = static_cast<uint32_t *>(a.counters);
-    return a.bf16 ? pa_launch<true>(a, pl, stream) : pa_launch<false>(a, pl, stream);
+    // units are counted in 32 bits: a batch with more of them runs in parts
+    PagedAttnArgs b = a;
+    const uint32_t step = paged_attn_seqs(a);
+    for (uint64_t s = 0; s < a.seqs; s += step) {
+        b.seqs = static_cast<uint32_t>(a.seqs - s < step ? a.seqs - s : step);
+        b.q = a.q + static_cast<int64_t>(s) * a.q_st[2];
+        b.y = a.y + static_cast<int64_t>(s) * a.y_st[2];
+        b.table = a.table + static_cast<int64_t>(s) * a.table_st[1];
+        b.lengths = a.lengths + static_cast<int64_t>(s) * a.lengths_st;
+        const hipError_t e = b.bf16 ? pa_launch<true>(b, pl, stream) : pa_launch<false>(b, pl, stream);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 } // namespace emel
