@@ -2619,7 +2619,8 @@ emel_status mul_mat_q4(bool q4k, const emel_tensor_view *w, const emel_tensor_vi
 {
     if (!data_ok(w, 1) || !data_ok(x, 4) || !data_ok(y, 4))
         return fail(EMEL_ERR_INVALID_ARGUMENT, "null view or data, or a misaligned pointer");
-    if (!extents_ok(*w, *x, *y)) return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent is past 2^31 - 1");
+    if (!extents_ok(*w, *x, *y) || w->ne[0] > 1u << 26)
+        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent is past 2^31 - 1, or k past 2^26");
     if (w->reserved != 0 || !(q4k ? packed_view_valid(*w, EMEL_DTYPE_Q4_K, 256, 144)
                                   : packed_view_valid(*w, EMEL_DTYPE_Q4_0, 32, 18)) ||
         !valid_f32(*x, true) || !valid_f32(*y, true))

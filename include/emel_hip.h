@@ -513,7 +513,8 @@ emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_
  * long k, which grows as the reductions' does.  Guards: a NULL view or data,
  * or an unaligned F32 pointer, is INVALID_ARGUMENT; a view that fails its
  * rules, or an overlap, INVALID_VIEW; extents that do not match,
- * SHAPE_MISMATCH; an extent past 2^31 - 1, UNSUPPORTED_OPERATION. */
+ * SHAPE_MISMATCH; an extent past 2^31 - 1 or a k past 2^26,
+ * UNSUPPORTED_OPERATION. */
 emel_status emel_op_mul_mat_q4_0(const emel_tensor_view *weights, const emel_tensor_view *x,
                                  const emel_tensor_view_mut *dst, emel_stream stream);
 emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_tensor_view *x,
