@@ -231,7 +231,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
     __shared__ float wm[kWaves][16], wl[kWaves][16], jl[16];
     __shared__ uint32_t scan[kWaves], found[2];
     __shared__ uint32_t last;
-    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t col = lane % 16, g = lane / 16;
     const uint32_t dim = a.dim, pitch = dim + 4; // of a head in joined
 

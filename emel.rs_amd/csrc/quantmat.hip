@@ -330,13 +330,13 @@ __global__ __launch_bounds__(kQmBlock) void k_qm_columns(QMatArgs a, QmPlan pl)
 
 // NR: a quarter of the columns, rounded up.  LDS: columns laid out here, else read from the workspace.
 template <bool Q4K, int NR, bool LDS>
-__global__ __launch_bounds__(kQmBlock, 4) void k_qm(QMatArgs a, QmPlan pl)
+__global__ __launch_bounds__(kQmBlock, 2) void k_qm(QMatArgs a, QmPlan pl)
 {
     constexpr int U = Q4K ? 2 : 4; // units in flight
     extern __shared__ u4 laid[];
     __shared__ float top[kQmWaves], downs[16];
     __shared__ float part[2][kQmWaves][NR][kWave];
-    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, j = lane % 16, g = lane / 16;
+    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), j = lane % 16, g = lane / 16;
     const uint32_t c0 = blockIdx.y * 16, n = a.n - c0 < 16 ? a.n - c0 : 16;
     const XLayout<Q4K> lay{(a.k + kUnit<Q4K> - 1) / kUnit<Q4K>, n};
     const uint32_t kw = pl.kw, tw = kQmWaves / kw, wk = wave % kw, wt = wave / kw;
