@@ -5,27 +5,41 @@
 // f16 d and dmin, eight 6-bit sc and m, 128 bytes of nibbles).
 //
 // Bound by the weights' bytes for the few columns of a decode step, if what is
-// done per weight stays small.  So the scales stay out of the inner product:
-// a 32-value group's nibbles are exact as f16 integers, and one 16x16x32
-// matrix instruction multiplies a group of 16 rows with up to 16 columns; the
-// scale then goes once into each group's f32 result.  x is f32, so a column
-// goes in as two halves, hi + lo, scaled by a power of two that brings its largest
-// value to [2^14, 2^15): 22 bits of every value down to 2^-16 of that, and
-// 2^-40 of it below.  Nibble-half products are exact, sums are f32.
-// A nibble becomes a half by and-or into 1024's mantissa and one packed
-// subtraction (or a packed fma for the high nibbles): 9 instructions for 8
-// weights, and about 5 more a group for lanes' exchange and scales.
+// done per weight stays small.  So scales and minima stay out of the inner
+// product: a matrix instruction multiplies a 32-value group of 16 rows with the columns,
+// nibbles as integers, and the group's scale goes once into its result.  x is
+// f32 and is not to lose by it; two ways, by the number of columns:
 //
-// Lane (j, g) of a wave works for row j of a tile of 16 rows.  Q4_0: it loads
-// the whole of every fourth block, and the four lanes of a row exchange so
-// that each instruction sees one block.  Q4_K: a block's nibbles are read 16
-// bytes a lane, two swaps make sub-blocks of them.  The order of values within a group
-// is whatever that gives; x is laid out in the same order.  The waves of a
-// workgroup share a tile's k range and add up through LDS.
+// k_qm_digits, up to four columns.  Each column's run of 256 values is a
+// fixed-point number of 30 bits and a sign, scaled by a power of two to its largest
+// value, and cut into four signed bytes.  The 16 columns of the 8-bit
+// instruction then hold 4 digits x 4 columns, and one instruction a group does
+// them all, exactly, in integers.  Eight weights cost three or four
+// instructions of unpacking, a group one LDS read, and a conversion and an fma
+// a column.  A value is off by 2^-30 of the largest of its 256 at most: less
+// than f32's own rounding of the sum that the largest is part of.
 //
-// hi + lo breaks 0 * inf and inf - inf, and a scale that is infinite times a
-// sum is not the sum of its products: an output that is not finite is
+// k_qm_halves, more columns.  A column goes in as two halves, hi + lo, scaled
+// by a power of two that brings its largest value to [2^14, 2^15): 22 bits of
+// every value down to 2^-16 of that, and 2^-40 of it below.  The 16 columns
+// of the f16 instruction are 16 columns, two instructions a group.  A nibble
+// becomes a half by and-or into 1024's mantissa and a packed subtraction (as a
+// subnormal half it would need neither, but the instruction drops as many
+// low bits of its sum as such a factor has leading zeros: 1e-5 off).
+//
+// Sums are f32, and their order depends on the sizes alone.
+//
+// Lane (j, g) of a wave works for row j of a tile of 16 rows.  It loads a
+// fourth of the row's 256-value unit, whole blocks of Q4_0 or 16 bytes of each
+// half of a Q4_K block, and the four lanes of a row exchange words so that each
+// instruction sees one group.  The order of values within a group is whatever
+// that gives; x is laid out in the same order.  The waves of a workgroup share
+// a tile's k range and add up through LDS.
+//
+// Neither digits nor halves hold infinities: an output that is not finite is
 // computed again as the formula stands, by the whole wave.
+#include <type_traits>
+
 #include "common.hpp"
 #include "launch.hpp"
 #include "libm_replica.hpp"
@@ -35,32 +49,20 @@ namespace {
 
 constexpr int kQmWaves = 8;
 constexpr int kQmBlock = kQmWaves * kWave;
-constexpr uint32_t kQmLds = 64 * 1024; // of laid-out columns: two workgroups fit a compute unit
+constexpr uint32_t kQmUnit = 256;      // values that a wave takes of a row at a time: eight groups
+constexpr uint32_t kQmLds = 70 * 1024; // of laid-out columns: two workgroups fit a compute unit
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef u4 u4_any __attribute__((aligned(1))); // packed rows may start at any byte
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef u4 u4_byte __attribute__((aligned(1))); // packed rows may start at any byte
+typedef u4 u4_word __attribute__((aligned(4)));
 typedef v4f v4f_any __attribute__((aligned(4)));
 
-// Per format: values of a unit (what a wave takes at a time), its bytes.
-template <bool Q4K>
-constexpr uint32_t kUnit = Q4K ? 256 : 128;
-
-// Columns as the matrix instruction reads them, in 16-byte pieces of 8 halves.
-// Column c of a group of 16 sits at [32-value group][part][c][lane row g]; Q4_K
-// adds each column's group sums (for the minima) at [unit][c][part].
-template <bool Q4K>
-struct XLayout {
-    uint32_t units, n; // n: columns laid out
-    __host__ __device__ uint32_t groups() const { return units * (kUnit<Q4K> / 32); }
-    __device__ uint32_t at(uint32_t group, uint32_t part, uint32_t c, uint32_t g) const { return ((group * 2 + part) * n + c) * 4 + g; }
-    __device__ uint32_t sum_at(uint32_t unit, uint32_t c, uint32_t part) const { return groups() * n * 8 + (unit * n + c) * 2 + part; }
-    __host__ __device__ uint64_t pieces() const { return static_cast<uint64_t>(groups()) * n * 8 + (Q4K ? units * n * 2 : 0); }
-};
-
 // Where the eight values of lane row g lie in their group: four from first
-// and four from second, dealt out evens before odds as the nibbles fall.
+// and four from second, dealt out as the nibbles fall.
 template <bool Q4K>
 __device__ __forceinline__ void value_places(uint32_t g, uint32_t &first, uint32_t &second)
 {
@@ -68,38 +70,150 @@ __device__ __forceinline__ void value_places(uint32_t g, uint32_t &first, uint32
     second = Q4K ? first + 4 : 16 + 4 * g;
 }
 
-__device__ __forceinline__ uint32_t pack(_Float16 a, _Float16 b)
-{
-    return __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
-}
-
-// The power of two that brings the largest finite magnitude into [2^14, 2^15), and its inverse.
-__device__ __forceinline__ void column_scale(float top, float &up, float &down)
-{
-    int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
-    e = top == 0.0f || e == 128 ? 0 : e < -110 ? -110 : e;
-    up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 14 - e) << 23);
-    down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - 14 + e) << 23);
-}
-
-// Lays out a column's eight values of (group, g): x points at the column.
+// Eight values of (group, g) of a column, times up; zeros past the column.
 template <bool Q4K>
-__device__ __forceinline__ void lay_out(const QMatArgs &a, const XLayout<Q4K> &lay, const float *x, float up, uint32_t group, uint32_t g, uint32_t c, u4 *to)
+__device__ __forceinline__ void load_values(const QMatArgs &a, const float *x, uint32_t group, uint32_t g, float v[8])
 {
     uint32_t p[2];
     value_places<Q4K>(g, p[0], p[1]);
-    float v[8];
     const uint32_t k0 = group * 32;
     if (k0 >= a.k) {
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     } else if (a.x_st[0] == 1) {
         const v4f lo = *reinterpret_cast<const v4f_any *>(x + k0 + p[0]), hi = *reinterpret_cast<const v4f_any *>(x + k0 + p[1]);
         for (int i = 0; i < 4; ++i) {
-            v[i] = lo[i] * up;
-            v[4 + i] = hi[i] * up;
+            v[i] = lo[i];
+            v[4 + i] = hi[i];
         }
     } else {
-        for (int i = 0; i < 8; ++i) v[i] = x[static_cast<int64_t>(k0 + p[i / 4] + i % 4) * a.x_st[0]] * up;
+        for (int i = 0; i < 8; ++i) v[i] = x[static_cast<int64_t>(k0 + p[i / 4] + i % 4) * a.x_st[0]];
+    }
+}
+
+// ---- columns as digits ---------------------------------------------------------------
+
+// In LDS, eight bytes each: digit d of unit u's group t at [u][t][d][column][lane
+// row], its group sums behind all of those at [u][d][column], and the units'
+// scales as floats behind all at [u][column].
+template <int N>
+struct Digits {
+    static constexpr uint32_t kUnit = 8 * 4 * N * 4;
+    static __host__ __device__ uint32_t sums(uint32_t units) { return units * kUnit; }
+    static __host__ __device__ uint32_t scales(uint32_t units) { return units * (kUnit + 4 * N); }
+    static __host__ __device__ uint64_t bytes(uint64_t units) { return units * ((kUnit + 4 * N) * 8 + N * 4); }
+};
+
+// The four signed bytes d0 + 2^8 d1 + 2^16 d2 + 2^24 d3 of v, |v| < 2^30.
+__device__ __forceinline__ uint32_t digits_of(float v)
+{
+    return (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v))) + 0x00808080u) ^ 0x00808080u;
+}
+
+// Byte b of four words, as word b.
+__device__ __forceinline__ void bytes4(const uint32_t t[4], uint32_t out[4])
+{
+    const uint32_t a = __builtin_amdgcn_perm(t[1], t[0], 0x05010400u), b = __builtin_amdgcn_perm(t[3], t[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(t[1], t[0], 0x07030602u), d = __builtin_amdgcn_perm(t[3], t[2], 0x07030602u);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v)
+{
+    return __builtin_bit_cast(float, dpp32<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+
+template <bool Q4K, int N>
+__device__ __forceinline__ void lay_out_digits(const QMatArgs &a, uint32_t units, u2 *to)
+{
+    for (uint32_t c = 0; c < N; ++c) {
+        if (c >= a.n) break;
+        const float *x = a.x + static_cast<int64_t>(c) * a.x_st[1];
+        // a unit per half wave: group i / 4 % 8, lane row i % 4
+        for (uint32_t i = threadIdx.x; i < units * 32; i += kQmBlock) {
+            const uint32_t unit = i / 32, t = i / 4 % 8, g = i % 4;
+            float v[8], top = 0.0f, zero = 0.0f;
+            load_values<Q4K>(a, x, i / 4, g, v);
+            for (int e = 0; e < 8; ++e) {
+                top = __builtin_fmaxf(top, __builtin_fabsf(v[e]));
+                zero = __builtin_fmaf(v[e], 0.0f, zero); // NaN from an infinity or NaN
+            }
+            top = __builtin_fmaxf(top, dpp_f32<kDppXor1>(top));
+            top = __builtin_fmaxf(top, dpp_f32<kDppXor2>(top));
+            top = __builtin_fmaxf(top, dpp_f32<kDppHalfMirror>(top));
+            top = __builtin_fmaxf(top, dpp_f32<kDppMirror>(top));
+            top = __builtin_fmaxf(top, __shfl_xor(top, 16, kWave));
+            const uint64_t odd = __ballot(!(zero == 0.0f));
+            // the largest to [2^29, 2^30)
+            int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
+            e = e == 128 ? 0 : e < -97 ? -97 : e;
+            const float up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 29 - e) << 23);
+            if (i % 32 == 0) // an output that meets what is not finite is computed again
+                reinterpret_cast<float *>(to + Digits<N>::scales(units))[unit * N + c] =
+                    (odd >> (threadIdx.x % kWave)) & 0xffffffffu ? __builtin_nanf("") : __builtin_bit_cast(float, static_cast<uint32_t>(127 - 29 + e) << 23);
+            float sum = 0.0f;
+            uint32_t w[2][4], d[2][4];
+            for (int q = 0; q < 8; ++q) {
+                const float s = v[q] * up;
+                sum += s;
+                w[q / 4][q % 4] = digits_of(s);
+            }
+            bytes4(w[0], d[0]);
+            bytes4(w[1], d[1]);
+            for (uint32_t q = 0; q < 4; ++q) to[unit * Digits<N>::kUnit + ((t * 4 + q) * N + c) * 4 + g] = u2{d[0][q], d[1][q]};
+            if constexpr (Q4K) { // sums of 32 values, by 2^-5
+                sum += dpp_f32<kDppXor1>(sum);
+                sum += dpp_f32<kDppXor2>(sum);
+                const uint32_t s = digits_of(sum * 0.03125f);
+                // lane row g writes digit g
+                reinterpret_cast<unsigned char *>(to + Digits<N>::sums(units) + (unit * 4 + g) * N + c)[t] = static_cast<unsigned char>(s >> (8 * g));
+            }
+        }
+    }
+}
+
+// ---- columns as halves -----------------------------------------------------------------
+
+// In the workspace, 16 bytes of 8 halves each, 16 columns side by side: unit u's
+// group t at [u][t][part][column][lane row], and behind all units, at [u][column]
+// [part], the eight groups' sums (parts 2 and 3 are zeros).
+constexpr uint32_t kHalvesUnit = 8 * 2 * 16 * 4;
+constexpr uint32_t halves_at(uint32_t t, uint32_t part) { return (t * 2 + part) * 16 * 4; }
+constexpr uint64_t halves_pieces(uint64_t units) { return units * (kHalvesUnit + 16 * 4); }
+
+__device__ __forceinline__ uint32_t pack(_Float16 a, _Float16 b)
+{
+    return __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
+}
+
+// The power of two that brings the largest magnitude into [2^14, 2^15), and
+// its inverse; 1 for a column of zeros or with an infinity.
+__device__ __forceinline__ void column_scale(float top, float &up, float &down)
+{
+    int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
+    e = top == 0.0f || e == 128 ? 14 : e < -110 ? -110 : e;
+    up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 14 - e) << 23);
+    down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - 14 + e) << 23);
+}
+
+// Lays out a column's eight values of (group, g): x points at the column.
+template <bool Q4K>
+__device__ __forceinline__ void lay_out_halves(const QMatArgs &a, const float *x, float up, uint32_t group, uint32_t g, uint32_t units, uint32_t c, u4 *to)
+{
+    float v[8];
+    load_values<Q4K>(a, x, group, g, v);
+    for (int i = 0; i < 8; ++i) v[i] *= up;
+    if constexpr (Q4K) { // the group's sum over its four lanes, by 2^-6 within f16's range
+        float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        sum += dpp_f32<kDppXor1>(sum);
+        sum += dpp_f32<kDppXor2>(sum);
+        sum *= 0.015625f;
+        const _Float16 h = static_cast<_Float16>(sum);
+        _Float16 *sums = reinterpret_cast<_Float16 *>(to + units * kHalvesUnit + ((group / 8) * 16 + c) * 4 + g);
+        sums[group % 8] = g == 0 ? h : g == 1 ? static_cast<_Float16>(sum - static_cast<float>(h)) : static_cast<_Float16>(0.0f);
     }
     // Q4_0 halves: evens and odds of both fours; Q4_K: of each four
     constexpr int order[2][8] = {{0, 2, 4, 6, 1, 3, 5, 7}, {0, 2, 1, 3, 4, 6, 5, 7}};
@@ -110,43 +224,9 @@ __device__ __forceinline__ void lay_out(const QMatArgs &a, const XLayout<Q4K> &l
         hi[i] = pack(h0, h1);
         lo[i] = pack(static_cast<_Float16>(x0 - static_cast<float>(h0)), static_cast<_Float16>(x1 - static_cast<float>(h1)));
     }
-    to[lay.at(group, 0, c, g)] = hi;
-    to[lay.at(group, 1, c, g)] = lo;
-    if constexpr (Q4K) { // the group's sum over its four lanes, by 2^-6 within f16's range
-        float s = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-        s += __shfl_xor(s, 1, kWave);
-        s += __shfl_xor(s, 2, kWave);
-        s *= 0.015625f;
-        const _Float16 h = static_cast<_Float16>(s);
-        if (g < 2) {
-            _Float16 *sums = reinterpret_cast<_Float16 *>(to + lay.sum_at(group / 8, c, g));
-            sums[group % 8] = g == 0 ? h : static_cast<_Float16>(s - static_cast<float>(h));
-        }
-    }
-}
-
-// One column of a workgroup's threads: its scale, then its pieces.  All threads
-// call it; top needs a float per wave.
-template <bool Q4K, int THREADS>
-__device__ __forceinline__ float lay_out_column(const QMatArgs &a, const XLayout<Q4K> &lay, uint32_t col, uint32_t c, u4 *to, float *top)
-{
-    const float *x = a.x + static_cast<int64_t>(col) * a.x_st[1];
-    float m = 0.0f;
-    if (a.x_st[0] == 1)
-        for (uint32_t k = threadIdx.x * 4; k < a.k; k += THREADS * 4) {
-            const v4f v = *reinterpret_cast<const v4f_any *>(x + k);
-            for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(v[i]));
-        }
-    else
-        for (uint32_t k = threadIdx.x; k < a.k; k += THREADS) m = __builtin_fmaxf(m, __builtin_fabsf(x[static_cast<int64_t>(k) * a.x_st[0]]));
-    m = wave_max_dpp(m);
-    if (threadIdx.x % kWave == 0) top[threadIdx.x / kWave] = m;
-    __syncthreads();
-    for (int w = 0; w < THREADS / kWave; ++w) m = __builtin_fmaxf(m, top[w]);
-    float up, down;
-    column_scale(m, up, down);
-    for (uint32_t i = threadIdx.x; i < lay.groups() * 4; i += THREADS) lay_out<Q4K>(a, lay, x, up, i / 4, i % 4, c, to);
-    return down;
+    u4 *at = to + (group / 8) * kHalvesUnit + c * 4 + g;
+    at[halves_at(group % 8, 0)] = hi;
+    at[halves_at(group % 8, 1)] = lo;
 }
 
 __device__ __forceinline__ float half_value(uint32_t h) { return hw_fp16_to_f32(static_cast<uint16_t>(h)); }
@@ -179,36 +259,51 @@ __device__ __forceinline__ float walk_row(const unsigned char *row, const float 
     return wave_sum(sum);
 }
 
-// Packed bytes of one unit as lane (j, g) loads them.
+// Packed bytes of one unit as lane (j, g) loads them: two Q4_0 blocks (d in
+// word 0's low and word 4's high half, nibbles between and behind), or a Q4_K
+// block's head and its lane's 16 bytes of both halves.
 template <bool Q4K>
 struct Raw;
 template <>
 struct Raw<false> {
-    u4 q;
-    uint32_t d;
+    u4 a, b;
+    uint32_t c;
 };
 template <>
 struct Raw<true> {
     u4 head, q[2];
 };
 
-__device__ __forceinline__ u4 load16(const unsigned char *p) { return *reinterpret_cast<const u4_any *>(p); }
-
+// WORDS: rows start at multiples of four bytes and hold whole pairs of blocks.
+template <bool WORDS>
 __device__ __forceinline__ void load_unit(Raw<false> &r, const unsigned char *row, uint32_t unit, uint32_t g, uint32_t blocks)
 {
-    const uint32_t b = unit * 4 + g;
-    const unsigned char *p = row + static_cast<uint64_t>(b < blocks ? b : blocks - 1) * 18;
-    uint16_t d;
-    __builtin_memcpy(&d, p, 2);
-    r.d = b < blocks ? d : 0; // past the row: nothing times zeros
-    r.q = load16(p + 2);
+    const uint32_t b = unit * 8 + 2 * g;
+    if constexpr (WORDS) {
+        const unsigned char *p = row + static_cast<uint64_t>(b < blocks ? b : blocks - 2) * 18;
+        r.a = *reinterpret_cast<const u4_word *>(p);
+        r.b = *reinterpret_cast<const u4_word *>(p + 16);
+        r.c = *reinterpret_cast<const uint32_t *>(p + 32);
+    } else { // a block at a time, put together as above
+        const unsigned char *p = row + static_cast<uint64_t>(b < blocks ? b : blocks - 1) * 18;
+        const unsigned char *s = row + static_cast<uint64_t>(b + 1 < blocks ? b + 1 : blocks - 1) * 18;
+        uint16_t last, d;
+        __builtin_memcpy(&last, p + 16, 2);
+        __builtin_memcpy(&d, s, 2);
+        r.a = *reinterpret_cast<const u4_byte *>(p);
+        const u4 q = *reinterpret_cast<const u4_byte *>(s + 2);
+        r.b = u4{last | static_cast<uint32_t>(d) << 16, q[0], q[1], q[2]};
+        r.c = q[3];
+    }
 }
+template <bool WORDS>
 __device__ __forceinline__ void load_unit(Raw<true> &r, const unsigned char *row, uint32_t unit, uint32_t g, uint32_t)
 {
+    typedef std::conditional_t<WORDS, u4_word, u4_byte> piece;
     const unsigned char *p = row + static_cast<uint64_t>(unit) * 144;
-    r.head = load16(p);
-    r.q[0] = load16(p + 16 + 16 * g);
-    r.q[1] = load16(p + 80 + 16 * g);
+    r.head = *reinterpret_cast<const piece *>(p);
+    r.q[0] = *reinterpret_cast<const piece *>(p + 16 + 16 * g);
+    r.q[1] = *reinterpret_cast<const piece *>(p + 80 + 16 * g);
 }
 
 __device__ __forceinline__ void swap16(uint32_t &a, uint32_t &b)
@@ -223,95 +318,285 @@ __device__ __forceinline__ void swap32(uint32_t &a, uint32_t &b)
     a = r[0];
     b = r[1];
 }
+// Word t of lane row g to word g of lane row t.
+__device__ __forceinline__ void transpose(uint32_t w[4])
+{
+    swap32(w[0], w[2]);
+    swap32(w[1], w[3]);
+    swap16(w[0], w[1]);
+    swap16(w[2], w[3]);
+}
+
+// ---- a unit made ready: words and scales of its eight groups ----------------------------
+
+template <bool Q4K>
+struct Unit;
+
+template <>
+struct Unit<false> {
+    uint32_t w[2][4]; // even and odd blocks
+    uint32_t d[4];    // eight halves
+
+    __device__ __forceinline__ Unit(const Raw<false> &r, uint32_t unit, uint32_t g, uint32_t blocks)
+    {
+        const uint32_t x[9] = {r.a[0], r.a[1], r.a[2], r.a[3], r.b[0], r.b[1], r.b[2], r.b[3], r.c};
+        for (int i = 0; i < 4; ++i) {
+            w[0][i] = __builtin_amdgcn_alignbit(x[i + 1], x[i], 16);
+            w[1][i] = x[5 + i];
+        }
+        transpose(w[0]);
+        transpose(w[1]);
+        uint32_t p = (x[0] & 0xffffu) | (x[4] & 0xffff0000u);
+        if (__builtin_expect((unit + 1) * 8 > blocks, 0)) { // past the row: nothing times zeros
+            const uint32_t b = unit * 8 + 2 * g;
+            p = b + 1 < blocks ? p : b < blocks ? p & 0xffffu : 0u;
+        }
+        d[0] = d[2] = p; // every lane of the row: all scales
+        swap32(d[0], d[2]);
+        d[1] = d[0];
+        d[3] = d[2];
+        swap16(d[0], d[1]);
+        swap16(d[2], d[3]);
+    }
+    __device__ __forceinline__ float scale(int t) const { return half_value(t % 2 ? d[t / 2] >> 16 : d[t / 2] & 0xffffu); }
+    // 16 (q - 8) as signed bytes: values 0-3 and 4-7 of the lane
+    __device__ __forceinline__ u2 bytes(int t) const
+    {
+        const uint32_t u = w[t % 2][t / 2] ^ 0x88888888u;
+        return u2{(u << 4) & 0xF0F0F0F0u, u & 0xF0F0F0F0u};
+    }
+    __device__ __forceinline__ u4 halves(int t) const; // q - 8
+};
+
+template <>
+struct Unit<true> {
+    uint32_t w[2][4];
+    uint32_t sc[2], mn[2];
+    float d, dmin;
+
+    __device__ __forceinline__ Unit(const Raw<true> &r, uint32_t, uint32_t, uint32_t)
+    {
+        const uint32_t h0 = r.head[0], s0 = r.head[1], s1 = r.head[2], s2 = r.head[3];
+        sc[0] = s0 & 0x3f3f3f3fu;
+        sc[1] = (s2 & 0x0f0f0f0fu) | ((s0 >> 2) & 0x30303030u);
+        mn[0] = s1 & 0x3f3f3f3fu;
+        mn[1] = ((s2 >> 4) & 0x0f0f0f0fu) | ((s1 >> 2) & 0x30303030u);
+        d = half_value(h0 & 0xffffu);
+        dmin = half_value(h0 >> 16);
+        for (int h = 0; h < 2; ++h) {
+            for (int i = 0; i < 4; ++i) w[h][i] = r.q[h][i];
+            swap32(w[h][0], w[h][2]); // words 0, 1: quarter 2 h of the block, words 2, 3: quarter 2 h + 1
+            swap32(w[h][1], w[h][3]);
+        }
+    }
+    __device__ __forceinline__ float scale(int t) const { return static_cast<float>((sc[t / 4] >> (8 * (t % 4))) & 255u); }
+    __device__ __forceinline__ u2 bytes(int t) const // q
+    {
+        const uint32_t u = w[t / 4][t / 2 % 2 * 2], v = w[t / 4][t / 2 % 2 * 2 + 1], s = t % 2 * 4;
+        return u2{(u >> s) & 0x0F0F0F0Fu, (v >> s) & 0x0F0F0F0Fu};
+    }
+    __device__ __forceinline__ u4 halves(int t) const; // q
+    __device__ __forceinline__ u4 minima() const       // as halves
+    {
+        u4 m;
+        for (int i = 0; i < 4; ++i) { // two bytes into 1024's mantissa
+            const v2h v = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, mn[i / 2], i % 2 ? 0x07030702u : 0x07010700u));
+            m[i] = __builtin_bit_cast(uint32_t, v - v2h{static_cast<_Float16>(1024.0f), static_cast<_Float16>(1024.0f)});
+        }
+        return m;
+    }
+};
 
 // Two nibbles, in bits 0-3 (or 4-7) of a word's halves, as halves minus `off`.
 __device__ __forceinline__ uint32_t low_nibbles(uint32_t u, _Float16 off)
 {
     const v2h v = __builtin_bit_cast(v2h, (u & 0x000F000Fu) | 0x64006400u);
-    return __builtin_bit_cast(uint32_t, v - v2h{static_cast<_Float16>(1024.0f + off), static_cast<_Float16>(1024.0f + off)});
+    const _Float16 o = static_cast<_Float16>(1024.0f) + off;
+    return __builtin_bit_cast(uint32_t, v - v2h{o, o});
 }
 __device__ __forceinline__ uint32_t high_nibbles(uint32_t u, _Float16 off)
 {
     const v2h v = __builtin_bit_cast(v2h, (u & 0x00F000F0u) | 0x64006400u);
-    const v2h s = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
-    const v2h o = {static_cast<_Float16>(-64.0f - off), static_cast<_Float16>(-64.0f - off)};
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, s, o));
+    const _Float16 s = static_cast<_Float16>(0.0625f), o = static_cast<_Float16>(-64.0f) - off;
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, v2h{s, s}, v2h{o, o}));
+}
+__device__ __forceinline__ u4 Unit<false>::halves(int t) const
+{
+    const uint32_t u = w[t % 2][t / 2], v = u >> 8;
+    return u4{low_nibbles(u, 8.0f), high_nibbles(u, 8.0f), low_nibbles(v, 8.0f), high_nibbles(v, 8.0f)};
+}
+__device__ __forceinline__ u4 Unit<true>::halves(int t) const
+{
+    const uint32_t u = w[t / 4][t / 2 % 2 * 2], v = w[t / 4][t / 2 % 2 * 2 + 1];
+    return t % 2 ? u4{high_nibbles(u, 0.0f), high_nibbles(u >> 8, 0.0f), high_nibbles(v, 0.0f), high_nibbles(v >> 8, 0.0f)}
+                 : u4{low_nibbles(u, 0.0f), low_nibbles(u >> 8, 0.0f), low_nibbles(v, 0.0f), low_nibbles(v >> 8, 0.0f)};
 }
 
+__device__ __forceinline__ v4i mfma(u2 x, u2 w)
+{
+    return __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x), __builtin_bit_cast(long, w), v4i{0, 0, 0, 0}, 0, 0, 0);
+}
 __device__ __forceinline__ v4f mfma(u4 x, u4 w, v4f c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, w), c, 0, 0, 0);
 }
 
-// acc[r] (column 4 r + g of row j) += this unit's products.
-template <int NR>
-__device__ __forceinline__ void do_unit(Raw<false> r, const XLayout<false> &lay, const u4 *xs, uint32_t unit, uint32_t c, uint32_t g, float *acc)
+// acc[i] (digit g of column i, of row j) += a unit's products.
+template <bool Q4K, int N>
+__device__ __forceinline__ void digits_unit(const Raw<Q4K> &raw, const u2 *xs, const u2 *sums, const float *scales, uint32_t unit, uint32_t g, uint32_t blocks, float (&acc)[N])
 {
-    uint32_t w[4] = {r.q[0], r.q[1], r.q[2], r.q[3]}; // word t of block g ...
-    swap32(w[0], w[2]);
-    swap32(w[1], w[3]);
-    swap16(w[0], w[1]);
-    swap16(w[2], w[3]); // ... to word g of block t
-    uint32_t d[4];
-    d[0] = d[2] = __builtin_bit_cast(uint32_t, half_value(r.d));
-    swap32(d[0], d[2]);
-    d[1] = d[0];
-    d[3] = d[2];
-    swap16(d[0], d[1]);
-    swap16(d[2], d[3]); // every lane of the row: block t's scale
+    const Unit<Q4K> un(raw, unit, g, blocks);
+    float part[N];
+    for (int i = 0; i < N; ++i) part[i] = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const uint32_t u = w[t], v = u >> 8;
-        const u4 q = {low_nibbles(u, 8.0f), high_nibbles(u, 8.0f), low_nibbles(v, 8.0f), high_nibbles(v, 8.0f)};
-        const uint32_t group = unit * 4 + t;
-        const v4f s = mfma(xs[lay.at(group, 0, c, g)], q, mfma(xs[lay.at(group, 1, c, g)], q, v4f{0.0f, 0.0f, 0.0f, 0.0f}));
-        const float f = __builtin_bit_cast(float, d[t]);
-        for (int i = 0; i < NR; ++i) acc[i] = __builtin_fmaf(f, s[i], acc[i]);
+    for (int t = 0; t < 8; ++t) {
+        const v4i p = mfma(xs[t * 4 * N * 4], un.bytes(t));
+        const float f = un.scale(t);
+        for (int i = 0; i < N; ++i) part[i] = __builtin_fmaf(f, static_cast<float>(p[i]), part[i]);
     }
+    if constexpr (Q4K) {
+        const v4i p = mfma(*sums, g == 0 ? u2{un.mn[0], un.mn[1]} : u2{0u, 0u});
+        for (int i = 0; i < N; ++i) part[i] = __builtin_fmaf(un.d, part[i], (un.dmin * -32.0f) * static_cast<float>(p[i]));
+    }
+    for (int i = 0; i < N; ++i) acc[i] = __builtin_fmaf(scales[i], part[i], acc[i]);
 }
 
-template <int NR>
-__device__ __forceinline__ void do_unit(Raw<true> r, const XLayout<true> &lay, const u4 *xs, uint32_t unit, uint32_t c, uint32_t g, float *acc)
+// acc[r][i] (tile r, column 4 i + g of row j) += the products of a unit of RT
+// tiles.  xs: the unit's pieces of the lane's column, sums: its group sums.
+template <bool Q4K, int NR, int RT>
+__device__ __forceinline__ void halves_unit(const Raw<Q4K> raw[RT], const u4 *xs, const u4 *sums, uint32_t unit, uint32_t g, uint32_t blocks, float (&acc)[RT][NR])
 {
-    const uint32_t h0 = r.head[0], s0 = r.head[1], s1 = r.head[2], s2 = r.head[3];
-    const uint32_t sc[2] = {s0 & 0x3f3f3f3fu, (s2 & 0x0f0f0f0fu) | ((s0 >> 2) & 0x30303030u)};
-    const uint32_t mn[2] = {s1 & 0x3f3f3f3fu, ((s2 >> 4) & 0x0f0f0f0fu) | ((s1 >> 2) & 0x30303030u)};
-    const float d = half_value(h0 & 0xffffu), dmin = half_value(h0 >> 16) * -64.0f;
-    float t[NR];
-    for (int i = 0; i < NR; ++i) t[i] = 0.0f;
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto all = [&](auto... R) {
+        const Unit<Q4K> un[RT] = {Unit<Q4K>(raw[R()], unit, g, blocks)...};
+        float part[RT][NR];
+        for (int r = 0; r < RT; ++r)
+            for (int i = 0; i < NR; ++i) part[r][i] = Q4K ? 0.0f : acc[r][i];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t w[4] = {r.q[h][0], r.q[h][1], r.q[h][2], r.q[h][3]};
-        swap32(w[0], w[2]); // words 0, 1: quarter 2 h of the block, words 2, 3: quarter 2 h + 1
-        swap32(w[1], w[3]);
+        for (int t = 0; t < 8; ++t) {
+            const u4 hi = xs[halves_at(t, 0)], lo = xs[halves_at(t, 1)];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) { // sub-block 4 h + b
-            const uint32_t u = w[b / 2 * 2], v = w[b / 2 * 2 + 1];
-            const u4 q = b % 2 ? u4{high_nibbles(u, 0.0f), high_nibbles(u >> 8, 0.0f), high_nibbles(v, 0.0f), high_nibbles(v >> 8, 0.0f)}
-                               : u4{low_nibbles(u, 0.0f), low_nibbles(u >> 8, 0.0f), low_nibbles(v, 0.0f), low_nibbles(v >> 8, 0.0f)};
-            const uint32_t group = unit * 8 + 4 * h + b;
-            const v4f s = mfma(xs[lay.at(group, 0, c, g)], q, mfma(xs[lay.at(group, 1, c, g)], q, v4f{0.0f, 0.0f, 0.0f, 0.0f}));
-            const float f = static_cast<float>((sc[h] >> (8 * b)) & 255u);
-            for (int i = 0; i < NR; ++i) t[i] = __builtin_fmaf(f, s[i], t[i]);
+            for (int r = 0; r < RT; ++r) {
+                const u4 q = un[r].halves(t);
+                const v4f p = mfma(hi, q, mfma(lo, q, zero));
+                const float f = un[r].scale(t);
+                for (int i = 0; i < NR; ++i) part[r][i] = __builtin_fmaf(f, p[i], part[r][i]);
+            }
         }
-    }
-    // the minima: their products with the groups' sums, hi for lane row 0, lo for 1
-    const u4 sums = xs[lay.sum_at(unit, c, g & 1)], none = {0, 0, 0, 0};
-    u4 m;
-    for (int i = 0; i < 4; ++i) { // bytes 2 i and 2 i + 1 into 1024's mantissa
-        const v2h v = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, mn[i / 2], i % 2 ? 0x07030702u : 0x05010400u));
-        m[i] = __builtin_bit_cast(uint32_t, v - v2h{static_cast<_Float16>(1024.0f), static_cast<_Float16>(1024.0f)});
-    }
-    const v4f s = mfma(g < 2 ? sums : none, m, v4f{0.0f, 0.0f, 0.0f, 0.0f});
-    for (int i = 0; i < NR; ++i) acc[i] = __builtin_fmaf(d, t[i], __builtin_fmaf(dmin, s[i], acc[i]));
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            if constexpr (Q4K) {
+                const v4f p = mfma(*sums, un[r].minima(), zero);
+                for (int i = 0; i < NR; ++i) acc[r][i] = __builtin_fmaf(un[r].d, part[r][i], __builtin_fmaf(un[r].dmin * -64.0f, p[i], acc[r][i]));
+            } else {
+                for (int i = 0; i < NR; ++i) acc[r][i] = part[r][i];
+            }
+        }
+    };
+    if constexpr (RT == 1) all(std::integral_constant<int, 0>());
+    else all(std::integral_constant<int, 0>(), std::integral_constant<int, 1>());
 }
 
 struct QmPlan {
+    uint32_t units;    // of k
     uint32_t tiles;    // of 16 rows
     uint32_t kw;       // waves along k; the others take further tiles
     uint32_t groups;   // of 16 columns
-    uint64_t x_pieces; // workspace pieces of a group (0: columns are laid out in LDS)
+    bool words;        // load_unit's
+    uint64_t x_pieces; // workspace pieces of a group (0: columns are digits in LDS)
 };
+
+// A wave's share: units [u0, u1) of its rows.
+struct QmShare {
+    uint32_t kw, tw, wt, u0, u1, blocks;
+    uint64_t row_bytes;
+    __device__ __forceinline__ QmShare(const QMatArgs &a, const QmPlan &pl, uint32_t wave, bool q4k)
+    {
+        kw = pl.kw;
+        tw = kQmWaves / kw; // both powers of two
+        wt = wave / kw;
+        const uint32_t wk = wave % kw;
+        u0 = static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * wk / kw);
+        u1 = static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * (wk + 1) / kw);
+        blocks = a.k / 32;
+        row_bytes = q4k ? static_cast<uint64_t>(a.k / 256) * 144 : static_cast<uint64_t>(blocks) * 18;
+    }
+};
+
+// Up to N <= 4 columns, as digits.
+template <bool Q4K, int N, bool WORDS>
+__global__ __launch_bounds__(kQmBlock, 4) void k_qm_digits(QMatArgs a, QmPlan pl)
+{
+    constexpr int U = 2; // units in flight
+    extern __shared__ u2 laid[];
+    __shared__ float part[2][kQmWaves][N][kWave];
+    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), j = lane % 16, g = lane / 16;
+    const QmShare sh(a, pl, wave, Q4K);
+    const unsigned char *w = static_cast<const unsigned char *>(a.w);
+    auto row_of = [&](uint32_t tile) { // of this wave's tile; past the last one, rows that are read and dropped
+        const uint64_t at = (static_cast<uint64_t>(tile) + sh.wt) * 16 + j;
+        return w + (at < a.m ? at : a.m - 1) * sh.row_bytes;
+    };
+    // the first weights are on their way while the columns are laid out
+    const uint32_t step = gridDim.x * sh.tw;
+    uint32_t tile = blockIdx.x * sh.tw;
+    const unsigned char *row = row_of(tile);
+    Raw<Q4K> raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if (sh.u0 + i < sh.u1) load_unit<WORDS>(raw[i], row, sh.u0 + i, g, sh.blocks);
+    lay_out_digits<Q4K, N>(a, pl.units, laid);
+    __syncthreads();
+    // slot j of the instruction's 16 columns is digit j / 4 of column j % 4 (the
+    // ones past n repeat the last), so that result i of lane row g is digit g of column i
+    const uint32_t c = j % 4 < a.n ? j % 4 : a.n - 1;
+    const u2 *xs = laid + (j / 4 * N + c) * 4 + g, *sums = laid + Digits<N>::sums(pl.units) + j / 4 * N + c;
+    const float *scales = reinterpret_cast<const float *>(laid + Digits<N>::scales(pl.units));
+    const float digit = __builtin_bit_cast(float, (127u + 8 * g) << 23) * (Q4K ? 1.0f : 0.0625f);
+    uint32_t turn = 0;
+    for (; tile < pl.tiles; tile += step, turn ^= 1) {
+        float acc[N];
+        for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+        const unsigned char *next = row_of(tile + step);
+        for (uint32_t u = sh.u0; u < sh.u1; u += U) {
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (u + i < sh.u1)
+                    digits_unit<Q4K, N>(raw[i], xs + (u + i) * Digits<N>::kUnit, sums + (u + i) * 4 * N, scales + (u + i) * N, u + i, g, sh.blocks, acc);
+                // the slot's next unit: of this tile, or of the next one
+                const bool more = u + i + U < sh.u1;
+                if (more || (u + U >= sh.u1 && sh.u0 + i < sh.u1))
+                    load_unit<WORDS>(raw[i], more ? row : next, more ? u + i + U : sh.u0 + i, g, sh.blocks);
+            }
+        }
+        row = next;
+        for (int i = 0; i < N; ++i) part[turn][wave][i][lane] = acc[i] * digit;
+        __syncthreads();
+        for (uint32_t e = wave; e < sh.tw * N; e += kQmWaves) { // a wave per tile and column
+            const uint32_t t = e / N, i = e % N;
+            if (i >= a.n) continue;
+            float v = 0.0f;
+            for (uint32_t k = 0; k < sh.kw; ++k) v += part[turn][t * sh.kw + k][i][lane];
+            // the digits' sum, the small ones first: lane rows 0 + 1, 2 + 3, then both
+            uint32_t p0 = __builtin_bit_cast(uint32_t, v), p1 = p0;
+            swap16(p0, p1);
+            v = __builtin_bit_cast(float, p0) + __builtin_bit_cast(float, p1);
+            p0 = p1 = __builtin_bit_cast(uint32_t, v);
+            swap32(p0, p1);
+            v = __builtin_bit_cast(float, p0) + __builtin_bit_cast(float, p1);
+            const uint64_t r = (static_cast<uint64_t>(tile) + t) * 16 + j;
+            const bool live = r < a.m && g == 0;
+            uint64_t odd = __ballot(live && !(__builtin_fabsf(v) < __builtin_inff()));
+            while (__builtin_expect(odd != 0, 0)) {
+                const int l = __builtin_ctzll(odd);
+                odd &= odd - 1;
+                const float f = walk_row<Q4K>(w + (r - j + l) * sh.row_bytes, a.x + static_cast<int64_t>(i) * a.x_st[1], a.x_st[0], a.k);
+                if (lane == static_cast<uint32_t>(l)) v = f;
+            }
+            if (live) a.y[static_cast<int64_t>(r) * a.y_st[0] + static_cast<int64_t>(i) * a.y_st[1]] = v;
+        }
+    }
+}
 
 // Lays out a column a workgroup in the workspace, and leaves its scale behind the pieces.
 template <bool Q4K>
@@ -319,82 +604,85 @@ __global__ __launch_bounds__(kQmBlock) void k_qm_columns(QMatArgs a, QmPlan pl)
 {
     __shared__ float top[kQmWaves];
     for (uint32_t col = blockIdx.x; col < a.n; col += gridDim.x) {
-        const uint32_t group = col / 16, n = a.n - group * 16 < 16 ? a.n - group * 16 : 16;
-        const XLayout<Q4K> lay{(a.k + kUnit<Q4K> - 1) / kUnit<Q4K>, n};
-        u4 *to = static_cast<u4 *>(a.workspace) + group * pl.x_pieces;
+        const float *x = a.x + static_cast<int64_t>(col) * a.x_st[1];
+        float m = 0.0f;
+        if (a.x_st[0] == 1)
+            for (uint32_t k = threadIdx.x * 4; k < a.k; k += kQmBlock * 4) {
+                const v4f v = *reinterpret_cast<const v4f_any *>(x + k);
+                for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(v[i]));
+            }
+        else
+            for (uint32_t k = threadIdx.x; k < a.k; k += kQmBlock) m = __builtin_fmaxf(m, __builtin_fabsf(x[static_cast<int64_t>(k) * a.x_st[0]]));
+        m = wave_max_dpp(m);
         __syncthreads(); // top of the column before
-        const float down = lay_out_column<Q4K, kQmBlock>(a, lay, col, col % 16, to, top);
+        if (threadIdx.x % kWave == 0) top[threadIdx.x / kWave] = m;
+        __syncthreads();
+        for (int w = 0; w < kQmWaves; ++w) m = __builtin_fmaxf(m, top[w]);
+        float up, down;
+        column_scale(m, up, down);
+        u4 *to = static_cast<u4 *>(a.workspace) + (col / 16) * pl.x_pieces;
+        for (uint32_t i = threadIdx.x; i < pl.units * 32; i += kQmBlock) lay_out_halves<Q4K>(a, x, up, i / 4, i % 4, pl.units, col % 16, to);
         if (threadIdx.x == 0) reinterpret_cast<float *>(static_cast<u4 *>(a.workspace) + pl.groups * pl.x_pieces)[col] = down;
     }
 }
 
-// NR: a quarter of the columns, rounded up.  LDS: columns laid out here, else read from the workspace.
-template <bool Q4K, int NR, bool LDS>
-__global__ __launch_bounds__(kQmBlock, 2) void k_qm(QMatArgs a, QmPlan pl)
+// Up to 16 columns a workgroup, as halves.  NR: a quarter of them, rounded up,
+// RT: tiles a wave takes at once, for one read of x.
+template <bool Q4K, int NR, int RT, bool WORDS>
+__global__ __launch_bounds__(kQmBlock, 4) void k_qm_halves(QMatArgs a, QmPlan pl)
 {
-    constexpr int U = Q4K ? 2 : 4; // units in flight
-    extern __shared__ u4 laid[];
-    __shared__ float top[kQmWaves], downs[16];
-    __shared__ float part[2][kQmWaves][NR][kWave];
+    constexpr int U = RT == 1 ? 2 : 1; // units in flight of each tile
+    __shared__ float part[2][kQmWaves][RT * NR][kWave];
     const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), j = lane % 16, g = lane / 16;
     const uint32_t c0 = blockIdx.y * 16, n = a.n - c0 < 16 ? a.n - c0 : 16;
-    const XLayout<Q4K> lay{(a.k + kUnit<Q4K> - 1) / kUnit<Q4K>, n};
-    const uint32_t kw = pl.kw, tw = kQmWaves / kw, wk = wave % kw, wt = wave / kw;
-    const uint32_t u0 = static_cast<uint32_t>(static_cast<uint64_t>(lay.units) * wk / kw);
-    const uint32_t u1 = static_cast<uint32_t>(static_cast<uint64_t>(lay.units) * (wk + 1) / kw);
-    const uint32_t blocks = a.k / 32;
-    const uint64_t row_bytes = Q4K ? static_cast<uint64_t>(a.k / 256) * 144 : static_cast<uint64_t>(blocks) * 18;
+    const QmShare sh(a, pl, wave, Q4K);
     const unsigned char *w = static_cast<const unsigned char *>(a.w);
-    auto row_of = [&](uint32_t tile) { // of this wave's tile; past the last one, rows that are read and dropped
-        const uint64_t r = (static_cast<uint64_t>(tile) + wt) * 16 + j;
-        return w + (r < a.m ? r : a.m - 1) * row_bytes;
+    auto row_of = [&](uint32_t tile, int r) {
+        const uint64_t at = (static_cast<uint64_t>(tile) + sh.wt * RT + r) * 16 + j;
+        return w + (at < a.m ? at : a.m - 1) * sh.row_bytes;
     };
-    // the first weights are on their way while the columns are laid out
-    uint32_t tile = blockIdx.x * tw;
-    const unsigned char *row = row_of(tile);
-    Raw<Q4K> raw[U];
+    const uint32_t step = gridDim.x * sh.tw * RT;
+    uint32_t tile = blockIdx.x * sh.tw * RT;
+    const unsigned char *row[RT];
+    for (int r = 0; r < RT; ++r) row[r] = row_of(tile, r);
+    Raw<Q4K> raw[U][RT];
 #pragma unroll
     for (int i = 0; i < U; ++i)
-        if (u0 + i < u1) load_unit(raw[i], row, u0 + i, g, blocks);
-    const u4 *xs;
-    if constexpr (LDS) {
-        for (uint32_t c = 0; c < n; ++c) {
-            if (c) __syncthreads();
-            const float down = lay_out_column<Q4K, kQmBlock>(a, lay, c0 + c, c, laid, top);
-            if (tid == 0) downs[c] = down;
-        }
-        xs = laid;
-    } else {
-        xs = static_cast<const u4 *>(a.workspace) + blockIdx.y * pl.x_pieces;
-        const float *d = reinterpret_cast<const float *>(static_cast<const u4 *>(a.workspace) + pl.groups * pl.x_pieces) + c0;
-        if (tid < n) downs[tid] = d[tid];
-    }
-    __syncthreads();
+        if (sh.u0 + i < sh.u1)
+            for (int r = 0; r < RT; ++r) load_unit<WORDS>(raw[i][r], row[r], sh.u0 + i, g, sh.blocks);
     // slot j of the instruction's 16 columns is column 4 (j % 4) + j / 4, so
     // that result i of lane row g is column 4 i + g; the slots past n repeat
     uint32_t c = (j % 4) * 4 + j / 4;
     c = c < n ? c : n - 1;
+    const u4 *xs = static_cast<const u4 *>(a.workspace) + blockIdx.y * pl.x_pieces + c * 4 + g;
+    const u4 *sums = xs + static_cast<uint64_t>(pl.units) * kHalvesUnit;
+    const float *downs = reinterpret_cast<const float *>(static_cast<const u4 *>(a.workspace) + pl.groups * pl.x_pieces) + c0;
     uint32_t turn = 0;
-    for (; tile < pl.tiles; tile += gridDim.x * tw, turn ^= 1) {
-        float acc[NR];
-        for (int i = 0; i < NR; ++i) acc[i] = 0.0f;
-        const unsigned char *next = row_of(tile + gridDim.x * tw);
-        for (uint32_t u = u0; u < u1; u += U) {
+    for (; tile < pl.tiles; tile += step, turn ^= 1) {
+        float acc[RT][NR];
+        for (int r = 0; r < RT; ++r)
+            for (int i = 0; i < NR; ++i) acc[r][i] = 0.0f;
+        const unsigned char *next[RT];
+        for (int r = 0; r < RT; ++r) next[r] = row_of(tile + step, r);
+        for (uint32_t u = sh.u0; u < sh.u1; u += U) {
 #pragma unroll
             for (int i = 0; i < U; ++i) {
-                if (u + i < u1) do_unit<NR>(raw[i], lay, xs, u + i, c, g, acc);
-                // the slot's next unit: of this tile, or of the next one
-                if (u + i + U < u1) load_unit(raw[i], row, u + i + U, g, blocks);
-                else if (u + U >= u1 && u0 + i < u1) load_unit(raw[i], next, u0 + i, g, blocks);
+                if (u + i < sh.u1)
+                    halves_unit<Q4K, NR, RT>(raw[i], xs + (u + i) * kHalvesUnit, sums + (u + i) * (16 * 4), u + i, g, sh.blocks, acc);
+                const bool more = u + i + U < sh.u1;
+                if (more || (u + U >= sh.u1 && sh.u0 + i < sh.u1))
+                    for (int r = 0; r < RT; ++r) load_unit<WORDS>(raw[i][r], more ? row[r] : next[r], more ? u + i + U : sh.u0 + i, g, sh.blocks);
             }
         }
-        row = next;
-        for (int i = 0; i < NR; ++i) part[turn][wave][i][lane] = acc[i];
+        for (int r = 0; r < RT; ++r) {
+            row[r] = next[r];
+            for (int i = 0; i < NR; ++i) part[turn][wave][r * NR + i][lane] = acc[r][i];
+        }
         __syncthreads();
-        for (uint32_t e = wave; e < tw * NR; e += kQmWaves) { // a wave per tile and quarter of columns
+        for (uint32_t e = wave; e < sh.tw * RT * NR; e += kQmWaves) { // a wave per tile and quarter of columns
             const uint32_t t = e / NR, i = e % NR, col = 4 * i + g;
             float v = 0.0f;
-            for (uint32_t s = 0; s < kw; ++s) v += part[turn][t * kw + s][i][lane];
+            for (uint32_t k = 0; k < sh.kw; ++k) v += part[turn][t / RT * sh.kw + k][t % RT * NR + i][lane];
             const uint64_t r = (static_cast<uint64_t>(tile) + t) * 16 + j;
             const bool live = r < a.m && col < n;
             v *= live ? downs[col] : 0.0f;
@@ -403,7 +691,7 @@ __global__ __launch_bounds__(kQmBlock, 2) void k_qm(QMatArgs a, QmPlan pl)
                 const int l = __builtin_ctzll(odd);
                 odd &= odd - 1;
                 const uint64_t rr = (static_cast<uint64_t>(tile) + t) * 16 + l % 16;
-                const float f = walk_row<Q4K>(w + rr * row_bytes, a.x + static_cast<int64_t>(c0 + 4 * i + l / 16) * a.x_st[1], a.x_st[0], a.k);
+                const float f = walk_row<Q4K>(w + rr * sh.row_bytes, a.x + static_cast<int64_t>(c0 + 4 * i + l / 16) * a.x_st[1], a.x_st[0], a.k);
                 if (lane == static_cast<uint32_t>(l)) v = f;
             }
             if (live) a.y[static_cast<int64_t>(r) * a.y_st[0] + static_cast<int64_t>(c0 + col) * a.y_st[1]] = v;
@@ -411,21 +699,7 @@ __global__ __launch_bounds__(kQmBlock, 2) void k_qm(QMatArgs a, QmPlan pl)
     }
 }
 
-template <bool Q4K>
-QmPlan qm_plan(const QMatArgs &a)
-{
-    QmPlan pl;
-    const uint32_t units = (a.k + kUnit<Q4K> - 1) / kUnit<Q4K>;
-    pl.tiles = static_cast<uint32_t>((static_cast<uint64_t>(a.m) + 15) / 16);
-    pl.kw = units >= 16 ? 8 : units >= 8 ? 4 : units >= 4 ? 2 : 1;
-    pl.groups = (a.n + 15) / 16;
-    const XLayout<Q4K> lay{units, a.n < 16 ? a.n : 16};
-    pl.x_pieces = pl.groups == 1 && lay.pieces() * 16 <= kQmLds ? 0 : lay.pieces();
-    return pl;
-}
-
-template <bool Q4K, int NR>
-void qm_launch(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
+uint32_t qm_cus()
 {
     static const uint32_t cus = [] {
         int dev = 0, n = 0;
@@ -433,41 +707,90 @@ void qm_launch(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
             n = 256;
         return static_cast<uint32_t>(n);
     }();
-    const uint32_t tw = kQmWaves / pl.kw, wgs = (pl.tiles + tw - 1) / tw;
-    const dim3 grid(wgs < 2 * cus ? wgs : 2 * cus, pl.groups);
-    if (pl.x_pieces) {
-        k_qm_columns<Q4K><<<a.n < 65536 ? a.n : 65536, kQmBlock, 0, stream>>>(a, pl);
-        k_qm<Q4K, NR, false><<<grid, kQmBlock, 0, stream>>>(a, pl);
-    } else {
-        const XLayout<Q4K> lay{(a.k + kUnit<Q4K> - 1) / kUnit<Q4K>, a.n};
-        k_qm<Q4K, NR, true><<<grid, kQmBlock, static_cast<uint32_t>(lay.pieces() * 16), stream>>>(a, pl);
+    return cus;
+}
+
+// Columns that are laid out as digits: up to four where they fit; 0: as halves.
+int qm_digits(const QMatArgs &a, uint32_t units)
+{
+    const uint64_t bytes[] = {Digits<1>::bytes(units), Digits<2>::bytes(units), Digits<3>::bytes(units), Digits<4>::bytes(units)};
+    return a.n <= 4 && bytes[a.n - 1] <= kQmLds ? static_cast<int>(a.n) : 0;
+}
+
+QmPlan qm_plan(const QMatArgs &a)
+{
+    QmPlan pl;
+    pl.units = (a.k + kQmUnit - 1) / kQmUnit;
+    pl.tiles = static_cast<uint32_t>((static_cast<uint64_t>(a.m) + 15) / 16);
+    pl.kw = pl.units >= 8 ? 8 : pl.units >= 4 ? 4 : pl.units >= 2 ? 2 : 1;
+    pl.groups = (a.n + 15) / 16;
+    pl.words = reinterpret_cast<uintptr_t>(a.w) % 4 == 0 && a.k % 64 == 0;
+    pl.x_pieces = qm_digits(a, pl.units) ? 0 : halves_pieces(pl.units);
+    return pl;
+}
+
+// Workgroups for tiles taken `per` at a time: even shares of what runs at once.
+uint32_t qm_grid(const QmPlan &pl, uint32_t per)
+{
+    const uint32_t wgs = (pl.tiles + per - 1) / per, most = 2 * qm_cus(), rounds = (wgs + most - 1) / most;
+    return (wgs + rounds - 1) / rounds;
+}
+
+template <bool Q4K, int N>
+void qm_run_digits(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
+{
+    const uint32_t grid = qm_grid(pl, kQmWaves / pl.kw), lds = static_cast<uint32_t>(Digits<N>::bytes(pl.units));
+    if (pl.words) k_qm_digits<Q4K, N, true><<<grid, kQmBlock, lds, stream>>>(a, pl);
+    else k_qm_digits<Q4K, N, false><<<grid, kQmBlock, lds, stream>>>(a, pl);
+}
+
+template <bool Q4K, int NR, int RT>
+void qm_run_halves(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
+{
+    const dim3 grid(qm_grid(pl, kQmWaves / pl.kw * RT), pl.groups);
+    k_qm_columns<Q4K><<<a.n < 65536 ? a.n : 65536, kQmBlock, 0, stream>>>(a, pl);
+    if (pl.words) k_qm_halves<Q4K, NR, RT, true><<<grid, kQmBlock, 0, stream>>>(a, pl);
+    else k_qm_halves<Q4K, NR, RT, false><<<grid, kQmBlock, 0, stream>>>(a, pl);
+}
+
+template <bool Q4K, int RT>
+void qm_run_halves(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
+{
+    switch ((a.n + 3) / 4) {
+    case 1: return qm_run_halves<Q4K, 1, RT>(a, pl, stream);
+    case 2: return qm_run_halves<Q4K, 2, RT>(a, pl, stream);
+    case 3: return qm_run_halves<Q4K, 3, RT>(a, pl, stream);
+    default: return qm_run_halves<Q4K, 4, RT>(a, pl, stream);
     }
 }
 
 template <bool Q4K>
-hipError_t qm_run(const QMatArgs &a, hipStream_t stream)
+void qm_run(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 {
-    const QmPlan pl = qm_plan<Q4K>(a);
-    switch ((a.n + 3) / 4) {
-    case 1: qm_launch<Q4K, 1>(a, pl, stream); break;
-    case 2: qm_launch<Q4K, 2>(a, pl, stream); break;
-    case 3: qm_launch<Q4K, 3>(a, pl, stream); break;
-    default: qm_launch<Q4K, 4>(a, pl, stream); break;
+    switch (qm_digits(a, pl.units)) {
+    case 1: return qm_run_digits<Q4K, 1>(a, pl, stream);
+    case 2: return qm_run_digits<Q4K, 2>(a, pl, stream);
+    case 3: return qm_run_digits<Q4K, 3>(a, pl, stream);
+    case 4: return qm_run_digits<Q4K, 4>(a, pl, stream);
     }
-    return hipGetLastError();
+    if (pl.tiles >= 4 * qm_cus()) qm_run_halves<Q4K, 2>(a, pl, stream); // two tiles a wave leave enough workgroups
+    else qm_run_halves<Q4K, 1>(a, pl, stream);
 }
 
 } // namespace
 
 uint64_t quant_mat_workspace_bytes(const QMatArgs &a)
 {
-    const QmPlan pl = a.q4k ? qm_plan<true>(a) : qm_plan<false>(a);
+    const QmPlan pl = qm_plan(a);
     return pl.x_pieces ? pl.groups * pl.x_pieces * 16 + static_cast<uint64_t>(a.n) * 4 : 0;
 }
 
 hipError_t launch_quant_mat(const QMatArgs &a, hipStream_t stream)
 {
-    return a.q4k ? qm_run<true>(a, stream) : qm_run<false>(a, stream);
+    const QmPlan pl = qm_plan(a);
+    if (a.q4k) qm_run<true>(a, pl, stream);
+    else qm_run<false>(a, pl, stream);
+    return hipGetLastError();
 }
 
 } // namespace emel
