@@ -19,10 +19,14 @@
 // a column.  A value is off by 2^-30 of the largest of its 256 at most: less
 // than f32's own rounding of the sum that the largest is part of.
 //
-// k_qm_halves, more columns.  A column goes in as two halves, hi + lo, scaled
-// by a power of two that brings its largest value to [2^14, 2^15): 22 bits of
-// every value down to 2^-16 of that, and 2^-40 of it below.  The 16 columns
-// of the f16 instruction are 16 columns, two instructions a group.  A nibble
+// k_qm_halves, more columns.  Each column's run of 256 values goes in as two
+// halves each, hi + lo, scaled by a power of two that brings its largest value to
+// [2^14, 2^15): 22 bits of every value down to 2^-16 of that, and 2^-40 of it
+// below.  The 16 columns of the f16 instruction are 16 columns, two
+// instructions a group.  k_qm_columns lays x out in the workspace, 4 bytes a
+// value; a workgroup stages half units of it in LDS, the next one on its way
+// in registers (read straight from the L2 the waves waited for it: 15 columns
+// of 4096x11008 38 us).  A nibble
 // becomes a half by and-or into 1024's mantissa and a packed subtraction (as a
 // subnormal half it would need neither, but the instruction drops as many
 // low bits of its sum as such a factor has leading zeros: 1e-5 off).
@@ -90,6 +94,37 @@ __device__ __forceinline__ void load_values(const QMatArgs &a, const float *x, u
     }
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v)
+{
+    return __builtin_bit_cast(float, dpp32<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+
+// Scales the eight values of each lane of a half wave, 256 in all, by the power
+// of two that brings the largest to [2^TOP, 2^(TOP + 1)); returns its inverse,
+// or NaN where a value is not finite (an output that meets it is computed again).
+template <int TOP>
+__device__ __forceinline__ float scale_unit(float v[8])
+{
+    float top = 0.0f, zero = 0.0f;
+    for (int e = 0; e < 8; ++e) {
+        top = __builtin_fmaxf(top, __builtin_fabsf(v[e]));
+        zero = __builtin_fmaf(v[e], 0.0f, zero); // NaN from an infinity or NaN
+    }
+    top = __builtin_fmaxf(top, dpp_f32<kDppXor1>(top));
+    top = __builtin_fmaxf(top, dpp_f32<kDppXor2>(top));
+    top = __builtin_fmaxf(top, dpp_f32<kDppHalfMirror>(top));
+    top = __builtin_fmaxf(top, dpp_f32<kDppMirror>(top));
+    top = __builtin_fmaxf(top, __shfl_xor(top, 16, kWave));
+    const uint64_t odd = __ballot(!(zero == 0.0f)) >> (threadIdx.x & 32);
+    constexpr int least = TOP - 126; // the power stays a normal number
+    int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
+    e = e == 128 ? 0 : e < least ? least : e;
+    const float up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + TOP - e) << 23);
+    for (int i = 0; i < 8; ++i) v[i] *= up;
+    return static_cast<uint32_t>(odd) ? __builtin_nanf("") : __builtin_bit_cast(float, static_cast<uint32_t>(127 - TOP + e) << 23);
+}
+
 // ---- columns as digits ---------------------------------------------------------------
 
 // In LDS, eight bytes each: digit d of unit u's group t at [u][t][d][column][lane
@@ -120,51 +155,33 @@ __device__ __forceinline__ void bytes4(const uint32_t t[4], uint32_t out[4])
     out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_f32(float v)
-{
-    return __builtin_bit_cast(float, dpp32<CTRL>(__builtin_bit_cast(uint32_t, v)));
-}
-
 template <bool Q4K, int N>
 __device__ __forceinline__ void lay_out_digits(const QMatArgs &a, uint32_t units, u2 *to)
 {
-    for (uint32_t c = 0; c < N; ++c) {
-        if (c >= a.n) break;
-        const float *x = a.x + static_cast<int64_t>(c) * a.x_st[1];
-        // a unit per half wave: group i / 4 % 8, lane row i % 4
-        for (uint32_t i = threadIdx.x; i < units * 32; i += kQmBlock) {
-            const uint32_t unit = i / 32, t = i / 4 % 8, g = i % 4;
-            float v[8], top = 0.0f, zero = 0.0f;
-            load_values<Q4K>(a, x, i / 4, g, v);
-            for (int e = 0; e < 8; ++e) {
-                top = __builtin_fmaxf(top, __builtin_fabsf(v[e]));
-                zero = __builtin_fmaf(v[e], 0.0f, zero); // NaN from an infinity or NaN
-            }
-            top = __builtin_fmaxf(top, dpp_f32<kDppXor1>(top));
-            top = __builtin_fmaxf(top, dpp_f32<kDppXor2>(top));
-            top = __builtin_fmaxf(top, dpp_f32<kDppHalfMirror>(top));
-            top = __builtin_fmaxf(top, dpp_f32<kDppMirror>(top));
-            top = __builtin_fmaxf(top, __shfl_xor(top, 16, kWave));
-            const uint64_t odd = __ballot(!(zero == 0.0f));
-            // the largest to [2^29, 2^30)
-            int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
-            e = e == 128 ? 0 : e < -97 ? -97 : e;
-            const float up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 29 - e) << 23);
-            if (i % 32 == 0) // an output that meets what is not finite is computed again
-                reinterpret_cast<float *>(to + Digits<N>::scales(units))[unit * N + c] =
-                    (odd >> (threadIdx.x % kWave)) & 0xffffffffu ? __builtin_nanf("") : __builtin_bit_cast(float, static_cast<uint32_t>(127 - 29 + e) << 23);
-            float sum = 0.0f;
+    // A unit of a column per half wave: group i / 4 % 8, lane row i % 4.  Four
+    // of them at a time, so that their loads overlap.
+    const uint32_t run = units * 32, all = run * a.n;
+    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 4 * kQmBlock) {
+        float v[4][8];
+#pragma unroll
+        for (uint32_t b = 0; b < 4; ++b) {
+            const uint32_t i = i0 + b * kQmBlock, c = N == 1 ? 0 : i / run, k = i - c * run;
+            if (i < all) load_values<Q4K>(a, a.x + static_cast<int64_t>(c) * a.x_st[1], k / 4, k % 4, v[b]);
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < 4; ++b) {
+            const uint32_t i = i0 + b * kQmBlock, c = N == 1 ? 0 : i / run, k = i - c * run;
+            if (i >= all) break;
+            const uint32_t unit = k / 32, t = k / 4 % 8, g = k % 4;
+            const float down = scale_unit<29>(v[b]);
+            if (k % 32 == 0) reinterpret_cast<float *>(to + Digits<N>::scales(units))[unit * N + c] = down;
             uint32_t w[2][4], d[2][4];
-            for (int q = 0; q < 8; ++q) {
-                const float s = v[q] * up;
-                sum += s;
-                w[q / 4][q % 4] = digits_of(s);
-            }
+            for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = digits_of(v[b][q]);
             bytes4(w[0], d[0]);
             bytes4(w[1], d[1]);
             for (uint32_t q = 0; q < 4; ++q) to[unit * Digits<N>::kUnit + ((t * 4 + q) * N + c) * 4 + g] = u2{d[0][q], d[1][q]};
             if constexpr (Q4K) { // sums of 32 values, by 2^-5
+                float sum = ((v[b][0] + v[b][1]) + (v[b][2] + v[b][3])) + ((v[b][4] + v[b][5]) + (v[b][6] + v[b][7]));
                 sum += dpp_f32<kDppXor1>(sum);
                 sum += dpp_f32<kDppXor2>(sum);
                 const uint32_t s = digits_of(sum * 0.03125f);
@@ -179,54 +196,48 @@ __device__ __forceinline__ void lay_out_digits(const QMatArgs &a, uint32_t units
 
 // In the workspace, 16 bytes of 8 halves each, 16 columns side by side: unit u's
 // group t at [u][t][part][column][lane row], and behind all units, at [u][column]
-// [part], the eight groups' sums (parts 2 and 3 are zeros).
+// [part], the eight groups' sums (parts 2 and 3 are zeros), and behind those
+// the units' scales, column 4 i + g at [u][g][i].
 constexpr uint32_t kHalvesUnit = 8 * 2 * 16 * 4;
 constexpr uint32_t halves_at(uint32_t t, uint32_t part) { return (t * 2 + part) * 16 * 4; }
-constexpr uint64_t halves_pieces(uint64_t units) { return units * (kHalvesUnit + 16 * 4); }
+constexpr uint64_t halves_pieces(uint64_t units) { return units * (kHalvesUnit + 16 * 4 + 4); }
 
 __device__ __forceinline__ uint32_t pack(_Float16 a, _Float16 b)
 {
     return __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
 }
 
-// The power of two that brings the largest magnitude into [2^14, 2^15), and
-// its inverse; 1 for a column of zeros or with an infinity.
-__device__ __forceinline__ void column_scale(float top, float &up, float &down)
-{
-    int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
-    e = top == 0.0f || e == 128 ? 14 : e < -110 ? -110 : e;
-    up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 14 - e) << 23);
-    down = __builtin_bit_cast(float, static_cast<uint32_t>(127 - 14 + e) << 23);
-}
-
-// Lays out a column's eight values of (group, g): x points at the column.
+// Column c of its group: a half wave's unit, lane i % 32 its (group, lane row).
 template <bool Q4K>
-__device__ __forceinline__ void lay_out_halves(const QMatArgs &a, const float *x, float up, uint32_t group, uint32_t g, uint32_t units, uint32_t c, u4 *to)
+__device__ __forceinline__ void lay_out_halves(const QMatArgs &a, const float *x, uint32_t units, uint32_t unit, uint32_t i, uint32_t c, u4 *to)
 {
+    const uint32_t t = i / 4, g = i % 4;
     float v[8];
-    load_values<Q4K>(a, x, group, g, v);
-    for (int i = 0; i < 8; ++i) v[i] *= up;
+    load_values<Q4K>(a, x, unit * 8 + t, g, v);
+    const float down = scale_unit<14>(v);
+    u4 *sums = to + static_cast<uint64_t>(units) * kHalvesUnit;
+    if (i == 0) reinterpret_cast<float *>(sums + units * (16 * 4))[unit * 16 + c % 4 * 4 + c / 4] = down;
     if constexpr (Q4K) { // the group's sum over its four lanes, by 2^-6 within f16's range
         float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         sum += dpp_f32<kDppXor1>(sum);
         sum += dpp_f32<kDppXor2>(sum);
         sum *= 0.015625f;
         const _Float16 h = static_cast<_Float16>(sum);
-        _Float16 *sums = reinterpret_cast<_Float16 *>(to + units * kHalvesUnit + ((group / 8) * 16 + c) * 4 + g);
-        sums[group % 8] = g == 0 ? h : g == 1 ? static_cast<_Float16>(sum - static_cast<float>(h)) : static_cast<_Float16>(0.0f);
+        reinterpret_cast<_Float16 *>(sums + (unit * 16 + c) * 4 + g)[t] =
+            g == 0 ? h : g == 1 ? static_cast<_Float16>(sum - static_cast<float>(h)) : static_cast<_Float16>(0.0f);
     }
     // Q4_0 halves: evens and odds of both fours; Q4_K: of each four
     constexpr int order[2][8] = {{0, 2, 4, 6, 1, 3, 5, 7}, {0, 2, 1, 3, 4, 6, 5, 7}};
     u4 hi, lo;
-    for (int i = 0; i < 4; ++i) {
-        const float x0 = v[order[Q4K][2 * i]], x1 = v[order[Q4K][2 * i + 1]];
+    for (int q = 0; q < 4; ++q) {
+        const float x0 = v[order[Q4K][2 * q]], x1 = v[order[Q4K][2 * q + 1]];
         const _Float16 h0 = static_cast<_Float16>(x0), h1 = static_cast<_Float16>(x1);
-        hi[i] = pack(h0, h1);
-        lo[i] = pack(static_cast<_Float16>(x0 - static_cast<float>(h0)), static_cast<_Float16>(x1 - static_cast<float>(h1)));
+        hi[q] = pack(h0, h1);
+        lo[q] = pack(static_cast<_Float16>(x0 - static_cast<float>(h0)), static_cast<_Float16>(x1 - static_cast<float>(h1)));
     }
-    u4 *at = to + (group / 8) * kHalvesUnit + c * 4 + g;
-    at[halves_at(group % 8, 0)] = hi;
-    at[halves_at(group % 8, 1)] = lo;
+    u4 *at = to + static_cast<uint64_t>(unit) * kHalvesUnit + c * 4 + g;
+    at[halves_at(t, 0)] = hi;
+    at[halves_at(t, 1)] = lo;
 }
 
 __device__ __forceinline__ float half_value(uint32_t h) { return hw_fp16_to_f32(static_cast<uint16_t>(h)); }
@@ -461,42 +472,6 @@ __device__ __forceinline__ void digits_unit(const Raw<Q4K> &raw, const u2 *xs, c
     for (int i = 0; i < N; ++i) acc[i] = __builtin_fmaf(scales[i], part[i], acc[i]);
 }
 
-// acc[r][i] (tile r, column 4 i + g of row j) += the products of a unit of RT
-// tiles.  xs: the unit's pieces of the lane's column, sums: its group sums.
-template <bool Q4K, int NR, int RT>
-__device__ __forceinline__ void halves_unit(const Raw<Q4K> raw[RT], const u4 *xs, const u4 *sums, uint32_t unit, uint32_t g, uint32_t blocks, float (&acc)[RT][NR])
-{
-    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto all = [&](auto... R) {
-        const Unit<Q4K> un[RT] = {Unit<Q4K>(raw[R()], unit, g, blocks)...};
-        float part[RT][NR];
-        for (int r = 0; r < RT; ++r)
-            for (int i = 0; i < NR; ++i) part[r][i] = Q4K ? 0.0f : acc[r][i];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const u4 hi = xs[halves_at(t, 0)], lo = xs[halves_at(t, 1)];
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const u4 q = un[r].halves(t);
-                const v4f p = mfma(hi, q, mfma(lo, q, zero));
-                const float f = un[r].scale(t);
-                for (int i = 0; i < NR; ++i) part[r][i] = __builtin_fmaf(f, p[i], part[r][i]);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            if constexpr (Q4K) {
-                const v4f p = mfma(*sums, un[r].minima(), zero);
-                for (int i = 0; i < NR; ++i) acc[r][i] = __builtin_fmaf(un[r].d, part[r][i], __builtin_fmaf(un[r].dmin * -64.0f, p[i], acc[r][i]));
-            } else {
-                for (int i = 0; i < NR; ++i) acc[r][i] = part[r][i];
-            }
-        }
-    };
-    if constexpr (RT == 1) all(std::integral_constant<int, 0>());
-    else all(std::integral_constant<int, 0>(), std::integral_constant<int, 1>());
-}
-
 struct QmPlan {
     uint32_t units;    // of k
     uint32_t tiles;    // of 16 rows
@@ -598,94 +573,115 @@ __global__ __launch_bounds__(kQmBlock, 4) void k_qm_digits(QMatArgs a, QmPlan pl
     }
 }
 
-// Lays out a column a workgroup in the workspace, and leaves its scale behind the pieces.
+// Lays out the columns in the workspace, a unit of a column per half wave.
 template <bool Q4K>
-__global__ __launch_bounds__(kQmBlock) void k_qm_columns(QMatArgs a, QmPlan pl)
+__global__ __launch_bounds__(kBlock) void k_qm_columns(QMatArgs a, QmPlan pl)
 {
-    __shared__ float top[kQmWaves];
-    for (uint32_t col = blockIdx.x; col < a.n; col += gridDim.x) {
-        const float *x = a.x + static_cast<int64_t>(col) * a.x_st[1];
-        float m = 0.0f;
-        if (a.x_st[0] == 1)
-            for (uint32_t k = threadIdx.x * 4; k < a.k; k += kQmBlock * 4) {
-                const v4f v = *reinterpret_cast<const v4f_any *>(x + k);
-                for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, __builtin_fabsf(v[i]));
-            }
-        else
-            for (uint32_t k = threadIdx.x; k < a.k; k += kQmBlock) m = __builtin_fmaxf(m, __builtin_fabsf(x[static_cast<int64_t>(k) * a.x_st[0]]));
-        m = wave_max_dpp(m);
-        __syncthreads(); // top of the column before
-        if (threadIdx.x % kWave == 0) top[threadIdx.x / kWave] = m;
-        __syncthreads();
-        for (int w = 0; w < kQmWaves; ++w) m = __builtin_fmaxf(m, top[w]);
-        float up, down;
-        column_scale(m, up, down);
-        u4 *to = static_cast<u4 *>(a.workspace) + (col / 16) * pl.x_pieces;
-        for (uint32_t i = threadIdx.x; i < pl.units * 32; i += kQmBlock) lay_out_halves<Q4K>(a, x, up, i / 4, i % 4, pl.units, col % 16, to);
-        if (threadIdx.x == 0) reinterpret_cast<float *>(static_cast<u4 *>(a.workspace) + pl.groups * pl.x_pieces)[col] = down;
+    const uint64_t all = static_cast<uint64_t>(pl.units) * a.n, step = static_cast<uint64_t>(gridDim.x) * (kBlock / 32);
+    for (uint64_t e = static_cast<uint64_t>(blockIdx.x) * (kBlock / 32) + threadIdx.x / 32; e < all; e += step) {
+        const uint32_t col = static_cast<uint32_t>(e / pl.units), unit = static_cast<uint32_t>(e % pl.units);
+        lay_out_halves<Q4K>(a, a.x + static_cast<int64_t>(col) * a.x_st[1], pl.units, unit, threadIdx.x % 32, col % 16,
+                            static_cast<u4 *>(a.workspace) + (col / 16) * pl.x_pieces);
     }
 }
 
 // Up to 16 columns a workgroup, as halves.  NR: a quarter of them, rounded up,
-// RT: tiles a wave takes at once, for one read of x.
-template <bool Q4K, int NR, int RT, bool WORDS>
-__global__ __launch_bounds__(kQmBlock, 4) void k_qm_halves(QMatArgs a, QmPlan pl)
+// KW: waves along k.
+template <bool Q4K, int NR, int KW, bool WORDS>
+__global__ __launch_bounds__(kQmBlock, KW == 8 ? 2 : 4) void k_qm_halves(QMatArgs a, QmPlan pl)
 {
-    constexpr int U = RT == 1 ? 2 : 1; // units in flight of each tile
-    __shared__ float part[2][kQmWaves][RT * NR][kWave];
+    constexpr uint32_t kHalf = kHalvesUnit / 2; // pieces of a half unit: one a thread
+    static_assert(kHalf == kQmBlock, "a thread stages one piece of each half unit");
+    extern __shared__ u4 stage[]; // [2][KW][kHalf]
+    __shared__ float part[2][kQmWaves][NR][kWave];
     const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), j = lane % 16, g = lane / 16;
     const uint32_t c0 = blockIdx.y * 16, n = a.n - c0 < 16 ? a.n - c0 : 16;
     const QmShare sh(a, pl, wave, Q4K);
+    const uint32_t steps = 2 * ((pl.units + KW - 1) / KW); // half units of the longest share
     const unsigned char *w = static_cast<const unsigned char *>(a.w);
-    auto row_of = [&](uint32_t tile, int r) {
-        const uint64_t at = (static_cast<uint64_t>(tile) + sh.wt * RT + r) * 16 + j;
+    auto row_of = [&](uint32_t tile) {
+        const uint64_t at = (static_cast<uint64_t>(tile) + sh.wt) * 16 + j;
         return w + (at < a.m ? at : a.m - 1) * sh.row_bytes;
     };
-    const uint32_t step = gridDim.x * sh.tw * RT;
-    uint32_t tile = blockIdx.x * sh.tw * RT;
-    const unsigned char *row[RT];
-    for (int r = 0; r < RT; ++r) row[r] = row_of(tile, r);
-    Raw<Q4K> raw[U][RT];
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-        if (sh.u0 + i < sh.u1)
-            for (int r = 0; r < RT; ++r) load_unit<WORDS>(raw[i][r], row[r], sh.u0 + i, g, sh.blocks);
     // slot j of the instruction's 16 columns is column 4 (j % 4) + j / 4, so
     // that result i of lane row g is column 4 i + g; the slots past n repeat
     uint32_t c = (j % 4) * 4 + j / 4;
     c = c < n ? c : n - 1;
-    const u4 *xs = static_cast<const u4 *>(a.workspace) + blockIdx.y * pl.x_pieces + c * 4 + g;
-    const u4 *sums = xs + static_cast<uint64_t>(pl.units) * kHalvesUnit;
-    const float *downs = reinterpret_cast<const float *>(static_cast<const u4 *>(a.workspace) + pl.groups * pl.x_pieces) + c0;
-    uint32_t turn = 0;
-    for (; tile < pl.tiles; tile += step, turn ^= 1) {
-        float acc[RT][NR];
-        for (int r = 0; r < RT; ++r)
-            for (int i = 0; i < NR; ++i) acc[r][i] = 0.0f;
-        const unsigned char *next[RT];
-        for (int r = 0; r < RT; ++r) next[r] = row_of(tile + step, r);
-        for (uint32_t u = sh.u0; u < sh.u1; u += U) {
+    const u4 *x = static_cast<const u4 *>(a.workspace) + blockIdx.y * pl.x_pieces;
+    const u4 *sums = x + static_cast<uint64_t>(pl.units) * kHalvesUnit;
+    const v4f *scales = reinterpret_cast<const v4f *>(sums + pl.units * (16 * 4)) + g;
+    sums += c * 4 + g;
+    const bool used = tid % 64 / 4 < n; // pieces of columns that are there
+    u4 piece[KW];
+    auto fetch = [&](uint32_t step) {
 #pragma unroll
-            for (int i = 0; i < U; ++i) {
-                if (u + i < sh.u1)
-                    halves_unit<Q4K, NR, RT>(raw[i], xs + (u + i) * kHalvesUnit, sums + (u + i) * (16 * 4), u + i, g, sh.blocks, acc);
-                const bool more = u + i + U < sh.u1;
-                if (more || (u + U >= sh.u1 && sh.u0 + i < sh.u1))
-                    for (int r = 0; r < RT; ++r) load_unit<WORDS>(raw[i][r], more ? row[r] : next[r], more ? u + i + U : sh.u0 + i, g, sh.blocks);
+        for (uint32_t k = 0; k < KW; ++k) {
+            const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * k / KW) * 2 + step;
+            if (used && first < static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * (k + 1) / KW) * 2)
+                piece[k] = x[static_cast<uint64_t>(first) * kHalf + tid];
+        }
+    };
+    const uint32_t step_tiles = gridDim.x * sh.tw;
+    uint32_t tile = blockIdx.x * sh.tw;
+    const unsigned char *row = row_of(tile);
+    fetch(0);
+    Raw<Q4K> raw;
+    if (sh.u0 < sh.u1) load_unit<WORDS>(raw, row, sh.u0, g, sh.blocks);
+    uint32_t turn = 0, buf = 0;
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (; tile < pl.tiles; tile += step_tiles, turn ^= 1) {
+        float acc[NR];
+        for (int i = 0; i < NR; ++i) acc[i] = 0.0f;
+        const unsigned char *next = row_of(tile + step_tiles);
+        for (uint32_t s = 0; s < steps; s += 2) {
+            const uint32_t u = sh.u0 + s / 2;
+            const bool live = u < sh.u1;
+            const Unit<Q4K> un(raw, u, g, sh.blocks); // of a share that has ended: not used
+            v4f scale = zero;
+            u4 sum = {0, 0, 0, 0};
+            if (live) {
+                scale = scales[u * 4];
+                if constexpr (Q4K) sum = sums[u * (16 * 4)];
+                if (u + 1 < sh.u1) load_unit<WORDS>(raw, row, u + 1, g, sh.blocks);
+                else load_unit<WORDS>(raw, next, sh.u0, g, sh.blocks);
+            }
+            float p[NR];
+            for (int i = 0; i < NR; ++i) p[i] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h, buf ^= 1) {
+                u4 *to = stage + buf * (KW * kHalf);
+#pragma unroll
+                for (uint32_t k = 0; k < KW; ++k) to[k * kHalf + tid] = piece[k];
+                fetch(s + h + 1 < steps ? s + h + 1 : 0); // of the next tile: the same again
+                __syncthreads();
+                const u4 *xs = to + wave % KW * kHalf + c * 4 + g;
+                if (live) {
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const u4 hi = xs[halves_at(t, 0)], lo = xs[halves_at(t, 1)], q = un.halves(4 * h + t);
+                        const v4f r = mfma(hi, q, mfma(lo, q, zero));
+                        const float f = un.scale(4 * h + t);
+                        for (int i = 0; i < NR; ++i) p[i] = __builtin_fmaf(f, r[i], p[i]);
+                    }
+                }
+            }
+            if (live) {
+                if constexpr (Q4K) {
+                    const v4f r = mfma(sum, un.minima(), zero);
+                    for (int i = 0; i < NR; ++i) p[i] = __builtin_fmaf(un.d, p[i], (un.dmin * -64.0f) * r[i]);
+                }
+                for (int i = 0; i < NR; ++i) acc[i] = __builtin_fmaf(scale[i], p[i], acc[i]);
             }
         }
-        for (int r = 0; r < RT; ++r) {
-            row[r] = next[r];
-            for (int i = 0; i < NR; ++i) part[turn][wave][r * NR + i][lane] = acc[r][i];
-        }
+        row = next;
+        for (int i = 0; i < NR; ++i) part[turn][wave][i][lane] = acc[i];
         __syncthreads();
-        for (uint32_t e = wave; e < sh.tw * RT * NR; e += kQmWaves) { // a wave per tile and quarter of columns
+        for (uint32_t e = wave; e < sh.tw * NR; e += kQmWaves) { // a wave per tile and quarter of columns
             const uint32_t t = e / NR, i = e % NR, col = 4 * i + g;
             float v = 0.0f;
-            for (uint32_t k = 0; k < sh.kw; ++k) v += part[turn][t / RT * sh.kw + k][t % RT * NR + i][lane];
+            for (uint32_t k = 0; k < KW; ++k) v += part[turn][t * KW + k][i][lane];
             const uint64_t r = (static_cast<uint64_t>(tile) + t) * 16 + j;
             const bool live = r < a.m && col < n;
-            v *= live ? downs[col] : 0.0f;
             uint64_t odd = __ballot(live && !(__builtin_fabsf(v) < __builtin_inff()));
             while (__builtin_expect(odd != 0, 0)) {
                 const int l = __builtin_ctzll(odd);
@@ -726,6 +722,9 @@ QmPlan qm_plan(const QMatArgs &a)
     pl.groups = (a.n + 15) / 16;
     pl.words = reinterpret_cast<uintptr_t>(a.w) % 4 == 0 && a.k % 64 == 0;
     pl.x_pieces = qm_digits(a, pl.units) ? 0 : halves_pieces(pl.units);
+    // halves: four waves along k share their stage with a second tile; eight
+    // where that leaves compute units idle
+    if (pl.x_pieces) pl.kw = static_cast<uint64_t>(pl.tiles) * pl.groups <= 2 * qm_cus() ? 8 : 4;
     return pl;
 }
 
@@ -744,23 +743,25 @@ void qm_run_digits(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
     else k_qm_digits<Q4K, N, false><<<grid, kQmBlock, lds, stream>>>(a, pl);
 }
 
-template <bool Q4K, int NR, int RT>
+template <bool Q4K, int NR, int KW>
 void qm_run_halves(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 {
-    const dim3 grid(qm_grid(pl, kQmWaves / pl.kw * RT), pl.groups);
-    k_qm_columns<Q4K><<<a.n < 65536 ? a.n : 65536, kQmBlock, 0, stream>>>(a, pl);
-    if (pl.words) k_qm_halves<Q4K, NR, RT, true><<<grid, kQmBlock, 0, stream>>>(a, pl);
-    else k_qm_halves<Q4K, NR, RT, false><<<grid, kQmBlock, 0, stream>>>(a, pl);
+    const uint64_t wgs = (static_cast<uint64_t>(pl.units) * a.n + kBlock / 32 - 1) / (kBlock / 32);
+    k_qm_columns<Q4K><<<static_cast<uint32_t>(wgs < 65536 ? wgs : 65536), kBlock, 0, stream>>>(a, pl);
+    const dim3 grid(qm_grid(pl, kQmWaves / KW), pl.groups);
+    constexpr uint32_t lds = 2 * KW * kHalvesUnit / 2 * 16;
+    if (pl.words) k_qm_halves<Q4K, NR, KW, true><<<grid, kQmBlock, lds, stream>>>(a, pl);
+    else k_qm_halves<Q4K, NR, KW, false><<<grid, kQmBlock, lds, stream>>>(a, pl);
 }
 
-template <bool Q4K, int RT>
+template <bool Q4K, int KW>
 void qm_run_halves(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 {
     switch ((a.n + 3) / 4) {
-    case 1: return qm_run_halves<Q4K, 1, RT>(a, pl, stream);
-    case 2: return qm_run_halves<Q4K, 2, RT>(a, pl, stream);
-    case 3: return qm_run_halves<Q4K, 3, RT>(a, pl, stream);
-    default: return qm_run_halves<Q4K, 4, RT>(a, pl, stream);
+    case 1: return qm_run_halves<Q4K, 1, KW>(a, pl, stream);
+    case 2: return qm_run_halves<Q4K, 2, KW>(a, pl, stream);
+    case 3: return qm_run_halves<Q4K, 3, KW>(a, pl, stream);
+    default: return qm_run_halves<Q4K, 4, KW>(a, pl, stream);
     }
 }
 
@@ -773,8 +774,8 @@ void qm_run(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
     case 3: return qm_run_digits<Q4K, 3>(a, pl, stream);
     case 4: return qm_run_digits<Q4K, 4>(a, pl, stream);
     }
-    if (pl.tiles >= 4 * qm_cus()) qm_run_halves<Q4K, 2>(a, pl, stream); // two tiles a wave leave enough workgroups
-    else qm_run_halves<Q4K, 1>(a, pl, stream);
+    if (pl.kw == 8) qm_run_halves<Q4K, 8>(a, pl, stream);
+    else qm_run_halves<Q4K, 4>(a, pl, stream);
 }
 
 } // namespace
@@ -782,7 +783,7 @@ void qm_run(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 uint64_t quant_mat_workspace_bytes(const QMatArgs &a)
 {
     const QmPlan pl = qm_plan(a);
-    return pl.x_pieces ? pl.groups * pl.x_pieces * 16 + static_cast<uint64_t>(a.n) * 4 : 0;
+    return pl.groups * pl.x_pieces * 16;
 }
 
 hipError_t launch_quant_mat(const QMatArgs &a, hipStream_t stream)
