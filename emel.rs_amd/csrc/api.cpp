@@ -2739,6 +2739,8 @@ emel_status paged_append(const emel_tensor_view *k, const emel_tensor_view *v, c
     if (!pools_alike(*kp, *vp) || !ne_is(k->ne, kp->ne[0], kp->ne[2], k->ne[2]) || !same_ne(*k, *v) ||
         !ne_is(slots->ne, k->ne[2], 1))
         return fail(EMEL_ERR_SHAPE_MISMATCH, "paged append takes [dim, heads, tokens], [tokens] and two pools alike");
+    if (kp->ne[0] * kp->ne[2] > 1u << 26)
+        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "dim * kv_heads is past 2^26");
     const Span ks = pages_span(*kp), vs = pages_span(*vp);
     for (const Span s : {span_of(*k, 4), span_of(*v, 4), span_of(*slots, 4)})
         if (!apart(s, ks) || !apart(s, vs)) return fail(EMEL_ERR_INVALID_VIEW, "the pages overlap a source");

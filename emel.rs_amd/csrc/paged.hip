@@ -20,28 +20,71 @@ __device__ __forceinline__ float from_half(uint16_t h)
     else return static_cast<float>(__builtin_bit_cast(_Float16, h));
 }
 
-// A workgroup per token.  Of tokens with one slot the last is stored: a
-// workgroup whose slot a later token names leaves it to that one.
-template <bool BF16>
-__global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a)
+// ---- new tokens into their slots ---------------------------------------------------------
+//
+// Bound by the tokens' bytes: 4 read and 2 written a value.  A workgroup takes
+// T consecutive tokens, eight values a lane and step.  Of tokens with one slot
+// the last is stored: each workgroup looks through the slots behind its own and leaves a
+// token whose slot a later one names to that one.  Eight tokens a workgroup
+// share that look (it reads 4 bytes of each later token, and 8001 tokens of 1024 values took
+// 37 us with one token a workgroup, bound by it); few tokens take one each, for
+// more workgroups.
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef u4 u4_any __attribute__((aligned(2))); // pools may start at any half
+typedef v4f v4f_any __attribute__((aligned(4)));
+
+// dim: values of a head, in eights where VEC.
+template <bool BF16, uint32_t T, bool VEC>
+__global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a, FastDiv page, FastDiv head, FastDiv token)
 {
+    __shared__ uint32_t gone;
     const uint64_t slots = static_cast<uint64_t>(a.page) * a.pages;
-    const uint32_t per = a.dim * a.kv_heads;
-    for (uint32_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-        const int32_t slot = a.slots[static_cast<int64_t>(t) * a.slots_st];
-        if (slot < 0 || static_cast<uint64_t>(slot) >= slots) continue;
-        bool later = false;
-        for (uint32_t u = t + 1 + threadIdx.x; u < a.tokens; u += kBlock)
-            later |= a.slots[static_cast<int64_t>(u) * a.slots_st] == slot;
-        if (__syncthreads_or(later)) continue;
-        const uint32_t p = static_cast<uint32_t>(slot) / a.page, i = static_cast<uint32_t>(slot) % a.page;
-        for (uint32_t e = threadIdx.x; e < per; e += kBlock) {
-            const int64_t h = e / a.dim, d = e % a.dim;
-            a.k_pool.data[p * a.k_pool.st_page + h * a.k_pool.st_head + i * a.k_pool.st_tok + d] =
-                to_half<BF16>(a.k[d * a.k_st[0] + h * a.k_st[1] + t * a.k_st[2]]);
-            a.v_pool.data[p * a.v_pool.st_page + h * a.v_pool.st_head + i * a.v_pool.st_tok + d] =
-                to_half<BF16>(a.v[d * a.v_st[0] + h * a.v_st[1] + t * a.v_st[2]]);
+    for (uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * T; t0 < a.tokens; t0 += static_cast<uint64_t>(gridDim.x) * T) {
+        int32_t mine[T];
+        uint32_t skip = 0;
+        for (uint32_t i = 0; i < T; ++i) {
+            mine[i] = t0 + i < a.tokens ? a.slots[static_cast<int64_t>(t0 + i) * a.slots_st] : -1;
+            if (mine[i] < 0 || static_cast<uint64_t>(mine[i]) >= slots) skip |= 1u << i;
         }
+        if (threadIdx.x == 0) gone = skip;
+        __syncthreads();
+        uint32_t later = 0;
+#pragma unroll 4
+        for (uint64_t u = t0 + 1 + threadIdx.x; u < a.tokens; u += kBlock) {
+            const int32_t s = a.slots[static_cast<int64_t>(u) * a.slots_st];
+            for (uint32_t i = 0; i < T; ++i) later |= s == mine[i] && u > t0 + i ? 1u << i : 0u;
+        }
+        if (later & ~skip) atomicOr(&gone, later);
+        __syncthreads();
+        const uint32_t drop = gone;
+        // an item: eight values (or one) of a head, of a token, of keys or values
+        for (uint32_t e = threadIdx.x; e < 2 * T * token.d; e += kBlock) {
+            const uint32_t i = token.div(e), r = e - i * token.d, k = i % T;
+            if ((drop >> k) & 1u) continue;
+            const uint32_t h = head.div(r), d = (r - h * head.d) * (VEC ? 8 : 1);
+            int32_t slot = mine[0]; // no index at run time: the slots stay in registers
+            for (uint32_t q = 1; q < T; ++q) slot = k == q ? mine[q] : slot;
+            const uint32_t p = page.div(static_cast<uint32_t>(slot)), at = static_cast<uint32_t>(slot) - p * page.d;
+            const bool val = i >= T;
+            const float *src = val ? a.v : a.k;
+            const int64_t *st = val ? a.v_st : a.k_st;
+            const PagePool &pool = val ? a.v_pool : a.k_pool;
+            src += d * st[0] + h * st[1] + static_cast<int64_t>(t0 + k) * st[2];
+            uint16_t *dst = pool.data + p * pool.st_page + h * pool.st_head + at * pool.st_tok + d;
+            if constexpr (VEC) {
+                const v4f lo = *reinterpret_cast<const v4f_any *>(src), hi = *reinterpret_cast<const v4f_any *>(src + 4);
+                u4 w;
+                for (int q = 0; q < 4; ++q) {
+                    const float x = q < 2 ? lo[2 * q] : hi[2 * q - 4], y = q < 2 ? lo[2 * q + 1] : hi[2 * q - 3];
+                    w[q] = to_half<BF16>(x) | static_cast<uint32_t>(to_half<BF16>(y)) << 16;
+                }
+                *reinterpret_cast<u4_any *>(dst) = w;
+            } else {
+                *dst = to_half<BF16>(*src);
+            }
+        }
+        __syncthreads(); // gone, of the next tokens
     }
 }
 
@@ -83,12 +126,8 @@ constexpr uint32_t pa_per_cu(int ks) { return 2; }
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-// pools may start at any half
-typedef u4 u4_any __attribute__((aligned(2)));
 typedef u2 u2_any __attribute__((aligned(2)));
-typedef v4f v4f_any __attribute__((aligned(4)));
 
 template <bool BF16>
 __device__ __forceinline__ v4f mfma32(u4 a, u4 b, v4f c)
@@ -655,11 +694,23 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
 
 } // namespace
 
+template <bool BF16, uint32_t T>
+static void pa_append(const PagedAppendArgs &a, hipStream_t stream)
+{
+    const bool vec = a.dim % 8 == 0 && a.k_st[0] == 1 && a.v_st[0] == 1;
+    const uint32_t head = vec ? a.dim / 8 : a.dim;
+    const uint64_t wgs = (static_cast<uint64_t>(a.tokens) + T - 1) / T;
+    const uint32_t grid = static_cast<uint32_t>(wgs < (1u << 20) ? wgs : 1u << 20);
+    const FastDiv page(a.page), per_head(head), per_token(head * a.kv_heads);
+    if (vec) k_pa_append<BF16, T, true><<<grid, kBlock, 0, stream>>>(a, page, per_head, per_token);
+    else k_pa_append<BF16, T, false><<<grid, kBlock, 0, stream>>>(a, page, per_head, per_token);
+}
+
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t stream)
 {
-    const uint32_t grid = a.tokens < (1u << 20) ? a.tokens : 1u << 20;
-    if (a.bf16) k_pa_append<true><<<grid, kBlock, 0, stream>>>(a);
-    else k_pa_append<false><<<grid, kBlock, 0, stream>>>(a);
+    const bool many = a.tokens >= 2048; // a workgroup per compute unit, of eight tokens
+    if (a.bf16) many ? pa_append<true, 8>(a, stream) : pa_append<true, 1>(a, stream);
+    else many ? pa_append<false, 8>(a, stream) : pa_append<false, 1>(a, stream);
     return hipGetLastError();
 }
 
