@@ -393,6 +393,20 @@ def test_logits_adjustment_is_the_definition(gpu, card, rows, history, biases, m
     assert_bits_equal(dev["logits"].cpu().numpy(), want, "in place")
 
 
+def test_logits_adjustment_of_a_history_past_16_bits(gpu):
+    """Counts and entry numbers that do not fit half a word."""
+    import torch
+
+    c = logits_case(9, 5003, 2, 70000, 66000, False)
+    c["history"][0, :69000] = 77  # one token, 69000 times over
+    c["history_len"][:] = 70000
+    want = adjusted(**c)
+    dev = {n: torch.from_numpy(v).to(gpu) for n, v in c.items()}
+    y = torch.empty(2, 5003, device=gpu)
+    run(logits_event(c, dev, y))
+    assert_bits_equal(y.cpu().numpy(), want, "long history")
+
+
 def test_logits_adjustment_strides(gpu):
     import torch
 
