@@ -270,38 +270,38 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
     __shared__ float wm[kWaves][16], wl[kWaves][16], jl[16];
     __shared__ uint32_t scan[kWaves], found[2];
     __shared__ uint32_t last;
-    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const uint32_t col = lane % 16, g = lane / 16;
+    const uint32_t thread = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(thread / kWave);
     const uint32_t dim = a.dim, pitch = dim + 4; // of a head in joined
 
     // This workgroup's run of units, and the sequence it starts in.  A row's
     // set-up and end cost about a unit: it counts as one more, but where there
     // is no more than a unit to a workgroup (that would only part the rows).
+    const uint32_t first_lane = thread % kWave;
     uint32_t total, run, cur, base; // base: the sequence's first unit
     uint32_t s, setup;
     int32_t s_len;
-    if (__builtin_expect(a.seqs <= kWave, 1)) { // every wave for itself: a sequence per lane
-        const int32_t len = lane < a.seqs ? pa_len(a, lane) : 0;
-        const uint32_t mine = lane < a.seqs ? pa_seq(a, len).units : 0;
+    if (__builtin_expect(a.seqs <= kWave, 1)) { // every wave for itself: a sequence per first_lane
+        const int32_t len = first_lane < a.seqs ? pa_len(a, first_lane) : 0;
+        const uint32_t mine = first_lane < a.seqs ? pa_seq(a, len).units : 0;
         uint32_t pre = wave_scan(mine);
         const uint32_t all = lane_u32(pre, kWave - 1);
         setup = all * pl.rows > gridDim.x;
         total = (all + setup * a.seqs) * pl.rows;
-        pre += setup * (lane + 1);
+        pre += setup * (first_lane + 1);
         run = pl.grid.div(total + gridDim.x - 1);
         cur = blockIdx.x * run;
         if (cur >= total) return;
-        s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__popcll(__ballot(lane < a.seqs && pre * pl.rows <= cur))));
+        s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__popcll(__ballot(first_lane < a.seqs && pre * pl.rows <= cur))));
         base = lane_u32(pre - mine - setup, s) * pl.rows;
         s_len = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len), s));
     } else {
         const uint32_t per = (a.seqs + kBlock - 1) / kBlock;
-        const uint32_t s0 = tid * per < a.seqs ? tid * per : a.seqs, s1 = s0 + per < a.seqs ? s0 + per : a.seqs;
+        const uint32_t s0 = thread * per < a.seqs ? thread * per : a.seqs, s1 = s0 + per < a.seqs ? s0 + per : a.seqs;
         uint32_t mine = 0;
 #pragma unroll 1
         for (uint32_t i = s0; i < s1; ++i) mine += pa_seq(a, pa_len(a, i)).units;
         uint32_t pre = wave_scan(mine);
-        if (lane == kWave - 1) scan[wave] = pre;
+        if (first_lane == kWave - 1) scan[wave] = pre;
         __syncthreads();
         uint32_t all = 0;
         for (int w = 0; w < kWaves; ++w) {
@@ -338,6 +338,12 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
     uint32_t row_at = base + row * units;
 
     while (cur < end) {
+        // What follows from the thread's number is worked out where it is used:
+        // the compiler would gather all of it ahead of this loop, some 470
+        // instructions that a workgroup of one short segment waits for.
+        uint32_t tid = thread;
+        asm volatile("" : "+v"(tid));
+        const uint32_t lane = tid % kWave, col = lane % 16, g = lane / 16;
         const uint32_t n0 = cur - row_at, n1 = end - row_at < units ? end - row_at : units;
         const uint32_t u0 = n0 > setup ? n0 - setup : 0, u1 = n1 - setup;
         const uint32_t kh = pl.hgroups.div(row), h0 = kh * pl.group + (row - kh * pl.hgroups.d) * 16;
@@ -582,6 +588,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
             }
             return top;
         };
+        asm volatile("" : "+v"(tid));
         const uint32_t cells = heads * dim; // dim is even: pairs do not cross heads
         float *out = a.y + static_cast<int64_t>(h0) * a.y_st[1] + static_cast<int64_t>(s) * a.y_st[2];
         auto put = [&](uint32_t h, uint32_t d, float x, float y) {
@@ -617,6 +624,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
             }
             __syncthreads();
             if (last) {
+                asm volatile("" : "+v"(tid));
                 auto piece = [&](uint32_t p) { return pl.parts + static_cast<size_t>(2 * (w0 + p) + (p == 0 ? 1 : 0)) * pl.slot; };
                 float *weight = joined; // [piece][head]
                 // The first loads of everything go out together: maxima and
