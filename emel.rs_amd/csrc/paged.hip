@@ -122,7 +122,7 @@ constexpr uint32_t kPaLine = 64;   // words between arrival counters (a cache li
 
 // Workgroups that a compute unit holds at once: the registers that their
 // launch bounds leave them.
-constexpr uint32_t pa_per_cu(int ks) { return 2; }
+constexpr uint32_t pa_per_cu(int ks) { return ks <= 2 ? 4 : ks <= 4 ? 3 : 2; }
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
@@ -193,7 +193,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v)
 // What a launch derives on the host.
 struct PaPlan {
     FastDiv page;       // tokens per page
-    FastDiv dim, grid, hgroups;
+    FastDiv dim, hgroups;
+    FastDiv grid, few;  // workgroups: all, and two a compute unit
     uint32_t group;     // query heads of a cache head
     uint32_t rows;      // rows of a sequence: kv_heads * hgroups
     uint32_t slot;      // floats of a workspace slot
@@ -273,6 +274,10 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
     const uint32_t thread = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(thread / kWave);
     const uint32_t dim = a.dim, pitch = dim + 4; // of a head in joined
 
+    // Rows of a few units are mostly set-up, which more workgroups hide; long
+    // ones stream best with two a compute unit (64 sequences of 90 to 9000
+    // tokens 106 us, 113 with three; 640 of 100 tokens 90 us, 77 with three).
+    auto share_of = [&](uint32_t units) { return units > 4 * a.seqs ? pl.few : pl.grid; };
     // This workgroup's run of units, and the sequence it starts in.  A row's
     // set-up and end cost about a unit: it counts as one more, but where there
     // is no more than a unit to a workgroup (that would only part the rows).
@@ -285,10 +290,11 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
         const uint32_t mine = first_lane < a.seqs ? pa_seq(a, len).units : 0;
         uint32_t pre = wave_scan(mine);
         const uint32_t all = lane_u32(pre, kWave - 1);
-        setup = all * pl.rows > gridDim.x;
+        const FastDiv share = share_of(all);
+        setup = all * pl.rows > share.d;
         total = (all + setup * a.seqs) * pl.rows;
         pre += setup * (first_lane + 1);
-        run = pl.grid.div(total + gridDim.x - 1);
+        run = share.div(total + share.d - 1);
         cur = blockIdx.x * run;
         if (cur >= total) return;
         s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__popcll(__ballot(first_lane < a.seqs && pre * pl.rows <= cur))));
@@ -308,11 +314,12 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
             if (static_cast<uint32_t>(w) < wave) pre += scan[w];
             all += scan[w];
         }
-        setup = all * pl.rows > gridDim.x;
+        const FastDiv share = share_of(all);
+        setup = all * pl.rows > share.d;
         pre += setup * s0 - mine;
         mine += setup * (s1 - s0);
         total = (all + setup * a.seqs) * pl.rows;
-        run = pl.grid.div(total + gridDim.x - 1);
+        run = share.div(total + share.d - 1);
         cur = blockIdx.x * run;
         if (cur >= total) return;
         if (mine && pre * pl.rows <= cur && cur < (pre + mine) * pl.rows) {
@@ -733,7 +740,7 @@ uint32_t pa_heads(const PagedAttnArgs &a) // of a row
 // Workgroups that run at once, by registers and LDS, and their LDS: more would
 // wait for a second round with as large a run each.
 struct PaGrid {
-    uint32_t workgroups, lds;
+    uint32_t workgroups, few, lds;
 };
 PaGrid pa_grid(const PagedAttnArgs &a)
 {
@@ -748,7 +755,7 @@ PaGrid pa_grid(const PagedAttnArgs &a)
     for (;; --per) {
         const uint32_t joined = 4 * pa_heads(a) * (a.dim + 4), weights = pa_heads(a) * cus * per;
         const uint32_t lds = 4 * (joined > weights ? joined : weights);
-        if (per == 1 || per * (fixed + lds) <= 160 * 1024) return {cus * per, lds};
+        if (per == 1 || per * (fixed + lds) <= 160 * 1024) return {cus * per, cus * (per < 2 ? per : 2), lds};
     }
 }
 
@@ -794,7 +801,9 @@ hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream)
     pl.group = a.heads / a.kv_heads;
     pl.hgroups = FastDiv((pl.group + 15) / 16);
     pl.rows = a.kv_heads * pl.hgroups.d;
-    pl.grid = FastDiv(pa_grid(a).workgroups);
+    const PaGrid grid = pa_grid(a);
+    pl.grid = FastDiv(grid.workgroups);
+    pl.few = FastDiv(grid.few);
     pl.slot = 32 + pa_heads(a) * a.dim;
     pl.parts = static_cast<float *>(a.workspace);
     pl.arrived = static_cast<uint32_t *>(a.counters);
