@@ -2822,7 +2822,7 @@ emel_status paged_attention(const emel_tensor_view *q, const emel_tensor_view *k
     a.soft_cap = soft_cap;
     a.window = static_cast<uint32_t>(window > kMaxExtent ? 0 : window); // longer than any sequence: none
     if (emel::paged_attn_seqs(a) == 0)
-        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "max pages * page * cache heads is past 2^38 tokens");
+        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "a sequence's cache heads hold 2^31 units of 128 tokens or more");
     StreamLease lease;
     const emel::PagedScratch need = emel::paged_attn_scratch(a);
     s = lease.acquire(as_stream(stream));

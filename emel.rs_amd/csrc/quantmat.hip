@@ -16,7 +16,8 @@
 // instruction then hold 4 digits x 4 columns, and one instruction a group does
 // them all, exactly, in integers.  Eight weights cost three or four
 // instructions of unpacking, a group one LDS read, and a conversion and an fma
-// a column.  A value is off by 2^-30 of the largest of its 256 at most: less
+// a column.  A value is off by 2^-30 of the largest of its 256 at most (by 2^-127
+// where that is below 2^-97: the scale stays a normal number): less
 // than f32's own rounding of the sum that the largest is part of.
 //
 // k_qm_halves, more columns.  Each column's run of 256 values goes in as two
@@ -780,18 +781,33 @@ void qm_run(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 
 } // namespace
 
+// Columns that are laid out and launched at a time: the workspace stays at
+// 68 bytes a value of k for each 16 of these, and the grid's second axis
+// within what a launch takes (65535 groups).
+constexpr uint32_t kQmColumns = 1u << 14;
+
 uint64_t quant_mat_workspace_bytes(const QMatArgs &a)
 {
-    const QmPlan pl = qm_plan(a);
+    QMatArgs b = a;
+    b.n = a.n < kQmColumns ? a.n : kQmColumns;
+    const QmPlan pl = qm_plan(b);
     return pl.groups * pl.x_pieces * 16;
 }
 
 hipError_t launch_quant_mat(const QMatArgs &a, hipStream_t stream)
 {
-    const QmPlan pl = qm_plan(a);
-    if (a.q4k) qm_run<true>(a, pl, stream);
-    else qm_run<false>(a, pl, stream);
-    return hipGetLastError();
+    QMatArgs b = a;
+    for (uint64_t c = 0; c < a.n; c += kQmColumns) {
+        b.n = static_cast<uint32_t>(a.n - c < kQmColumns ? a.n - c : kQmColumns);
+        b.x = a.x + static_cast<int64_t>(c) * a.x_st[1];
+        b.y = a.y + static_cast<int64_t>(c) * a.y_st[1];
+        const QmPlan pl = qm_plan(b);
+        if (a.q4k) qm_run<true>(b, pl, stream);
+        else qm_run<false>(b, pl, stream);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 } // namespace emel

@@ -505,13 +505,17 @@ emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_
  * sources: nb = [1, row bytes, ...], k a multiple of 32 resp. 256), x is F32
  * [k, n, 1, 1], dst F32 [m, n, 1, 1]; x and dst may have any strides, dst's
  * elements disjoint and apart from both sources.  W[r, k] is the value that
- * get_rows gives: (q - 8) d for Q4_0, d sc q - dmin m for Q4_K.  Each x is
- * read to 22 bits below its leading one (values under 2^-16 of their
- * column's largest lose further low bits), products are exact and sums are
- * f32, in an order that depends on the sizes alone; infinities and NaN go
- * through as in the formula.  Wants the stream's workspace for n > 4 or a
- * long k, which grows as the reductions' does.  Guards: a NULL view or data,
- * or an unaligned F32 pointer, is INVALID_ARGUMENT; a view that fails its
+ * get_rows gives: (q - 8) d for Q4_0, d sc q - dmin m for Q4_K.  x is read in
+ * runs of 256 values along k, to 2^-30 of a run's largest value (to 2^-127
+ * where that is below 2^-97) for up to four columns, else to 22 bits of each value
+ * down to 2^-16 of the run's largest and to 2^-40 of the largest below.
+ * Products are exact, sums are f32, in an order that depends on the sizes
+ * alone; infinities and NaN go through as in the formula.  More than four
+ * columns, or a k whose columns do not fit LDS as digits (past 17152 for one column, 4096
+ * for four), want the stream's workspace, which grows as the reductions'
+ * does: graphs captured from one stream share it, and run one after the
+ * other, or are captured from streams of their own.  Guards: a NULL view or
+ * data, or an unaligned F32 pointer, is INVALID_ARGUMENT; a view that fails its
  * rules, or an overlap, INVALID_VIEW; extents that do not match,
  * SHAPE_MISMATCH; an extent past 2^31 - 1 or a k past 2^26,
  * UNSUPPORTED_OPERATION. */
@@ -546,15 +550,17 @@ emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_ten
  * when the kernel runs, so a captured call follows them.  A sequence of
  * length 0 gets zeros.  One whose length is negative or past max pages * page, or that
  * reaches a page id outside the pool, gets NaN, and nothing outside the pool
- * is read.  What lies behind a sequence's length, and before its window, is
- * never read.  Scores, softmax and sums are f32; q and the softmax weights
+ * is read.  What lies behind a sequence's length, and before its window,
+ * does not count, NaN or not.  Scores, softmax and sums are f32; q and the softmax weights
  * keep 22 bits (F16 pools) or 24 (BF16) in products with the cached halves.
  * Wants the stream's workspace, which grows as the reductions' does: graphs
  * captured from one stream share it, and run one after the other, or are
  * captured from streams of their own.
  *
  * Guards of both: as mul_mat_q4_0; parameters that are not finite, or a
- * negative soft_cap, are INVALID_PARAMETERS. */
+ * negative soft_cap, are INVALID_PARAMETERS; dim * kv_heads past 2^26 in an
+ * append, and max pages * page past 2^31 - 1, or 2^31 units of 128 tokens for one
+ * sequence's cache heads, in an attention, UNSUPPORTED_OPERATION. */
 emel_status emel_op_paged_kv_append(const emel_tensor_view *k, const emel_tensor_view *v,
                                     const emel_tensor_view *slots, const emel_tensor_view_mut *k_pages,
                                     const emel_tensor_view_mut *v_pages, emel_stream stream);

@@ -47,7 +47,9 @@ def product(form, rows, x):
     x is taken as hi + lo halves of 11 bits each, an error of 2^-23 of the value, or of 2^-39 of the column's
     largest value where lo is subnormal; products of a half and a nibble are exact; sums of up to k / 32 + 128 f32
     terms in a row (a block's in the matrix unit, then blocks, then waves), each off by at most 2^-23 of the sum of
-    magnitudes so far."""
+    magnitudes so far.  As digits, x is off by 2^-30 of the largest of its 256 instead, T: sum |w| T 2^-30 is within the
+    first term where T is below 2^14 times the run's mean weighted size, as in a run of 256 normal values (T about 3) or
+    of those with one 1000 times as large."""
     hi, lo = weight_terms(form, rows)
     x = x.astype(np.float64)
     k = x.shape[1]

@@ -104,6 +104,35 @@ def test_product_range_of_values(gpu, form, n):
 
 
 @pytest.mark.parametrize("form", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("n", [1, 4, 6])
+def test_product_of_values_near_the_smallest(gpu, form, n):
+    """Runs whose largest value is below 2^-97 keep an absolute precision of 2^-127 a value."""
+    import torch
+
+    k, m = 512, 40
+    rows, x = inputs(88 + n, form, k, m, n)
+    x *= np.float32(2.0**-110)
+    y = torch.empty(n, m, device=gpu)
+    run(EVENT[form](packed(torch.from_numpy(rows).to(gpu), form, k, m), view(torch.from_numpy(x).to(gpu)), out(y)))
+    want, tol = product(form, rows, x)
+    hi, lo = weight_terms(form, rows)
+    within(y.cpu().numpy(), want, tol + (np.abs(hi) + np.abs(lo)).sum(1) * 2.0**-127 + 2.0**-140, "small")
+
+
+def test_product_of_more_columns_than_a_launch_takes(gpu):
+    """Columns run in parts of 2^14; more than 65535 groups of 16 of them would not fit a grid."""
+    import torch
+
+    k, m, n = 32, 5, (1 << 20) + 3
+    rows = packed_rows(3, "q4_0", k, m)
+    x = torch.randn(n, k, device=gpu, generator=torch.Generator(gpu).manual_seed(5))
+    y = torch.empty(n, m, device=gpu)
+    run(EVENT["q4_0"](packed(torch.from_numpy(rows).to(gpu), "q4_0", k, m), view(x), out(y)))
+    want, tol = product("q4_0", rows, x.cpu().numpy())
+    within(y.cpu().numpy(), want, tol, "columns")
+
+
+@pytest.mark.parametrize("form", ["q4_0", "q4_k"])
 @pytest.mark.parametrize("n", [1, 3, 9])
 def test_product_infinities_and_nan_as_in_the_formula(gpu, form, n):
     import torch
@@ -565,3 +594,41 @@ def test_streams_do_not_share_scratch(gpu):
     for c, (r, x), (_, _, y) in zip(cases, weights, dev):
         check_attention(c)
         within(y.cpu().numpy(), *product("q4_k", r, x), "stream")
+
+
+def test_a_capture_needs_its_scratch_beforehand(gpu):
+    """Under capture a call whose scratch must grow is refused, and nothing of it is recorded; a reserve ahead lets it in."""
+    import ctypes
+
+    import torch
+
+    handle = ctypes.c_void_p()  # a stream of its own: one of torch's pool may have scratch already
+    assert eh.load().emel_stream_create(ctypes.byref(handle)) == eh.Status.OK
+    stream = torch.cuda.ExternalStream(handle.value)
+    kernel = eh.Kernel(stream.cuda_stream, synchronous=False)
+    c = attend_case(gpu, False, 8, 2, 64, 16, [700, 90], "token", 21)
+    rows, x = inputs(61, "q4_k", 1024, 300, 9)
+    w, x_dev, y = torch.from_numpy(rows).to(gpu), torch.from_numpy(x).to(gpu), torch.full((9, 300), 7.0, device=gpu)
+    events = attend_event(c), eh.OpMulMatQ4K(packed(w, "q4_k", 1024, 300), view(x_dev), out(y))
+    c["y"].fill_(7.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert [kernel.process_event(e) for e in events] == [eh.Status.STREAM_CAPTURE] * 2
+        x_dev.mul_(1.0)  # a graph of no nodes is no test of one
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (c["y"] == 7.0).all() and (y == 7.0).all()
+    assert eh.stream_reserve(32 << 20, 1 << 20, stream.cuda_stream) == eh.Status.OK
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert [kernel.process_event(e) for e in events] == [eh.Status.OK] * 2
+    for _ in range(3):
+        c["y"].fill_(7.0)
+        y.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(c)
+        within(y.cpu().numpy(), *product("q4_k", rows, x), "captured")
+    del graph
+    assert eh.load().emel_stream_destroy(handle) == eh.Status.OK
