@@ -10,8 +10,8 @@ None has a counterpart in the reference's events; include/emel_hip.h holds
 their formulas, layouts and guards.  Every view is device memory.  An event
 may be kept and processed again: it then reads and writes the same views,
 with what they hold by then.  Its operands' C views are laid out once, on
-construction, so an event is immutable (a call of six views 2.5 us against
-5 us with the views rebuilt).
+construction, so an event is immutable (a call of six views takes the host
+3.9 us, 6.3 us with the event built anew).
 """
 from __future__ import annotations
 
