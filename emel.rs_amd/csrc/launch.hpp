@@ -243,7 +243,7 @@ struct QMatArgs {
     int64_t x_st[2];     // element strides
     float *y;            // [m, n]
     int64_t y_st[2];
-    void *workspace;     // quant_mat_workspace_bytes
+    void *workspace;     // at least quant_mat_workspace_bytes
 };
 
 uint64_t quant_mat_workspace_bytes(const QMatArgs &args);

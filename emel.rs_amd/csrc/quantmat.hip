@@ -24,13 +24,17 @@
 // halves each, hi + lo, scaled by a power of two that brings its largest value to
 // [2^14, 2^15): 22 bits of every value down to 2^-16 of that, and 2^-40 of it
 // below.  The 16 columns of the f16 instruction are 16 columns, two
-// instructions a group.  k_qm_columns lays x out in the workspace, 4 bytes a
-// value; a workgroup stages half units of it in LDS, the next one on its way
-// in registers (read straight from the L2 the waves waited for it: 15 columns
-// of 4096x11008 38 us).  A nibble
+// instructions a group.  A workgroup lays a chunk of k, up to four units, of 16
+// columns out in LDS and takes a run of tiles through it, a tile a wave,
+// without another barrier; k_qm_sum adds up the chunks.  (Columns laid out by a
+// kernel of their own and staged by half units, each workgroup over all of k:
+// 15 columns of 4096x11008 20.7 us against 15.5, 16 of 4096x40000 56 against 35.)  A nibble
 // becomes a half by and-or into 1024's mantissa and a packed subtraction (as a
 // subnormal half it would need neither, but the instruction drops as many
 // low bits of its sum as such a factor has leading zeros: 1e-5 off).
+// Of 15.5 us of 4096x11008 about 9.6 are the launch and the weights (25 MB from
+// the L2 and the Infinity Cache), 2.3 the columns' layout, 2 to 3 the
+// matrix instructions and what surrounds them, 2 to 3 k_qm_sum.
 //
 // Sums are f32, and their order depends on the sizes alone.
 //
@@ -38,8 +42,8 @@
 // fourth of the row's 256-value unit, whole blocks of Q4_0 or 16 bytes of each
 // half of a Q4_K block, and the four lanes of a row exchange words so that each
 // instruction sees one group.  The order of values within a group is whatever
-// that gives; x is laid out in the same order.  The waves of a workgroup share
-// a tile's k range and add up through LDS.
+// that gives; x is laid out in the same order.  As digits, the waves of a
+// workgroup share a tile's k range and add up through LDS.
 //
 // Neither digits nor halves hold infinities: an output that is not finite is
 // computed again as the formula stands, by the whole wave.
@@ -195,28 +199,26 @@ __device__ __forceinline__ void lay_out_digits(const QMatArgs &a, uint32_t units
 
 // ---- columns as halves -----------------------------------------------------------------
 
-// In the workspace, 16 bytes of 8 halves each, 16 columns side by side: unit u's
-// group t at [u][t][part][column][lane row], and behind all units, at [u][column]
-// [part], the eight groups' sums (parts 2 and 3 are zeros), and behind those
-// the units' scales, column 4 i + g at [u][g][i].
+// In LDS, 16 bytes of 8 halves each, 16 columns side by side: unit u's group t
+// at [u][t][part][column][lane row], and behind all units, at [u][column][part],
+// the eight groups' sums (parts 2 and 3 are zeros), and behind those the
+// units' scales, column 4 i + g at [u][g][i].
 constexpr uint32_t kHalvesUnit = 8 * 2 * 16 * 4;
+constexpr uint32_t kHalvesBytes = (kHalvesUnit + 16 * 4 + 4) * 16; // of a unit
 constexpr uint32_t halves_at(uint32_t t, uint32_t part) { return (t * 2 + part) * 16 * 4; }
-constexpr uint64_t halves_pieces(uint64_t units) { return units * (kHalvesUnit + 16 * 4 + 4); }
 
 __device__ __forceinline__ uint32_t pack(_Float16 a, _Float16 b)
 {
     return __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
 }
 
-// Column c of its group: a half wave's unit, lane i % 32 its (group, lane row).
+// Column c's unit, by a half wave: lane i % 32 holds its (group, lane row).
 template <bool Q4K>
-__device__ __forceinline__ void lay_out_halves(const QMatArgs &a, const float *x, uint32_t units, uint32_t unit, uint32_t i, uint32_t c, u4 *to)
+__device__ __forceinline__ void lay_out_halves(float v[8], uint32_t units, uint32_t unit, uint32_t i, uint32_t c, u4 *to)
 {
     const uint32_t t = i / 4, g = i % 4;
-    float v[8];
-    load_values<Q4K>(a, x, unit * 8 + t, g, v);
     const float down = scale_unit<14>(v);
-    u4 *sums = to + static_cast<uint64_t>(units) * kHalvesUnit;
+    u4 *sums = to + units * kHalvesUnit;
     if (i == 0) reinterpret_cast<float *>(sums + units * (16 * 4))[unit * 16 + c % 4 * 4 + c / 4] = down;
     if constexpr (Q4K) { // the group's sum over its four lanes, by 2^-6 within f16's range
         float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
@@ -236,7 +238,7 @@ __device__ __forceinline__ void lay_out_halves(const QMatArgs &a, const float *x
         hi[q] = pack(h0, h1);
         lo[q] = pack(static_cast<_Float16>(x0 - static_cast<float>(h0)), static_cast<_Float16>(x1 - static_cast<float>(h1)));
     }
-    u4 *at = to + static_cast<uint64_t>(unit) * kHalvesUnit + c * 4 + g;
+    u4 *at = to + unit * kHalvesUnit + c * 4 + g;
     at[halves_at(t, 0)] = hi;
     at[halves_at(t, 1)] = lo;
 }
@@ -474,12 +476,13 @@ __device__ __forceinline__ void digits_unit(const Raw<Q4K> &raw, const u2 *xs, c
 }
 
 struct QmPlan {
-    uint32_t units;    // of k
-    uint32_t tiles;    // of 16 rows
-    uint32_t kw;       // waves along k; the others take further tiles
-    uint32_t groups;   // of 16 columns
-    bool words;        // load_unit's
-    uint64_t x_pieces; // workspace pieces of a group (0: columns are digits in LDS)
+    uint32_t units;  // of k
+    uint32_t tiles;  // of 16 rows
+    uint32_t kw;     // digits: waves along k; the others take further tiles
+    bool words;      // load_unit's
+    uint32_t groups; // halves: of 16 columns
+    uint32_t chunks; // parts of k
+    uint32_t parts;  // workgroups of a chunk, each with a run of tiles
 };
 
 // A wave's share: units [u0, u1) of its rows.
@@ -574,125 +577,121 @@ __global__ __launch_bounds__(kQmBlock, 4) void k_qm_digits(QMatArgs a, QmPlan pl
     }
 }
 
-// Lays out the columns in the workspace, a unit of a column per half wave.
-template <bool Q4K>
-__global__ __launch_bounds__(kBlock) void k_qm_columns(QMatArgs a, QmPlan pl)
+// Up to 16 columns a workgroup, as halves.  NR: a quarter of them, rounded up.
+template <bool Q4K, int NR, bool WORDS>
+__global__ __launch_bounds__(kQmBlock, 4) void k_qm_halves(QMatArgs a, QmPlan pl)
 {
-    const uint64_t all = static_cast<uint64_t>(pl.units) * a.n, step = static_cast<uint64_t>(gridDim.x) * (kBlock / 32);
-    for (uint64_t e = static_cast<uint64_t>(blockIdx.x) * (kBlock / 32) + threadIdx.x / 32; e < all; e += step) {
-        const uint32_t col = static_cast<uint32_t>(e / pl.units), unit = static_cast<uint32_t>(e % pl.units);
-        lay_out_halves<Q4K>(a, a.x + static_cast<int64_t>(col) * a.x_st[1], pl.units, unit, threadIdx.x % 32, col % 16,
-                            static_cast<u4 *>(a.workspace) + (col / 16) * pl.x_pieces);
-    }
-}
-
-// Up to 16 columns a workgroup, as halves.  NR: a quarter of them, rounded up,
-// KW: waves along k.
-template <bool Q4K, int NR, int KW, bool WORDS>
-__global__ __launch_bounds__(kQmBlock, KW == 8 ? 2 : 4) void k_qm_halves(QMatArgs a, QmPlan pl)
-{
-    constexpr uint32_t kHalf = kHalvesUnit / 2; // pieces of a half unit: one a thread
-    static_assert(kHalf == kQmBlock, "a thread stages one piece of each half unit");
-    extern __shared__ u4 stage[]; // [2][KW][kHalf]
-    __shared__ float part[2][kQmWaves][NR][kWave];
+    constexpr int U = 2; // units in flight
+    extern __shared__ u4 pieces[];
     const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), j = lane % 16, g = lane / 16;
     const uint32_t c0 = blockIdx.y * 16, n = a.n - c0 < 16 ? a.n - c0 : 16;
-    const QmShare sh(a, pl, wave, Q4K);
-    const uint32_t steps = 2 * ((pl.units + KW - 1) / KW); // half units of the longest share
+    const uint32_t chunk = blockIdx.x / pl.parts, part = blockIdx.x - chunk * pl.parts;
+    const uint32_t u0 = static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * chunk / pl.chunks);
+    const uint32_t u1 = static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * (chunk + 1) / pl.chunks), units = u1 - u0;
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(pl.tiles) * (part + 1) / pl.parts);
+    uint32_t tile = static_cast<uint32_t>(static_cast<uint64_t>(pl.tiles) * part / pl.parts) + wave;
+    const uint32_t blocks = a.k / 32;
+    const uint64_t row_bytes = Q4K ? static_cast<uint64_t>(a.k / 256) * 144 : static_cast<uint64_t>(blocks) * 18;
     const unsigned char *w = static_cast<const unsigned char *>(a.w);
-    auto row_of = [&](uint32_t tile) {
-        const uint64_t at = (static_cast<uint64_t>(tile) + sh.wt) * 16 + j;
-        return w + (at < a.m ? at : a.m - 1) * sh.row_bytes;
+    auto row_of = [&](uint32_t t) { // past the last one, rows that are read and dropped
+        const uint64_t at = static_cast<uint64_t>(t) * 16 + j;
+        return w + (at < a.m ? at : a.m - 1) * row_bytes;
     };
+    // the first weights are on their way while the columns are laid out
+    const unsigned char *row = row_of(tile);
+    Raw<Q4K> raw[U];
+#pragma unroll
+    for (uint32_t i = 0; i < U; ++i)
+        if (i < units) load_unit<WORDS>(raw[i], row, u0 + i, g, blocks);
+    // a unit of a column per half wave, two at a time, so that their loads overlap
+    const uint32_t i32 = lane % 32, halves = 2 * kQmWaves;
+    for (uint32_t e0 = tid / 32; e0 < units * n; e0 += 2 * halves) {
+        float v[2][8];
+#pragma unroll
+        for (uint32_t b = 0; b < 2; ++b) {
+            const uint32_t e = e0 + b * halves, c = e / units, unit = e - c * units;
+            if (e < units * n) load_values<Q4K>(a, a.x + static_cast<int64_t>(c0 + c) * a.x_st[1], (u0 + unit) * 8 + i32 / 4, i32 % 4, v[b]);
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < 2; ++b) {
+            const uint32_t e = e0 + b * halves, c = e / units, unit = e - c * units;
+            if (e < units * n) lay_out_halves<Q4K>(v[b], units, unit, i32, c, pieces);
+        }
+    }
+    __syncthreads();
     // slot j of the instruction's 16 columns is column 4 (j % 4) + j / 4, so
     // that result i of lane row g is column 4 i + g; the slots past n repeat
     uint32_t c = (j % 4) * 4 + j / 4;
     c = c < n ? c : n - 1;
-    const u4 *x = static_cast<const u4 *>(a.workspace) + blockIdx.y * pl.x_pieces;
-    const u4 *sums = x + static_cast<uint64_t>(pl.units) * kHalvesUnit;
-    const v4f *scales = reinterpret_cast<const v4f *>(sums + pl.units * (16 * 4)) + g;
-    sums += c * 4 + g;
-    const bool used = tid % 64 / 4 < n; // pieces of columns that are there
-    u4 piece[KW];
-    auto fetch = [&](uint32_t step) {
-#pragma unroll
-        for (uint32_t k = 0; k < KW; ++k) {
-            const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * k / KW) * 2 + step;
-            if (used && first < static_cast<uint32_t>(static_cast<uint64_t>(pl.units) * (k + 1) / KW) * 2)
-                piece[k] = x[static_cast<uint64_t>(first) * kHalf + tid];
-        }
-    };
-    const uint32_t step_tiles = gridDim.x * sh.tw;
-    uint32_t tile = blockIdx.x * sh.tw;
-    const unsigned char *row = row_of(tile);
-    fetch(0);
-    Raw<Q4K> raw;
-    if (sh.u0 < sh.u1) load_unit<WORDS>(raw, row, sh.u0, g, sh.blocks);
-    uint32_t turn = 0, buf = 0;
+    const u4 *x = pieces + c * 4 + g, *sums = pieces + units * kHalvesUnit + c * 4 + g;
+    const v4f *scales = reinterpret_cast<const v4f *>(pieces + units * (kHalvesUnit + 16 * 4)) + g;
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (; tile < pl.tiles; tile += step_tiles, turn ^= 1) {
+    float *to = static_cast<float *>(a.workspace) + (static_cast<uint64_t>(blockIdx.y) * pl.chunks + chunk) * pl.tiles * (NR * kWave) + lane;
+    for (; tile < end; tile += kQmWaves) {
         float acc[NR];
         for (int i = 0; i < NR; ++i) acc[i] = 0.0f;
-        const unsigned char *next = row_of(tile + step_tiles);
-        for (uint32_t s = 0; s < steps; s += 2) {
-            const uint32_t u = sh.u0 + s / 2;
-            const bool live = u < sh.u1;
-            const Unit<Q4K> un(raw, u, g, sh.blocks); // of a share that has ended: not used
-            v4f scale = zero;
-            u4 sum = {0, 0, 0, 0};
-            if (live) {
-                scale = scales[u * 4];
-                if constexpr (Q4K) sum = sums[u * (16 * 4)];
-                if (u + 1 < sh.u1) load_unit<WORDS>(raw, row, u + 1, g, sh.blocks);
-                else load_unit<WORDS>(raw, next, sh.u0, g, sh.blocks);
-            }
-            float p[NR];
-            for (int i = 0; i < NR; ++i) p[i] = 0.0f;
+        const unsigned char *next = row_of(tile + kQmWaves);
+        for (uint32_t u = 0; u < units; u += U) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h, buf ^= 1) {
-                u4 *to = stage + buf * (KW * kHalf);
+            for (uint32_t i = 0; i < U; ++i) {
+                if (u + i < units) {
+                    const Unit<Q4K> un(raw[i], u0 + u + i, g, blocks);
+                    const u4 *xs = x + (u + i) * kHalvesUnit;
+                    float p[NR];
+                    for (int q = 0; q < NR; ++q) p[q] = 0.0f;
 #pragma unroll
-                for (uint32_t k = 0; k < KW; ++k) to[k * kHalf + tid] = piece[k];
-                fetch(s + h + 1 < steps ? s + h + 1 : 0); // of the next tile: the same again
-                __syncthreads();
-                const u4 *xs = to + wave % KW * kHalf + c * 4 + g;
-                if (live) {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const u4 hi = xs[halves_at(t, 0)], lo = xs[halves_at(t, 1)], q = un.halves(4 * h + t);
-                        const v4f r = mfma(hi, q, mfma(lo, q, zero));
-                        const float f = un.scale(4 * h + t);
-                        for (int i = 0; i < NR; ++i) p[i] = __builtin_fmaf(f, r[i], p[i]);
+                    for (int t = 0; t < 8; ++t) {
+                        const u4 q = un.halves(t);
+                        const v4f r = mfma(xs[halves_at(t, 0)], q, mfma(xs[halves_at(t, 1)], q, zero));
+                        const float f = un.scale(t);
+                        for (int k = 0; k < NR; ++k) p[k] = __builtin_fmaf(f, r[k], p[k]);
                     }
+                    if constexpr (Q4K) {
+                        const v4f r = mfma(sums[(u + i) * (16 * 4)], un.minima(), zero);
+                        for (int k = 0; k < NR; ++k) p[k] = __builtin_fmaf(un.d, p[k], (un.dmin * -64.0f) * r[k]);
+                    }
+                    const v4f scale = scales[(u + i) * 4];
+                    for (int k = 0; k < NR; ++k) acc[k] = __builtin_fmaf(scale[k], p[k], acc[k]);
                 }
-            }
-            if (live) {
-                if constexpr (Q4K) {
-                    const v4f r = mfma(sum, un.minima(), zero);
-                    for (int i = 0; i < NR; ++i) p[i] = __builtin_fmaf(un.d, p[i], (un.dmin * -64.0f) * r[i]);
-                }
-                for (int i = 0; i < NR; ++i) acc[i] = __builtin_fmaf(scale[i], p[i], acc[i]);
+                // the slot's next unit: of this tile, or of the next one
+                const bool more = u + i + U < units;
+                if (more || (u + U >= units && i < units))
+                    load_unit<WORDS>(raw[i], more ? row : next, u0 + (more ? u + i + U : i), g, blocks);
             }
         }
         row = next;
-        for (int i = 0; i < NR; ++i) part[turn][wave][i][lane] = acc[i];
-        __syncthreads();
-        for (uint32_t e = wave; e < sh.tw * NR; e += kQmWaves) { // a wave per tile and quarter of columns
-            const uint32_t t = e / NR, i = e % NR, col = 4 * i + g;
-            float v = 0.0f;
-            for (uint32_t k = 0; k < KW; ++k) v += part[turn][t * KW + k][i][lane];
-            const uint64_t r = (static_cast<uint64_t>(tile) + t) * 16 + j;
-            const bool live = r < a.m && col < n;
-            uint64_t odd = __ballot(live && !(__builtin_fabsf(v) < __builtin_inff()));
-            while (__builtin_expect(odd != 0, 0)) {
-                const int l = __builtin_ctzll(odd);
-                odd &= odd - 1;
-                const uint64_t rr = (static_cast<uint64_t>(tile) + t) * 16 + l % 16;
-                const float f = walk_row<Q4K>(w + rr * sh.row_bytes, a.x + static_cast<int64_t>(c0 + 4 * i + l / 16) * a.x_st[1], a.x_st[0], a.k);
-                if (lane == static_cast<uint32_t>(l)) v = f;
-            }
-            if (live) a.y[static_cast<int64_t>(r) * a.y_st[0] + static_cast<int64_t>(c0 + col) * a.y_st[1]] = v;
+        for (int i = 0; i < NR; ++i) to[static_cast<uint64_t>(tile) * (NR * kWave) + i * kWave] = acc[i];
+    }
+}
+
+// Adds up the chunks' parts, a wave per tile and quarter of columns.
+template <bool Q4K, int NR>
+__global__ __launch_bounds__(kBlock) void k_qm_sum(QMatArgs a, QmPlan pl)
+{
+    const uint32_t lane = threadIdx.x % kWave, j = lane % 16, g = lane / 16;
+    const uint64_t run = static_cast<uint64_t>(pl.tiles) * NR, all = run * pl.groups;
+    const uint64_t row_bytes = Q4K ? static_cast<uint64_t>(a.k / 256) * 144 : static_cast<uint64_t>(a.k / 32) * 18;
+    const unsigned char *w = static_cast<const unsigned char *>(a.w);
+    for (uint64_t e = static_cast<uint64_t>(blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave; e < all; e += static_cast<uint64_t>(gridDim.x) * (kBlock / kWave)) {
+        const uint64_t group = e / run, at = e - group * run, tile = at / NR;
+        const float *from = static_cast<const float *>(a.workspace) + (group * pl.chunks * run + at) * kWave + lane;
+        float v = 0.0f;
+        for (uint32_t k0 = 0; k0 < pl.chunks; k0 += 8) {
+            float p[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) p[k] = k0 + k < pl.chunks ? from[(k0 + k) * run * kWave] : 0.0f;
+            for (int k = 0; k < 8; ++k) v += p[k];
         }
+        const uint64_t r = tile * 16 + j, col = group * 16 + 4 * (at - tile * NR) + g;
+        const bool live = r < a.m && col < a.n;
+        uint64_t odd = __ballot(live && !(__builtin_fabsf(v) < __builtin_inff()));
+        while (__builtin_expect(odd != 0, 0)) {
+            const int l = __builtin_ctzll(odd);
+            odd &= odd - 1;
+            const float f = walk_row<Q4K>(w + (tile * 16 + l % 16) * row_bytes, a.x + static_cast<int64_t>(col - g + l / 16) * a.x_st[1], a.x_st[0], a.k);
+            if (lane == static_cast<uint32_t>(l)) v = f;
+        }
+        if (live) a.y[static_cast<int64_t>(r) * a.y_st[0] + static_cast<int64_t>(col) * a.y_st[1]] = v;
     }
 }
 
@@ -716,18 +715,32 @@ int qm_digits(const QMatArgs &a, uint32_t units)
 
 QmPlan qm_plan(const QMatArgs &a)
 {
-    QmPlan pl;
+    QmPlan pl{};
     pl.units = (a.k + kQmUnit - 1) / kQmUnit;
     pl.tiles = static_cast<uint32_t>((static_cast<uint64_t>(a.m) + 15) / 16);
     pl.kw = pl.units >= 8 ? 8 : pl.units >= 4 ? 4 : pl.units >= 2 ? 2 : 1;
-    pl.groups = (a.n + 15) / 16;
     pl.words = reinterpret_cast<uintptr_t>(a.w) % 4 == 0 && a.k % 64 == 0;
-    pl.x_pieces = qm_digits(a, pl.units) ? 0 : halves_pieces(pl.units);
-    // halves: four waves along k share their stage with a second tile; eight
-    // where that leaves compute units idle
-    if (pl.x_pieces) pl.kw = static_cast<uint64_t>(pl.tiles) * pl.groups <= 2 * qm_cus() ? 8 : 4;
+    pl.groups = (a.n + 15) / 16;
+    // Halves, by sets of a tile a wave and chunk.  Four units (68 KB, two
+    // workgroups a compute unit) write the fewest parts: 5 columns of
+    // 4096x151936 99 us, 103 with two units.  Fewer sets go in chunks of two
+    // units, to a workgroup a compute unit: 15 columns of 4096x11008 15.5 us, 16.3
+    // with two workgroups, 17.3 with four units; and of one unit where those
+    // leave compute units idle: 12 columns of 1024x2000 7.4 us, 8.3 with two units.
+    const uint64_t sets = (static_cast<uint64_t>(pl.tiles) + kQmWaves - 1) / kQmWaves;
+    auto work = [&](uint32_t chunk) { return sets * pl.groups * ((pl.units + chunk - 1) / chunk); };
+    const bool large = work(4) >= 4 * qm_cus();
+    const uint32_t chunk = large ? 4 : work(2) >= qm_cus() ? 2 : 1;
+    pl.chunks = (pl.units + chunk - 1) / chunk;
+    uint64_t parts = (large ? 2 : 1) * qm_cus() / (static_cast<uint64_t>(pl.chunks) * pl.groups);
+    // In eights, a row's chunks run on one of the eight XCDs, whose L2 holds
+    // the lines that two chunks share.
+    if (parts > 8) parts = parts / 8 * 8;
+    pl.parts = static_cast<uint32_t>(parts < 1 ? 1 : parts < sets ? parts : sets);
     return pl;
 }
+
+uint32_t qm_quarter(const QMatArgs &a) { return a.n > 12 ? 4 : (a.n + 3) / 4; }
 
 // Workgroups for tiles taken `per` at a time: even shares of what runs at once.
 uint32_t qm_grid(const QmPlan &pl, uint32_t per)
@@ -744,26 +757,15 @@ void qm_run_digits(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
     else k_qm_digits<Q4K, N, false><<<grid, kQmBlock, lds, stream>>>(a, pl);
 }
 
-template <bool Q4K, int NR, int KW>
+template <bool Q4K, int NR>
 void qm_run_halves(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 {
-    const uint64_t wgs = (static_cast<uint64_t>(pl.units) * a.n + kBlock / 32 - 1) / (kBlock / 32);
-    k_qm_columns<Q4K><<<static_cast<uint32_t>(wgs < 65536 ? wgs : 65536), kBlock, 0, stream>>>(a, pl);
-    const dim3 grid(qm_grid(pl, kQmWaves / KW), pl.groups);
-    constexpr uint32_t lds = 2 * KW * kHalvesUnit / 2 * 16;
-    if (pl.words) k_qm_halves<Q4K, NR, KW, true><<<grid, kQmBlock, lds, stream>>>(a, pl);
-    else k_qm_halves<Q4K, NR, KW, false><<<grid, kQmBlock, lds, stream>>>(a, pl);
-}
-
-template <bool Q4K, int KW>
-void qm_run_halves(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
-{
-    switch ((a.n + 3) / 4) {
-    case 1: return qm_run_halves<Q4K, 1, KW>(a, pl, stream);
-    case 2: return qm_run_halves<Q4K, 2, KW>(a, pl, stream);
-    case 3: return qm_run_halves<Q4K, 3, KW>(a, pl, stream);
-    default: return qm_run_halves<Q4K, 4, KW>(a, pl, stream);
-    }
+    const dim3 grid(pl.chunks * pl.parts, pl.groups);
+    const uint32_t lds = (pl.units + pl.chunks - 1) / pl.chunks * kHalvesBytes;
+    if (pl.words) k_qm_halves<Q4K, NR, true><<<grid, kQmBlock, lds, stream>>>(a, pl);
+    else k_qm_halves<Q4K, NR, false><<<grid, kQmBlock, lds, stream>>>(a, pl);
+    const uint64_t sums = (static_cast<uint64_t>(pl.tiles) * NR * pl.groups + kBlock / kWave - 1) / (kBlock / kWave);
+    k_qm_sum<Q4K, NR><<<static_cast<uint32_t>(sums < 65536 ? sums : 65536), kBlock, 0, stream>>>(a, pl);
 }
 
 template <bool Q4K>
@@ -775,37 +777,64 @@ void qm_run(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
     case 3: return qm_run_digits<Q4K, 3>(a, pl, stream);
     case 4: return qm_run_digits<Q4K, 4>(a, pl, stream);
     }
-    if (pl.kw == 8) qm_run_halves<Q4K, 8>(a, pl, stream);
-    else qm_run_halves<Q4K, 4>(a, pl, stream);
+    switch (qm_quarter(a)) {
+    case 1: return qm_run_halves<Q4K, 1>(a, pl, stream);
+    case 2: return qm_run_halves<Q4K, 2>(a, pl, stream);
+    case 3: return qm_run_halves<Q4K, 3>(a, pl, stream);
+    default: return qm_run_halves<Q4K, 4>(a, pl, stream);
+    }
+}
+
+// Products run in parts of columns and rows whose partial sums take about 256 MB of
+// workspace at most: kilobytes, by tile, 16 columns and chunk of k.
+constexpr uint64_t kQmPartials = 1u << 18;
+
+struct QmPart {
+    uint32_t rows, columns;
+};
+QmPart qm_part(const QMatArgs &a)
+{
+    const QmPlan pl = qm_plan(a);
+    if (qm_digits(a, pl.units)) return {a.m, a.n};
+    const uint64_t all = static_cast<uint64_t>(pl.chunks) * pl.tiles;
+    uint64_t groups = all * pl.groups <= kQmPartials ? pl.groups : all < kQmPartials ? kQmPartials / all : 1;
+    if (groups > 4096) groups = 4096; // within a grid's second axis
+    const uint64_t tiles = all * groups <= kQmPartials ? pl.tiles : pl.chunks * kQmWaves < kQmPartials ? kQmPartials / pl.chunks : kQmWaves;
+    const uint64_t rows = tiles * 16, columns = groups * 16;
+    return {static_cast<uint32_t>(rows < a.m ? rows : a.m), static_cast<uint32_t>(columns < a.n ? columns : a.n)};
 }
 
 } // namespace
 
-// Columns that are laid out and launched at a time: the workspace stays at
-// 68 bytes a value of k for each 16 of these, and the grid's second axis
-// within what a launch takes (65535 groups).
-constexpr uint32_t kQmColumns = 1u << 14;
-
 uint64_t quant_mat_workspace_bytes(const QMatArgs &a)
 {
+    const QmPart part = qm_part(a);
     QMatArgs b = a;
-    b.n = a.n < kQmColumns ? a.n : kQmColumns;
+    b.m = part.rows;
+    b.n = part.columns;
     const QmPlan pl = qm_plan(b);
-    return pl.groups * pl.x_pieces * 16;
+    if (qm_digits(b, pl.units)) return 0;
+    return static_cast<uint64_t>(pl.chunks) * pl.tiles * pl.groups * qm_quarter(b) * kWave * sizeof(float);
 }
 
 hipError_t launch_quant_mat(const QMatArgs &a, hipStream_t stream)
 {
+    const QmPart part = qm_part(a);
+    const uint64_t row_bytes = static_cast<uint64_t>(a.k) / (a.q4k ? 256 : 32) * (a.q4k ? 144 : 18);
     QMatArgs b = a;
-    for (uint64_t c = 0; c < a.n; c += kQmColumns) {
-        b.n = static_cast<uint32_t>(a.n - c < kQmColumns ? a.n - c : kQmColumns);
-        b.x = a.x + static_cast<int64_t>(c) * a.x_st[1];
-        b.y = a.y + static_cast<int64_t>(c) * a.y_st[1];
-        const QmPlan pl = qm_plan(b);
-        if (a.q4k) qm_run<true>(b, pl, stream);
-        else qm_run<false>(b, pl, stream);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+    for (uint64_t r = 0; r < a.m; r += part.rows) {
+        b.m = static_cast<uint32_t>(a.m - r < part.rows ? a.m - r : part.rows);
+        b.w = static_cast<const unsigned char *>(a.w) + r * row_bytes;
+        for (uint64_t c = 0; c < a.n; c += part.columns) {
+            b.n = static_cast<uint32_t>(a.n - c < part.columns ? a.n - c : part.columns);
+            b.x = a.x + static_cast<int64_t>(c) * a.x_st[1];
+            b.y = a.y + static_cast<int64_t>(r) * a.y_st[0] + static_cast<int64_t>(c) * a.y_st[1];
+            const QmPlan pl = qm_plan(b);
+            if (b.q4k) qm_run<true>(b, pl, stream);
+            else qm_run<false>(b, pl, stream);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
     }
     return hipSuccess;
 }

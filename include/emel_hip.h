@@ -512,8 +512,8 @@ emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_
  * Products are exact, sums are f32, in an order that depends on the sizes
  * alone; infinities and NaN go through as in the formula.  More than four
  * columns, or a k whose columns do not fit LDS as digits (past 17152 for one column, 4096
- * for four), want the stream's workspace, which grows as the reductions'
- * does: graphs captured from one stream share it, and run one after the
+ * for four), want the stream's workspace (partial sums, up to about 256 MB),
+ * which grows as the reductions' does: graphs captured from one stream share it, and run one after the
  * other, or are captured from streams of their own.  Guards: a NULL view or
  * data, or an unaligned F32 pointer, is INVALID_ARGUMENT; a view that fails its
  * rules, or an overlap, INVALID_VIEW; extents that do not match,

@@ -27,18 +27,29 @@ def product(rec, k, m, n, q4k=False, nb=None):
 @pytest.mark.parametrize("n,fits", [(1, 17152), (2, 8448), (3, 5632), (4, 4096)])
 def test_up_to_four_columns_are_digits_where_they_fit(rec, q4k, n, fits):
     assert kernels(product(rec, fits, 4096, n, q4k)) == ["k_qm_digits"]
-    assert kernels(product(rec, fits + 256, 4096, n, q4k)) == ["k_qm_columns", "k_qm_halves"]
-    assert kernels(product(rec, 256, 4096, n + 4, q4k)) == ["k_qm_columns", "k_qm_halves"]
+    assert kernels(product(rec, fits + 256, 4096, n, q4k)) == ["k_qm_halves", "k_qm_sum"]
+    assert kernels(product(rec, 256, 4096, n + 4, q4k)) == ["k_qm_halves", "k_qm_sum"]
 
 
-@pytest.mark.parametrize("n,launches", [(1 << 14, 1), ((1 << 14) + 5, 2), (1 << 21, 128)])
-def test_many_columns_run_in_parts(rec, n, launches):
-    got = product(rec, 64, 33, n)
-    assert kernels(got) == ["k_qm_columns", "k_qm_halves"] * launches
+@pytest.mark.parametrize("k,m,n,launches", [
+    (64, 33, 1 << 16, 1), (64, 33, (1 << 16) + 5, 2), (64, 33, 1 << 21, 32),  # columns, by a grid's second axis
+    (4096, 11008, 64, 1), (4096, 11008, 2000, 2), (4096, 151936, 64, 1), (4096, 151936, 102, 2),  # by the partial sums' 256 MB
+    (32, 1 << 22, 16, 1), (32, (1 << 22) + 1, 16, 2), (11008, 1 << 22, 32, 24), (1 << 26, 300, 5, 3)])  # rows
+def test_large_products_run_in_parts(rec, k, m, n, launches):
+    assert kernels(product(rec, k, m, n)) == ["k_qm_halves", "k_qm_sum"] * launches
 
 
 def test_columns_left_over_are_digits(rec):
-    assert kernels(product(rec, 64, 33, (1 << 14) + 2)) == ["k_qm_columns", "k_qm_halves", "k_qm_digits"]
+    assert kernels(product(rec, 64, 33, (1 << 16) + 2)) == ["k_qm_halves", "k_qm_sum", "k_qm_digits"]
+
+
+@pytest.mark.parametrize("k,m,n,lds,grid", [
+    (4096, 151936, 5, 4, 4 * 128), (4096, 40000, 16, 4, 4 * 128),  # four units a chunk, two workgroups a compute unit
+    (4096, 11008, 15, 2, 8 * 32), (4096, 4096, 8, 2, 8 * 32),       # two, and one
+    (1024, 2000, 12, 1, 4 * 16), (256, 16, 5, 1, 1)])               # where that leaves compute units idle
+def test_chunks_of_many_columns(rec, k, m, n, lds, grid):
+    halves = product(rec, k, m, n)[0]
+    assert (halves.lds, halves.grid) == (lds * 17472, grid)
 
 
 @pytest.mark.parametrize("dim,strided", [(64, False), (60, False), (64, True)])

@@ -120,7 +120,7 @@ def test_product_of_values_near_the_smallest(gpu, form, n):
 
 
 def test_product_of_more_columns_than_a_launch_takes(gpu):
-    """Columns run in parts of 2^14; more than 65535 groups of 16 of them would not fit a grid."""
+    """Columns run in parts; more than 65535 groups of 16 of them would not fit a grid."""
     import torch
 
     k, m, n = 32, 5, (1 << 20) + 3
@@ -130,6 +130,23 @@ def test_product_of_more_columns_than_a_launch_takes(gpu):
     run(EVENT["q4_0"](packed(torch.from_numpy(rows).to(gpu), "q4_0", k, m), view(x), out(y)))
     want, tol = product("q4_0", rows, x.cpu().numpy())
     within(y.cpu().numpy(), want, tol, "columns")
+
+
+def test_product_of_more_rows_than_a_launch_takes(gpu):
+    """Rows run in parts of 2^22 where k is short; the rows on both sides of the cut, the ends and some between."""
+    import torch
+
+    k, m, n = 32, (1 << 22) + 37, 5
+    some = packed_rows(4, "q4_0", k, 4096)
+    pick = np.arange(m) % 4093
+    rows = torch.from_numpy(some).to(gpu)[torch.from_numpy(pick).to(gpu)].contiguous()
+    x = rng(6).standard_normal((n, k)).astype(np.float32)
+    y = torch.empty(n, m, device=gpu)
+    run(EVENT["q4_0"](packed(rows, "q4_0", k, m), view(torch.from_numpy(x).to(gpu)), out(y)))
+    want, tol = product("q4_0", some, x)
+    got = y.cpu().numpy()
+    for a, b in ((0, 5000), ((1 << 21) - 7, (1 << 21) + 300), ((1 << 22) - 300, m)):
+        within(got[:, a:b], want[:, pick[a:b]], tol[:, pick[a:b]], f"rows {a}")
 
 
 @pytest.mark.parametrize("form", ["q4_0", "q4_k"])
