@@ -8,7 +8,7 @@
 // token there, in LDS (integer atomics: the result does not depend on their
 // order), then passes over the run once.  Both fit one word a token where there
 // are fewer than 2^16 of either, which leaves a compute unit eight workgroups
-// instead of four (64 rows of 151936 with a history of 2048 and a mask: 21.0 us against 27.2).  Each of a row's runs reads the whole
+// instead of four (64 rows of 151936 with a history of 2048 and a mask: 21.0 us, 3.8 TB/s, against 27.2).  Each of a row's runs reads the whole
 // history and all its biases: a few KB from the L2 for 16 KB of logits.  Runs
 // start at 16-byte boundaries of the output, wherever its rows start.
 #include "common.hpp"

@@ -10,7 +10,7 @@
 // nibbles as integers, and the group's scale goes once into its result.  x is
 // f32 and is not to lose by it; two ways, by the number of columns:
 //
-// k_qm_digits, up to four columns.  Each column's run of 256 values is a
+// k_qm_digits, up to four columns where they fit LDS.  Each column's run of 256 values is a
 // fixed-point number of 30 bits and a sign, scaled by a power of two to its largest
 // value, and cut into four signed bytes.  The 16 columns of the 8-bit
 // instruction then hold 4 digits x 4 columns, and one instruction a group does
@@ -19,8 +19,10 @@
 // a column.  A value is off by 2^-30 of the largest of its 256 at most (by 2^-127
 // where that is below 2^-97: the scale stays a normal number): less
 // than f32's own rounding of the sum that the largest is part of.
+// One column of 4096x4096 5.3 us (a launch, the layout, one round of loads),
+// three of 4096x151936 78 us: 4.5 TB/s.
 //
-// k_qm_halves, more columns.  Each column's run of 256 values goes in as two
+// k_qm_halves, all others.  Each column's run of 256 values goes in as two
 // halves each, hi + lo, scaled by a power of two that brings its largest value to
 // [2^14, 2^15): 22 bits of every value down to 2^-16 of that, and 2^-40 of it
 // below.  The 16 columns of the f16 instruction are 16 columns, two
@@ -59,7 +61,7 @@ namespace {
 constexpr int kQmWaves = 8;
 constexpr int kQmBlock = kQmWaves * kWave;
 constexpr uint32_t kQmUnit = 256;      // values that a wave takes of a row at a time: eight groups
-constexpr uint32_t kQmLds = 70 * 1024; // of laid-out columns: two workgroups fit a compute unit
+constexpr uint32_t kQmLds = 80 * 1024, kQmLdsAlone = 110 * 1024; // of a workgroup: two fit a compute unit, or one
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -706,11 +708,19 @@ uint32_t qm_cus()
     return cus;
 }
 
-// Columns that are laid out as digits: up to four where they fit; 0: as halves.
-int qm_digits(const QMatArgs &a, uint32_t units)
+// Columns that are laid out as digits: up to four whose digits and waves' sums
+// let two workgroups share a compute unit, or one where there is no more than a
+// tile to each; 0: as halves.  Every workgroup lays out all of k: 4 columns of
+// 4096x4096 7.9 us against 9.4 as halves, of 4096x11008 18.7 (a workgroup a
+// compute unit) against 13.1; 2 columns of 11008x4096 (97 KB) 11.3 against 15.0, 4 of
+// 8192x4096 (149 KB) 12.3 against 11.9, of 8192x1024 11.2 against 8.9.
+int qm_digits(const QMatArgs &a)
 {
+    if (a.n > 4) return 0;
+    const uint64_t units = (static_cast<uint64_t>(a.k) + kQmUnit - 1) / kQmUnit;
     const uint64_t bytes[] = {Digits<1>::bytes(units), Digits<2>::bytes(units), Digits<3>::bytes(units), Digits<4>::bytes(units)};
-    return a.n <= 4 && bytes[a.n - 1] <= kQmLds ? static_cast<int>(a.n) : 0;
+    const uint64_t lds = bytes[a.n - 1] + a.n * (2 * kQmBlock * sizeof(float));
+    return lds <= kQmLds || (lds <= kQmLdsAlone && a.m <= 16 * qm_cus()) ? static_cast<int>(a.n) : 0;
 }
 
 QmPlan qm_plan(const QMatArgs &a)
@@ -771,7 +781,7 @@ void qm_run_halves(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 template <bool Q4K>
 void qm_run(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
 {
-    switch (qm_digits(a, pl.units)) {
+    switch (qm_digits(a)) {
     case 1: return qm_run_digits<Q4K, 1>(a, pl, stream);
     case 2: return qm_run_digits<Q4K, 2>(a, pl, stream);
     case 3: return qm_run_digits<Q4K, 3>(a, pl, stream);
@@ -795,7 +805,7 @@ struct QmPart {
 QmPart qm_part(const QMatArgs &a)
 {
     const QmPlan pl = qm_plan(a);
-    if (qm_digits(a, pl.units)) return {a.m, a.n};
+    if (qm_digits(a)) return {a.m, a.n};
     const uint64_t all = static_cast<uint64_t>(pl.chunks) * pl.tiles;
     uint64_t groups = all * pl.groups <= kQmPartials ? pl.groups : all < kQmPartials ? kQmPartials / all : 1;
     if (groups > 4096) groups = 4096; // within a grid's second axis
@@ -809,12 +819,18 @@ QmPart qm_part(const QMatArgs &a)
 uint64_t quant_mat_workspace_bytes(const QMatArgs &a)
 {
     const QmPart part = qm_part(a);
-    QMatArgs b = a;
-    b.m = part.rows;
-    b.n = part.columns;
-    const QmPlan pl = qm_plan(b);
-    if (qm_digits(b, pl.units)) return 0;
-    return static_cast<uint64_t>(pl.chunks) * pl.tiles * pl.groups * qm_quarter(b) * kWave * sizeof(float);
+    uint64_t most = 0;
+    for (const uint32_t m : {part.rows, a.m % part.rows}) // whole parts and what is left of them
+        for (const uint32_t n : {part.columns, a.n % part.columns}) {
+            QMatArgs b = a;
+            b.m = m;
+            b.n = n;
+            if (m == 0 || n == 0 || qm_digits(b)) continue;
+            const QmPlan pl = qm_plan(b);
+            const uint64_t bytes = static_cast<uint64_t>(pl.chunks) * pl.tiles * pl.groups * qm_quarter(b) * kWave * sizeof(float);
+            most = bytes > most ? bytes : most;
+        }
+    return most;
 }
 
 hipError_t launch_quant_mat(const QMatArgs &a, hipStream_t stream)

@@ -506,15 +506,15 @@ emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_
  * [k, n, 1, 1], dst F32 [m, n, 1, 1]; x and dst may have any strides, dst's
  * elements disjoint and apart from both sources.  W[r, k] is the value that
  * get_rows gives: (q - 8) d for Q4_0, d sc q - dmin m for Q4_K.  x is read in
- * runs of 256 values along k, to 2^-30 of a run's largest value (to 2^-127
- * where that is below 2^-97) for up to four columns, else to 22 bits of each value
+ * runs of 256 values along k: up to four columns to 2^-30 of a run's largest
+ * value (to 2^-127 where that is below 2^-97), more columns, or a k whose columns
+ * do not fit LDS (past 18688 for one column, 3840 for four), to 22 bits of each value
  * down to 2^-16 of the run's largest and to 2^-40 of the largest below.
  * Products are exact, sums are f32, in an order that depends on the sizes
- * alone; infinities and NaN go through as in the formula.  More than four
- * columns, or a k whose columns do not fit LDS as digits (past 17152 for one column, 4096
- * for four), want the stream's workspace (partial sums, up to about 256 MB),
- * which grows as the reductions' does: graphs captured from one stream share it, and run one after the
- * other, or are captured from streams of their own.  Guards: a NULL view or
+ * alone; infinities and NaN go through as in the formula.  The second form
+ * wants the stream's workspace (partial sums, up to about 256 MB), which grows as
+ * the reductions' does: graphs captured from one stream share it, and run
+ * one after the other, or are captured from streams of their own.  Guards: a NULL view or
  * data, or an unaligned F32 pointer, is INVALID_ARGUMENT; a view that fails its
  * rules, or an overlap, INVALID_VIEW; extents that do not match,
  * SHAPE_MISMATCH; an extent past 2^31 - 1 or a k past 2^26,

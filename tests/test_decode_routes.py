@@ -24,11 +24,13 @@ def product(rec, k, m, n, q4k=False, nb=None):
 
 
 @pytest.mark.parametrize("q4k", [False, True])
-@pytest.mark.parametrize("n,fits", [(1, 17152), (2, 8448), (3, 5632), (4, 4096)])
-def test_up_to_four_columns_are_digits_where_they_fit(rec, q4k, n, fits):
-    assert kernels(product(rec, fits, 4096, n, q4k)) == ["k_qm_digits"]
-    assert kernels(product(rec, fits + 256, 4096, n, q4k)) == ["k_qm_halves", "k_qm_sum"]
-    assert kernels(product(rec, 256, 4096, n + 4, q4k)) == ["k_qm_halves", "k_qm_sum"]
+@pytest.mark.parametrize("n,fits,alone", [(1, 18688, 26112), (2, 8704, 12544), (3, 5376, 7936), (4, 3840, 5632)])
+def test_up_to_four_columns_are_digits_where_they_fit(rec, q4k, n, fits, alone):
+    digits, halves = ["k_qm_digits"], ["k_qm_halves", "k_qm_sum"]
+    for m, k in ((11008, fits), (4096, alone)):  # two workgroups a compute unit, or one with a tile to each
+        assert kernels(product(rec, k, m, n, q4k)) == digits
+        assert kernels(product(rec, k + 256, m, n, q4k)) == halves
+    assert kernels(product(rec, 256, 4096, n + 4, q4k)) == halves
 
 
 @pytest.mark.parametrize("k,m,n,launches", [
