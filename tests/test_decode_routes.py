@@ -80,6 +80,7 @@ def test_attention_with_more_units_than_are_counted_runs_in_parts(rec):
     # 2^22 tokens at most: 2^15 + 1 units a sequence and cache head
     assert len(attention(rec, 32000, 1 << 18)) == 1
     assert len(attention(rec, 33000, 1 << 18)) == 2
+    assert len(attention(rec, 1100, 1 << 14, page=256, kv=64, heads=64, dim=8)) == 2
     assert len(attention(rec, 70, (1 << 27) - 1, kv=127, heads=127)) == 70
     with pytest.raises(RuntimeError, match="UNSUPPORTED_OPERATION"):
         attention(rec, 1, (1 << 27) - 1, kv=128, heads=128)

@@ -374,6 +374,44 @@ def test_attention_refuses_to_read_outside_the_pool(gpu):
     check_attention(c, skip=range(5))
 
 
+def test_cache_past_32_bit_offsets(gpu):
+    """Pools of more than 2^32 halves: tokens appended to their first and last pages, and attention over those."""
+    import torch
+
+    kv, page, dim, tokens = 4, 64, 128, 300
+    pages = (1 << 17) + 9  # of 2^15 halves
+    kp, vp = (torch.empty(pages, kv, page, dim, dtype=torch.float16, device=gpu) for _ in range(2))
+    assert kp.numel() > 1 << 32
+    table = torch.tensor([[0, pages - 1, 1, pages - 2, pages // 2], [pages - 5, 2, pages - 4, pages - 3, pages - 6]], dtype=torch.int32, device=gpu)
+    q = torch.from_numpy(rng(70).standard_normal((2, 8, dim)).astype(np.float32)).to(gpu)
+    c = {"q": q, "kp": kp, "vp": vp, "table": table, "lengths": torch.tensor([tokens, tokens - 7], dtype=torch.int32, device=gpu), "y": torch.empty_like(q)}
+    at = torch.arange(tokens, device=gpu)
+    for s in range(2):
+        k, v = (torch.from_numpy(rng(71 + 2 * s + i).standard_normal((tokens, kv, dim)).astype(np.float32)).to(gpu) for i in range(2))
+        slots = (table[s][at // page] * page + at % page).to(torch.int32)
+        run(eh.OpPagedKvAppend(view(k), view(v), view(slots), out(kp), out(vp)))
+        where = table[s].long()[at // page]
+        assert torch.equal(kp[where, :, at % page], k.half()) and torch.equal(vp[where, :, at % page], v.half())
+    run(attend_event(c))
+    check_attention(c)
+
+
+def test_attention_in_parts_of_a_batch(gpu):
+    """A table so wide that its units, counted before the lengths are known, pass 2^31: the batch runs in parts."""
+    import torch
+
+    seqs, heads = 1100, 64
+    few = attend_case(gpu, False, heads, heads, 8, 256, [int(n) for n in rng(81).integers(0, 500, 40)], "head", 80)
+    at = torch.arange(seqs, device=gpu) * 7 % 40
+    table = torch.full((seqs, 1 << 14), -1, dtype=torch.int32, device=gpu)
+    table[:, :few["table"].shape[1]] = few["table"][at]
+    q = torch.from_numpy(rng(82).standard_normal((seqs, heads, 8)).astype(np.float32)).to(gpu)
+    c = {**few, "q": q, "table": table, "lengths": few["lengths"][at].contiguous(), "y": torch.full_like(q, 5.0)}
+    run(attend_event(c))
+    check_attention(c, skip=set(range(seqs)) - {*range(0, 60), *range(1000, 1100)})
+    assert c["y"].isfinite().all() and not (c["y"] == 5.0).any()
+
+
 @pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (3, 1, 40)])
 def test_attention_strides(gpu, heads, kv, dim):
     """q and dst with heads and dims in other orders, the index tensors by columns, pools that start at any half."""
