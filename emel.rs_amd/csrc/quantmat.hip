@@ -744,7 +744,8 @@ QmPlan qm_plan(const QMatArgs &a)
     pl.chunks = (pl.units + chunk - 1) / chunk;
     uint64_t parts = (large ? 2 : 1) * qm_cus() / (static_cast<uint64_t>(pl.chunks) * pl.groups);
     // In eights, a row's chunks run on one of the eight XCDs, whose L2 holds
-    // the lines that two chunks share.
+    // the lines that two chunks share (15 columns of 4096x11008 in 88 parts
+    // 17.1 us, in 86 18.5).
     if (parts > 8) parts = parts / 8 * 8;
     pl.parts = static_cast<uint32_t>(parts < 1 ? 1 : parts < sets ? parts : sets);
     return pl;

@@ -50,6 +50,17 @@ def test_product_matches_the_formula(gpu, form, k, m, n):
 
 
 @pytest.mark.parametrize("form", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("k,m,n", [(18688, 4112, 1), (18944, 4112, 1), (26112, 20, 1), (26368, 20, 1), (12544, 33, 2), (12800, 33, 2), (5632, 20, 4), (5888, 20, 4), (32768, 50, 7)])
+def test_product_at_the_limits_of_its_lds(gpu, form, k, m, n):
+    import torch
+
+    rows, x = inputs(k + m, form, k, m, n)
+    y = torch.empty(n, m, device=gpu)
+    run(EVENT[form](packed(torch.from_numpy(rows).to(gpu), form, k, m), view(torch.from_numpy(x).to(gpu)), out(y)))
+    within(y.cpu().numpy(), *product(form, rows, x), f"{k} {m} {n}")
+
+
+@pytest.mark.parametrize("form", ["q4_0", "q4_k"])
 @pytest.mark.parametrize("m,n", [(40000, 1), (40000, 3), (9000, 16), (5000, 64)])
 def test_product_of_many_rows(gpu, form, m, n):
     import torch
