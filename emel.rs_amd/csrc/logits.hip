@@ -2,14 +2,17 @@
 // rows of logits, ahead of the sampler.
 //
 // Bound by one read and one write of the logits; what goes with them is
-// sparse.  A workgroup takes a run of kLaTokens tokens of one row, 16 a
-// thread, whose logits it loads first.  While they are on their way it counts
+// sparse.  A workgroup takes a run of 4096 tokens of one row, 16 a
+// thread, whose logits it loads first, or of 1024, 4 a thread, where all
+// of those run at once: up to kLaFew logits, what counts is the chain of a run's
+// loads, and shorter runs clear and walk fewer cells (one row of 151936 4.1 us
+// against 5.8, eight 7.2 against 9.3, sixteen 10.9 against 10.1).  While they are on their way it counts
 // the row's history ids that fall in its run, and the last bias entry of each
 // token there, in LDS (integer atomics: the result does not depend on their
 // order), then passes over the run once.  Both fit one word a token where there
 // are fewer than 2^16 of either, which leaves a compute unit eight workgroups
 // instead of four (64 rows of 151936 with a history of 2048 and a mask: 21.0 us, 3.8 TB/s, against 27.2).  Each of a row's runs reads the whole
-// history and all its biases: a few KB from the L2 for 16 KB of logits.  Runs
+// history and all its biases: a few KB from the L2 for 4 or 16 KB of logits.  Runs
 // start at 16-byte boundaries of the output, wherever its rows start.
 #include "common.hpp"
 #include "launch.hpp"
@@ -17,8 +20,8 @@
 namespace emel {
 namespace {
 
-constexpr uint32_t kLaTokens = 4096;
-constexpr uint32_t kLaQuads = kLaTokens / 4 / kBlock; // float4 per thread
+constexpr uint64_t kLaFew = 1u << 21; // 1024 tokens for each of eight workgroups on 256 compute units
+constexpr uint32_t la_tokens(uint32_t quads) { return quads * 4 * kBlock; }
 
 __device__ __forceinline__ float row_value(const RowTable &t, uint32_t row, float none)
 {
@@ -28,9 +31,11 @@ __device__ __forceinline__ float row_value(const RowTable &t, uint32_t row, floa
 // PACKED: count in the low half of a word, entry in the high half.
 // VEC: both rows have unit stride and the same place in a 16-byte line.
 // INPLACE: only tokens that change are read and written.
-template <bool PACKED, bool VEC, bool INPLACE>
+// Q: float4 a thread.
+template <uint32_t Q, bool PACKED, bool VEC, bool INPLACE>
 __global__ __launch_bounds__(kBlock) void k_la_adjust(LogitsAdjustArgs a, uint32_t runs, uint64_t items)
 {
+    constexpr uint32_t kLaTokens = la_tokens(Q);
     __shared__ __attribute__((aligned(16))) uint32_t count[kLaTokens];
     __shared__ __attribute__((aligned(16))) uint32_t entry[PACKED ? 4 : kLaTokens]; // 1 + the last bias entry
     __shared__ uint32_t words[kLaTokens / 32 + 2];
@@ -42,17 +47,17 @@ __global__ __launch_bounds__(kBlock) void k_la_adjust(LogitsAdjustArgs a, uint32
         const int64_t shift = VEC ? (reinterpret_cast<uintptr_t>(y) / 4) % 4 : 0;
         const int64_t t0 = static_cast<int64_t>(it % runs) * kLaTokens - shift, card = a.card; // t0 + i is token of cell i
         if (t0 >= card) continue; // a run that only other rows have
-        float4 v[kLaQuads];
+        float4 v[Q];
         auto cell = [&](uint32_t q) { return 4 * (tid + q * kBlock); };
         auto whole = [&](uint32_t q) { return t0 + cell(q) >= 0 && t0 + cell(q) + 3 < card; };
         if constexpr (VEC && !INPLACE) {
 #pragma unroll
-            for (uint32_t q = 0; q < kLaQuads; ++q)
+            for (uint32_t q = 0; q < Q; ++q)
                 if (whole(q)) v[q] = ld_nt(reinterpret_cast<const float4 *>(x + t0 + cell(q)));
         }
         __syncthreads(); // the cells of the run before
         const uint4 none = make_uint4(0, 0, 0, 0);
-        for (uint32_t q = 0; q < kLaQuads; ++q) {
+        for (uint32_t q = 0; q < Q; ++q) {
             *reinterpret_cast<uint4 *>(count + cell(q)) = none;
             if constexpr (!PACKED) *reinterpret_cast<uint4 *>(entry + cell(q)) = none;
         }
@@ -100,7 +105,7 @@ __global__ __launch_bounds__(kBlock) void k_la_adjust(LogitsAdjustArgs a, uint32
         };
         auto masked_at = [&](int64_t t) { return a.allowed.data && !((words[t / 32 - w0] >> (t % 32)) & 1u); };
 #pragma unroll
-        for (uint32_t q = 0; q < kLaQuads; ++q) {
+        for (uint32_t q = 0; q < Q; ++q) {
             const uint32_t i = cell(q);
             const int64_t t = t0 + i;
             uint4 c = *reinterpret_cast<const uint4 *>(count + i), e;
@@ -143,13 +148,16 @@ __global__ __launch_bounds__(kBlock) void k_la_adjust(LogitsAdjustArgs a, uint32
     }
 }
 
-template <bool PACKED>
-void la_launch(const LogitsAdjustArgs &a, bool vec, bool inplace, uint32_t grid, uint32_t runs, uint64_t items, hipStream_t stream)
+template <uint32_t Q, bool PACKED>
+void la_launch(const LogitsAdjustArgs &a, bool vec, bool inplace, hipStream_t stream)
 {
-    if (vec && inplace) k_la_adjust<PACKED, true, true><<<grid, kBlock, 0, stream>>>(a, runs, items);
-    else if (vec) k_la_adjust<PACKED, true, false><<<grid, kBlock, 0, stream>>>(a, runs, items);
-    else if (inplace) k_la_adjust<PACKED, false, true><<<grid, kBlock, 0, stream>>>(a, runs, items);
-    else k_la_adjust<PACKED, false, false><<<grid, kBlock, 0, stream>>>(a, runs, items);
+    const uint64_t runs = (static_cast<uint64_t>(a.card) + (vec ? 3 : 0) + la_tokens(Q) - 1) / la_tokens(Q);
+    const uint64_t items = runs * a.rows;
+    const uint32_t grid = static_cast<uint32_t>(items < (1u << 20) ? items : 1u << 20), n = static_cast<uint32_t>(runs);
+    if (vec && inplace) k_la_adjust<Q, PACKED, true, true><<<grid, kBlock, 0, stream>>>(a, n, items);
+    else if (vec) k_la_adjust<Q, PACKED, true, false><<<grid, kBlock, 0, stream>>>(a, n, items);
+    else if (inplace) k_la_adjust<Q, PACKED, false, true><<<grid, kBlock, 0, stream>>>(a, n, items);
+    else k_la_adjust<Q, PACKED, false, false><<<grid, kBlock, 0, stream>>>(a, n, items);
 }
 
 } // namespace
@@ -159,11 +167,10 @@ hipError_t launch_logits_adjust(const LogitsAdjustArgs &a, hipStream_t stream)
     const bool inplace = a.x == a.y; // and then of one layout
     const uint64_t apart = (reinterpret_cast<uintptr_t>(a.x) ^ reinterpret_cast<uintptr_t>(a.y)) % 16;
     const bool vec = a.x_st == 1 && a.y_st == 1 && apart == 0 && (a.rows == 1 || (a.x_row - a.y_row) % 4 == 0);
-    const uint64_t runs = (static_cast<uint64_t>(a.card) + (vec ? 3 : 0) + kLaTokens - 1) / kLaTokens;
-    const uint64_t items = runs * a.rows;
-    const uint32_t grid = static_cast<uint32_t>(items < (1u << 20) ? items : 1u << 20), n = static_cast<uint32_t>(runs);
-    if (a.history.entries < 65536 && a.bias.entries < 65535) la_launch<true>(a, vec, inplace, grid, n, items, stream);
-    else la_launch<false>(a, vec, inplace, grid, n, items, stream);
+    const bool packed = a.history.entries < 65536 && a.bias.entries < 65535;
+    const bool few = static_cast<uint64_t>(a.card) * a.rows <= kLaFew;
+    if (few) packed ? la_launch<1, true>(a, vec, inplace, stream) : la_launch<1, false>(a, vec, inplace, stream);
+    else packed ? la_launch<4, true>(a, vec, inplace, stream) : la_launch<4, false>(a, vec, inplace, stream);
     return hipGetLastError();
 }
 

@@ -99,14 +99,20 @@ def test_logits_counts_and_entries_share_a_word_where_they_fit(rec, history, bia
     t = lambda slot, ne, dtype=I32: view(slot, ne, dtype=dtype)  # noqa: E731
     got, = rec.launches(eh.OpLogitsAdjust(view(0, [1000, 2, 1, 1]), view(1, [1000, 2, 1, 1], mut=True), history=t(2, [history, 2, 1, 1]),
                                           bias_ids=t(3, [biases, 2, 1, 1]), bias=t(4, [biases, 2, 1, 1], eh.DType.F32)))
-    assert ("k_la_adjust<true" in got.name) == packed
+    assert ("u, true, true, false>" in got.name) == packed
 
 
 def test_logits_rows_out_of_step_are_not_read_by_fours(rec):
     def vec(nb_x, nb_y, rows=3, at=0):
         got, = rec.launches(eh.OpLogitsAdjust(view(0, [1000, rows, 1, 1], nb_x), view(1, [1000, rows, 1, 1], nb_y, mut=True, offset=at)))
-        return re.search(r"k_la_adjust<\w+, (\w+), false", got.name).group(1) == "true"
+        return re.search(r"k_la_adjust<\w+, \w+, (\w+), false", got.name).group(1) == "true"
 
     dense = [4, 4000, 12000, 12000]
     assert vec(None, None) and vec(dense, [4, 4016, 12048, 12048]) and vec(None, None, rows=1)
     assert not vec(dense, [4, 4004, 12012, 12012]) and not vec([8, 8000, 24000, 24000], None) and not vec(None, None, at=4)
+
+
+@pytest.mark.parametrize("card,rows,tokens", [(151936, 13, 1024), (151936, 14, 4096), (1 << 21, 1, 1024), ((1 << 21) + 1, 1, 4096), (5, 1000, 1024)])
+def test_logits_that_run_at_once_take_shorter_runs(rec, card, rows, tokens):
+    got, = rec.launches(eh.OpLogitsAdjust(view(0, [card, rows, 1, 1]), view(1, [card, rows, 1, 1], mut=True)))
+    assert f"k_la_adjust<{tokens // 1024}u," in got.name

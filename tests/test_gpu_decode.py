@@ -488,6 +488,28 @@ def test_logits_adjustment_is_the_definition(gpu, card, rows, history, biases, m
     assert_bits_equal(dev["logits"].cpu().numpy(), want, "in place")
 
 
+@pytest.mark.parametrize("card,rows,history,biases,mask", [(151937, 15, 0, 0, False), (151937, 15, 700, 9, True), (2200001, 1, 70000, 66000, True)])
+def test_logits_adjustment_of_many_logits(gpu, card, rows, history, biases, mask):
+    """More logits than run at once in the shorter runs: apart, in place, and with a step of two."""
+    import torch
+
+    c = logits_case(card + rows, card, rows, history, biases, mask)
+    want = adjusted(**c)
+    dev = {n: torch.from_numpy(v).to(gpu) for n, v in c.items()}
+    y = torch.full((rows, card), 7.0, device=gpu)
+    run(logits_event(c, dev, y))
+    assert_bits_equal(y.cpu().numpy(), want, "apart")
+    y = torch.full((rows, 2 * card), 7.0, device=gpu)
+    run(logits_event(c, dev, y[:, 1::2]))
+    assert_bits_equal(y[:, 1::2].cpu().numpy(), want, "steps of two")
+    assert (y[:, 0::2] == 7.0).all()
+    two = torch.stack([dev["logits"], dev["logits"]], -1)[..., 0]
+    run(logits_event(c, {**dev, "logits": two}, two))
+    assert_bits_equal(two.cpu().numpy(), want, "in place, steps of two")
+    run(logits_event(c, dev, dev["logits"]))
+    assert_bits_equal(dev["logits"].cpu().numpy(), want, "in place")
+
+
 def test_logits_adjustment_of_a_history_past_16_bits(gpu):
     """Counts and entry numbers that do not fit half a word."""
     import torch
