@@ -17,9 +17,16 @@
 // them all, exactly, in integers.  Eight weights cost three or four
 // instructions of unpacking, a group one LDS read, and a conversion and an fma
 // a column.  A value is off by 2^-30 of the largest of its 256 at most (by 2^-127
-// where that is below 2^-97: the scale stays a normal number): less
-// than f32's own rounding of the sum that the largest is part of.
-// One column of 4096x4096 5.3 us (a launch, the layout, one round of loads),
+// where that is below 2^-97: the scale stays a normal number).  While most of
+// the run is within 2^-9 of its largest, that is less than f32's rounding of
+// a sum of such products.  It is not where a few values stand far above the
+// rest and meet small or zero weights (10^4 times: 5e-6 of the result), so a
+// workgroup that finds two runs side by side of whose nonzero values more than
+// a quarter is below 2^-9 of their run's largest lays out what the digits left
+// over, as four more of them, goes through its tiles again and adds that: 60
+// bits, at twice the time (one column of 4096x4096 9.2 us).  To look for such
+// runs costs 0.2 us there.
+// One column of 4096x4096 5.6 us (a launch, the layout, one round of loads),
 // three of 4096x151936 78 us: 4.5 TB/s.
 //
 // k_qm_halves, all others.  Each column's run of 256 values goes in as two
@@ -145,10 +152,26 @@ struct Digits {
     static __host__ __device__ uint64_t bytes(uint64_t units) { return units * ((kUnit + 4 * N) * 8 + N * 4); }
 };
 
-// The four signed bytes d0 + 2^8 d1 + 2^16 d2 + 2^24 d3 of v, |v| < 2^30.
+// The four signed bytes d0 + 2^8 d1 + 2^16 d2 + 2^24 d3 of v, |v| < 2^30;
+// LEFT: of 2^30 times what they leave of v.
+template <bool LEFT>
 __device__ __forceinline__ uint32_t digits_of(float v)
 {
-    return (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(v))) + 0x00808080u) ^ 0x00808080u;
+    float n = __builtin_rintf(v);
+    if constexpr (LEFT) n = __builtin_rintf((v - n) * 0x1p30f);
+    return (static_cast<uint32_t>(static_cast<int>(n)) + 0x00808080u) ^ 0x00808080u;
+}
+
+// Whether more than a quarter of the nonzero values of a wave's two units, as
+// scale_unit<29> leaves them, are below 2^21.
+__device__ __forceinline__ bool units_wide(const float v[8])
+{
+    const uint32_t all = 8 * __builtin_popcountll(__ballot(true));
+    uint32_t small = 0, zero = 0;
+    for (int i = 0; i < 8; ++i) small += __builtin_popcountll(__ballot(__builtin_fabsf(v[i]) < 0x1p21f));
+    if (__builtin_expect(4 * small <= all, 1)) return false;
+    for (int i = 0; i < 8; ++i) zero += __builtin_popcountll(__ballot(v[i] == 0.0f));
+    return 4 * (small - zero) > all - zero;
 }
 
 // Byte b of four words, as word b.
@@ -162,28 +185,32 @@ __device__ __forceinline__ void bytes4(const uint32_t t[4], uint32_t out[4])
     out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
-template <bool Q4K, int N>
-__device__ __forceinline__ void lay_out_digits(const QMatArgs &a, uint32_t units, u2 *to)
+// Returns whether units of this wave's are wide.
+template <bool Q4K, int N, bool LEFT>
+__device__ __forceinline__ bool lay_out_digits(const QMatArgs &a, uint32_t units, u2 *to, uint32_t tid)
 {
+    bool wide = false;
     // A unit of a column per half wave: group i / 4 % 8, lane row i % 4.  Four
-    // of them at a time, so that their loads overlap.
+    // of them at a time, so that their loads overlap (LEFT is rare: one).
+    constexpr uint32_t B = LEFT ? 1 : 4;
     const uint32_t run = units * 32, all = run * a.n;
-    for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 4 * kQmBlock) {
-        float v[4][8];
+    for (uint32_t i0 = tid; i0 < all; i0 += B * kQmBlock) {
+        float v[B][8];
 #pragma unroll
-        for (uint32_t b = 0; b < 4; ++b) {
+        for (uint32_t b = 0; b < B; ++b) {
             const uint32_t i = i0 + b * kQmBlock, c = N == 1 ? 0 : i / run, k = i - c * run;
             if (i < all) load_values<Q4K>(a, a.x + static_cast<int64_t>(c) * a.x_st[1], k / 4, k % 4, v[b]);
         }
 #pragma unroll
-        for (uint32_t b = 0; b < 4; ++b) {
+        for (uint32_t b = 0; b < B; ++b) {
             const uint32_t i = i0 + b * kQmBlock, c = N == 1 ? 0 : i / run, k = i - c * run;
             if (i >= all) break;
             const uint32_t unit = k / 32, t = k / 4 % 8, g = k % 4;
             const float down = scale_unit<29>(v[b]);
+            if constexpr (!LEFT) wide |= units_wide(v[b]);
             if (k % 32 == 0) reinterpret_cast<float *>(to + Digits<N>::scales(units))[unit * N + c] = down;
             uint32_t w[2][4], d[2][4];
-            for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = digits_of(v[b][q]);
+            for (int q = 0; q < 8; ++q) w[q / 4][q % 4] = digits_of<LEFT>(v[b][q]);
             bytes4(w[0], d[0]);
             bytes4(w[1], d[1]);
             for (uint32_t q = 0; q < 4; ++q) to[unit * Digits<N>::kUnit + ((t * 4 + q) * N + c) * 4 + g] = u2{d[0][q], d[1][q]};
@@ -191,12 +218,13 @@ __device__ __forceinline__ void lay_out_digits(const QMatArgs &a, uint32_t units
                 float sum = ((v[b][0] + v[b][1]) + (v[b][2] + v[b][3])) + ((v[b][4] + v[b][5]) + (v[b][6] + v[b][7]));
                 sum += dpp_f32<kDppXor1>(sum);
                 sum += dpp_f32<kDppXor2>(sum);
-                const uint32_t s = digits_of(sum * 0.03125f);
+                const uint32_t s = digits_of<LEFT>(sum * 0.03125f);
                 // lane row g writes digit g
                 reinterpret_cast<unsigned char *>(to + Digits<N>::sums(units) + (unit * 4 + g) * N + c)[t] = static_cast<unsigned char>(s >> (8 * g));
             }
         }
     }
+    return wide;
 }
 
 // ---- columns as halves -----------------------------------------------------------------
@@ -511,6 +539,7 @@ __global__ __launch_bounds__(kQmBlock, 4) void k_qm_digits(QMatArgs a, QmPlan pl
     constexpr int U = 2; // units in flight
     extern __shared__ u2 laid[];
     __shared__ float part[2][kQmWaves][N][kWave];
+    __shared__ uint32_t wides[kQmWaves];
     const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave), j = lane % 16, g = lane / 16;
     const QmShare sh(a, pl, wave, Q4K);
     const unsigned char *w = static_cast<const unsigned char *>(a.w);
@@ -526,16 +555,35 @@ __global__ __launch_bounds__(kQmBlock, 4) void k_qm_digits(QMatArgs a, QmPlan pl
 #pragma unroll
     for (int i = 0; i < U; ++i)
         if (sh.u0 + i < sh.u1) load_unit<WORDS>(raw[i], row, sh.u0 + i, g, sh.blocks);
-    lay_out_digits<Q4K, N>(a, pl.units, laid);
+    const bool wide = lay_out_digits<Q4K, N, false>(a, pl.units, laid, tid);
+    if (lane == 0) wides[wave] = wide;
     __syncthreads();
+    bool again = __any(wides[lane % kQmWaves]); // the digits left something over
     // slot j of the instruction's 16 columns is digit j / 4 of column j % 4 (the
     // ones past n repeat the last), so that result i of lane row g is digit g of column i
     const uint32_t c = j % 4 < a.n ? j % 4 : a.n - 1;
     const u2 *xs = laid + (j / 4 * N + c) * 4 + g, *sums = laid + Digits<N>::sums(pl.units) + j / 4 * N + c;
     const float *scales = reinterpret_cast<const float *>(laid + Digits<N>::scales(pl.units));
-    const float digit = __builtin_bit_cast(float, (127u + 8 * g) << 23) * (Q4K ? 1.0f : 0.0625f);
+    float digit = __builtin_bit_cast(float, (127u + 8 * g) << 23) * (Q4K ? 1.0f : 0.0625f);
     uint32_t turn = 0;
-    for (; tile < pl.tiles; tile += step, turn ^= 1) {
+    bool left = false; // the digits laid out are what the first ones left
+    for (;; tile += step, turn ^= 1) {
+        if (tile >= pl.tiles) {
+            if (__builtin_expect(!again, 1)) break;
+            again = false;
+            left = true;
+            digit *= 0x1p-30f;
+            tile = blockIdx.x * sh.tw;
+            __syncthreads(); // the first digits are read
+            uint32_t thread = threadIdx.x;
+            asm volatile("" : "+v"(thread)); // what the layout derives from it takes no registers ahead of here
+            lay_out_digits<Q4K, N, true>(a, pl.units, laid, thread);
+            __syncthreads();
+            row = row_of(tile);
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+                if (sh.u0 + i < sh.u1) load_unit<WORDS>(raw[i], row, sh.u0 + i, g, sh.blocks);
+        }
         float acc[N];
         for (int i = 0; i < N; ++i) acc[i] = 0.0f;
         const unsigned char *next = row_of(tile + step);
@@ -568,13 +616,15 @@ __global__ __launch_bounds__(kQmBlock, 4) void k_qm_digits(QMatArgs a, QmPlan pl
             const uint64_t r = (static_cast<uint64_t>(tile) + t) * 16 + j;
             const bool live = r < a.m && g == 0;
             uint64_t odd = __ballot(live && !(__builtin_fabsf(v) < __builtin_inff()));
+            float *y = a.y + static_cast<int64_t>(r) * a.y_st[0] + static_cast<int64_t>(i) * a.y_st[1];
+            if (__builtin_expect(left, 0) && live) v += *y; // this lane's own; one that is not finite is walked once more
             while (__builtin_expect(odd != 0, 0)) {
                 const int l = __builtin_ctzll(odd);
                 odd &= odd - 1;
                 const float f = walk_row<Q4K>(w + (r - j + l) * sh.row_bytes, a.x + static_cast<int64_t>(i) * a.x_st[1], a.x_st[0], a.k);
                 if (lane == static_cast<uint32_t>(l)) v = f;
             }
-            if (live) a.y[static_cast<int64_t>(r) * a.y_st[0] + static_cast<int64_t>(i) * a.y_st[1]] = v;
+            if (live) *y = v;
         }
     }
 }

@@ -507,7 +507,9 @@ emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_
  * elements disjoint and apart from both sources.  W[r, k] is the value that
  * get_rows gives: (q - 8) d for Q4_0, d sc q - dmin m for Q4_K.  x is read in
  * runs of 256 values along k: up to four columns to 2^-30 of a run's largest
- * value (to 2^-127 where that is below 2^-97), more columns, or a k whose columns
+ * value (to 2^-127 where that is below 2^-97), and to 2^-60 of it, at twice the
+ * time, once more than a quarter of the nonzero values of two neighbouring runs
+ * are below 2^-9 of their run's largest; more columns, or a k whose columns
  * do not fit LDS (past 18688 for one column, 3840 for four), to 22 bits of each value
  * down to 2^-16 of the run's largest and to 2^-40 of the largest below.
  * Products are exact, sums are f32, in an order that depends on the sizes

@@ -1,0 +1,57 @@
+"""GPU: the served-token operators on cases whose result is exact."""
+import numpy as np
+import pytest
+
+import emel_hip as eh
+from decode_exact import exact_product, exact_rows, outlier_columns
+from decode_reference import out, packed, view
+
+pytestmark = pytest.mark.gpu
+
+EVENT = {"q4_0": eh.OpMulMatQ4_0, "q4_k": eh.OpMulMatQ4K}
+
+
+def run(event):
+    status = eh.Kernel().process_event(event)
+    assert status == eh.Status.OK, eh.last_error()
+
+
+def product(gpu, form, rows, x):
+    import torch
+
+    (n, k), m = x.shape, len(rows)
+    y = torch.full((n, m), 7.0, device=gpu)
+    run(EVENT[form](packed(torch.from_numpy(rows).to(gpu), form, k, m), view(torch.from_numpy(x).to(gpu)), out(y)))
+    return y.cpu().numpy()
+
+
+@pytest.mark.parametrize("form,k", [("q4_0", 64), ("q4_0", 4128), ("q4_0", 3840), ("q4_k", 256), ("q4_k", 3840)])
+@pytest.mark.parametrize("n", [1, 2, 3, 4])
+@pytest.mark.parametrize("big", [2.0**-3, 1.0, 2.0**12, 2.0**20, 2.0**30, 2.0**40])
+def test_product_beside_values_that_tower_over_the_rest(gpu, form, k, n, big):
+    """Values that meet zero weights take nothing from the precision of the others."""
+    x, at = outlier_columns(k + n, k, n, big)
+    rows = exact_rows(n, form, k, 70, at)
+    got = product(gpu, form, rows, x)
+    assert np.array_equal(got, exact_product(form, rows, x, 2.0**-14))
+
+
+@pytest.mark.parametrize("form", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("m,n", [(17000, 1), (9001, 3), (40000, 4)])
+def test_product_of_many_rows_beside_towering_values(gpu, form, m, n):
+    x, at = outlier_columns(m, 512, n, 2.0**18)
+    rows = exact_rows(n, form, 512, m, at)
+    assert np.array_equal(product(gpu, form, rows, x), exact_product(form, rows, x, 2.0**-14))
+
+
+@pytest.mark.parametrize("form", ["q4_0", "q4_k"])
+def test_product_with_one_towering_and_one_infinite_column(gpu, form):
+    x, at = outlier_columns(5, 1024, 3, 2.0**25)
+    rows = exact_rows(6, form, 1024, 90, at)
+    want = exact_product(form, rows, x, 2.0**-14)
+    x[1, 77], x[2, 900] = np.inf, np.nan
+    got = product(gpu, form, rows, x)
+    assert np.array_equal(got[0], want[0]) and np.isnan(got[2]).all()
+    plain = exact_product(form, rows[:, :], np.where(np.arange(1024) == 77, 1, 0)[None].astype(np.float32))[0]
+    assert np.array_equal(np.isnan(got[1]), plain == 0)
+    assert np.array_equal(got[1][plain != 0], np.sign(plain[plain != 0]) * np.inf)
