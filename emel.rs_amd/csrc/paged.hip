@@ -28,11 +28,18 @@ __device__ __forceinline__ float from_half(uint16_t h)
 // token whose slot a later one names to that one.  Eight tokens a workgroup
 // share that look (it reads 4 bytes of each later token, and 8001 tokens of 1024 values took
 // 37 us with one token a workgroup, bound by it, and 25.8 with eight: 3.8 TB/s);
-// few tokens take one each, for more workgroups.
+// few tokens take one each, for more workgroups.  A launch takes 2^17 tokens
+// at most, so that the looks grow with the tokens and not with their square: of
+// tokens in different launches the later launch's is stored, being later.
+// (2^17 tokens of 1024 values 1000 us, 2^18 2000 against 4000 in one launch;
+// 2^20 of 64 values 7.2 ms against 60.  Up to 2^15 tokens the looks are
+// a small part: 2^15 of 1024 values 106 us.)
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef u4 u4_any __attribute__((aligned(2))); // pools may start at any half
 typedef v4f v4f_any __attribute__((aligned(4)));
+
+constexpr uint32_t kPaAppend = 1u << 17; // tokens of a launch
 
 // dim: values of a head, in eights where VEC.
 template <bool BF16, uint32_t T, bool VEC>
@@ -40,51 +47,49 @@ __global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a, FastDiv
 {
     __shared__ uint32_t gone;
     const uint64_t slots = static_cast<uint64_t>(a.page) * a.pages;
-    for (uint64_t t0 = static_cast<uint64_t>(blockIdx.x) * T; t0 < a.tokens; t0 += static_cast<uint64_t>(gridDim.x) * T) {
-        int32_t mine[T];
-        uint32_t skip = 0;
-        for (uint32_t i = 0; i < T; ++i) {
-            mine[i] = t0 + i < a.tokens ? a.slots[static_cast<int64_t>(t0 + i) * a.slots_st] : -1;
-            if (mine[i] < 0 || static_cast<uint64_t>(mine[i]) >= slots) skip |= 1u << i;
-        }
-        if (threadIdx.x == 0) gone = skip;
-        __syncthreads();
-        uint32_t later = 0;
+    const uint32_t t0 = blockIdx.x * T;
+    int32_t mine[T];
+    uint32_t skip = 0;
+    for (uint32_t i = 0; i < T; ++i) {
+        mine[i] = t0 + i < a.tokens ? a.slots[static_cast<int64_t>(t0 + i) * a.slots_st] : -1;
+        if (mine[i] < 0 || static_cast<uint64_t>(mine[i]) >= slots) skip |= 1u << i;
+    }
+    if (threadIdx.x == 0) gone = skip;
+    __syncthreads();
+    uint32_t later = 0;
 #pragma unroll 4
-        for (uint64_t u = t0 + 1 + threadIdx.x; u < a.tokens; u += kBlock) {
-            const int32_t s = a.slots[static_cast<int64_t>(u) * a.slots_st];
-            for (uint32_t i = 0; i < T; ++i) later |= s == mine[i] && u > t0 + i ? 1u << i : 0u;
-        }
-        if (later & ~skip) atomicOr(&gone, later);
-        __syncthreads();
-        const uint32_t drop = gone;
-        // an item: eight values (or one) of a head, of a token, of keys or values
-        for (uint32_t e = threadIdx.x; e < 2 * T * token.d; e += kBlock) {
-            const uint32_t i = token.div(e), r = e - i * token.d, k = i % T;
-            if ((drop >> k) & 1u) continue;
-            const uint32_t h = head.div(r), d = (r - h * head.d) * (VEC ? 8 : 1);
-            int32_t slot = mine[0]; // no index at run time: the slots stay in registers
-            for (uint32_t q = 1; q < T; ++q) slot = k == q ? mine[q] : slot;
-            const uint32_t p = page.div(static_cast<uint32_t>(slot)), at = static_cast<uint32_t>(slot) - p * page.d;
-            const bool val = i >= T;
-            const float *src = val ? a.v : a.k;
-            const int64_t *st = val ? a.v_st : a.k_st;
-            const PagePool &pool = val ? a.v_pool : a.k_pool;
-            src += d * st[0] + h * st[1] + static_cast<int64_t>(t0 + k) * st[2];
-            uint16_t *dst = pool.data + p * pool.st_page + h * pool.st_head + at * pool.st_tok + d;
-            if constexpr (VEC) {
-                const v4f lo = *reinterpret_cast<const v4f_any *>(src), hi = *reinterpret_cast<const v4f_any *>(src + 4);
-                u4 w;
-                for (int q = 0; q < 4; ++q) {
-                    const float x = q < 2 ? lo[2 * q] : hi[2 * q - 4], y = q < 2 ? lo[2 * q + 1] : hi[2 * q - 3];
-                    w[q] = to_half<BF16>(x) | static_cast<uint32_t>(to_half<BF16>(y)) << 16;
-                }
-                *reinterpret_cast<u4_any *>(dst) = w;
-            } else {
-                *dst = to_half<BF16>(*src);
+    for (uint32_t u = t0 + 1 + threadIdx.x; u < a.tokens; u += kBlock) {
+        const int32_t s = a.slots[static_cast<int64_t>(u) * a.slots_st];
+        for (uint32_t i = 0; i < T; ++i) later |= s == mine[i] && u > t0 + i ? 1u << i : 0u;
+    }
+    if (later & ~skip) atomicOr(&gone, later);
+    __syncthreads();
+    const uint32_t drop = gone;
+    // an item: eight values (or one) of a head, of a token, of keys or values
+    for (uint32_t e = threadIdx.x; e < 2 * T * token.d; e += kBlock) {
+        const uint32_t i = token.div(e), r = e - i * token.d, k = i % T;
+        if ((drop >> k) & 1u) continue;
+        const uint32_t h = head.div(r), d = (r - h * head.d) * (VEC ? 8 : 1);
+        int32_t slot = mine[0]; // no index at run time: the slots stay in registers
+        for (uint32_t q = 1; q < T; ++q) slot = k == q ? mine[q] : slot;
+        const uint32_t p = page.div(static_cast<uint32_t>(slot)), at = static_cast<uint32_t>(slot) - p * page.d;
+        const bool val = i >= T;
+        const float *src = val ? a.v : a.k;
+        const int64_t *st = val ? a.v_st : a.k_st;
+        const PagePool &pool = val ? a.v_pool : a.k_pool;
+        src += d * st[0] + h * st[1] + static_cast<int64_t>(t0 + k) * st[2];
+        uint16_t *dst = pool.data + p * pool.st_page + h * pool.st_head + at * pool.st_tok + d;
+        if constexpr (VEC) {
+            const v4f lo = *reinterpret_cast<const v4f_any *>(src), hi = *reinterpret_cast<const v4f_any *>(src + 4);
+            u4 w;
+            for (int q = 0; q < 4; ++q) {
+                const float x = q < 2 ? lo[2 * q] : hi[2 * q - 4], y = q < 2 ? lo[2 * q + 1] : hi[2 * q - 3];
+                w[q] = to_half<BF16>(x) | static_cast<uint32_t>(to_half<BF16>(y)) << 16;
             }
+            *reinterpret_cast<u4_any *>(dst) = w;
+        } else {
+            *dst = to_half<BF16>(*src);
         }
-        __syncthreads(); // gone, of the next tokens
     }
 }
 
@@ -719,8 +724,7 @@ static void pa_append(const PagedAppendArgs &a, hipStream_t stream)
 {
     const bool vec = a.dim % 8 == 0 && a.k_st[0] == 1 && a.v_st[0] == 1;
     const uint32_t head = vec ? a.dim / 8 : a.dim;
-    const uint64_t wgs = (static_cast<uint64_t>(a.tokens) + T - 1) / T;
-    const uint32_t grid = static_cast<uint32_t>(wgs < (1u << 20) ? wgs : 1u << 20);
+    const uint32_t grid = (a.tokens + T - 1) / T;
     const FastDiv page(a.page), per_head(head), per_token(head * a.kv_heads);
     if (vec) k_pa_append<BF16, T, true><<<grid, kBlock, 0, stream>>>(a, page, per_head, per_token);
     else k_pa_append<BF16, T, false><<<grid, kBlock, 0, stream>>>(a, page, per_head, per_token);
@@ -728,10 +732,19 @@ static void pa_append(const PagedAppendArgs &a, hipStream_t stream)
 
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t stream)
 {
-    const bool many = a.tokens >= 2048; // a workgroup per compute unit, of eight tokens
-    if (a.bf16) many ? pa_append<true, 8>(a, stream) : pa_append<true, 1>(a, stream);
-    else many ? pa_append<false, 8>(a, stream) : pa_append<false, 1>(a, stream);
-    return hipGetLastError();
+    PagedAppendArgs b = a;
+    for (uint64_t t = 0; t < a.tokens; t += kPaAppend) {
+        b.tokens = static_cast<uint32_t>(a.tokens - t < kPaAppend ? a.tokens - t : kPaAppend);
+        b.k = a.k + static_cast<int64_t>(t) * a.k_st[2];
+        b.v = a.v + static_cast<int64_t>(t) * a.v_st[2];
+        b.slots = a.slots + static_cast<int64_t>(t) * a.slots_st;
+        const bool many = b.tokens >= 2048; // a workgroup per compute unit, of eight tokens
+        if (b.bf16) many ? pa_append<true, 8>(b, stream) : pa_append<true, 1>(b, stream);
+        else many ? pa_append<false, 8>(b, stream) : pa_append<false, 1>(b, stream);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 namespace {

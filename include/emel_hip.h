@@ -537,7 +537,9 @@ emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_ten
  * v[:, :, t] (F32 [dim, kv_heads, tokens, 1]), rounded to the nearest half,
  * into slot slots[t] (I32 [tokens, 1, 1, 1], device memory).  A slot that is
  * negative or past the pool skips its token; of tokens with the same slot
- * the last one is stored.
+ * the last one is stored.  To know it, up to 2^17 tokens are compared with one
+ * another: that is little beside the copy up to 2^15 tokens of 1024 values (106 us),
+ * and 8 ns a token from 2^17 on, however narrow a token is.
  *
  * emel_op_paged_attention attends from one new token of each sequence:
  *   dst[:, h, s] = sum over j of softmax_j(f(scale q[:, h, s] . k_j)) v_j

@@ -1,9 +1,20 @@
-"""CPU: that the exact cases notice what they are for, on results with a mistake planted in them."""
+"""CPU: that the exact cases notice what they are for, on results with a mistake planted in them, and what the
+operators launch for very many tokens, rows or columns."""
+import re
+
 import numpy as np
 import pytest
 
+import emel_hip as eh
 from decode_exact import exact_product, exact_rows, outlier_columns
 from decode_reference import weight_terms
+from launch_recorder import Recorder
+from launch_recorder import view as wide_view
+
+
+@pytest.fixture(scope="module")
+def rec():
+    return Recorder()
 
 
 def fixed_point(x, bits):
@@ -32,3 +43,14 @@ def test_thirty_bits_are_too_few_beside_towering_values(form, big):
     hi, lo = weight_terms(form, rows)
     assert (fixed_point(x, 30) @ (hi - lo).T != want).mean() > 0.95
     assert np.array_equal(fixed_point(x, 60) @ (hi - lo).T, want)
+
+
+@pytest.mark.parametrize("tokens,launches", [(1 << 17, 1), ((1 << 17) + 1, 2), (1 << 20, 8), ((1 << 31) - 1, 1 << 14)])
+def test_append_looks_through_no_more_tokens_than_a_launch_takes(rec, tokens, launches):
+    """Each workgroup looks through all later slots of its launch, so a launch's tokens bound what a token costs."""
+    kv = [wide_view(i, [8, 1, tokens, 1]) for i in (0, 1)]
+    pools = [wide_view(i, [8, 16, 1, 9000], dtype=eh.DType.F16, mut=True) for i in (2, 3)]
+    got = rec.launches(eh.OpPagedKvAppend(*kv, wide_view(4, [tokens, 1, 1, 1], dtype=eh.DType.I32), *pools))
+    per = [int(re.search(r", (\d)u,", g.name).group(1)) for g in got]
+    assert len(got) == launches and sum(g.grid * p for g, p in zip(got, per)) in range(tokens, tokens + 8)
+    assert max(g.grid * p for g, p in zip(got, per)) == 1 << 17

@@ -5,6 +5,7 @@ import pytest
 import emel_hip as eh
 from decode_exact import exact_product, exact_rows, outlier_columns
 from decode_reference import out, packed, view
+from helpers import rng
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,25 @@ def test_product_with_one_towering_and_one_infinite_column(gpu, form):
     plain = exact_product(form, rows[:, :], np.where(np.arange(1024) == 77, 1, 0)[None].astype(np.float32))[0]
     assert np.array_equal(np.isnan(got[1]), plain == 0)
     assert np.array_equal(got[1][plain != 0], np.sign(plain[plain != 0]) * np.inf)
+
+
+@pytest.mark.parametrize("tokens", [(1 << 17) - 1, (1 << 17) + 1, (1 << 17) + 3000, (1 << 18) + 9])
+def test_append_of_more_tokens_than_a_launch_takes(gpu, tokens):
+    """Slots named again within a launch and by later ones: the last token is stored, whichever launch has it."""
+    import torch
+
+    pages, page, dim = 500, 100, 8
+    g = rng(tokens)
+    slots = g.integers(-5, pages * page + 5, tokens).astype(np.int32)
+    slots[[3, 70000, tokens - 1]] = 77
+    k = torch.arange(tokens, device=gpu, dtype=torch.int32)[:, None, None].expand(tokens, 1, dim).contiguous()
+    k = k % 2039 + torch.arange(dim, device=gpu)  # whole numbers that f16 holds
+    v = (k // 7 - 100).float()
+    pool = torch.full((2, pages, 1, page, dim), -5.0, device=gpu, dtype=torch.float16)
+    run(eh.OpPagedKvAppend(view(k.float()), view(v), view(torch.from_numpy(slots).to(gpu)), out(pool[0]), out(pool[1])))
+    last = np.full(pages * page, -1)
+    live = np.flatnonzero((slots >= 0) & (slots < pages * page))
+    last[slots[live]] = live  # numpy stores the last of equal indices
+    at = torch.from_numpy(last).to(gpu)
+    for got, src in zip(pool.view(2, pages * page, dim), (k[:, 0].half(), v[:, 0].half())):
+        assert torch.equal(got, torch.where((at < 0)[:, None], torch.full_like(got, -5.0), src[at.clamp(min=0)]))
