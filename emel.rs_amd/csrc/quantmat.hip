@@ -846,8 +846,10 @@ void qm_run(const QMatArgs &a, const QmPlan &pl, hipStream_t stream)
     }
 }
 
-// Products run in parts of columns and rows whose partial sums take about 256 MB of
-// workspace at most: kilobytes, by tile, 16 columns and chunk of k.
+// Products run in parts of columns and rows whose partial sums take 256 MB of
+// workspace at most: kilobytes, by tile, 16 columns and chunk of k.  Parts are
+// of eight tiles, one a wave, or more, but where k is so long that
+// the sums of fewer fill it (k past 2^25: 2^16 chunks of it are 64 MB a tile).
 constexpr uint64_t kQmPartials = 1u << 18;
 
 struct QmPart {
@@ -860,7 +862,11 @@ QmPart qm_part(const QMatArgs &a)
     const uint64_t all = static_cast<uint64_t>(pl.chunks) * pl.tiles;
     uint64_t groups = all * pl.groups <= kQmPartials ? pl.groups : all < kQmPartials ? kQmPartials / all : 1;
     if (groups > 4096) groups = 4096; // within a grid's second axis
-    const uint64_t tiles = all * groups <= kQmPartials ? pl.tiles : pl.chunks * kQmWaves < kQmPartials ? kQmPartials / pl.chunks : kQmWaves;
+    uint64_t tiles = pl.tiles;
+    if (all * groups > kQmPartials) { // one group: a tile and chunk take quarters of a kilobyte
+        const uint64_t fit = kQmPartials * 4 / qm_quarter(a) / pl.chunks;
+        tiles = pl.chunks * kQmWaves < kQmPartials ? kQmPartials / pl.chunks : fit < kQmWaves ? fit : kQmWaves;
+    }
     const uint64_t rows = tiles * 16, columns = groups * 16;
     return {static_cast<uint32_t>(rows < a.m ? rows : a.m), static_cast<uint32_t>(columns < a.n ? columns : a.n)};
 }

@@ -514,7 +514,7 @@ emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_
  * down to 2^-16 of the run's largest and to 2^-40 of the largest below.
  * Products are exact, sums are f32, in an order that depends on the sizes
  * alone; infinities and NaN go through as in the formula.  The second form
- * wants the stream's workspace (partial sums, up to about 256 MB), which grows as
+ * wants the stream's workspace (partial sums, up to 256 MB), which grows as
  * the reductions' does: graphs captured from one stream share it, and run
  * one after the other, or are captured from streams of their own.  Guards: a NULL view or
  * data, or an unaligned F32 pointer, is INVALID_ARGUMENT; a view that fails its

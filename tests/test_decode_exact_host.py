@@ -1,5 +1,6 @@
 """CPU: that the exact cases notice what they are for, on results with a mistake planted in them, and what the
 operators launch for very many tokens, rows or columns."""
+import ctypes
 import re
 
 import numpy as np
@@ -54,3 +55,15 @@ def test_append_looks_through_no_more_tokens_than_a_launch_takes(rec, tokens, la
     per = [int(re.search(r", (\d)u,", g.name).group(1)) for g in got]
     assert len(got) == launches and sum(g.grid * p for g, p in zip(got, per)) in range(tokens, tokens + 8)
     assert max(g.grid * p for g, p in zip(got, per)) == 1 << 17
+
+
+@pytest.mark.parametrize("k,m,n", [(1 << 26, 300, 16), (1 << 26, 300, 12), (1 << 26, 300, 5), (1 << 26, 17, 70), (3 << 24, 200, 16), (1 << 25, 200, 16),
+                                   (11008, 1 << 22, 32), (4096, 151936, 102), (64, 33, 1 << 21)])
+def test_partial_sums_stay_within_256_mb(rec, k, m, n):
+    w = eh.TensorView(1 << 43, eh.Layout.packed(eh.DType.Q4_0, [k, m, 1, 1]), 1 << 62)
+    stream = ctypes.c_void_p(0x1000 + 16 * (k + m + n))  # its own: a stream's workspace only grows
+    event = eh.OpMulMatQ4_0(w, wide_view(1, [k, n, 1, 1]), wide_view(2, [m, n, 1, 1], mut=True))
+    assert eh.Status(event._call(rec.lib, stream)) == eh.Status.OK
+    work, counters = ctypes.c_uint64(), ctypes.c_uint64()
+    assert rec.lib.emel_stream_workspace(stream, ctypes.byref(work), ctypes.byref(counters)) == 0
+    assert 1 << 20 <= work.value <= 256 << 20

@@ -58,6 +58,28 @@ def test_product_with_one_towering_and_one_infinite_column(gpu, form):
     assert np.array_equal(got[1][plain != 0], np.sign(plain[plain != 0]) * np.inf)
 
 
+@pytest.mark.parametrize("k,n", [(1 << 26, 16), (1 << 26, 1), (3 << 24, 11)])
+def test_product_of_the_longest_rows(gpu, k, n):
+    """Rows so long that a part of the product has fewer tiles than a workgroup has waves."""
+    import torch
+
+    m, g = 70, torch.Generator(gpu).manual_seed(k + n)
+    w = torch.randint(0, 256, (m, k // 32, 18), dtype=torch.uint8, device=gpu, generator=g)
+    w[:, :, 0], w[:, :, 1] = 0x00, 0x24  # the f16 2^-6
+    at = torch.randint(0, k, (4000,), device=gpu, generator=g)
+    at[:3] = torch.tensor([0, k - 1, k // 2], device=gpu)
+    at = at.unique()
+    x = torch.zeros(n, k, device=gpu)
+    x[:, at] = torch.randint(-400, 401, (n, at.numel()), device=gpu, generator=g).float()
+    y = torch.full((n, m), 7.0, device=gpu)
+    run(eh.OpMulMatQ4_0(packed(w, "q4_0", k, m), view(x), out(y)))
+    byte = w[:, at // 32, 2 + at % 16].int()
+    q = torch.where(at % 32 < 16, byte & 15, byte >> 4) - 8
+    want = x[:, at].double() @ q.double().t().contiguous() / 64
+    assert (x[:, at].abs().double() @ q.abs().double().t().contiguous()).max() < 2**23
+    assert torch.equal(y.double(), want)
+
+
 @pytest.mark.parametrize("tokens", [(1 << 17) - 1, (1 << 17) + 1, (1 << 17) + 3000, (1 << 18) + 9])
 def test_append_of_more_tokens_than_a_launch_takes(gpu, tokens):
     """Slots named again within a launch and by later ones: the last token is stored, whichever launch has it."""
