@@ -510,8 +510,11 @@ emel_status emel_op_get_rows_q4_k(const emel_tensor_view *src, const emel_index_
  * value (to 2^-127 where that is below 2^-97), and to 2^-60 of it, at twice the
  * time, once more than a quarter of the nonzero values of two neighbouring runs
  * are below 2^-9 of their run's largest; more columns, or a k whose columns
- * do not fit LDS (past 18688 for one column, 3840 for four), to 22 bits of each value
- * down to 2^-16 of the run's largest and to 2^-40 of the largest below.
+ * do not fit LDS, to 22 bits of each value down to 2^-16 of the run's largest
+ * and to 2^-40 of the largest below.  One to four columns fit with k up to
+ * 18688, 8704, 5376 and 3840, and up to 26112, 12544, 7936 and 5632 where m is
+ * at most 16 rows a compute unit (4096 on 256 of them); the last columns of a
+ * product of very many, which runs in parts, may go in either form.
  * Products are exact, sums are f32, in an order that depends on the sizes
  * alone; infinities and NaN go through as in the formula.  The second form
  * wants the stream's workspace (partial sums, up to 256 MB), which grows as
