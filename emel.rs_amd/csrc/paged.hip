@@ -125,7 +125,10 @@ __global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a, FastDiv
 //
 // Splitting a factor into parts breaks 0 * inf and inf - inf.  A wave whose
 // results are not all finite walks its tokens again one by one in f32, as the
-// formula stands, and takes those.
+// formula stands, and takes those.  So does one whose sums pass 2^97, which
+// bf16's range allows: their weighted mean is finite where the sums of this wave or of
+// the row's waves together are not.  The walk takes bf16 values by 2^-34, and a maximum
+// 34 above its own, which is what the joins weigh a part by.
 
 constexpr uint32_t kPaUnit = 128;  // tokens of a unit, 32 a wave
 constexpr uint32_t kPaLine = 64;   // words between arrival counters (a cache line each)
@@ -527,13 +530,14 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
         // the wave's part: [head][dim], dims of lane row c = 4 g + i
         float *own = joined + wave * heads * pitch;
         l = rows16(l, [](float x, float y) { return x + y; });
-        v4f zero = {l * 0.0f, 0.0f, 0.0f, 0.0f}; // stays zero while all is finite
+        v4f size = {l, 0.0f, 0.0f, 0.0f};
         for (int j = 0; j < VW; ++j)
-            for (int i = 0; i < 4; ++i) zero[i] = __builtin_fmaf(acc[j][i], 0.0f, zero[i]);
-        const bool odd = !((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f);
+            for (int i = 0; i < 4; ++i) size[i] += __builtin_fabsf(acc[j][i]);
+        const bool odd = !((size[0] + size[1]) + (size[2] + size[3]) < (BF16 ? 0x1p97f : __builtin_inff()));
         bad = __any(bad);
         if (__builtin_expect(__any(odd && col < heads) && !bad, 0)) {
             // as the formula stands: a head and a token at a time, a lane four dims
+            constexpr float down = BF16 ? 0x1p-34f : 1.0f, above = BF16 ? 34.0f : 0.0f;
             for (uint32_t h = 0; h < heads; ++h) {
                 const float *q = a.q + static_cast<int64_t>(h0 + h) * a.q_st[1] + static_cast<int64_t>(s) * a.q_st[2];
                 float qv[4], av[4] = {}, mm = -__builtin_inff(), ll = 0.0f;
@@ -559,16 +563,16 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS)) void k_pa_attn(PagedAttnArgs
                         const float e = __builtin_amdgcn_exp2f(zz - ref);
                         ll = ll * f + e;
                         for (uint32_t i = 0; i < 4; ++i)
-                            if (4 * lane + i < dim) av[i] = av[i] * f + e * from_half<BF16>(vp[4 * lane + i]);
+                            if (4 * lane + i < dim) av[i] = av[i] * f + e * (from_half<BF16>(vp[4 * lane + i]) * down);
                         mm = m1;
                     }
                 }
-                const float lift = BF16 ? 1.0f : 16384.0f;
+                const float lift = BF16 ? 1.0f : 16384.0f; // as the parts of waves that do not walk
                 for (uint32_t i = 0; i < 4; ++i)
                     if (4 * lane + i < dim) own[h * pitch + 4 * lane + i] = av[i] * lift;
                 if (lane == 0) {
-                    wm[wave][h] = mm;
-                    wl[wave][h] = ll * lift;
+                    wm[wave][h] = mm + above;
+                    wl[wave][h] = ll * (lift * down);
                 }
             }
         } else if (col < heads) {

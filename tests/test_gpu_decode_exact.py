@@ -100,3 +100,55 @@ def test_append_of_more_tokens_than_a_launch_takes(gpu, tokens):
     at = torch.from_numpy(last).to(gpu)
     for got, src in zip(pool.view(2, pages * page, dim), (k[:, 0].half(), v[:, 0].half())):
         assert torch.equal(got, torch.where((at < 0)[:, None], torch.full_like(got, -5.0), src[at.clamp(min=0)]))
+
+
+def attention(gpu, kind, q, k, v, lengths, scale=0.0, page=16, **more):
+    """The operator over keys and values [seqs, kv_heads, positions, dim] put into pages in a mixed order."""
+    import torch
+
+    seqs, kv, most, dim = k.shape
+    per = -(-most // page)
+    ids = torch.from_numpy(rng(most).permutation(seqs * per)).to(gpu)
+    pools = []
+    for src in (k, v):
+        pad = torch.zeros(seqs, kv, per * page, dim, device=gpu, dtype=kind)
+        pad[:, :, :most] = src.to(kind)
+        pool = torch.empty(seqs * per, kv, page, dim, device=gpu, dtype=kind)
+        pool[ids] = pad.view(seqs, kv, per, page, dim).transpose(1, 2).reshape(seqs * per, kv, page, dim)
+        pools.append(pool)
+    y = torch.full(q.shape, 7.0, device=gpu)
+    run(eh.OpPagedAttention(view(q), view(pools[0]), view(pools[1]), view(ids.view(seqs, per).int()), view(torch.tensor(lengths, dtype=torch.int32, device=gpu)),
+                            out(y), scale=scale, **more))
+    return y
+
+
+@pytest.mark.parametrize("lengths", [[2, 5, 40], [300, 1, 4000], [20000, 3, 33]])
+@pytest.mark.parametrize("dim", [8, 128, 256])
+def test_attention_of_values_whose_sum_overflows(gpu, dim, lengths):
+    """The mean of values near bf16's largest is finite, though their sum is not; the means are exact (flat scores)."""
+    import torch
+
+    seqs, kv, heads, most = 3, 2, 4, max(lengths)
+    v = torch.full((seqs, kv, most, dim), 3 * 2.0**126, device=gpu)  # three quarters of the largest power of two
+    v[:, :, :, 1::2] = -(2.0**127)
+    v[:, 1, 1::2, 2::4] = 0.0  # every other position
+    v[2] = 2.0**-60
+    q = torch.ones(seqs, heads, dim, device=gpu)
+    got = attention(gpu, torch.bfloat16, q, v[:, :, :, :] * 0, v, lengths).double().cpu()
+    for s, n in enumerate(lengths):
+        want = v[s, :, :n].double().mean(1).repeat_interleave(heads // kv, 0).cpu()
+        # a product with the reciprocal of a sum, each off by half a step, and the join's weighted parts
+        assert (abs(got[s] - want) <= abs(want) * 2.0**-21).all(), (s, n)
+
+
+@pytest.mark.parametrize("where", [0, 1999])
+def test_attention_of_one_value_that_overflows_beside_small_ones(gpu, where):
+    """Waves with huge sums and others are joined at one scale."""
+    import torch
+
+    v = torch.ones(1, 1, 2000, 64, device=gpu)
+    v[0, 0, where] = 2.0**127
+    v[0, 0, where - 1, 5] = -(2.0**127)
+    got = attention(gpu, torch.bfloat16, torch.ones(1, 4, 64, device=gpu), v * 0, v, [2000]).double().cpu()
+    want = v[0, 0].double().mean(0).cpu().expand(4, 64)
+    assert (abs(got[0] - want) <= abs(v[0, 0].double()).mean(0).cpu() * 2.0**-21).all()
