@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import emel_hip as eh
-from decode_exact import exact_product, exact_rows, outlier_columns
+from decode_exact import exact_product, exact_rows, outlier_columns, whole_columns
 from decode_reference import out, packed, view
 from helpers import rng
 
@@ -152,3 +152,21 @@ def test_attention_of_one_value_that_overflows_beside_small_ones(gpu, where):
     got = attention(gpu, torch.bfloat16, torch.ones(1, 4, 64, device=gpu), v * 0, v, [2000]).double().cpu()
     want = v[0, 0].double().mean(0).cpu().expand(4, 64)
     assert (abs(got[0] - want) <= abs(v[0, 0].double()).mean(0).cpu() * 2.0**-21).all()
+
+
+@pytest.mark.parametrize("form", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("n,idle", [(1, [0]), (3, [1]), (4, [0, 3]), (15, [14]), (16, [2, 3, 7]), (33, [0, 16, 32])])
+def test_product_beside_columns_that_nobody_filled(gpu, form, n, idle):
+    """Columns of NaN, or with one, are NaN in every row, whatever weights they meet; the others are as without them."""
+    x = whole_columns(n, form, 1024, n)
+    rows = exact_rows(n, form, 1024, 200)
+    want = exact_product(form, rows, x)
+    for i, c in enumerate(idle):
+        x[c, :: 1 if i % 2 == 0 else 1024] = np.nan
+        want[c] = np.nan
+    rows.reshape(200, -1, 18 if form == "q4_0" else 144)[7, 0, :2] = np.array([np.inf], np.float16).view(np.uint8)
+    got = product(gpu, form, rows, x)
+    assert np.isnan(got[idle]).all()
+    rest = [c for c in range(n) if c not in idle]
+    got, want = np.delete(got[rest], 7, 1), np.delete(want[rest], 7, 1)
+    assert np.array_equal(got, want)
