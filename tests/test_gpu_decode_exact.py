@@ -170,3 +170,23 @@ def test_product_beside_columns_that_nobody_filled(gpu, form, n, idle):
     rest = [c for c in range(n) if c not in idle]
     got, want = np.delete(got[rest], 7, 1), np.delete(want[rest], 7, 1)
     assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (20, 1, 72), (3, 3, 8), (4, 2, 256)])
+def test_attention_beside_queries_that_nobody_filled(gpu, bf16, heads, kv, dim):
+    """A head whose query holds a NaN is NaN, unless its sequence is empty; the others are as without it."""
+    import torch
+
+    kind, lengths = (torch.bfloat16, torch.float16)[not bf16], [700, 0, 33, 5000, 1]
+    g = torch.Generator(gpu).manual_seed(dim)
+    v = torch.randint(-9, 10, (5, kv, 5000, dim), device=gpu, generator=g).float()
+    q = torch.randn(5, heads, dim, device=gpu, generator=g)
+    plain = attention(gpu, kind, q, v * 0, v, lengths, scale=1.0)
+    q[0, heads - 1, dim - 1] = q[3, 0, 3] = q[4, 0] = float("nan")
+    q[1] = float("nan")
+    got = attention(gpu, kind, q, v * 0, v, lengths, scale=1.0)
+    filled = ~q.isnan().any(2)
+    filled[1] = True
+    assert torch.equal(got[filled], plain[filled]) and got[~filled].isnan().all()
+    assert (got[1] == 0).all()
