@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import emel_hip as eh
-from decode_exact import exact_product, exact_rows, outlier_columns
+from decode_exact import cancelling, cancelling_attention, exact_product, exact_rows, flat_means_differ, flat_values, outlier_columns, whole_columns
 from decode_reference import weight_terms
 from launch_recorder import Recorder
 from launch_recorder import view as wide_view
@@ -67,3 +67,53 @@ def test_partial_sums_stay_within_256_mb(rec, k, m, n):
     work, counters = ctypes.c_uint64(), ctypes.c_uint64()
     assert rec.lib.emel_stream_workspace(stream, ctypes.byref(work), ctypes.byref(counters)) == 0
     assert 1 << 20 <= work.value <= 256 << 20
+
+
+def nearest(x, bits):
+    """x to `bits` significant bits."""
+    with np.errstate(divide="ignore"):
+        unit = 2.0 ** (np.floor(np.log2(np.abs(np.where(x == 0, 1, x)))) - bits + 1)
+    return np.rint(x / unit) * unit
+
+
+def cut(x, bits):
+    """x cut after `bits` significant bits."""
+    unit = 2.0 ** (np.floor(np.log2(np.abs(np.where(x == 0, 1, x)))) - bits + 1)
+    return np.trunc(x / unit) * unit
+
+
+@pytest.mark.parametrize("form,k", [("q4_0", 4096), ("q4_0", 32768), ("q4_k", 4096), ("q4_k", 11008)])
+def test_lost_low_halves_and_lost_values_show(form, k):
+    """Columns to 11 bits, or without one value, differ from the exact results nearly everywhere."""
+    x, rows = whole_columns(1, form, k, 5), exact_rows(2, form, k, 60)
+    want = exact_product(form, rows, x)
+    hi, lo = weight_terms(form, rows)
+    assert (nearest(x, 11) @ (hi - lo).T != want).mean() > 0.95
+    without = x.copy()
+    without[:, k // 2] = 0
+    changed = (hi - lo)[:, k // 2] != 0
+    assert ((without @ (hi - lo).T != want) == ((x[:, k // 2] != 0)[:, None] & changed)).all()
+
+
+@pytest.mark.parametrize("n", [1, 33, 20000, 150000])
+def test_a_lost_or_doubled_position_shows(n):
+    v = flat_values(n, 1, 1, n, 16)[0]
+    mean = v.sum(1, dtype=np.float64) / n
+    assert not flat_means_differ(mean.astype(np.float32), v, n).any()
+    for j in {0, n // 2, n - 1}:
+        for sign in (1, -1):
+            off = (mean + sign * v[:, j] / n).astype(np.float32)
+            assert np.array_equal(flat_means_differ(off, v, n)[0], v[0, j] != 0)
+
+
+@pytest.mark.parametrize("dim", [8, 64, 136, 256])
+@pytest.mark.parametrize("part", ["q: f16, one half", "q: bf16, two parts", "weights: f16, one half", "weights: bf16, two parts"])
+def test_lost_parts_of_queries_and_weights_show(dim, part):
+    kept = (lambda x: nearest(x, 11)) if "f16, one" in part else (lambda x: cut(x, 16))
+    seen = []
+    for seed in range(8):
+        q, k, v = cancelling(seed, 1, 4, 3, dim)
+        want, tol = cancelling_attention(q, k, v, 3)
+        got, _ = cancelling_attention(q, k, v, 3, **{"q_part" if part[0] == "q" else "p_part": kept})
+        seen.append((abs(got - want) > tol).mean())
+    assert min(seen) > 0.1, seen

@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 
 import emel_hip as eh
-from decode_exact import exact_product, exact_rows, outlier_columns, whole_columns
+from decode_exact import (POWER, cancelling, cancelling_attention, exact_product, exact_rows, exact_scale, flat_means_differ, flat_values,
+                          outlier_columns, whole_columns)
 from decode_reference import out, packed, view
 from helpers import rng
 
@@ -190,3 +191,69 @@ def test_attention_beside_queries_that_nobody_filled(gpu, bf16, heads, kv, dim):
     filled[1] = True
     assert torch.equal(got[filled], plain[filled]) and got[~filled].isnan().all()
     assert (got[1] == 0).all()
+
+
+@pytest.mark.parametrize("form,k", [("q4_0", 32), ("q4_0", 288), ("q4_0", 4096), ("q4_0", 4128), ("q4_0", 11008), ("q4_0", 18688), ("q4_0", 32768),
+                                    ("q4_k", 256), ("q4_k", 1280), ("q4_k", 4096), ("q4_k", 11008), ("q4_k", 16384)])
+@pytest.mark.parametrize("m,n", [(70, 1), (257, 2), (33, 3), (100, 4), (47, 5), (64, 13), (31, 16), (50, 33)])
+def test_product_keeps_every_bit_of_whole_numbers(gpu, form, k, m, n):
+    x, rows = whole_columns(k + n, form, k, n), exact_rows(m, form, k, m)
+    assert np.array_equal(product(gpu, form, rows, x), exact_product(form, rows, x))
+
+
+@pytest.mark.parametrize("form", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("m,n", [(40000, 1), (20000, 4), (40000, 7), (11008, 15), (9000, 64)])
+def test_product_of_many_rows_keeps_every_bit(gpu, form, m, n):
+    x, rows = whole_columns(m, form, 1024, n), exact_rows(n, form, 1024, m)
+    assert np.array_equal(product(gpu, form, rows, x), exact_product(form, rows, x))
+
+
+FLAT = [(1, 1, 64), (8, 1, 128), (17, 1, 8), (4, 2, 40), (6, 3, 104), (2, 1, 136), (5, 1, 200), (16, 1, 256), (32, 8, 128)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("heads,kv,dim", FLAT)
+def test_attention_counts_every_position_once(gpu, bf16, heads, kv, dim):
+    """Flat scores, values that name their positions: lengths around units, waves and the runs of workgroups."""
+    import torch
+
+    lengths = [1, 2, 31, 32, 33, 127, 128, 129, 255, 256, 257, 0, 500, 639, 641, 1500, 2047, 2049, 3000]
+    v = flat_values(dim, len(lengths), kv, max(lengths), dim)
+    q = torch.ones(len(lengths), heads, dim, device=gpu)
+    vt = torch.from_numpy(v).to(gpu)
+    for window in (0, 1, 32, 100, 1000):
+        got = attention(gpu, (torch.float16, torch.bfloat16)[bf16], q, vt * 0, vt, lengths, scale=0.0, page=(24, 1, 16, 7, 256)[window % 5], window=window).cpu().numpy()
+        for s, n in enumerate(lengths):
+            if n:
+                assert not flat_means_differ(got[s], v[s], n, window).any(), (n, window)
+            else:
+                assert (got[s] == 0).all()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(8, 1, 128), (1, 1, 64), (20, 1, 8), (4, 2, 256), (32, 8, 128), (3, 1, 96)])
+@pytest.mark.parametrize("positions", [[8191], [12000, 1], [20000], [33000, 5, 129], [70001], [150000]])
+def test_attention_counts_every_position_of_long_sequences_once(gpu, heads, kv, dim, positions):
+    """As above, with rows of more than 64 parts."""
+    import torch
+
+    v = flat_values(positions[0] + dim, len(positions), kv, positions[0], dim)
+    vt = torch.from_numpy(v).to(gpu)
+    got = attention(gpu, torch.float16, torch.ones(len(positions), heads, dim, device=gpu), vt * 0, vt, positions, scale=0.0, page=64).cpu().numpy()
+    for s, n in enumerate(positions):
+        assert not flat_means_differ(got[s], v[s], n).any(), n
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("dim", list(range(8, 257, 8)))
+def test_attention_keeps_every_part_of_queries_and_weights(gpu, bf16, dim):
+    """Scores that are differences of large numbers in q, in every dim, over three positions and over some hundreds."""
+    import torch
+
+    heads, kv, most = 4, 2, dim + 200
+    lengths = [3] * 24 + [dim + 9, most]
+    cases = [cancelling(dim + s, kv, heads, most, dim) for s in range(len(lengths))]
+    q, k, v = (torch.from_numpy(np.stack(t)).to(gpu) for t in zip(*cases))
+    got = attention(gpu, (torch.float16, torch.bfloat16)[bf16], q, k, v, lengths, scale=exact_scale(POWER)).double().cpu().numpy()
+    for s, n in enumerate(lengths):
+        want, tol = cancelling_attention(*cases[s], n)
+        assert (np.abs(got[s] - want) <= tol).all(), (n, (np.abs(got[s] - want) / np.maximum(tol, 1e-30)).max())
