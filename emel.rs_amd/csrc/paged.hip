@@ -111,8 +111,13 @@ __global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a, FastDiv
 //            the VW dims from VW c on of tokens 4g .. 4g+3 of both 16-token
 //            tiles; 16-bit permutes of its own registers turn them into operands,
 //            and its scores are the other operand where they stand.
-// The weights P go in as halves that add up to f32's 24 bits for bf16, 22 for
-// f16 (hi + lo, scaled by 2^14 so that lo stays normal down to 2^-28 of the largest).
+// The weights P, and q, go in as halves that add up to f32's 24 bits for bf16
+// (three) and 22 for f16 (hi + lo): a third f16 half would be half as many
+// instructions again for less than f32's sums over a head's dims or a sequence's
+// tokens lose.  f16's are scaled so that the largest is near 2^14: lo keeps its 11 bits down
+// to 2^-16 of that, and 2^-39 of it below, where lo is subnormal (hi is from
+// 2^-28 on).  A subnormal factor also costs the instruction low bits: halves of
+// the cache below 2^-14 count to about 2^-38 of what they are multiplied by.
 // A wave's (m, l, out) are joined through LDS, a row's segments of several
 // workgroups through the workspace by the last of them to finish: stores and
 // loads at agent scope and an arrival counter, as in reduce.hip.  The order

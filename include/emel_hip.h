@@ -558,8 +558,11 @@ emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_ten
  * length 0 gets zeros.  One whose length is negative or past max pages * page, or that
  * reaches a page id outside the pool, gets NaN, and nothing outside the pool
  * is read.  What lies behind a sequence's length, and before its window,
- * does not count, NaN or not.  Scores, softmax and sums are f32; q and the softmax weights
- * keep 22 bits (F16 pools) or 24 (BF16) in products with the cached halves.
+ * does not count, NaN or not.  Scores, softmax and sums are f32.  q and the
+ * softmax weights keep 24 bits in products with BF16 halves.  With F16 halves
+ * they keep 22, down to 2^-16 of the head's largest element of q or of its
+ * largest weight, and 2^-39 of that below; and F16 halves below 2^-14, which are
+ * subnormal, count to about 2^-38 of what they are multiplied by.
  * Wants the stream's workspace, which grows as the reductions' does: graphs
  * captured from one stream share it, and run one after the other, or are
  * captured from streams of their own.

@@ -5,6 +5,7 @@ import pytest
 import emel_hip as eh
 from decode_exact import (POWER, cancelling, cancelling_attention, exact_product, exact_rows, exact_scale, flat_means_differ, flat_values,
                           outlier_columns, whole_columns)
+from decode_reference import attention as reference
 from decode_reference import out, packed, view
 from helpers import rng
 
@@ -257,3 +258,21 @@ def test_attention_keeps_every_part_of_queries_and_weights(gpu, bf16, dim):
     for s, n in enumerate(lengths):
         want, tol = cancelling_attention(*cases[s], n)
         assert (np.abs(got[s] - want) <= tol).all(), (n, (np.abs(got[s] - want) / np.maximum(tol, 1e-30)).max())
+
+
+@pytest.mark.parametrize("dim", [8, 128, 256])
+@pytest.mark.parametrize("size", [2.0**-24, 2.0**-20, 2.0**-17])
+def test_attention_over_subnormal_halves(gpu, dim, size):
+    """F16 values below 2^-14 count to 2^-38 of their weights, each instruction's largest: 2^-37 of the sum, at most."""
+    import torch
+
+    lengths, most = [1, 33, 700], 700
+    g = rng(dim)
+    k = g.standard_normal((3, 2, most, dim)).astype(np.float16)
+    v = (g.integers(-7, 8, (3, 2, most, dim)) * size).astype(np.float16)
+    q = g.standard_normal((3, 4, dim)).astype(np.float32)
+    up = lambda t: torch.from_numpy(t.astype(np.float32)).to(gpu)  # noqa: E731
+    got = attention(gpu, torch.float16, up(q), up(k), up(v), lengths, scale=dim**-0.5).double().cpu().numpy()
+    for s, n in enumerate(lengths):
+        want, tol = reference(q[s].astype(np.float64), *(t[s, :, :n].astype(np.float64).transpose(1, 0, 2) for t in (k, v)), dim**-0.5, 0.0)
+        assert (np.abs(got[s] - want) <= tol + 2.0**-37).all(), (n, np.abs(got[s] - want).max())
