@@ -27,7 +27,7 @@ __device__ __forceinline__ float from_half(uint16_t h)
 // the last is stored: each workgroup looks through the slots behind its own and leaves a
 // token whose slot a later one names to that one.  Eight tokens a workgroup
 // share that look (it reads 4 bytes of each later token, and 8001 tokens of 1024 values took
-// 37 us with one token a workgroup, bound by it, and 25.8 with eight: 3.8 TB/s);
+// 37 us with one token a workgroup, bound by it, and 23.9 with eight: 4.1 TB/s);
 // few tokens take one each, for more workgroups.  A launch takes 2^17 tokens
 // at most, so that the looks grow with the tokens and not with their square: of
 // tokens in different launches the later launch's is stored, being later.
