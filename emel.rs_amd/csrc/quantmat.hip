@@ -790,7 +790,7 @@ int qm_digits(const QMatArgs &a)
     if (a.n > 4) return 0;
     const uint64_t units = (static_cast<uint64_t>(a.k) + kQmUnit - 1) / kQmUnit;
     const uint64_t bytes[] = {Digits<1>::bytes(units), Digits<2>::bytes(units), Digits<3>::bytes(units), Digits<4>::bytes(units)};
-    const uint64_t lds = bytes[a.n - 1] + a.n * (2 * kQmBlock * sizeof(float));
+    const uint64_t lds = bytes[a.n - 1] + a.n * (2 * kQmBlock * sizeof(float)) + kQmWaves * sizeof(uint32_t);
     return lds <= kQmLds || (lds <= kQmLdsAlone && a.m <= 16 * qm_cus()) ? static_cast<int>(a.n) : 0;
 }
 

@@ -276,3 +276,65 @@ def test_attention_over_subnormal_halves(gpu, dim, size):
     for s, n in enumerate(lengths):
         want, tol = reference(q[s].astype(np.float64), *(t[s, :, :n].astype(np.float64).transpose(1, 0, 2) for t in (k, v)), dim**-0.5, 0.0)
         assert (np.abs(got[s] - want) <= tol + 2.0**-37).all(), (n, np.abs(got[s] - want).max())
+
+
+@pytest.mark.parametrize("form", ["q4_0", "q4_k"])
+@pytest.mark.parametrize("n", [1, 4, 9])
+def test_a_captured_product_follows_its_columns(gpu, form, n):
+    """What a replay finds in its columns decides how it goes: whole numbers, towering values, NaN, and whole numbers again."""
+    import torch
+
+    k, m = 1024, 300
+    tower, at = outlier_columns(n, k, n, 2.0**20)
+    rows = exact_rows(n, form, k, m, at)
+    whole = whole_columns(n, form, k, n)
+    plain = (whole, exact_product(form, rows, whole))
+    empty = whole.copy()
+    empty[n - 1] = np.nan
+    with_empty = plain[1].copy()
+    with_empty[n - 1] = np.nan
+    w, x, y = torch.from_numpy(rows).to(gpu), torch.zeros(n, k, device=gpu), torch.zeros(n, m, device=gpu)
+    stream = torch.cuda.Stream()
+    kernel = eh.Kernel(stream.cuda_stream, synchronous=False)
+    event = EVENT[form](packed(w, form, k, m), view(x), out(y))
+    torch.cuda.synchronize()
+    assert kernel.process_event(event) == eh.Status.OK  # sizes the stream's workspace
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert kernel.process_event(event) == eh.Status.OK
+    steps = [plain, (empty, with_empty), plain, plain]
+    if n <= 4:  # more columns keep 22 bits beside such values
+        steps[1:1] = [(tower, exact_product(form, rows, tower, 2.0**-14)), plain]
+    for values, want in steps:
+        x.copy_(torch.from_numpy(values))
+        y.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(y.cpu().numpy(), want, equal_nan=True)
+
+
+def test_a_captured_append_of_several_launches_follows_its_slots(gpu):
+    import torch
+
+    tokens, pages, page, dim = (1 << 17) + 500, 40, 64, 8
+    k = (torch.arange(tokens, device=gpu) % 2039).float()[:, None, None].expand(tokens, 1, dim).contiguous()
+    slots = torch.zeros(tokens, dtype=torch.int32, device=gpu)
+    pool = torch.zeros(2, pages, 1, page, dim, device=gpu, dtype=torch.bfloat16)
+    stream = torch.cuda.Stream()
+    kernel = eh.Kernel(stream.cuda_stream, synchronous=False)
+    event = eh.OpPagedKvAppend(view(k), view(-k), view(slots), out(pool[0]), out(pool[1]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert kernel.process_event(event) == eh.Status.OK
+    for seed in range(3):
+        ids = rng(seed).integers(-9, pages * page, tokens).astype(np.int32)
+        slots.copy_(torch.from_numpy(ids))
+        pool.fill_(1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        last = np.full(pages * page, -1)
+        last[ids[ids >= 0]] = np.flatnonzero(ids >= 0)
+        want = torch.where(torch.from_numpy(last < 0).to(gpu)[:, None], torch.ones(1, device=gpu), k[torch.from_numpy(last).to(gpu).clamp(min=0), 0]).bfloat16()
+        assert torch.equal(pool[0].view(-1, dim), want) and (pool[1].view(-1, dim) == -want)[torch.from_numpy(last >= 0).to(gpu)].all()
