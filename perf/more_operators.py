@@ -24,8 +24,9 @@ import torch
 
 own = False
 
-# bytes of a block of 32 values: an f16 scale d, then 32 signed bytes q (d q), or 16 bytes of two nibbles q (d (q - 8))
+# bytes of a block of 32 values: an f16 scale d, and 32 signed bytes q (d q), or 16 bytes of two nibbles q (d (q - 8))
 BLOCK = {"q8_0": 34, "q4_0": 18}
+NIBBLES = [0, 2, 4, 6, 1, 3, 5, 7]  # which of eight values each nibble holds, lowest bits first
 
 
 def listed():
@@ -244,31 +245,39 @@ def _events(c, s):
 def _encode(kind, x):
     """Rows of f32 values as packed bytes.  Of a block's 32 values the scale is the largest magnitude / 127, or the value
     of the largest magnitude (the first of equal ones) / -8, rounded to f32 and then to f16; a value is the nearest
-    whole number of scales, ties to even, within the format's range."""
+    whole number of scales, ties to even, within the format's range.  Numbers come first, by eights: the first eight
+    of every block, then the second, the third and the fourth; the blocks' scales follow."""
     b = x.reshape(-1, 32)
-    size, at = b.abs().max(1)
+    size = b.abs().amax(1)
     if kind == "q8_0":
         d = size.double() / torch.full_like(size, 127.0).double()
     else:
         d = b.gather(1, b.abs().eq(size[:, None]).to(torch.int8).argmax(1, keepdim=True))[:, 0] * -0.125
     d = d.float().clamp(-65504.0, 65504.0).half()
     n = torch.where(d[:, None] == 0, 0.0, torch.round(b.double() / d.double()[:, None]))  # 64 bits tell which side of a half a quotient is
-    out = torch.empty(b.shape[0], BLOCK[kind], dtype=torch.uint8, device=x.device)
-    out[:, :2] = d[:, None].view(torch.uint8)
     if kind == "q8_0":
-        out[:, 2:] = n.clamp(-127, 127).to(torch.int8).view(torch.uint8)
-    else:
-        q = (n.clamp(-8, 7) + 8).to(torch.uint8)
-        out[:, 2:] = q[:, :16] | (q[:, 16:] << 4)
-    return out.view(*x.shape[:-1], -1)
+        q = n.clamp(-127, 127).to(torch.int8).view(torch.uint8)
+    else:  # of an eight: values 0, 2, 4, 6, then 1, 3, 5, 7, four bits each
+        q = (n.clamp(-8, 7) + 8).to(torch.uint8).view(-1, 8)[:, NIBBLES]
+        q = q[:, 0::2] | (q[:, 1::2] << 4)
+    blocks = x.shape[-1] // 32
+    rows = torch.cat([q.reshape(x.numel() // x.shape[-1], blocks, 4, -1).transpose(1, 2).flatten(1), d.view(-1, blocks).view(torch.uint8)], 1)
+    return rows.view(*x.shape[:-1], -1)
 
 
 def _decode(kind, b):
     """Packed rows as f32 values."""
-    r = b.reshape(-1, BLOCK[kind])
-    d, q = r[:, :2].contiguous().view(torch.float16).float(), r[:, 2:].contiguous()
-    v = q.view(torch.int8).float() if kind == "q8_0" else torch.cat([q & 15, q >> 4], 1).float() - 8.0
-    return (v * d).view(*b.shape[:-1], -1)
+    blocks = b.shape[-1] // BLOCK[kind]
+    rows = b.reshape(-1, b.shape[-1])
+    d, q = rows[:, -2 * blocks:].contiguous().view(torch.float16).float(), rows[:, :-2 * blocks]
+    if kind == "q8_0":
+        v = q.contiguous().view(torch.int8).float()
+    else:
+        q = q.reshape(-1, 4)
+        v = torch.empty(q.shape[0], 8, device=b.device)
+        v[:, NIBBLES] = torch.stack([q & 15, q >> 4], 2).flatten(1).float() - 8.0
+    v = v.view(-1, 4, blocks, 8).transpose(1, 2).flatten(2)  # [rows, blocks, 32]
+    return (v * d[:, :, None]).view(*b.shape[:-1], -1)
 
 
 def _pairs(c):
@@ -358,15 +367,20 @@ def exact(c, seed):
     s = prepare(c, seed)
 
     def values(kind, rows):
-        """Packed rows [..., bytes] in 64 bits, a block's scale first."""
-        b = rows.reshape(-1, BLOCK[kind]).to(torch.int32)
-        d = (b[:, 0] | (b[:, 1] << 8)).to(torch.int16).view(torch.float16).double()
-        out = torch.empty(b.shape[0], 32, dtype=torch.float64, device="cuda")
-        for j in range(32):
+        """Packed rows [..., bytes] in 64 bits, a value at a time."""
+        b = rows.reshape(-1, rows.shape[-1]).to(torch.int32)
+        blocks = rows.shape[-1] // BLOCK[kind]
+        out = torch.empty(b.shape[0], 32 * blocks, dtype=torch.float64, device="cuda")
+        for i in range(32 * blocks):
+            j, eight, at = i // 32, i % 32 // 8, i % 8
+            low = (32 if kind == "q8_0" else 16) * blocks + 2 * j
+            d = (b[:, low] | (b[:, low + 1] << 8)).to(torch.int16).view(torch.float16).double()
             if kind == "q8_0":
-                out[:, j] = d * (b[:, 2 + j] - 256 * (b[:, 2 + j] // 128))
-            else:
-                out[:, j] = d * ((b[:, 2 + j % 16] // 16 if j > 15 else b[:, 2 + j % 16] % 16) - 8)
+                q = b[:, 8 * (eight * blocks + j) + at]
+                out[:, i] = d * (q - 256 * (q // 128))
+            else:  # even values in the first two bytes, odd ones in the last two
+                q = b[:, 4 * (eight * blocks + j) + 2 * (at % 2) + at // 4]
+                out[:, i] = d * ((q // 16 if at // 2 % 2 else q % 16) - 8)
         return out.view(*rows.shape[:-1], -1)
 
     def rounded(kind, x):
