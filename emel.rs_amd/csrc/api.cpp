@@ -2656,6 +2656,128 @@ emel_status mul_mat_q4(bool q4k, const emel_tensor_view *w, const emel_tensor_vi
     return launched(emel::launch_quant_mat(a, as_stream(stream)));
 }
 
+// Whether no element of a shares a byte with one of b, by a sufficient rule:
+// their spans are apart, or both have one stride per token, each token's
+// elements lie within it, and the tokens of b lie in the gaps between those of a.
+template <class A, class B>
+bool tokens_apart(const A &a, const B &b)
+{
+    if (apart(span_of(a, 4), span_of(b, 4))) return true;
+    const Operand ao = operand(a, 4), bo = operand(b, 4);
+    const uint64_t step = static_cast<uint64_t>(ao.st[2]) * 4;
+    if (a.ne[2] < 2 || b.ne[2] < 2 || ao.st[2] != bo.st[2]) return false;
+    auto bytes = [](const Operand &o) {
+        u128 n = 4;
+        for (int d = 0; d < 2; ++d) n += static_cast<u128>(o.ne[d] - 1) * static_cast<uint64_t>(o.st[d]) * 4;
+        return n;
+    };
+    const uintptr_t al = reinterpret_cast<uintptr_t>(a.data), bl = reinterpret_cast<uintptr_t>(b.data);
+    const uint64_t at = bl >= al ? (bl - al) % step : (step - (al - bl) % step) % step;
+    return bytes(ao) <= at && at + bytes(bo) <= step;
+}
+
+emel_status rope(const emel_rope_request *r, emel_stream stream)
+{
+    if (!r || !data_ok(r->q, 4) || !data_ok(r->q_out, 4) || !data_ok(r->positions, 4) || (r->k && !data_ok(r->k, 4)) ||
+        (r->k_out && !data_ok(r->k_out, 4)) || (r->factors && !data_ok(r->factors, 4)))
+        return fail(EMEL_ERR_INVALID_ARGUMENT, "null request, view or data, or a misaligned pointer");
+    constexpr uint32_t kFlags = EMEL_ROPE_ADJACENT | EMEL_ROPE_IN_TURN | EMEL_ROPE_OWN_FREQUENCIES | EMEL_ROPE_BACKWARD;
+    if ((!r->k) != (!r->k_out) || (r->flags & ~kFlags))
+        return fail(EMEL_ERR_INVALID_REQUEST, "k goes with k_out, flags are those of emel_rope_flag");
+    const emel_tensor_view &q = *r->q, &p = *r->positions;
+    const emel_tensor_view_mut &qo = *r->q_out;
+    if (!extents_ok(q, qo, p) || (r->k && !extents_ok(*r->k, *r->k_out)) || (r->factors && !extents_ok(*r->factors)) ||
+        q.ne[0] > 1u << 24 || q.ne[1] + (r->k ? r->k->ne[1] : 0) > kMaxExtent)
+        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent, or both heads', is past 2^31 - 1, or dim past 2^24");
+    if (!valid_f32(q, true) || !valid_f32(qo, true) || !valid_i32(p) ||
+        (r->k && (!valid_f32(*r->k, true) || !valid_f32(*r->k_out, true))) || (r->factors && !valid_f32(*r->factors, true)))
+        return fail(EMEL_ERR_INVALID_VIEW, "rope view failed validation");
+    const uint64_t axes = p.ne[1];
+    uint64_t pairs = 0;
+    for (const uint32_t n : r->sections) pairs += n;
+    if (!same_ne(q, qo) || q.ne[3] != 1 || !ne_is(p.ne, q.ne[2], axes) || axes > 4 ||
+        (r->k && (!ne_is(r->k->ne, q.ne[0], r->k->ne[1], q.ne[2]) || !same_ne(*r->k, *r->k_out))) ||
+        (r->factors && !ne_is(r->factors->ne, pairs, 1)))
+        return fail(EMEL_ERR_SHAPE_MISMATCH, "rope takes [dim, heads, tokens], [tokens, axes] and [pairs]");
+    for (uint64_t d = axes; d < 4; ++d)
+        if (r->sections[d]) return fail(EMEL_ERR_INVALID_PARAMETERS, "a section past the last axis");
+    if (pairs == 0 || 2 * pairs > q.ne[0]) return fail(EMEL_ERR_INVALID_PARAMETERS, "sections hold one pair to dim / 2");
+    if (!std::isfinite(r->base) || r->base <= 0.0f || !std::isfinite(r->scale) || !std::isfinite(r->magnitude))
+        return fail(EMEL_ERR_INVALID_PARAMETERS, "base, scale and magnitude are finite, base > 0");
+    const emel_tensor_view_mut *outs[] = {r->q_out, r->k_out};
+    const emel_tensor_view *ins[] = {r->q, r->k};
+    for (int o = 0; o < (r->k ? 2 : 1); ++o) {
+        const Span ys = span_of(*outs[o], 4);
+        if (!apart(ys, span_of(p, 4)) || (r->factors && !apart(ys, span_of(*r->factors, 4))))
+            return fail(EMEL_ERR_INVALID_VIEW, "an output overlaps positions or factors");
+        if (!overlap_ok(*outs[o], 4, *ins[o], 4) && !tokens_apart(*outs[o], *ins[o]))
+            return fail(EMEL_ERR_INVALID_VIEW, "an output partially overlaps its input");
+        if (r->k && !tokens_apart(*outs[o], *ins[1 - o]))
+            return fail(EMEL_ERR_INVALID_VIEW, "an output overlaps the other input");
+        if (!elements_disjoint(*outs[o], 4)) return fail(EMEL_ERR_INVALID_VIEW, "output elements overlap one another");
+    }
+    if (r->k && !tokens_apart(*r->q_out, *r->k_out)) return fail(EMEL_ERR_INVALID_VIEW, "q_out overlaps k_out");
+    emel_status s = ensure_device();
+    if (s != EMEL_OK) return s;
+
+    emel::RopeArgs a{};
+    a.dim = static_cast<uint32_t>(q.ne[0]);
+    a.pairs = static_cast<uint32_t>(pairs);
+    a.tokens = static_cast<uint32_t>(q.ne[2]);
+    for (int o = 0; o < (r->k ? 2 : 1); ++o) {
+        const Operand x = operand(*ins[o], 4), y = operand(*outs[o], 4);
+        emel::RopeTensor &t = o ? a.k : a.q;
+        t.x = static_cast<const float *>(x.data);
+        t.y = static_cast<float *>(y.data);
+        for (int d = 0; d < 3; ++d) {
+            t.x_st[d] = x.st[d];
+            t.y_st[d] = y.st[d];
+        }
+        t.heads = static_cast<uint32_t>(x.ne[1]);
+    }
+    a.pos = static_cast<const int32_t *>(p.data);
+    a.pos_st[0] = static_cast<int64_t>(p.nb[0] / 4);
+    a.pos_st[1] = static_cast<int64_t>(p.nb[1] / 4);
+    if (r->factors) {
+        a.factors = static_cast<const float *>(r->factors->data);
+        a.factors_st = operand(*r->factors, 4).st[0];
+    }
+    a.own = r->flags & EMEL_ROPE_OWN_FREQUENCIES;
+    a.adjacent = r->flags & EMEL_ROPE_ADJACENT;
+    a.back = r->flags & EMEL_ROPE_BACKWARD;
+    // Runs of pairs whose axes take turns: with EMEL_ROPE_IN_TURN one from each
+    // section's end to the next longer one's, else one for each section.
+    int n = 0;
+    for (uint32_t at = 0, round = 0; at < pairs; ++n) {
+        emel::RopeRun &run = a.runs[n];
+        run = {at, 0, 0, 0};
+        if (r->flags & EMEL_ROPE_IN_TURN) {
+            uint32_t next = UINT32_MAX;
+            run.round = round;
+            for (uint32_t d = 0; d < 4; ++d) {
+                if (r->sections[d] <= round) continue;
+                run.axes |= d << (2 * run.live++);
+                next = std::min(next, r->sections[d]);
+            }
+            at += (next - round) * run.live;
+            round = next;
+        } else {
+            while (r->sections[round] == 0) ++round; // here the section's number
+            run.live = 1;
+            run.axes = round;
+            at += r->sections[round++];
+        }
+    }
+    for (; n < 4; ++n) a.runs[n] = {UINT32_MAX, 0, 1, 0};
+    for (int d = 0; d < 4; ++d) {
+        const uint64_t count = a.own ? r->sections[d] : pairs;
+        a.rate[d] = count ? std::log2(static_cast<double>(r->base)) / static_cast<double>(count) : 0.0;
+    }
+    a.quarters = static_cast<double>(r->scale) * 0.6366197723675814; // 2 / pi
+    a.magnitude = r->magnitude;
+    return launched(emel::launch_rope(a, as_stream(stream)));
+}
+
 // A pool of pages: halves with unit stride along dim.
 template <class V>
 bool pages_valid(const V &v)
@@ -2915,6 +3037,11 @@ emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_ten
                                  const emel_tensor_view_mut *dst, emel_stream stream)
 {
     return entry([&] { return mul_mat_q4(true, weights, x, dst, stream); });
+}
+
+emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream)
+{
+    return entry([&] { return rope(request, stream); });
 }
 
 emel_status emel_op_paged_kv_append(const emel_tensor_view *k, const emel_tensor_view *v,

@@ -249,6 +249,37 @@ struct QMatArgs {
 uint64_t quant_mat_workspace_bytes(const QMatArgs &args);
 hipError_t launch_quant_mat(const QMatArgs &args, hipStream_t stream);
 
+// ---- rotary positions (rope.hip) ----------------------------------------------------
+
+struct RopeTensor { // [dim, heads, tokens]; absent: no heads
+    const float *x;
+    float *y;
+    int64_t x_st[3], y_st[3]; // element strides
+    uint32_t heads;
+};
+
+// Pairs from `start` on are dealt out to `live` axes in turn (two bits each of
+// `axes`), each of which has `round` pairs before them.
+struct RopeRun {
+    uint32_t start, round, live, axes;
+};
+
+struct RopeArgs {
+    uint32_t dim, pairs, tokens;
+    RopeTensor q, k;
+    const int32_t *pos;   // [tokens, axes]
+    int64_t pos_st[2];
+    const float *factors; // [pairs], null: 1
+    int64_t factors_st;
+    RopeRun runs[4];      // by start; unused ones start past the pairs
+    double rate[4];       // log2 of the base by the exponent's count, of each axis
+    double quarters;      // quarter turns of a position at exponent 0
+    float magnitude;
+    bool own, adjacent, back;
+};
+
+hipError_t launch_rope(const RopeArgs &args, hipStream_t stream);
+
 // ---- paged key-value cache (paged.hip) --------------------------------------------
 
 // One pool of pages of halves, [dim, page, kv_heads, pages]; strides in halves.

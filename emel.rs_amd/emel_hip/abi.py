@@ -282,6 +282,22 @@ class CLogitsAdjustRequest(ctypes.Structure):
         "allowed")] + [("reserved", ctypes.c_uint64)]
 
 
+class CRopeRequest(ctypes.Structure):
+    """emel_rope_request: operands by pointer, absent ones NULL."""
+
+    _fields_ = [(name, ctypes.POINTER(CView)) for name in ("q", "q_out", "k", "k_out", "positions", "factors")] + [
+        ("sections", ctypes.c_uint32 * 4), ("flags", ctypes.c_uint32), ("base", ctypes.c_float),
+        ("scale", ctypes.c_float), ("magnitude", ctypes.c_float)]
+
+
+class RopeFlag(enum.IntFlag):
+    """emel_rope_flag: how pairs are formed and dealt out, and the gradient's direction."""
+    ADJACENT = 1
+    IN_TURN = 2
+    OWN_FREQUENCIES = 4
+    BACKWARD = 8
+
+
 _V = ctypes.POINTER(CView)
 _S = ctypes.c_void_p
 _ST = ctypes.c_int
@@ -351,6 +367,7 @@ SIGNATURES = {
     "emel_stream_copy": [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, _S],
     "emel_op_mul_mat_q4_0": [_V, _V, _V, _S],
     "emel_op_mul_mat_q4_k": [_V, _V, _V, _S],
+    "emel_op_rope": [ctypes.POINTER(CRopeRequest), _S],
     "emel_op_paged_kv_append": [_V, _V, _V, _V, _V, _S],
     "emel_op_paged_attention": [_V, _V, _V, _V, _V, ctypes.c_float, ctypes.c_uint64, ctypes.c_float, _V, _S],
     "emel_logits_adjust": [ctypes.POINTER(CLogitsAdjustRequest), _S],

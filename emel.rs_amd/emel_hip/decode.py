@@ -2,6 +2,7 @@
 
     kernel.process_event(OpMulMatQ4K(TensorView(w, Layout.packed(DType.Q4_K, [k, m, 1, 1])),
                                      TensorView(x, ...), TensorViewMut(y, ...)))
+    kernel.process_event(OpRope(q, q, positions, [16, 24, 24], k=k, k_out=k, base=1e6))
     kernel.process_event(OpPagedKvAppend(k, v, slots, k_pages, v_pages))
     kernel.process_event(OpPagedAttention(q, k_pages, v_pages, page_table, lengths, out, scale=dim ** -0.5))
     kernel.process_event(OpLogitsAdjust(logits, logits, history=ids, repeat=r, allowed=bits))
@@ -17,7 +18,7 @@ from __future__ import annotations
 
 import ctypes
 
-from .abi import CLogitsAdjustRequest
+from .abi import CLogitsAdjustRequest, CRopeRequest, RopeFlag
 from .views import TensorView, TensorViewMut
 
 
@@ -51,6 +52,30 @@ class OpMulMatQ4K(OpMulMatQ4_0):
 
     __slots__ = ()
     _fn = "emel_op_mul_mat_q4_k"
+
+
+class OpRope(_Event):
+    """Queries, and keys where k and k_out are given, turned by their positions on one to four axes (emel_op_rope).
+
+    sections holds the pairs of each axis; an output may be its input itself."""
+
+    __slots__ = ()
+    _fn = "emel_op_rope"
+
+    def __init__(self, q: TensorView, q_out: TensorViewMut, positions: TensorView, sections, *,
+                 k: TensorView | None = None, k_out: TensorViewMut | None = None, factors: TensorView | None = None,
+                 base: float = 10000.0, scale: float = 1.0, magnitude: float = 1.0, adjacent: bool = False,
+                 in_turn: bool = False, own_frequencies: bool = False, backward: bool = False):
+        r = CRopeRequest()
+        self._views = (q, q_out, k, k_out, positions, factors)
+        for (name, _), view in zip(CRopeRequest._fields_, self._views):
+            if view is not None:
+                setattr(r, name, ctypes.pointer(view.c()))
+        r.sections[:len(sections)] = [int(n) for n in sections]
+        r.base, r.scale, r.magnitude = base, scale, magnitude
+        r.flags = (RopeFlag.ADJACENT * adjacent | RopeFlag.IN_TURN * in_turn
+                   | RopeFlag.OWN_FREQUENCIES * own_frequencies | RopeFlag.BACKWARD * backward)
+        self._args = (ctypes.byref(r),)
 
 
 class OpPagedKvAppend(_Event):

@@ -48,6 +48,84 @@ impl HipEvent for OpMulMatQ4<'_> {
     }
 }
 
+/// Queries, and keys where given, turned by their positions on one to four
+/// axes.
+#[derive(Debug)]
+pub struct OpRope<'a> {
+    q: DeviceView<'a>,
+    q_out: DeviceViewMut<'a>,
+    k: Option<(DeviceView<'a>, DeviceViewMut<'a>)>,
+    positions: DeviceView<'a>,
+    factors: Option<DeviceView<'a>>,
+    sections: [u32; 4],
+    flags: u32,
+    base: f32,
+    scale: f32,
+    magnitude: f32,
+}
+
+impl<'a> OpRope<'a> {
+    /// Pairs of values half the turned ones apart, `sections` of them for each
+    /// axis, with frequencies from `base`; validation occurs when it is
+    /// dispatched.
+    #[must_use]
+    pub const fn new(q: DeviceView<'a>, q_out: DeviceViewMut<'a>, positions: DeviceView<'a>, sections: [u32; 4], base: f32) -> Self {
+        Self { q, q_out, k: None, positions, factors: None, sections, flags: 0, base, scale: 1.0, magnitude: 1.0 }
+    }
+
+    /// The tokens' keys, turned with them.
+    #[must_use]
+    pub const fn with_keys(mut self, k: DeviceView<'a>, k_out: DeviceViewMut<'a>) -> Self {
+        self.k = Some((k, k_out));
+        self
+    }
+
+    /// What each pair's frequency is divided by.
+    #[must_use]
+    pub const fn with_factors(mut self, factors: DeviceView<'a>) -> Self {
+        self.factors = Some(factors);
+        self
+    }
+
+    /// What positions, and the results, are multiplied by.
+    #[must_use]
+    pub const fn with_scale(mut self, scale: f32, magnitude: f32) -> Self {
+        self.scale = scale;
+        self.magnitude = magnitude;
+        self
+    }
+
+    /// `ffi::EMEL_ROPE_ADJACENT` and its neighbours.
+    #[must_use]
+    pub const fn with_flags(mut self, flags: u32) -> Self {
+        self.flags = flags;
+        self
+    }
+}
+
+impl HipEvent for OpRope<'_> {
+    type Output = Result<(), HipError>;
+
+    fn dispatch(self, kernel: &mut HipKernel) -> Self::Output {
+        let request = ffi::EmelRopeRequest {
+            q: self.q.as_ffi(),
+            q_out: self.q_out.as_ffi(),
+            k: raw(self.k.as_ref().map(|k| &k.0)),
+            k_out: self.k.as_ref().map_or(core::ptr::null(), |k| core::ptr::from_ref(k.1.as_ffi())),
+            positions: self.positions.as_ffi(),
+            factors: raw(self.factors.as_ref()),
+            sections: self.sections,
+            flags: self.flags,
+            base: self.base,
+            scale: self.scale,
+            magnitude: self.magnitude,
+        };
+        // SAFETY: the request's views live until the call returns and describe
+        // live device memory, checked by the library.
+        HipError::check(kernel.call(|s| unsafe { ffi::emel_op_rope(&raw const request, s) }))
+    }
+}
+
 /// Writes new tokens' keys and values into their slots of the page pools.
 #[derive(Debug)]
 pub struct OpPagedKvAppend<'a> {

@@ -96,6 +96,11 @@ pub const EMEL_BINARY_MUL: u32 = 2;
 pub const EMEL_BINARY_DIV: u32 = 3;
 
 // ---- emel_generic_op ----
+pub const EMEL_ROPE_ADJACENT: u32 = 1;
+pub const EMEL_ROPE_IN_TURN: u32 = 2;
+pub const EMEL_ROPE_OWN_FREQUENCIES: u32 = 4;
+pub const EMEL_ROPE_BACKWARD: u32 = 8;
+
 pub const EMEL_GENERIC_DUP: u32 = 0;
 pub const EMEL_GENERIC_ADD: u32 = 1;
 pub const EMEL_GENERIC_ADD_ID: u32 = 2;
@@ -286,6 +291,23 @@ pub struct EmelSampleRows {
     pub top_stride: u64,
 }
 
+/// `emel_rope_request`: absent operands are null.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct EmelRopeRequest {
+    pub q: *const EmelTensorView,
+    pub q_out: *const EmelTensorViewMut,
+    pub k: *const EmelTensorView,
+    pub k_out: *const EmelTensorViewMut,
+    pub positions: *const EmelTensorView,
+    pub factors: *const EmelTensorView,
+    pub sections: [u32; 4],
+    pub flags: u32,
+    pub base: f32,
+    pub scale: f32,
+    pub magnitude: f32,
+}
+
 /// `emel_logits_adjust_request`: absent operands are null.
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -380,6 +402,7 @@ unsafe extern "C" {
     pub fn emel_op_get_rows_q4_k(src: *const EmelTensorView, indices: *const EmelIndexView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_op_mul_mat_q4_0(weights: *const EmelTensorView, x: *const EmelTensorView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_op_mul_mat_q4_k(weights: *const EmelTensorView, x: *const EmelTensorView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
+    pub fn emel_op_rope(request: *const EmelRopeRequest, stream: Stream) -> Status;
     pub fn emel_op_paged_kv_append(k: *const EmelTensorView, v: *const EmelTensorView, slots: *const EmelTensorView, k_pages: *const EmelTensorViewMut, v_pages: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_op_paged_attention(q: *const EmelTensorView, k_pages: *const EmelTensorView, v_pages: *const EmelTensorView, page_table: *const EmelTensorView, lengths: *const EmelTensorView, scale: f32, window: u64, soft_cap: f32, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_generic_dispatch(request: *const EmelGenericRequest, stream: Stream) -> Status;

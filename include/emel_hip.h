@@ -529,6 +529,65 @@ emel_status emel_op_mul_mat_q4_0(const emel_tensor_view *weights, const emel_ten
 emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_tensor_view *x,
                                  const emel_tensor_view_mut *dst, emel_stream stream);
 
+/* ---- rotary positions ---------------------------------------------------------------
+ * No counterpart in the pinned path, whose wire opcode ROPE has no route: the
+ * positions that a decoder turns its queries and keys by before the cache
+ * takes them, and an image encoder its patches.
+ *
+ * q and q_out are F32 [dim, heads, tokens, 1]; k and k_out, both or neither,
+ * [dim, kv_heads, tokens, 1].  An output may be exactly its input (in place); else
+ * outputs and inputs share no byte (heads of one buffer side by side, as a
+ * fused projection leaves them, are fine).  positions is I32 [tokens, axes, 1, 1]
+ * with one to four axes, as a text's token (one axis) or an image's time,
+ * height and width; any I32 counts, negative ones too.  sections[a] is the
+ * number of pairs that axis a turns, 0 past the last axis; n = their sum, 2 n <=
+ * dim.  The first 2 n values of a head form n pairs, values i and i + n, or with
+ * EMEL_ROPE_ADJACENT 2 i and 2 i + 1; values behind them are copied.  Pair i belongs
+ * to the axis in whose section it lies, the sections one after the other, or
+ * with EMEL_ROPE_IN_TURN dealt out one pair to each axis in turn as long as
+ * it has any left.  With p the token's position on that axis,
+ *   angle = p * scale * base^(-i / n) / factors[i]
+ *   x' = magnitude (x cos angle - y sin angle)
+ *   y' = magnitude (x sin angle + y cos angle)
+ * where EMEL_ROPE_OWN_FREQUENCIES counts pairs along their own axis: i is the
+ * pair's number on it, and n its section.  factors is F32 [n, 1, 1, 1], by the
+ * pair's number in the head (NULL: 1).  EMEL_ROPE_BACKWARD takes the angle's opposite: from
+ * the gradient of a result it makes that of its input.
+ * Angles are worked out in 64 bits (off by 2^-50 of themselves at most), cos
+ * and sin rounded to f32.  Positions and factors are device memory, read when the kernel
+ * runs.
+ *
+ * Guards: a NULL request, view or data, or a misaligned pointer, is
+ * INVALID_ARGUMENT; k without k_out, or a flag that is none of these,
+ * INVALID_REQUEST; a view that fails its rules, or an overlap, INVALID_VIEW;
+ * extents that do not match, or more than four axes, SHAPE_MISMATCH; no pairs, more than
+ * dim holds, a section past the last axis, a base that is not finite and above 0, a
+ * scale or magnitude that is not finite, INVALID_PARAMETERS; an extent, or
+ * the heads of q and k together, past 2^31 - 1, or a dim past 2^24,
+ * UNSUPPORTED_OPERATION. */
+typedef enum emel_rope_flag {
+    EMEL_ROPE_ADJACENT = 1,
+    EMEL_ROPE_IN_TURN = 2,
+    EMEL_ROPE_OWN_FREQUENCIES = 4,
+    EMEL_ROPE_BACKWARD = 8
+} emel_rope_flag;
+
+typedef struct emel_rope_request {
+    const emel_tensor_view *q;
+    const emel_tensor_view_mut *q_out;
+    const emel_tensor_view *k;         /* NULL when absent, with k_out */
+    const emel_tensor_view_mut *k_out;
+    const emel_tensor_view *positions;
+    const emel_tensor_view *factors;   /* NULL when absent */
+    uint32_t sections[4];
+    uint32_t flags;                    /* emel_rope_flag bits */
+    float base;
+    float scale;
+    float magnitude;
+} emel_rope_request;
+
+emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream);
+
 /* ---- paged key-value cache ---------------------------------------------------------
  * No counterpart in the pinned path.  The cache is two pools of pages, one for
  * keys and one for values: F16 or BF16 views [dim, page, kv_heads, pages]
