@@ -2778,25 +2778,44 @@ emel_status rope(const emel_rope_request *r, emel_stream stream)
     return launched(emel::launch_rope(a, as_stream(stream)));
 }
 
-// A pool of pages: halves with unit stride along dim.
+// Bytes of a token's head in a pool: dim halves with unit stride, or a packed
+// row of dim / 32 blocks; 0: no page type.
+template <class V>
+uint64_t page_row(const V &v)
+{
+    switch (v.dtype) {
+    case EMEL_DTYPE_F16:
+    case EMEL_DTYPE_BF16: return 2 * v.ne[0];
+    case EMEL_DTYPE_Q8_0: return v.ne[0] / 32 * 34;
+    case EMEL_DTYPE_Q4_0: return v.ne[0] / 32 * 18;
+    default: return 0;
+    }
+}
+
+template <class V>
+bool packed_pages(const V &v)
+{
+    return v.dtype == EMEL_DTYPE_Q8_0 || v.dtype == EMEL_DTYPE_Q4_0;
+}
+
 template <class V>
 bool pages_valid(const V &v)
 {
     uint64_t count;
-    if ((v.dtype != EMEL_DTYPE_F16 && v.dtype != EMEL_DTYPE_BF16) || v.reserved != 0) return false;
-    if (!element_count(v, count) || v.nb[0] != 2) return false;
+    if (page_row(v) == 0 || v.reserved != 0 || !element_count(v, count)) return false;
+    if (packed_pages(v) ? v.nb[0] != 1 || v.ne[0] % 32 != 0 : v.nb[0] != 2) return false;
     for (int d = 1; d < 4; ++d)
         if (v.ne[d] > 1 && (v.nb[d] < 2 || v.nb[d] % 2 != 0)) return false;
-    uint64_t st[4];
-    for (int d = 0; d < 4; ++d) st[d] = v.ne[d] > 1 ? v.nb[d] : 0;
-    return span_fits(v, st, 2);
+    uint64_t st[4] = {0, 0, 0, 0};
+    for (int d = 1; d < 4; ++d) st[d] = v.ne[d] > 1 ? v.nb[d] : 0;
+    return span_fits(v, st, page_row(v));
 }
 
 template <class V>
 Span pages_span(const V &v)
 {
-    uintptr_t bytes = 2;
-    for (int d = 0; d < 4; ++d) bytes += (v.ne[d] - 1) * (v.ne[d] > 1 ? v.nb[d] : 0);
+    uintptr_t bytes = page_row(v);
+    for (int d = 1; d < 4; ++d) bytes += (v.ne[d] - 1) * (v.ne[d] > 1 ? v.nb[d] : 0);
     const uintptr_t lo = reinterpret_cast<uintptr_t>(v.data);
     return {lo, lo + bytes};
 }
@@ -2805,49 +2824,64 @@ template <class V>
 emel::PagePool pool_of(const V &v)
 {
     auto st = [&](int d) { return static_cast<int64_t>(v.ne[d] > 1 ? v.nb[d] / 2 : 0); };
-    return {static_cast<uint16_t *>(const_cast<void *>(static_cast<const void *>(v.data))), st(1), st(2), st(3)};
+    const emel::PoolKind kind = v.dtype == EMEL_DTYPE_F16    ? emel::PoolKind::F16
+                                : v.dtype == EMEL_DTYPE_BF16 ? emel::PoolKind::Bf16
+                                : v.dtype == EMEL_DTYPE_Q8_0 ? emel::PoolKind::Q8_0
+                                                             : emel::PoolKind::Q4_0;
+    return {static_cast<uint16_t *>(const_cast<void *>(static_cast<const void *>(v.data))), st(1), st(2), st(3), kind};
 }
 
 // Whether no slot of either pool shares a byte with another, by the rule of
-// elements_disjoint.  Pools of one layout that lie inside one another's span
-// (keys and values side by side in each page) count as one tensor with a
-// dimension of two more.
+// elements_disjoint over rows.  Pools of one layout that lie inside one another's
+// span (keys and values side by side in each page) count as one tensor with a
+// dimension of two more: the higher pool's rows stand `apart` bytes above
+// the lower one's.
 bool pools_disjoint(const emel_tensor_view_mut &k, const emel_tensor_view_mut &v)
 {
     struct Dim {
         uint64_t ne, st;
+        bool pair;
     };
-    auto rule = [](Dim *d, int n) {
+    // span: of one row, of the lower pool and of the higher one
+    auto rule = [](Dim *d, int n, u128 low, u128 high) {
         for (int i = 1; i < n; ++i)
             for (int j = i; j > 0 && d[j].st < d[j - 1].st; --j) std::swap(d[j], d[j - 1]);
-        u128 span = 2;
         for (int i = 0; i < n; ++i) {
-            if (d[i].st < span) return false;
-            span += static_cast<u128>(d[i].ne - 1) * d[i].st;
+            if (d[i].pair) {
+                if (d[i].st < low) return false;
+                low = high = d[i].st + high;
+                continue;
+            }
+            if (d[i].st < low || d[i].st < high) return false;
+            low += static_cast<u128>(d[i].ne - 1) * d[i].st;
+            high += static_cast<u128>(d[i].ne - 1) * d[i].st;
         }
         return true;
     };
     auto dims = [](const emel_tensor_view_mut &t, Dim *d) {
         int n = 0;
-        for (int i = 0; i < 4; ++i)
-            if (t.ne[i] > 1) d[n++] = {t.ne[i], t.nb[i]};
+        for (int i = 1; i < 4; ++i)
+            if (t.ne[i] > 1) d[n++] = {t.ne[i], t.nb[i], false};
         return n;
     };
-    Dim d[5];
-    if (!rule(d, dims(k, d)) || !rule(d, dims(v, d))) return false;
+    Dim d[4];
+    const u128 kr = page_row(k), vr = page_row(v);
+    if (!rule(d, dims(k, d), kr, kr) || !rule(d, dims(v, d), vr, vr)) return false;
     const Span ks = pages_span(k), vs = pages_span(v);
     if (apart(ks, vs)) return true;
-    for (int i = 0; i < 4; ++i)
+    for (int i = 1; i < 4; ++i)
         if (k.ne[i] > 1 && k.nb[i] != v.nb[i]) return false;
     const int n = dims(k, d);
-    d[n] = {2, ks.lo < vs.lo ? vs.lo - ks.lo : ks.lo - vs.lo};
-    return rule(d, n + 1);
+    const bool k_low = ks.lo < vs.lo;
+    d[n] = {2, k_low ? vs.lo - ks.lo : ks.lo - vs.lo, true};
+    return rule(d, n + 1, k_low ? kr : vr, k_low ? vr : kr);
 }
 
+// Pools of one shape and type; packed ones may differ in type.
 template <class A, class B>
 bool pools_alike(const A &k, const B &v)
 {
-    return k.dtype == v.dtype && same_ne(k, v);
+    return (k.dtype == v.dtype || (packed_pages(k) && packed_pages(v))) && same_ne(k, v);
 }
 
 emel_status paged_append(const emel_tensor_view *k, const emel_tensor_view *v, const emel_tensor_view *slots,
@@ -2871,7 +2905,6 @@ emel_status paged_append(const emel_tensor_view *k, const emel_tensor_view *v, c
     if (s != EMEL_OK) return s;
     const Operand ko = operand(*k, 4), vo = operand(*v, 4);
     emel::PagedAppendArgs a{};
-    a.bf16 = kp->dtype == EMEL_DTYPE_BF16;
     a.dim = static_cast<uint32_t>(kp->ne[0]);
     a.page = static_cast<uint32_t>(kp->ne[1]);
     a.kv_heads = static_cast<uint32_t>(kp->ne[2]);
@@ -2888,6 +2921,48 @@ emel_status paged_append(const emel_tensor_view *k, const emel_tensor_view *v, c
     a.k_pool = pool_of(*kp);
     a.v_pool = pool_of(*vp);
     return launched(emel::launch_paged_append(a, as_stream(stream)));
+}
+
+emel_status paged_read(const emel_tensor_view *kp, const emel_tensor_view *vp, const emel_tensor_view *slots,
+                       const emel_tensor_view_mut *k, const emel_tensor_view_mut *v, emel_stream stream)
+{
+    if (!data_ok(k, 4) || !data_ok(v, 4) || !data_ok(slots, 4) || !data_ok(kp, 2) || !data_ok(vp, 2))
+        return fail(EMEL_ERR_INVALID_ARGUMENT, "null view or data, or a misaligned pointer");
+    if (!extents_ok(*k, *v, *slots, *kp, *vp)) return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "an extent is past 2^31 - 1");
+    if (!valid_f32(*k, true) || !valid_f32(*v, true) || !valid_i32(*slots) || !pages_valid(*kp) || !pages_valid(*vp))
+        return fail(EMEL_ERR_INVALID_VIEW, "paged read view failed validation");
+    if (!pools_alike(*kp, *vp) || !ne_is(k->ne, kp->ne[0], kp->ne[2], k->ne[2]) || !same_ne(*k, *v) ||
+        !ne_is(slots->ne, k->ne[2], 1))
+        return fail(EMEL_ERR_SHAPE_MISMATCH, "paged read takes two pools alike, [tokens] and [dim, heads, tokens]");
+    if (kp->ne[0] * kp->ne[2] > 1u << 26)
+        return fail(EMEL_ERR_UNSUPPORTED_OPERATION, "dim * kv_heads is past 2^26");
+    for (const emel_tensor_view_mut *o : {k, v}) {
+        const Span os = span_of(*o, 4);
+        if (!apart(os, pages_span(*kp)) || !apart(os, pages_span(*vp)) || !apart(os, span_of(*slots, 4)))
+            return fail(EMEL_ERR_INVALID_VIEW, "an output overlaps a source");
+        if (!elements_disjoint(*o, 4)) return fail(EMEL_ERR_INVALID_VIEW, "output elements overlap one another");
+    }
+    if (!tokens_apart(*k, *v)) return fail(EMEL_ERR_INVALID_VIEW, "k overlaps v");
+    emel_status s = ensure_device();
+    if (s != EMEL_OK) return s;
+    const Operand ko = operand(*k, 4), vo = operand(*v, 4);
+    emel::PagedReadArgs a{};
+    a.dim = static_cast<uint32_t>(kp->ne[0]);
+    a.page = static_cast<uint32_t>(kp->ne[1]);
+    a.kv_heads = static_cast<uint32_t>(kp->ne[2]);
+    a.pages = static_cast<uint32_t>(kp->ne[3]);
+    a.tokens = static_cast<uint32_t>(k->ne[2]);
+    a.k_pool = pool_of(*kp);
+    a.v_pool = pool_of(*vp);
+    a.slots = static_cast<const int32_t *>(slots->data);
+    a.slots_st = static_cast<int64_t>(slots->nb[0] / 4);
+    a.k = static_cast<float *>(ko.data);
+    a.v = static_cast<float *>(vo.data);
+    for (int d = 0; d < 3; ++d) {
+        a.k_st[d] = ko.st[d];
+        a.v_st[d] = vo.st[d];
+    }
+    return launched(emel::launch_paged_read(a, as_stream(stream)));
 }
 
 emel_status paged_attention(const emel_tensor_view *q, const emel_tensor_view *kp, const emel_tensor_view *vp,
@@ -2919,7 +2994,6 @@ emel_status paged_attention(const emel_tensor_view *q, const emel_tensor_view *k
     if (s != EMEL_OK) return s;
     const Operand qo = operand(*q, 4), yo = operand(*y, 4);
     emel::PagedAttnArgs a{};
-    a.bf16 = kp->dtype == EMEL_DTYPE_BF16;
     a.dim = static_cast<uint32_t>(kp->ne[0]);
     a.page = static_cast<uint32_t>(kp->ne[1]);
     a.kv_heads = static_cast<uint32_t>(kp->ne[2]);
@@ -3049,6 +3123,13 @@ emel_status emel_op_paged_kv_append(const emel_tensor_view *k, const emel_tensor
                                     const emel_tensor_view_mut *v_pages, emel_stream stream)
 {
     return entry([&] { return paged_append(k, v, slots, k_pages, v_pages, stream); });
+}
+
+emel_status emel_op_paged_kv_read(const emel_tensor_view *k_pages, const emel_tensor_view *v_pages,
+                                  const emel_tensor_view *slots, const emel_tensor_view_mut *k,
+                                  const emel_tensor_view_mut *v, emel_stream stream)
+{
+    return entry([&] { return paged_read(k_pages, v_pages, slots, k, v, stream); });
 }
 
 emel_status emel_op_paged_attention(const emel_tensor_view *q, const emel_tensor_view *k_pages,

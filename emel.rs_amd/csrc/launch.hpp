@@ -282,14 +282,19 @@ hipError_t launch_rope(const RopeArgs &args, hipStream_t stream);
 
 // ---- paged key-value cache (paged.hip) --------------------------------------------
 
-// One pool of pages of halves, [dim, page, kv_heads, pages]; strides in halves.
+enum class PoolKind : uint32_t { F16 = 0, Bf16, Q8_0, Q4_0 };
+
+// One pool of pages, [dim, page, kv_heads, pages]; strides in halves (two
+// bytes), which rows of packed values are multiples of.
 struct PagePool {
     uint16_t *data;
     int64_t st_tok, st_head, st_page;
+    PoolKind kind;
+
+    __host__ __device__ bool packed() const { return kind >= PoolKind::Q8_0; }
 };
 
 struct PagedAppendArgs {
-    bool bf16;
     uint32_t dim, page, kv_heads, pages, tokens;
     const float *k, *v;  // [dim, kv_heads, tokens]
     int64_t k_st[3], v_st[3];
@@ -300,8 +305,18 @@ struct PagedAppendArgs {
 
 hipError_t launch_paged_append(const PagedAppendArgs &args, hipStream_t stream);
 
+struct PagedReadArgs {
+    uint32_t dim, page, kv_heads, pages, tokens;
+    PagePool k_pool, v_pool;
+    const int32_t *slots;
+    int64_t slots_st;
+    float *k, *v;        // [dim, kv_heads, tokens]
+    int64_t k_st[3], v_st[3];
+};
+
+hipError_t launch_paged_read(const PagedReadArgs &args, hipStream_t stream);
+
 struct PagedAttnArgs {
-    bool bf16;
     uint32_t dim, page, kv_heads, pages, heads, seqs, max_pages;
     const float *q;      // [dim, heads, seqs]
     int64_t q_st[3];

@@ -369,6 +369,7 @@ SIGNATURES = {
     "emel_op_mul_mat_q4_k": [_V, _V, _V, _S],
     "emel_op_rope": [ctypes.POINTER(CRopeRequest), _S],
     "emel_op_paged_kv_append": [_V, _V, _V, _V, _V, _S],
+    "emel_op_paged_kv_read": [_V, _V, _V, _V, _V, _S],
     "emel_op_paged_attention": [_V, _V, _V, _V, _V, ctypes.c_float, ctypes.c_uint64, ctypes.c_float, _V, _S],
     "emel_logits_adjust": [ctypes.POINTER(CLogitsAdjustRequest), _S],
     "emel_generic_dispatch": [ctypes.POINTER(CGenericRequest), _S],

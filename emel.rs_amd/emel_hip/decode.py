@@ -4,6 +4,7 @@
                                      TensorView(x, ...), TensorViewMut(y, ...)))
     kernel.process_event(OpRope(q, q, positions, [16, 24, 24], k=k, k_out=k, base=1e6))
     kernel.process_event(OpPagedKvAppend(k, v, slots, k_pages, v_pages))
+    kernel.process_event(OpPagedKvRead(k_pages, v_pages, slots, k, v))
     kernel.process_event(OpPagedAttention(q, k_pages, v_pages, page_table, lengths, out, scale=dim ** -0.5))
     kernel.process_event(OpLogitsAdjust(logits, logits, history=ids, repeat=r, allowed=bits))
 
@@ -79,13 +80,25 @@ class OpRope(_Event):
 
 
 class OpPagedKvAppend(_Event):
-    """Writes new tokens' keys and values into their slots of the page pools (emel_op_paged_kv_append)."""
+    """Writes new tokens' keys and values into their slots of the page pools (emel_op_paged_kv_append).
+
+    Pools hold halves (F16, BF16), or packed rows (Q8_0, Q4_0: Layout.packed), which quantises them."""
 
     __slots__ = ()
     _fn = "emel_op_paged_kv_append"
 
     def __init__(self, k: TensorView, v: TensorView, slots: TensorView, k_pages: TensorViewMut, v_pages: TensorViewMut):
         self._bind((k, v, slots, k_pages, v_pages))
+
+
+class OpPagedKvRead(_Event):
+    """Keys and values of the slots named, read back from the page pools as f32 (emel_op_paged_kv_read)."""
+
+    __slots__ = ()
+    _fn = "emel_op_paged_kv_read"
+
+    def __init__(self, k_pages: TensorView, v_pages: TensorView, slots: TensorView, k: TensorViewMut, v: TensorViewMut):
+        self._bind((k_pages, v_pages, slots, k, v))
 
 
 class OpPagedAttention(_Event):

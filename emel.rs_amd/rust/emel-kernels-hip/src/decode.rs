@@ -126,7 +126,8 @@ impl HipEvent for OpRope<'_> {
     }
 }
 
-/// Writes new tokens' keys and values into their slots of the page pools.
+/// Writes new tokens' keys and values into their slots of the page pools, as
+/// halves or packed rows.
 #[derive(Debug)]
 pub struct OpPagedKvAppend<'a> {
     k: DeviceView<'a>,
@@ -159,6 +160,42 @@ impl HipEvent for OpPagedKvAppend<'_> {
         // SAFETY: live device views, checked by the library; the kernel skips
         // slots outside the pools.
         HipError::check(kernel.call(|s| unsafe { ffi::emel_op_paged_kv_append(k, v, t, kp, vp, s) }))
+    }
+}
+
+/// Keys and values of the slots named, read back from the page pools as f32.
+#[derive(Debug)]
+pub struct OpPagedKvRead<'a> {
+    k_pages: DeviceView<'a>,
+    v_pages: DeviceView<'a>,
+    slots: DeviceView<'a>,
+    k: DeviceViewMut<'a>,
+    v: DeviceViewMut<'a>,
+}
+
+impl<'a> OpPagedKvRead<'a> {
+    /// Creates the event; validation occurs when it is dispatched.
+    #[must_use]
+    pub const fn new(
+        k_pages: DeviceView<'a>,
+        v_pages: DeviceView<'a>,
+        slots: DeviceView<'a>,
+        k: DeviceViewMut<'a>,
+        v: DeviceViewMut<'a>,
+    ) -> Self {
+        Self { k_pages, v_pages, slots, k, v }
+    }
+}
+
+impl HipEvent for OpPagedKvRead<'_> {
+    type Output = Result<(), HipError>;
+
+    fn dispatch(self, kernel: &mut HipKernel) -> Self::Output {
+        let (kp, vp, t) = (self.k_pages.as_ffi(), self.v_pages.as_ffi(), self.slots.as_ffi());
+        let (k, v) = (self.k.as_ffi(), self.v.as_ffi());
+        // SAFETY: live device views, checked by the library; the kernel skips
+        // slots outside the pools.
+        HipError::check(kernel.call(|s| unsafe { ffi::emel_op_paged_kv_read(kp, vp, t, k, v, s) }))
     }
 }
 

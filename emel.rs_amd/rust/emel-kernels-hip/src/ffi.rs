@@ -404,6 +404,7 @@ unsafe extern "C" {
     pub fn emel_op_mul_mat_q4_k(weights: *const EmelTensorView, x: *const EmelTensorView, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_op_rope(request: *const EmelRopeRequest, stream: Stream) -> Status;
     pub fn emel_op_paged_kv_append(k: *const EmelTensorView, v: *const EmelTensorView, slots: *const EmelTensorView, k_pages: *const EmelTensorViewMut, v_pages: *const EmelTensorViewMut, stream: Stream) -> Status;
+    pub fn emel_op_paged_kv_read(k_pages: *const EmelTensorView, v_pages: *const EmelTensorView, slots: *const EmelTensorView, k: *const EmelTensorViewMut, v: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_op_paged_attention(q: *const EmelTensorView, k_pages: *const EmelTensorView, v_pages: *const EmelTensorView, page_table: *const EmelTensorView, lengths: *const EmelTensorView, scale: f32, window: u64, soft_cap: f32, dst: *const EmelTensorViewMut, stream: Stream) -> Status;
     pub fn emel_generic_dispatch(request: *const EmelGenericRequest, stream: Stream) -> Status;
     pub fn emel_sample_temperature_top_k(request: *const EmelSampleTemperatureTopKRequest, stream: Stream) -> Status;

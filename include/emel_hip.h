@@ -590,18 +590,37 @@ emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream);
 
 /* ---- paged key-value cache ---------------------------------------------------------
  * No counterpart in the pinned path.  The cache is two pools of pages, one for
- * keys and one for values: F16 or BF16 views [dim, page, kv_heads, pages]
- * with nb[0] == 2 and any other strides (a token's heads side by side, or a
- * head's tokens, or both pools interleaved in one allocation), the same type
- * and extents for both.  Slot p * page + t is token t of page p.
+ * keys and one for values, of the same extents: views [dim, page, kv_heads, pages]
+ * of halves (F16 or BF16, the same for both, nb[0] == 2) or of packed rows
+ * (each Q8_0 or Q4_0, nb[0] == 1, dim a multiple of 32), with any other strides
+ * that are multiples of 2 (a token's heads side by side, or a head's tokens, or
+ * both pools interleaved in one allocation).  Slot p * page + t is token t of page p.
+ *
+ * A packed row is one token's head: B = dim / 32 blocks of 32 values, each
+ * an f16 scale d and whole numbers n, of which value d n is made.  It has the bytes of
+ * a Q8_0 or Q4_0 row (34 or 18 a block) in an order of the cache's own.  The numbers
+ * come first, by eights: the first eight of every block, then the second, third and
+ * fourth of every one; value 32 b + 8 g + i is of eight g B + b.  In Q8_0 an eight
+ * is its numbers as eight signed bytes; in Q4_0 n + 8 takes four bits, and an
+ * eight is four bytes that hold, low bits first, values 0 2, 4 6, 1 3 and 5 7.  The
+ * B scales follow.  A scale that is not finite stands for NaN.
  *
  * emel_op_paged_kv_append writes token t's keys k[:, :, t] and values
- * v[:, :, t] (F32 [dim, kv_heads, tokens, 1]), rounded to the nearest half,
- * into slot slots[t] (I32 [tokens, 1, 1, 1], device memory).  A slot that is
+ * v[:, :, t] (F32 [dim, kv_heads, tokens, 1]), rounded to the nearest half or
+ * packed, into slot slots[t] (I32 [tokens, 1, 1, 1], device memory).  A slot that is
  * negative or past the pool skips its token; of tokens with the same slot
  * the last one is stored.  To know it, up to 2^17 tokens are compared with one
  * another: that is little beside the copy up to 2^15 tokens of 1024 values (106 us),
- * and 8 ns a token from 2^17 on, however narrow a token is.
+ * and 8 ns a token from 2^17 on, however narrow a token is.  Packed, a block's scale is
+ * its largest magnitude / 127 (Q8_0), or its value of largest magnitude, the
+ * first of equal ones, / -8 (Q4_0), rounded to f32 and then to f16, at most
+ * 65504; a number is the nearest to x / d, ties to even, within -127 .. 127
+ * resp. -8 .. 7, and 0 where d is 0.  A block with an infinity or a NaN becomes
+ * NaN (d = 0x7e00, numbers 0).
+ *
+ * emel_op_paged_kv_read writes what slot slots[t] holds to k[:, :, t] and v[:, :, t]
+ * (F32 [dim, kv_heads, tokens, 1]), exactly; a slot that is negative or
+ * past the pool leaves its token as it was.  A slot may be named any number of times.
  *
  * emel_op_paged_attention attends from one new token of each sequence:
  *   dst[:, h, s] = sum over j of softmax_j(f(scale q[:, h, s] . k_j)) v_j
@@ -611,8 +630,8 @@ emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream);
  * dst are F32 [dim, heads, seqs, 1]; heads is a multiple of kv_heads, and
  * head h reads cache head h / (heads / kv_heads).  Position j of sequence s
  * is token j % page of page page_table[j / page, s] (I32 [max pages, seqs, 1,
- * 1]); lengths is I32 [seqs, 1, 1, 1].  dim is a multiple of 8, at most 256
- * (else UNSUPPORTED_OPERATION).  Both index tensors are device memory, read
+ * 1]); lengths is I32 [seqs, 1, 1, 1].  dim is a multiple of 8 (of 32 for packed rows), at
+ * most 256 (else UNSUPPORTED_OPERATION).  Both index tensors are device memory, read
  * when the kernel runs, so a captured call follows them.  A sequence of
  * length 0 gets zeros.  One whose length is negative or past max pages * page, or that
  * reaches a page id outside the pool, gets NaN, and nothing outside the pool
@@ -621,18 +640,23 @@ emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream);
  * softmax weights keep 24 bits in products with BF16 halves.  With F16 halves
  * they keep 22, down to 2^-16 of the head's largest element of q or of its
  * largest weight, and 2^-39 of that below; and F16 halves below 2^-14, which are
- * subnormal, count to about 2^-38 of what they are multiplied by.
+ * subnormal, count to about 2^-38 of what they are multiplied by.  Packed rows'
+ * numbers are exact in their products; q keeps 22 bits as with F16, and so does a weight
+ * by its block's scale, relative to the largest such product of that block of dims.
  * Wants the stream's workspace, which grows as the reductions' does: graphs
  * captured from one stream share it, and run one after the other, or are
  * captured from streams of their own.
  *
- * Guards of both: as mul_mat_q4_0; parameters that are not finite, or a
+ * Guards of all: as mul_mat_q4_0; parameters that are not finite, or a
  * negative soft_cap, are INVALID_PARAMETERS; dim * kv_heads past 2^26 in an
- * append, and max pages * page past 2^31 - 1, or 2^31 units of 128 tokens for one
+ * append or a read, and max pages * page past 2^31 - 1, or 2^31 units of 128 tokens for one
  * sequence's cache heads, in an attention, UNSUPPORTED_OPERATION. */
 emel_status emel_op_paged_kv_append(const emel_tensor_view *k, const emel_tensor_view *v,
                                     const emel_tensor_view *slots, const emel_tensor_view_mut *k_pages,
                                     const emel_tensor_view_mut *v_pages, emel_stream stream);
+emel_status emel_op_paged_kv_read(const emel_tensor_view *k_pages, const emel_tensor_view *v_pages,
+                                  const emel_tensor_view *slots, const emel_tensor_view_mut *k,
+                                  const emel_tensor_view_mut *v, emel_stream stream);
 emel_status emel_op_paged_attention(const emel_tensor_view *q, const emel_tensor_view *k_pages,
                                     const emel_tensor_view *v_pages, const emel_tensor_view *page_table,
                                     const emel_tensor_view *lengths, float scale, uint64_t window, float soft_cap,
