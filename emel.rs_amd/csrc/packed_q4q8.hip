@@ -1,0 +1,8 @@
+// packed_q4q8.hip -- the attention over pages of Q4_0 keys and Q8_0 values.
+#include "packed_attn.hpp"
+
+namespace emel {
+
+template hipError_t packed_attn<PaPages::Q4Q8>(const PagedAttnArgs &, const PaPlan &, uint32_t, uint32_t, hipStream_t);
+
+} // namespace emel

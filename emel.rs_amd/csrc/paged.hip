@@ -73,12 +73,6 @@ __global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a, FastDiv
 // the scale as it is stored: the quotient by 1/d is off by one at most, and
 // x - n d, which is exact in f32 (x is a multiple of 2^-25 d or below d / 2), says so.
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_f32(float v)
-{
-    return __builtin_bit_cast(float, dpp32<CTRL>(__builtin_bit_cast(uint32_t, v)));
-}
-
 // The nearest whole number of scales in x, ties to even; inv is 1 / d or near it.
 __device__ __forceinline__ float nearest(float x, float d, float inv)
 {
@@ -306,8 +300,34 @@ PaPages pa_pages(const PagedAttnArgs &a)
 // Workgroups that run at once, by registers and LDS, and their LDS: more would
 // wait for a second round with as large a run each.
 struct PaGrid {
-    uint32_t workgroups, few, lds;
+    uint32_t workgroups, few, side, lds;
 };
+
+// Packed rows side by side: as many as the rows and a die's workgroups divide by.
+uint32_t pa_side(const PagedAttnArgs &a, uint32_t workgroups)
+{
+    if (!a.k_pool.packed()) return 1;
+    const uint64_t group = a.heads / a.kv_heads, rows = a.kv_heads * ((group + 15) / 16);
+    uint32_t side = 1;
+    while (side < 8 && rows % (2 * side) == 0 && workgroups % (2 * side * kDies) == 0) side *= 2;
+    return side;
+}
+
+// Columns of a packed row's head: as many as 16 columns and its blocks allow.
+uint32_t pa_fold(const PagedAttnArgs &a)
+{
+    const uint32_t group = a.heads / a.kv_heads;
+    uint32_t f = 8;
+    while (f > 1 && (f / 2 >= a.dim / 32 || group * f > 16)) f /= 2;
+    return f;
+}
+
+// Floats of a workspace slot.
+uint32_t pa_slot(const PagedAttnArgs &a)
+{
+    return 2 * kPaLead + pa_heads(a) * a.dim;
+}
+
 PaGrid pa_grid(const PagedAttnArgs &a)
 {
     static const uint32_t cus = [] {
@@ -316,12 +336,16 @@ PaGrid pa_grid(const PagedAttnArgs &a)
             n = 256;
         return static_cast<uint32_t>(n);
     }();
-    const uint32_t ks = (a.dim + 31) / 32, fixed = 4096 + ks * 3 * 1024;
+    const uint32_t ks = (a.dim + 31) / 32, fixed = a.k_pool.packed() ? 4096 + ks * 1024 : 4096 + ks * 3 * 1024;
+    const uint32_t sets = (ks + pa_fold(a) - 1) / pa_fold(a);
+    const uint32_t planes = a.k_pool.packed() ? sets * 2 * (kWave + 1) * 4 : 0; // of score operands
     uint32_t per = pa_per_cu(pa_pages(a), static_cast<int>(ks));
     for (;; --per) {
-        const uint32_t joined = 4 * pa_heads(a) * (a.dim + 4), weights = pa_heads(a) * cus * per;
-        const uint32_t lds = 4 * (joined > weights ? joined : weights);
-        if (per == 1 || per * (fixed + lds) <= 160 * 1024) return {cus * per, cus * (per < 2 ? per : 2), lds};
+        const uint32_t side = pa_side(a, cus * per);
+        const uint32_t joined = 4 * pa_heads(a) * (a.dim + 4), weights = (a.k_pool.packed() ? kPaLead : 0) + pa_heads(a) * (cus * per / side);
+        uint32_t lds = 4 * (joined > weights ? joined : weights);
+        if (lds < 4 * planes) lds = 4 * planes;
+        if (per == 1 || per * (fixed + lds) <= 160 * 1024) return {cus * per, cus * (per < 2 ? per : 2), side, lds};
     }
 }
 
@@ -346,7 +370,7 @@ hipError_t pa_launch(const PagedAttnArgs &a, const PaPlan &pl, uint32_t grid, ui
 PagedScratch paged_attn_scratch(const PagedAttnArgs &a)
 {
     const uint64_t n = pa_grid(a).workgroups;
-    return {n * 2 * (32 + static_cast<uint64_t>(pa_heads(a)) * a.dim) * sizeof(float), n * kPaLine * sizeof(uint32_t)};
+    return {n * 2 * pa_slot(a) * sizeof(float), n * kPaLine * sizeof(uint32_t)};
 }
 
 uint32_t paged_attn_seqs(const PagedAttnArgs &a)
@@ -366,9 +390,10 @@ hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream)
     pl.hgroups = FastDiv((pl.group + 15) / 16);
     pl.rows = a.kv_heads * pl.hgroups.d;
     const PaGrid grid = pa_grid(a);
-    pl.grid = FastDiv(grid.workgroups);
+    pl.side = grid.side;
+    pl.grid = FastDiv(grid.workgroups / pl.side);
     pl.few = FastDiv(grid.few);
-    pl.slot = 32 + pa_heads(a) * a.dim;
+    pl.slot = pa_slot(a);
     pl.parts = static_cast<float *>(a.workspace);
     pl.arrived = static_cast<uint32_t *>(a.counters);
     // units are counted in 32 bits: a batch with more of them runs in parts
@@ -380,11 +405,16 @@ hipError_t launch_paged_attn(const PagedAttnArgs &a, hipStream_t stream)
         b.y = a.y + static_cast<int64_t>(s) * a.y_st[2];
         b.table = a.table + static_cast<int64_t>(s) * a.table_st[1];
         b.lengths = a.lengths + static_cast<int64_t>(s) * a.lengths_st;
-        const PaPages pages = pa_pages(a);
+        hipError_t e = hipSuccess;
         const uint32_t n = grid.workgroups, lds = grid.lds;
-        const hipError_t e = pages == PaPages::F16    ? pa_launch<PaPages::F16>(b, pl, n, lds, stream)
-                             : pages == PaPages::Bf16 ? pa_launch<PaPages::Bf16>(b, pl, n, lds, stream)
-                                                      : launch_packed_attn(pages, b, pl, n, lds, stream);
+        switch (pa_pages(a)) {
+        case PaPages::F16: e = pa_launch<PaPages::F16>(b, pl, n, lds, stream); break;
+        case PaPages::Bf16: e = pa_launch<PaPages::Bf16>(b, pl, n, lds, stream); break;
+        case PaPages::Q8Q8: e = packed_attn<PaPages::Q8Q8>(b, pl, n, lds, stream); break;
+        case PaPages::Q8Q4: e = packed_attn<PaPages::Q8Q4>(b, pl, n, lds, stream); break;
+        case PaPages::Q4Q8: e = packed_attn<PaPages::Q4Q8>(b, pl, n, lds, stream); break;
+        case PaPages::Q4Q4: e = packed_attn<PaPages::Q4Q4>(b, pl, n, lds, stream); break;
+        }
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

@@ -27,6 +27,12 @@ __device__ __forceinline__ float from_half(uint16_t h)
     else return static_cast<float>(__builtin_bit_cast(_Float16, h));
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v)
+{
+    return __builtin_bit_cast(float, dpp32<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+
 // A block's scale: what is not finite stands for NaN.
 __device__ __forceinline__ float pk_scale(uint16_t bits)
 {
@@ -37,6 +43,8 @@ __device__ __forceinline__ float pk_scale(uint16_t bits)
 // ---- attention -----------------------------------------------------------------------------
 
 constexpr uint32_t kPaUnit = 128;  // tokens of a unit, 32 a wave
+constexpr uint32_t kPaLead = 16;   // packed: heads of a row
+constexpr uint32_t kDies = 8;      // that blocks are dealt to in turn
 constexpr uint32_t kPaLine = 64;   // words between arrival counters (a cache line each)
 
 // What the pages of keys and of values hold.
@@ -54,12 +62,14 @@ struct PaPlan {
     uint32_t group;     // query heads of a cache head
     uint32_t rows;      // rows of a sequence: kv_heads * hgroups
     uint32_t slot;      // floats of a workspace slot
+    uint32_t side;      // packed: rows side by side
     float *parts;       // 2 slots a workgroup
     uint32_t *arrived;  // a counter per workgroup, zero between launches
 };
 
-hipError_t launch_packed_attn(PaPages pages, const PagedAttnArgs &args, const PaPlan &plan, uint32_t grid, uint32_t lds,
-                              hipStream_t stream);
+// The launch over packed pages, a source for each pair of types.
+template <PaPages PAGES>
+hipError_t packed_attn(const PagedAttnArgs &args, const PaPlan &plan, uint32_t grid, uint32_t lds, hipStream_t stream);
 
 // ---- new tokens ------------------------------------------------------------------------------
 

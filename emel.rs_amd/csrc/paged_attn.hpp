@@ -92,40 +92,43 @@ __device__ __forceinline__ void split(float x, uint32_t part[3])
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ uint32_t pk_low(uint32_t x, float less)
+// `magic` is twice the half 1024.
+
+__device__ __forceinline__ uint32_t pk_low(uint32_t x, float less, uint32_t magic)
 {
     const _Float16 l = static_cast<_Float16>(less);
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, x | 0x64006400u) - v2h{l, l});
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, x | magic) - v2h{l, l});
 }
-__device__ __forceinline__ uint32_t pk_high(uint32_t x)
+__device__ __forceinline__ uint32_t pk_high(uint32_t x, uint32_t magic)
 {
-    const v2h y = __builtin_bit_cast(v2h, x | 0x64006400u), part = {0.0625f16, 0.0625f16}, less = {-72.0f16, -72.0f16};
+    const v2h y = __builtin_bit_cast(v2h, x | magic), part = {0.0625f16, 0.0625f16}, less = {-72.0f16, -72.0f16};
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(y, part, less));
 }
 
 // An eight of Q4_0, and of Q8_0, in order.
-__device__ __forceinline__ u4 pk_halves4(uint32_t w)
+__device__ __forceinline__ u4 pk_halves4(uint32_t w, uint32_t magic)
 {
     const uint32_t s = w >> 8;
-    return u4{pk_low(w & 0x000f000fu, 1032.0f), pk_high(w & 0x00f000f0u), pk_low(s & 0x000f000fu, 1032.0f), pk_high(s & 0x00f000f0u)};
+    return u4{pk_low(w & 0x000f000fu, 1032.0f, magic), pk_high(w & 0x00f000f0u, magic), pk_low(s & 0x000f000fu, 1032.0f, magic),
+              pk_high(s & 0x00f000f0u, magic)};
 }
-__device__ __forceinline__ u4 pk_halves8(uint32_t w0, uint32_t w1)
+__device__ __forceinline__ u4 pk_halves8(uint32_t w0, uint32_t w1, uint32_t magic)
 {
     w0 ^= 0x80808080u;
     w1 ^= 0x80808080u;
-    return u4{pk_low(__builtin_amdgcn_perm(0, w0, 0x0c010c00u), 1152.0f), pk_low(__builtin_amdgcn_perm(0, w0, 0x0c030c02u), 1152.0f),
-              pk_low(__builtin_amdgcn_perm(0, w1, 0x0c010c00u), 1152.0f), pk_low(__builtin_amdgcn_perm(0, w1, 0x0c030c02u), 1152.0f)};
+    return u4{pk_low(__builtin_amdgcn_perm(0, w0, 0x0c010c00u), 1152.0f, magic), pk_low(__builtin_amdgcn_perm(0, w0, 0x0c030c02u), 1152.0f, magic),
+              pk_low(__builtin_amdgcn_perm(0, w1, 0x0c010c00u), 1152.0f, magic), pk_low(__builtin_amdgcn_perm(0, w1, 0x0c030c02u), 1152.0f, magic)};
 }
 
 // One value of two tokens: the byte that `pick` takes of each, and of Q4_0 its j-th nibble.
-__device__ __forceinline__ uint32_t pk_pair4(uint32_t a, uint32_t b, uint32_t pick, int j)
+__device__ __forceinline__ uint32_t pk_pair4(uint32_t a, uint32_t b, uint32_t pick, int j, uint32_t magic)
 {
     const uint32_t x = __builtin_amdgcn_perm(b, a, pick);
-    return j ? pk_high(x & 0x00f000f0u) : pk_low(x & 0x000f000fu, 1032.0f);
+    return j ? pk_high(x & 0x00f000f0u, magic) : pk_low(x & 0x000f000fu, 1032.0f, magic);
 }
-__device__ __forceinline__ uint32_t pk_pair8(uint32_t a, uint32_t b, uint32_t pick)
+__device__ __forceinline__ uint32_t pk_pair8(uint32_t a, uint32_t b, uint32_t pick, uint32_t magic)
 {
-    return pk_low(__builtin_amdgcn_perm(b, a, pick) ^ 0x00800080u, 1152.0f);
+    return pk_low(__builtin_amdgcn_perm(b, a, pick) ^ 0x00800080u, 1152.0f, magic);
 }
 
 // Value d of a packed row.
@@ -227,9 +230,144 @@ __device__ __forceinline__ float pa_weight(float m, float ref)
     return __builtin_amdgcn_exp2f(m - (ref == -__builtin_inff() ? 0.0f : ref));
 }
 
+// ---- the end of a packed segment -------------------------------------------------------------
+//
+// The waves' parts joined into the result, or into this workgroup's slot of the
+// workspace and by the last workgroup of the row from all slots, as the halves'
+// rows end; a slot is the heads' maxima, their sums and values.
+
+struct PaEnd {
+    bool empty, whole;
+    uint32_t heads, h0, s, w0, lane_row, pieces; // w0: the row's first bundle
+};
+
+__device__ __forceinline__ void pa_ends(const PagedAttnArgs &a, const PaPlan &pl, const PaEnd &n, float *slot, float *joined,
+                                        const float *wm, const float *wl, uint32_t *last, uint32_t tid)
+{
+    constexpr uint32_t kWaves = kBlock / kWave;
+    const uint32_t dim = a.dim, pitch = dim + 4, all = n.heads, cells = all * dim;
+    float *out = a.y + static_cast<int64_t>(n.h0) * a.y_st[1] + static_cast<int64_t>(n.s) * a.y_st[2];
+    auto put = [&](uint32_t h, uint32_t d, float x, float y) {
+        float *o = out + static_cast<int64_t>(d) * a.y_st[0] + static_cast<int64_t>(h) * a.y_st[1];
+        o[0] = x;
+        o[a.y_st[0]] = y;
+    };
+    // the waves' maximum and sum of a head, and each wave's weight
+    auto join = [&](uint32_t h, float f[kWaves], float &sum) {
+        float top = wm[h];
+        for (uint32_t w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, wm[w * 16 + h]);
+        sum = 0.0f;
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            f[w] = pa_weight(wm[w * 16 + h], top);
+            sum += wl[w * 16 + h] * f[w];
+        }
+        return top;
+    };
+    for (uint32_t e = 2 * tid; e < cells; e += 2 * kBlock) {
+        const uint32_t h = pl.dim.div(e), d = e - h * dim;
+        float f[kWaves], sum, x = 0.0f, y = 0.0f;
+        join(h, f, sum);
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            const float *from = joined + (w * all + h) * pitch + d;
+            x += from[0] * f[w];
+            y += from[1] * f[w];
+        }
+        if (!n.whole) pa_store2(slot + 2 * kPaLead + e, x, y);
+        else if (n.empty) put(h, d, 0.0f, 0.0f);
+        else put(h, d, x * (1.0f / sum), y * (1.0f / sum));
+    }
+    if (__builtin_expect(n.whole, 0)) return;
+    if (tid < all) {
+        float f[kWaves], sum;
+        pa_store(slot + tid, join(tid, f, sum));
+        pa_store(slot + kPaLead + tid, sum);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t *arrived = pl.arrived + static_cast<size_t>(n.w0 * pl.side + n.lane_row) * kPaLine;
+        *last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n.pieces - 1;
+        if (*last) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!*last) return;
+    // Short code, as a row's last workgroup is the only one that runs it: what it
+    // would take longest for is instructions that no cache holds.
+    const uint32_t pieces = n.pieces;
+    const size_t stride = static_cast<size_t>(2) * pl.side * pl.slot;
+    const float *from = pl.parts + static_cast<size_t>(2 * (n.w0 * pl.side + n.lane_row)) * pl.slot;
+    auto piece = [&](uint32_t p) { return from + p * stride + (p == 0 ? pl.slot : 0); };
+    float *jl = joined, *weight = joined + kPaLead; // each head's sum, [piece][head]
+    constexpr uint32_t kAtOnce = 16;
+    float2 v[kAtOnce] = {};
+    auto ask = [&](uint32_t p0, uint32_t e) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i)
+            if (p0 + i < pieces) v[i] = pa_load2(piece(p0 + i) + 2 * kPaLead + e);
+    };
+    // The first loads of everything go out together: the thread's first pair,
+    // maxima and sums (16 threads a head).
+    if (2 * tid < cells) ask(0, 2 * tid);
+    const uint32_t h1 = tid / 16 < all ? tid / 16 : 0, i1 = tid % 16;
+    float pm[4], ps[4], top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t p = i1 + 16 * i;
+        pm[i] = p < pieces ? pa_load(piece(p) + h1) : -__builtin_inff();
+        ps[i] = p < pieces ? pa_load(piece(p) + kPaLead + h1) : 0.0f;
+        top = __builtin_fmaxf(top, pm[i]);
+    }
+#pragma unroll 1
+    for (uint32_t p = i1 + 64; p < pieces; p += 16) top = __builtin_fmaxf(top, pa_load(piece(p) + h1));
+    for (int d = 8; d > 0; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 16));
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const float f = pa_weight(pm[i], top);
+        sum += ps[i] * f;
+        if (i1 + 16 * i < pieces) weight[(i1 + 16 * i) * all + h1] = f;
+    }
+#pragma unroll 1
+    for (uint32_t p = i1 + 64; p < pieces; p += 16) {
+        const float f = pa_weight(pa_load(piece(p) + h1), top);
+        sum += pa_load(piece(p) + kPaLead + h1) * f;
+        weight[p * all + h1] = f;
+    }
+    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 16);
+    if (i1 == 0 && tid / 16 < all) jl[h1] = sum;
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t e = 2 * tid; e < cells; e += 2 * kBlock) {
+        const uint32_t h = pl.dim.div(e);
+        const float *f = weight + h;
+        float x = 0.0f, y = 0.0f;
+#pragma unroll 1
+        for (uint32_t p0 = 0; p0 < pieces; p0 += kAtOnce) {
+            if (p0 > 0 || e != 2 * tid) ask(p0, e);
+#pragma unroll
+            for (uint32_t i = 0; i < kAtOnce; ++i, f += all)
+                if (p0 + i < pieces) {
+                    x += v[i].x * *f;
+                    y += v[i].y * *f;
+                }
+        }
+        const float scale = 1.0f / jl[h];
+        put(h, e - h * dim, n.empty ? 0.0f : x * scale, n.empty ? 0.0f : y * scale);
+    }
+}
+
 // KS: 32-dim steps of a score; VW: dims of a lane's values (4, 8, 12 or 16; 2
 // KS of packed pages).
-template <PaPages PAGES, int KS, int VW>
+// FOLD: of packed pages, the columns of a product that a head takes (1, 2, 4 or
+// 8, with 16 columns for all heads of a row); 0 of halves.  Column p of a head stands for every
+// block b with b % FOLD == p.  Its query is 0 in the other blocks, so what the
+// products of a set of FOLD consecutive blocks add up in it is one block's part of a
+// score, to be scaled by that block; a head's columns are added last.  Its weights
+// are by the scales of its own block of a set, and of the rows of a set's values only
+// those of that block count, the others are never looked at.  A lane so scales and splits
+// 8 weights a set and step, not a block and step, and its rows may be of any of a set's
+// blocks: it loads what lies side by side.  All of that costs as many matrix instructions
+// as FOLD 1 does.
+template <PaPages PAGES, int KS, int VW, int FOLD = 0>
 __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
 {
     constexpr bool BF16 = PAGES == PaPages::Bf16, PACKED = PAGES > PaPages::Bf16;
@@ -238,9 +376,17 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
     constexpr bool K4 = PAGES >= PaPages::Q4Q8, V4 = PAGES == PaPages::Q8Q4 || PAGES == PaPages::Q4Q4;
     constexpr int KI = K4 ? 8 : 16, VI = V4 ? 8 : 16; // packed: halves of a block's whole numbers
     constexpr int kAcc = PACKED ? 2 * KS : VW;
+    constexpr int F = PACKED ? FOLD : 1, kSets = PACKED ? (KS + F - 1) / F : 1;
+    // packed: blocks of set e; words that a lane loads of a token's, and of those before
+    constexpr auto blocks_of = [](int e) { return e < KS / F ? F : KS - e * F; };
+    constexpr auto words_of = [](int n) { return V4 ? (n + 3) / 4 : (n + 1) / 2; };
+    constexpr int kWords = PACKED ? KS / F * words_of(F) + (KS % F ? words_of(KS % F) : 0) : 1;
     constexpr float kLift = BF16 ? 0.0f : 14.0f;
-    extern __shared__ __attribute__((aligned(16))) float joined[];            // [wave][head of the group][dim]
-    __shared__ u4 qop[KS * P * kWave];           // score operands, lane after lane
+    // [wave][head of the group][dim]; packed: before that the score operands, by
+    // planes of 64 lanes and a zero
+    extern __shared__ __attribute__((aligned(16))) float joined[];
+    __shared__ u4 qop[PACKED ? 1 : KS * P * kWave]; // score operands, lane after lane
+    constexpr uint32_t kPlane = kWave + 1;
     __shared__ int64_t off[kWaves][2][32];       // a step's tokens in the key and value pools
     __shared__ float scales[PACKED ? kWaves : 1][2][PACKED ? KS : 1][32]; // packed: of their blocks
     __shared__ float wm[kWaves][16], wl[kWaves][16], jl[16];
@@ -252,10 +398,16 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
     // Rows of a few units are mostly set-up, which more workgroups hide; long
     // ones stream best with two a compute unit (64 sequences of 90 to 9000
     // tokens 106 us, 113 with three; 640 of 100 tokens 90 us, 77 with three).
-    auto share_of = [&](uint32_t units) { return units > 4 * a.seqs ? pl.few : pl.grid; };
+    auto share_of = [&](uint32_t units) { return !PACKED && units > 4 * a.seqs ? pl.few : pl.grid; };
     // This workgroup's run of units, and the sequence it starts in.  A row's
     // set-up and end cost about a unit: it counts as one more, but where there
     // is no more than a unit to a workgroup (that would only part the rows).
+    // Packed rows are short, and a token's heads share cache lines: `side` rows
+    // go to as many workgroups of one die, which walk the same tokens at one time
+    // (blocks are dealt to eight dies in turn).  `block` counts such bundles.
+    const uint32_t turn = blockIdx.x / kDies, lane_row = PACKED ? turn % pl.side : 0;
+    const uint32_t block = PACKED ? turn / pl.side * kDies + blockIdx.x % kDies : blockIdx.x;
+    const uint32_t rows = PACKED ? pl.rows / pl.side : pl.rows;
     const uint32_t first_lane = thread % kWave;
     uint32_t total, run, cur, base; // base: the sequence's first unit
     uint32_t s, setup;
@@ -266,14 +418,14 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         uint32_t pre = wave_scan(mine);
         const uint32_t all = lane_u32(pre, kWave - 1);
         const FastDiv share = share_of(all);
-        setup = all * pl.rows > share.d;
-        total = (all + setup * a.seqs) * pl.rows;
+        setup = all * rows > share.d;
+        total = (all + setup * a.seqs) * rows;
         pre += setup * (first_lane + 1);
         run = share.div(total + share.d - 1);
-        cur = blockIdx.x * run;
+        cur = block * run;
         if (cur >= total) return;
-        s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__popcll(__ballot(first_lane < a.seqs && pre * pl.rows <= cur))));
-        base = lane_u32(pre - mine - setup, s) * pl.rows;
+        s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__popcll(__ballot(first_lane < a.seqs && pre * rows <= cur))));
+        base = lane_u32(pre - mine - setup, s) * rows;
         s_len = static_cast<int32_t>(lane_u32(static_cast<uint32_t>(len), s));
     } else {
         const uint32_t per = (a.seqs + kBlock - 1) / kBlock;
@@ -290,17 +442,17 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
             all += scan[w];
         }
         const FastDiv share = share_of(all);
-        setup = all * pl.rows > share.d;
+        setup = all * rows > share.d;
         pre += setup * s0 - mine;
         mine += setup * (s1 - s0);
-        total = (all + setup * a.seqs) * pl.rows;
+        total = (all + setup * a.seqs) * rows;
         run = share.div(total + share.d - 1);
-        cur = blockIdx.x * run;
+        cur = block * run;
         if (cur >= total) return;
-        if (mine && pre * pl.rows <= cur && cur < (pre + mine) * pl.rows) {
+        if (mine && pre * rows <= cur && cur < (pre + mine) * rows) {
             uint32_t i = s0;
 #pragma unroll 1
-            for (uint32_t u = pa_seq(a, pa_len(a, i)).units + setup; (pre + u) * pl.rows <= cur; u = pa_seq(a, pa_len(a, i)).units + setup) {
+            for (uint32_t u = pa_seq(a, pa_len(a, i)).units + setup; (pre + u) * rows <= cur; u = pa_seq(a, pa_len(a, i)).units + setup) {
                 pre += u;
                 ++i;
             }
@@ -309,7 +461,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         }
         __syncthreads();
         s = found[0];
-        base = found[1] * pl.rows;
+        base = found[1] * rows;
         s_len = pa_len(a, s);
     }
     const uint32_t end = cur + run < total ? cur + run : total;
@@ -326,11 +478,13 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         uint32_t tid = thread;
         asm volatile("" : "+v"(tid));
         const uint32_t lane = tid % kWave, col = lane % 16, g = lane / 16;
-        // packed: the bytes of a word of two tokens that hold the lane's values
-        const uint32_t pick = 0x0c040c00u + (V4 ? col % 4 : col % 2 * 2) * 0x10001u;
+        // the head of a column, and which of each set's blocks it stands for
+        const uint32_t head = col / F, part = col % F, quarter = col % 4;
         const uint32_t n0 = cur - row_at, n1 = end - row_at < units ? end - row_at : units;
         const uint32_t u0 = n0 > setup ? n0 - setup : 0, u1 = n1 - setup;
-        const uint32_t kh = pl.hgroups.div(row), h0 = kh * pl.group + (row - kh * pl.hgroups.d) * 16;
+        if (PACKED && n1 <= setup) break; // a row's start, whose units are all another's
+        const uint32_t mine = PACKED ? row * pl.side + lane_row : row;
+        const uint32_t kh = pl.hgroups.div(mine), h0 = kh * pl.group + (mine - kh * pl.hgroups.d) * 16;
         const uint32_t heads = (kh + 1) * pl.group - h0 < 16 ? (kh + 1) * pl.group - h0 : 16;
 
         const uint16_t *kbase = a.k_pool.data + static_cast<int64_t>(kh) * a.k_pool.st_head;
@@ -349,17 +503,18 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         auto page_of = [&](uint32_t t) {
             return t < t_end ? table[static_cast<int64_t>(pl.page.div(sq.first + t)) * a.table_st[0]] : 0;
         };
-        int32_t next = page_of(t0 + lane % 32);
+        int32_t next = PACKED ? 0 : page_of(t0 + lane % 32);
 
         // score operands, lane (col, g): dims 32 e + 8 g .. + 7 of head col;
         // each wave lays out every fourth e
         float inv = 1.0f;
+        u4 *planes = reinterpret_cast<u4 *>(joined);
         {
-            const float *q = a.q + static_cast<int64_t>(h0 + col) * a.q_st[1] + static_cast<int64_t>(s) * a.q_st[2];
+            const float *q = a.q + static_cast<int64_t>(h0 + head) * a.q_st[1] + static_cast<int64_t>(s) * a.q_st[2];
             const float c = a.soft_cap > 0.0f ? a.scale / a.soft_cap : a.scale * 1.44269504088896340736f;
             auto eight = [&](uint32_t e, float x[8]) {
                 const uint32_t d = 32 * e + 8 * g;
-                if (col < heads && d < dim) {
+                if (head < heads && d < dim) {
                     if (__builtin_expect(a.q_st[0] == 1, 1)) {
                         const v4f lo = *reinterpret_cast<const v4f_any *>(q + d), hi = *reinterpret_cast<const v4f_any *>(q + d + 4);
                         for (int i = 0; i < 4; ++i) {
@@ -367,19 +522,39 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                             x[4 + i] = hi[i] * c;
                         }
                     } else {
-                        for (int i = 0; i < 8; ++i) x[i] = q[static_cast<int64_t>(d + i) * a.q_st[0]] * c;
+                        if constexpr (PACKED) {
+                            const float *from = q + static_cast<int64_t>(d) * a.q_st[0];
+#pragma unroll 1
+                            for (int i = 0; i < 8; ++i, from += a.q_st[0])
+                                for (int j = 0; j < 8; ++j) x[j] = i == j ? *from * c : x[j];
+                        } else {
+                            for (int i = 0; i < 8; ++i) x[i] = q[static_cast<int64_t>(d + i) * a.q_st[0]] * c;
+                        }
                     }
                 } else {
                     for (int i = 0; i < 8; ++i) x[i] = 0.0f;
                 }
             };
             float up = 1.0f;
+            constexpr int kKept = kSets <= 4 ? kSets : 1;
+            float own_q[kKept][8]; // packed: of the column's blocks, where they are few
             if constexpr (!BF16) { // the head's largest value to [2^14, 2^15)
                 float top = 0.0f;
                 auto fold = [&](const float x[8]) {
                     for (int i = 0; i < 8; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(x[i]));
                 };
-                if constexpr (KS <= 4) { // all loads at once
+                if constexpr (PACKED) {
+                    if constexpr (kKept == kSets) {
+                        for (int e = 0; e < kSets; ++e) eight(e * F + part, own_q[e]);
+                        for (int e = 0; e < kSets; ++e) fold(own_q[e]);
+                    } else {
+#pragma unroll 1
+                        for (int e = 0; e < kSets; ++e) {
+                            eight(e * F + part, own_q[0]);
+                            fold(own_q[0]);
+                        }
+                    }
+                } else if constexpr (KS <= 4) { // all loads at once
                     float x[KS][8];
                     for (int e = 0; e < KS; ++e) eight(e, x[e]);
                     for (int e = 0; e < KS; ++e) fold(x[e]);
@@ -392,13 +567,40 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                     }
                 }
                 top = rows16(top, [](float u, float v) { return __builtin_fmaxf(u, v); });
+                if constexpr (F > 1)
+                    for (int x = 1; x < F; x *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, x, kWave));
                 int e = static_cast<int>((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 127;
                 e = top == 0.0f || e == 128 ? 0 : e < -110 ? -110 : e; // infinite: the wave walks below
                 up = __builtin_bit_cast(float, static_cast<uint32_t>(127 + 14 - e) << 23);
                 inv = __builtin_bit_cast(float, static_cast<uint32_t>(127 - 14 + e) << 23);
             }
+            if constexpr (PACKED) {
+                auto lay = [&](uint32_t e, const float x[8]) {
+                    u4 w[P];
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t even[3], odd[3];
+                        split<false>(x[2 * i] * up, even);
+                        split<false>(x[2 * i + 1] * up, odd);
+                        for (int p = 0; p < P; ++p) w[p][i] = even[p] | (odd[p] << 16);
+                    }
+                    for (int p = 0; p < P; ++p) {
+                        planes[(e * P + p) * kPlane + lane] = w[p];
+                        if (lane == 0) planes[(e * P + p) * kPlane + kWave] = u4{0, 0, 0, 0};
+                    }
+                };
+                if constexpr (kKept == kSets) {
+                    for (int e = 0; e < kSets; ++e)
+                        if (static_cast<uint32_t>(e) == wave) lay(e, own_q[e]);
+                } else {
 #pragma unroll 1
-            for (uint32_t e = wave; e < KS; e += kWaves) {
+                    for (uint32_t e = wave; e < kSets; e += kWaves) {
+                        eight(e * F + part, own_q[0]);
+                        lay(e, own_q[0]);
+                    }
+                }
+            }
+#pragma unroll 1
+            for (uint32_t e = wave; e < (PACKED ? 0 : KS); e += kWaves) {
                 float x[8];
                 eight(e, x);
                 u4 w[P];
@@ -412,7 +614,177 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
             }
         }
         __syncthreads();
-        for (; t0 < t_end; t0 += kPaUnit) {
+        // The packed loop runs ahead of itself: a step's keys are asked for when
+        // the last one's scores are done with theirs, its values behind the last
+        // one's sums, so each load has half a step of instructions to come in.
+        uint32_t kw[2][PACKED ? (K4 ? 1 : 2) * KS : 1];
+        uint32_t vw[8][kWords];              // the words of each token that hold the lane's values
+        uint16_t bits[PACKED ? KS : 1];      // the scales of lane % 32's token, of keys or values
+        uint32_t inside = 0; // the place of its token in the page `next`
+        // Behind the end the last token stands for what is missing, so that
+        // these loads need no branch, which would have to wait for them.
+        auto ask_page = [&](uint32_t t) {
+            t = sq.first + (t < t_end ? t : t_end - 1);
+            const uint32_t page = pl.page.div(t);
+            inside = t - page * pl.page.d;
+            next = table[static_cast<int64_t>(page) * a.table_st[0]];
+        };
+        auto ask_keys = [&](uint32_t t1) {
+            const bool ok = static_cast<uint32_t>(next) < a.pages;
+            bad |= !ok;
+            const int64_t p = ok ? next : 0, i = inside;
+            const PagePool &pool = lane < 32 ? a.k_pool : a.v_pool;
+            const int64_t o = p * pool.st_page + i * pool.st_tok;
+            __builtin_amdgcn_wave_barrier();
+            off[wave][lane / 32][lane % 32] = o;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            ask_page(t1 + lane % 32 + kPaUnit);
+            const uint16_t *row = (lane < 32 ? kbase + KI * KS : vbase + VI * KS) + o; // a row's last KS halves
+            __builtin_memcpy(bits, row, sizeof bits);
+            for (int b = 0; b < 2; ++b) __builtin_memcpy(kw[b], kbase + off[wave][0][16 * b + col] + g * (KI * KS / 4), sizeof kw[b]);
+        };
+        // Of a quarter of a set's numbers, which lie side by side, four lanes take
+        // a quarter each: bytes from `skip` on, of a word that two or all of them load where it is less.
+        constexpr int kByte = V4 ? 1 : 2; // bytes of a lane and block
+        auto skip = [&](int n) { return n * kByte == 1 ? 0u : n * kByte == 2 ? quarter / 2 * 4 : quarter * n * kByte; };
+        auto first = [&](int n) { return n * kByte == 1 ? quarter : n * kByte == 2 ? quarter % 2 * 2 : 0u; };
+        auto ask_values = [&] {
+            for (int b = 0; b < 8; ++b) {
+                const uint8_t *p = reinterpret_cast<const uint8_t *>(vbase + off[wave][1][16 * (b / 4) + 4 * g + b % 4] + col / 4 * (VI * KS / 4));
+                for (int e = 0; e < kSets; ++e) {
+                    const int n = blocks_of(e);
+                    __builtin_memcpy(&vw[b][e * words_of(F)], p + 4 * kByte * F * e + skip(n), 4 * words_of(n));
+                }
+            }
+        };
+        // the scales of this step into LDS; what is not a token counts for nothing
+        auto place_scales = [&] {
+            float d[KS];
+            bool over = false;
+            for (int e = 0; e < KS; ++e) {
+                d[e] = t0 + lane % 32 < t_end || lane < 32 ? pk_scale(bits[e]) : 0.0f;
+                over |= __builtin_fabsf(d[e]) * unit[e] > 1.0f;
+            }
+            // A value's scale larger than all before: acc goes by a power of two
+            // that holds it, and eight times as large ones, so that few steps
+            // come by here.
+            if (__any(over && lane >= 32)) {
+                float f[kSets];
+                for (float &x : f) x = 1.0f;
+                for (int e = 0; e < KS; ++e) {
+                    const float top = wave_max_dpp(lane < 32 ? 0.0f : __builtin_fabsf(d[e]));
+                    if (top * unit[e] > 1.0f) {
+                        const uint32_t to = (250u << 23) - (__builtin_bit_cast(uint32_t, top) & 0x7f800000u);
+                        if (part == static_cast<uint32_t>(e % F))
+                            f[e / F] = __builtin_bit_cast(float, (127u << 23) + to - __builtin_bit_cast(uint32_t, unit[e]));
+                        unit[e] = __builtin_bit_cast(float, to);
+                    }
+                }
+                for (int j = 0; j < kAcc; ++j) acc[j] *= f[j / (2 * F)];
+            }
+            __builtin_amdgcn_wave_barrier();
+            for (int e = 0; e < KS; ++e) scales[wave][lane / 32][e][lane % 32] = d[e] * (lane < 32 ? 1.0f : unit[e]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        };
+        // the scales of the column's block of set e, of the lane's four tokens of tile b
+        auto four = [&](int of, int e, int b) {
+            const uint32_t at = e * F + part;
+            return *reinterpret_cast<const v4f *>(&scales[wave][of][KS % F == 0 || at < KS ? at : 0][16 * b + 4 * g]);
+        };
+        uint32_t magic = 0x64006400u; // in a register: an instruction holds one constant
+        asm volatile("" : "+v"(magic));
+        if constexpr (PACKED) {
+            if (t0 < t_end) {
+                ask_page(t0 + lane % 32);
+                ask_keys(t0);
+                ask_values();
+            }
+        }
+        for (; PACKED && t0 < t_end; t0 += kPaUnit) {
+            const bool more = t0 + kPaUnit < t_end;
+            float z[8];
+            place_scales();
+            v4f sum[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            for (int e = 0; e < kSets; ++e) {
+                v4f c[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                for (int i = e * F; i < e * F + blocks_of(e); ++i) {
+                    const uint32_t at = part == static_cast<uint32_t>(i % F) ? lane : kWave; // no other block's
+                    u4 x[2];
+                    for (int b = 0; b < 2; ++b) {
+                        if constexpr (K4) x[b] = pk_halves4(kw[b][i], magic);
+                        else x[b] = pk_halves8(kw[b][2 * i], kw[b][2 * i + 1], magic);
+                    }
+                    for (int p = P - 1; p >= 0; --p)
+                        for (int b = 0; b < 2; ++b) c[b] = mfma32<false>(x[b], planes[(e * P + p) * kPlane + at], c[b]);
+                }
+                for (int b = 0; b < 2; ++b) {
+                    const v4f d = four(0, e, b);
+                    for (int i = 0; i < 4; ++i)
+                        sum[b][i] = blocks_of(e) == F || part < static_cast<uint32_t>(blocks_of(e)) ? __builtin_fmaf(c[b][i], d[i], sum[b][i]) : sum[b][i];
+                }
+            }
+            for (int i = 0; i < 8; ++i) {
+                float x = sum[i / 4][i % 4];
+                if constexpr (F > 1) x += dpp_f32<kDppXor1>(x);
+                if constexpr (F > 2) x += dpp_f32<kDppXor2>(x);
+                if constexpr (F > 4) x += dpp_f32<kDppHalfMirror>(x);
+                z[i] = x * inv;
+            }
+            if (more) ask_keys(t0 + kPaUnit);
+            if (__builtin_expect(a.soft_cap > 0.0f, 0))
+                for (int i = 0; i < 8; ++i) z[i] = pa_tanh(z[i]) * (a.soft_cap * 1.44269504088896340736f);
+            if (t0 + 32 > t_end)
+                for (int b = 0; b < 8; ++b)
+                    if (t0 + 16 * (b / 4) + 4 * g + b % 4 >= t_end) z[b] = -__builtin_inff();
+            float top = z[0];
+            for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, z[i]);
+            top = rows16(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+            if (__any(top > m)) {
+                const float m1 = __builtin_fmaxf(m, top);
+                const float f = m1 > m ? __builtin_amdgcn_exp2f(m - m1) : 1.0f; // m = -inf: 0
+                l *= f;
+                for (int j = 0; j < kAcc; ++j) acc[j] *= f;
+                m = m1;
+            }
+            const float ref = (m == -__builtin_inff() ? 0.0f : m) - kLift;
+            float w[8];
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(z[i] - ref);
+                l += w[i];
+            }
+            for (int e = 0; e < kSets; ++e) {
+                u4 hi, lo; // the weights by a block's scales, as halves that add up to 22 bits
+                for (int b = 0; b < 2; ++b) {
+                    const v4f d = four(1, e, b);
+                    for (int i = 0; i < 2; ++i) {
+                        const float *x = w + 4 * b + 2 * i;
+                        const v2h h = __builtin_convertvector((v2f{x[0] * d[2 * i], x[1] * d[2 * i + 1]}), v2h);
+                        const v2f r = {__builtin_fmaf(x[0], d[2 * i], -static_cast<float>(h[0])),
+                                       __builtin_fmaf(x[1], d[2 * i + 1], -static_cast<float>(h[1]))};
+                        hi[2 * b + i] = __builtin_bit_cast(uint32_t, h);
+                        lo[2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
+                    }
+                }
+                const int n = blocks_of(e);
+                for (int j = 0; j < 2 * n; ++j) {
+                    // the lane's j-th number of the set, of tokens 2i and 2i + 1
+                    const int byte = V4 ? j / 2 : j, word = e * words_of(F) + byte / 4;
+                    const uint32_t pick = 0x0c040c00u + (first(n) + byte % 4) * 0x10001u;
+                    u4 x;
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (V4) x[i] = pk_pair4(vw[2 * i][word], vw[2 * i + 1][word], pick, j % 2, magic);
+                        else x[i] = pk_pair8(vw[2 * i][word], vw[2 * i + 1][word], pick, magic);
+                    }
+                    v4f &sum = acc[2 * F * e + j];
+                    sum = mfma32<false>(x, lo, sum);
+                    sum = mfma32<false>(x, hi, sum);
+                }
+            }
+            if (more) ask_values();
+        }
+        for (; !PACKED && t0 < t_end; t0 += kPaUnit) {
             {
                 const uint32_t t = t0 + lane % 32;
                 const bool ok = t < t_end && static_cast<uint32_t>(next) < a.pages;
@@ -420,62 +792,12 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                 const int64_t p = ok ? next : 0, i = ok ? pl.page.mod(sq.first + t) : 0;
                 const PagePool &pool = lane < 32 ? a.k_pool : a.v_pool;
                 __builtin_amdgcn_wave_barrier();
-                const int64_t o = p * pool.st_page + i * pool.st_tok;
-                off[wave][lane / 32][lane % 32] = o;
-                if constexpr (PACKED) {
-                    // the token's scales, a row's last KS halves; what is not a token counts for nothing
-                    const uint16_t *row = (lane < 32 ? kbase + KI * KS : vbase + VI * KS) + o;
-                    uint16_t bits[KS];
-                    __builtin_memcpy(bits, row, sizeof bits);
-                    float d[KS];
-                    bool over = false;
-                    for (int e = 0; e < KS; ++e) {
-                        d[e] = t < t_end || lane < 32 ? pk_scale(bits[e]) : 0.0f;
-                        over |= lane >= 32 && __builtin_fabsf(d[e]) * unit[e] > 1.0f;
-                    }
-                    if (__any(over)) { // larger than all before: acc goes by a power of two that holds them
-                        for (int e = 0; e < KS; ++e) {
-                            const float top = wave_max_dpp(lane < 32 ? 0.0f : __builtin_fabsf(d[e]));
-                            if (top * unit[e] > 1.0f) {
-                                const float to = __builtin_bit_cast(float, (253u << 23) - (__builtin_bit_cast(uint32_t, top) & 0x7f800000u));
-                                acc[2 * e] *= to / unit[e];
-                                acc[2 * e + 1] *= to / unit[e];
-                                unit[e] = to;
-                            }
-                        }
-                    }
-                    for (int e = 0; e < KS; ++e) scales[wave][lane / 32][e][lane % 32] = lane < 32 ? d[e] : d[e] * unit[e];
-                }
+                off[wave][lane / 32][lane % 32] = p * pool.st_page + i * pool.st_tok;
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
                 next = page_of(t + kPaUnit);
             }
-            float z[8];
-            u4 k[2][PACKED ? 1 : KS];
-            uint32_t v[8][PACKED ? 1 : VW / 2];
-            uint32_t vp[8][PACKED ? KS : 1]; // packed: the words of each token that hold the lane's values
-            if constexpr (PACKED) {
-                uint32_t kw[2][(K4 ? 1 : 2) * KS];
-                for (int b = 0; b < 2; ++b) __builtin_memcpy(kw[b], kbase + off[wave][0][16 * b + col] + g * (KI * KS / 4), sizeof kw[b]);
-                for (int b = 0; b < 8; ++b) {
-                    const uint16_t *p = vbase + off[wave][1][16 * (b / 4) + 4 * g + b % 4] + col / 4 * (VI * KS / 4);
-                    if constexpr (V4) __builtin_memcpy(vp[b], p, sizeof vp[b]);
-                    else for (int e = 0; e < KS; ++e) __builtin_memcpy(&vp[b][e], p + 4 * e + col % 4 / 2 * 2, 4);
-                }
-                for (int b = 0; b < 2; ++b) {
-                    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (int e = 0; e < KS; ++e) {
-                        u4 x;
-                        if constexpr (K4) x = pk_halves4(kw[b][e]);
-                        else x = pk_halves8(kw[b][2 * e], kw[b][2 * e + 1]);
-                        v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
-                        for (int p = P - 1; p >= 0; --p) c = mfma32<false>(x, qop[(e * P + p) * kWave + lane], c);
-                        const v4f d = *reinterpret_cast<const v4f *>(&scales[wave][0][e][16 * b + 4 * g]);
-                        for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(c[i], d[i], sum[i]);
-                    }
-                    for (int i = 0; i < 4; ++i) z[4 * b + i] = sum[i] * inv;
-                }
-            } else {
+            u4 k[2][KS];
             for (int b = 0; b < 2; ++b) {
                 const uint16_t *p = kbase + off[wave][0][16 * b + col];
                 for (int e = 0; e < KS; ++e) {
@@ -483,6 +805,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                     k[b][e] = *reinterpret_cast<const u4_any *>(p + (d < dim ? d : 0)); // q is 0 past dim
                 }
             }
+            uint32_t v[8][VW / 2];
             for (int b = 0; b < 8; ++b) {
                 const uint16_t *p = vbase + off[wave][1][16 * (b / 4) + 4 * g + b % 4];
                 // eights first, then fours behind the eights of all 16 lanes
@@ -498,12 +821,12 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                     v[b][VW / 2 - 1] = x[1];
                 }
             }
+            float z[8];
             for (int b = 0; b < 2; ++b) {
                 v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
                 for (int e = 0; e < KS; ++e)
                     for (int p = P - 1; p >= 0; --p) c = mfma32<BF16>(k[b][e], qop[(e * P + p) * kWave + lane], c);
                 for (int i = 0; i < 4; ++i) z[4 * b + i] = BF16 ? c[i] : c[i] * inv;
-            }
             }
             if (__builtin_expect(a.soft_cap > 0.0f, 0))
                 for (int i = 0; i < 8; ++i) z[i] = pa_tanh(z[i]) * (a.soft_cap * 1.44269504088896340736f);
@@ -511,8 +834,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                 for (int b = 0; b < 8; ++b) {
                     if (t0 + 16 * (b / 4) + 4 * g + b % 4 < t_end) continue;
                     z[b] = -__builtin_inff();
-                    if constexpr (!PACKED)
-                        for (int i = 0; i < VW / 2; ++i) v[b][i] = 0;
+                    for (int i = 0; i < VW / 2; ++i) v[b][i] = 0;
                 }
             }
             float top = z[0];
@@ -522,40 +844,10 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                 const float m1 = __builtin_fmaxf(m, top);
                 const float f = m1 > m ? __builtin_amdgcn_exp2f(m - m1) : 1.0f; // m = -inf: 0
                 l *= f;
-                for (int j = 0; j < kAcc; ++j) acc[j] *= f;
+                for (int j = 0; j < VW; ++j) acc[j] *= f;
                 m = m1;
             }
             const float ref = (m == -__builtin_inff() ? 0.0f : m) - kLift;
-            if constexpr (PACKED) {
-                float w[8];
-                for (int i = 0; i < 8; ++i) {
-                    w[i] = __builtin_amdgcn_exp2f(z[i] - ref);
-                    l += w[i];
-                }
-                for (int e = 0; e < KS; ++e) {
-                    u4 hi, lo; // the weights by the block's scales, as halves that add up to 22 bits
-                    for (int b = 0; b < 2; ++b) {
-                        const v4f d = *reinterpret_cast<const v4f *>(&scales[wave][1][e][16 * b + 4 * g]);
-                        for (int i = 0; i < 2; ++i) {
-                            const v2f x = {w[4 * b + 2 * i] * d[2 * i], w[4 * b + 2 * i + 1] * d[2 * i + 1]};
-                            const v2h h = __builtin_convertvector(x, v2h);
-                            const v2f r = {x[0] - static_cast<float>(h[0]), x[1] - static_cast<float>(h[1])};
-                            hi[2 * b + i] = __builtin_bit_cast(uint32_t, h);
-                            lo[2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
-                        }
-                    }
-                    for (int j = 0; j < 2; ++j) {
-                        u4 x;
-                        for (int i = 0; i < 4; ++i) { // the lane's j-th value of the block, of tokens 2i and 2i + 1
-                            if constexpr (V4) x[i] = pk_pair4(vp[2 * i][e], vp[2 * i + 1][e], pick, j);
-                            else x[i] = pk_pair8(vp[2 * i][e], vp[2 * i + 1][e], pick + 0x10001u * j);
-                        }
-                        acc[2 * e + j] = mfma32<false>(x, lo, acc[2 * e + j]);
-                        acc[2 * e + j] = mfma32<false>(x, hi, acc[2 * e + j]);
-                    }
-                }
-                continue;
-            }
             uint32_t part[8][3];
             for (int i = 0; i < 8; ++i) {
                 const float w = __builtin_amdgcn_exp2f(z[i] - ref);
@@ -573,17 +865,38 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
             }
         }
 
-        if constexpr (PACKED)
-            for (int j = 0; j < kAcc; ++j) acc[j] *= 1.0f / unit[j / 2];
+        // packed: of each set the eight g of the column's block, from the rows 4 g
+        // + i that hold its numbers
+        float eight[kSets][8];
+        for (int e = 0; PACKED && e < kSets; ++e) {
+            const int n = blocks_of(e);
+            float u = unit[e * F];
+            for (int i = 0; i < 8; ++i) {
+                constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7}; // Q4_0: the nibble of each value
+                const int at = V4 ? order[i] : i;
+                auto of = [&](int b) { // number `at` of the set's block b: row by row, 2 n of them
+                    const int q = 8 * b + at;
+                    return acc[2 * F * e + q % (2 * n)][q / (2 * n)];
+                };
+                eight[e][i] = of(0);
+                for (int b = 1; b < n; ++b) eight[e][i] = part == static_cast<uint32_t>(b) ? of(b) : eight[e][i];
+            }
+            for (int b = 1; b < n; ++b) u = part == static_cast<uint32_t>(b) ? unit[e * F + b] : u;
+            const float by = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, u)); // 1 / u
+            for (float &x : eight[e]) x *= by;
+        }
         // the wave's part: [head][dim], dims of lane row c = 4 g + i
         float *own = joined + wave * heads * pitch;
         l = rows16(l, [](float x, float y) { return x + y; });
         v4f size = {l, 0.0f, 0.0f, 0.0f};
-        for (int j = 0; j < kAcc; ++j)
+        for (int e = 0; PACKED && e < kSets; ++e)
+            for (int i = 0; i < 8; ++i) size[i % 4] += part < static_cast<uint32_t>(blocks_of(e)) ? __builtin_fabsf(eight[e][i]) : 0.0f;
+        for (int j = 0; j < (PACKED ? 0 : kAcc); ++j)
             for (int i = 0; i < 4; ++i) size[i] += __builtin_fabsf(acc[j][i]);
         const bool odd = !((size[0] + size[1]) + (size[2] + size[3]) < (BF16 ? 0x1p97f : __builtin_inff()));
         bad = __any(bad);
-        if (__builtin_expect(__any(odd && col < heads) && !bad, 0)) {
+        if constexpr (PACKED) __syncthreads(); // the operands' place is the joins' from here on
+        if (__builtin_expect(__any(odd && head < heads) && !bad, 0)) {
             // as the formula stands: a head and a token at a time, a lane four dims
             constexpr float down = BF16 ? 0x1p-34f : 1.0f, above = BF16 ? 34.0f : 0.0f;
             for (uint32_t h = 0; h < heads; ++h) {
@@ -630,18 +943,17 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                     wl[wave][h] = ll * (lift * down);
                 }
             }
-        } else if (col < heads) {
-            if (g == 0) {
-                wm[wave][col] = m;
-                wl[wave][col] = bad ? __builtin_nanf("") : l;
+        } else if (head < heads) {
+            if (g == 0 && part == 0) {
+                wm[wave][head] = m;
+                wl[wave][head] = bad ? __builtin_nanf("") : l;
             }
-            if constexpr (PACKED) {
-                for (int e = 0; e < KS; ++e) {
-                    const v4f &x = acc[2 * e], &y = acc[2 * e + 1]; // Q4_0: values 0 4 1 5 and 2 6 3 7 of the eight, Q8_0: even and odd
-                    float *o = own + col * pitch + 32 * e + 8 * g;
-                    *reinterpret_cast<v4f *>(o) = V4 ? v4f{x[0], x[2], y[0], y[2]} : v4f{x[0], y[0], x[1], y[1]};
-                    *reinterpret_cast<v4f *>(o + 4) = V4 ? v4f{x[1], x[3], y[1], y[3]} : v4f{x[2], y[2], x[3], y[3]};
-                }
+            for (int e = 0; PACKED && e < kSets; ++e) {
+                const float *x = eight[e];
+                float *o = own + head * pitch + 32 * (e * F + part) + 8 * g;
+                if (part >= static_cast<uint32_t>(blocks_of(e))) continue;
+                *reinterpret_cast<v4f *>(o) = v4f{x[0], x[1], x[2], x[3]};
+                *reinterpret_cast<v4f *>(o + 4) = v4f{x[4], x[5], x[6], x[7]};
             }
             for (int i = 0; i < (PACKED ? 0 : 4); ++i) {
                 const uint32_t c = 4 * g + i;
@@ -658,9 +970,11 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
             }
         }
         __syncthreads();
-        const bool whole = n0 == 0 && n1 == units;
-        const uint32_t w0 = n0 == 0 ? blockIdx.x : row_at / run; // the row's first workgroup
-        float *slot = pl.parts + static_cast<size_t>(2 * blockIdx.x + (n0 == 0 ? 1 : 0)) * pl.slot;
+        const bool begins = PACKED ? u0 == 0 : n0 == 0;
+        const bool whole = begins && n1 == units;
+        const uint32_t w0 = begins ? block : (row_at + (PACKED ? setup : 0)) / run; // the row's first workgroup
+        const uint32_t own_block = PACKED ? block * pl.side + lane_row : block;
+        float *slot = pl.parts + static_cast<size_t>(2 * own_block + (begins ? 1 : 0)) * pl.slot;
         // the waves' maximum and sum of a head, and each wave's weight
         auto join = [&](uint32_t h, float f[kWaves], float &sum) {
             float top = wm[0][h];
@@ -673,6 +987,19 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
             return top;
         };
         asm volatile("" : "+v"(tid));
+        if constexpr (PACKED) {
+            pa_ends(a, pl, PaEnd{sq.tokens == 0 && !sq.bad, whole, heads, h0, s, w0, lane_row, (row_at + units - 1) / run - w0 + 1}, slot, joined,
+                    &wm[0][0], &wl[0][0], &last, tid);
+            __syncthreads(); // the next segment reuses the shared arrays
+            cur = row_at + n1;
+            row_at += units;
+            if (++row == rows && cur < end) {
+                row = 0;
+                sq = pa_seq(a, pa_len(a, ++s));
+                units = sq.units + setup;
+            }
+            continue;
+        }
         const uint32_t cells = heads * dim; // dim is even: pairs do not cross heads
         float *out = a.y + static_cast<int64_t>(h0) * a.y_st[1] + static_cast<int64_t>(s) * a.y_st[2];
         auto put = [&](uint32_t h, uint32_t d, float x, float y) {
@@ -776,7 +1103,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         __syncthreads(); // the next segment reuses the shared arrays
         cur = row_at + n1;
         row_at += units;
-        if (++row == pl.rows && cur < end) {
+        if (++row == rows && cur < end) {
             row = 0;
             sq = pa_seq(a, pa_len(a, ++s));
             units = sq.units + setup;

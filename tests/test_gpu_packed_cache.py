@@ -228,11 +228,11 @@ def cached(c, s, window=0):
 
 def tolerance(c, v, tol):
     """attention()'s, and what a weight times its block's scale loses as two halves: 2^-22 of itself, which is within that,
-    or 2^-38 of the block's largest such product, of n tokens with numbers up to the format's end.  In blocks of random
+    or 2^-35 of the block's largest such product, of n tokens with numbers up to the format's end.  In blocks of random
     numbers the largest value is an eighth of that end or more."""
     big = 8 * np.abs(v).reshape(*v.shape[:2], -1, 32).max((0, 3))  # [kv, block]
     share = np.repeat(np.repeat(big, 32, 1), c["q"].shape[1] // len(big), 0)
-    return tol + share * len(v) * 2.0**-38
+    return tol + share * len(v) * 2.0**-35
 
 
 def check_attention(c, window=0, cap=0.0, scale=None, skip=()):
