@@ -73,83 +73,130 @@ __global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a, FastDiv
 // the scale as it is stored: the quotient by 1/d is off by one at most, and
 // x - n d, which is exact in f32 (x is a multiple of 2^-25 d or below d / 2), says so.
 
-// The nearest whole number of scales in x, ties to even; inv is 1 / d or near it.
-__device__ __forceinline__ float nearest(float x, float d, float inv)
+// What is to be added to n so that it is the nearest whole number of scales in
+// x, ties to even, for an n that is off by one at most.
+__device__ __forceinline__ float off_by(float x, float n, float d)
 {
-    float n = __builtin_rintf(x * inv);
     const float over = __builtin_fmaf(-n, d, x) * (d < 0.0f ? -1.0f : 1.0f), half = 0.5f * __builtin_fabsf(d);
     const bool odd = static_cast<int>(n) & 1;
-    if (over > half || (over == half && odd)) n += 1.0f;
-    else if (over < -half || (over == -half && odd)) n -= 1.0f;
-    return n;
+    return over > half || (over == half && odd) ? 1.0f : over < -half || (over == -half && odd) ? -1.0f : 0.0f;
 }
 
 // Packs a lane's eight values of a block; every lane of a quad is active.
 __device__ __forceinline__ void pack_eight(bool q4, const float x[8], uint8_t *row, uint32_t blocks, uint32_t eight)
 {
     const uint32_t block = eight / 4, part = eight % 4, unit = part * blocks + block;
-    float top = 0.0f;
-    bool fine = true;
+    float high = -__builtin_inff(), low = high, zero = 0.0f; // the largest value, the largest opposite one, 0 or NaN
     for (int i = 0; i < 8; ++i) {
-        top = __builtin_fmaxf(top, __builtin_fabsf(x[i]));
-        fine &= __builtin_fabsf(x[i]) < __builtin_inff();
+        high = __builtin_fmaxf(high, x[i]);
+        low = __builtin_fmaxf(low, -x[i]);
+        zero = __builtin_fmaf(x[i], 0.0f, zero);
     }
-    top = __builtin_fmaxf(top, dpp_f32<kDppXor1>(top));
-    top = __builtin_fmaxf(top, dpp_f32<kDppXor2>(top));
-    uint32_t odd = fine ? 0u : 1u;
-    odd |= dpp32<kDppXor1>(odd);
-    odd |= dpp32<kDppXor2>(odd);
-    float d;
-    if (q4) { // the first value of that magnitude: its number and sign
+    high = __builtin_fmaxf(high, dpp_f32<kDppXor1>(high));
+    low = __builtin_fmaxf(low, dpp_f32<kDppXor1>(low));
+    zero += dpp_f32<kDppXor1>(zero);
+    high = __builtin_fmaxf(high, dpp_f32<kDppXor2>(high));
+    low = __builtin_fmaxf(low, dpp_f32<kDppXor2>(low));
+    zero += dpp_f32<kDppXor2>(zero);
+    const float top = __builtin_fmaxf(high, low);
+    const bool fine = zero == 0.0f;
+    float d = top * (high > low ? -0.125f : 0.125f);
+    if (!q4) {
+        d = top / 127.0f;
+    } else if (__any(high == low)) { // both signs: the first value of that magnitude, by its number and sign
         uint32_t first = ~0u;
         for (int i = 7; i >= 0; --i)
             if (__builtin_fabsf(x[i]) == top) first = (8 * part + i) << 1 | (__builtin_bit_cast(uint32_t, x[i]) >> 31);
         first = min(first, dpp32<kDppXor1>(first));
         first = min(first, dpp32<kDppXor2>(first));
-        d = top * (first & 1 ? 0.125f : -0.125f);
-    } else {
-        d = top / 127.0f;
+        d = high == low ? top * (first & 1 ? 0.125f : -0.125f) : d;
     }
     const _Float16 scale = static_cast<_Float16>(__builtin_fminf(__builtin_fmaxf(d, -65504.0f), 65504.0f));
     d = static_cast<float>(scale);
-    const float inv = d == 0.0f || odd ? 0.0f : 1.0f / d;
-    float n[8];
-    for (int i = 0; i < 8; ++i) n[i] = inv == 0.0f ? 0.0f : nearest(x[i], d, inv);
+    const float inv = d == 0.0f || !fine ? 0.0f : __builtin_amdgcn_rcpf(d);
+    float n[8], most = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+        n[i] = fine ? __builtin_rintf(x[i] * inv) : 0.0f;
+        most = __builtin_fmaxf(most, __builtin_fabsf(__builtin_fmaf(-n[i], d, x[i])));
+    }
+    if (__any(most >= 0.5f * __builtin_fabsf(d))) // seldom: a tie, or 1 / d rounded to the wrong side of one
+        for (int i = 0; i < 8; ++i) n[i] += inv == 0.0f ? 0.0f : off_by(x[i], n[i], d);
     uint16_t *scales = reinterpret_cast<uint16_t *>(row + (q4 ? 16 : 32) * blocks);
-    if (part == 0) scales[block] = odd ? uint16_t{0x7e00} : __builtin_bit_cast(uint16_t, scale);
+    if (part == 0) scales[block] = fine ? __builtin_bit_cast(uint16_t, scale) : uint16_t{0x7e00};
     if (q4) {
         uint32_t w = 0;
-        for (int i = 0; i < 8; ++i) {
-            const int q = static_cast<int>(__builtin_fminf(__builtin_fmaxf(n[i], -8.0f), 7.0f)) + 8;
-            w |= static_cast<uint32_t>(q) << (4 * (i / 2 + i % 2 * 4));
-        }
+        for (int i = 0; i < 8; ++i)
+            w |= static_cast<uint32_t>(static_cast<int>(__builtin_fminf(__builtin_fmaxf(n[i], -8.0f), 7.0f)) + 8) << (4 * (i / 2 + i % 2 * 4));
         *reinterpret_cast<u1_any *>(row + 4 * unit) = w;
     } else {
         u2 w = {0, 0};
-        for (int i = 0; i < 8; ++i) {
-            const int q = static_cast<int>(__builtin_fminf(__builtin_fmaxf(n[i], -127.0f), 127.0f));
-            w[i / 4] |= (static_cast<uint32_t>(q) & 255u) << (8 * (i % 4));
-        }
+        for (int i = 0; i < 8; ++i)
+            w[i / 4] |= (static_cast<uint32_t>(static_cast<int>(__builtin_fminf(__builtin_fmaxf(n[i], -127.0f), 127.0f))) & 255u) << (8 * (i % 4));
         *reinterpret_cast<u2_any *>(row + 8 * unit) = w;
     }
 }
 
-// Eight consecutive values of a packed row, whatever its type.
-__device__ __forceinline__ void unpack_eight(bool q4, const uint8_t *row, uint32_t blocks, uint32_t eight, float x[8])
+// How a workgroup's waves share `jobs` tokens, keys and values apart, of
+// `items` lanes' work each: a wave takes the items of one run of 64 for every
+// wpc-th job, so that a token's place is the same for its lanes and worked out once.
+struct WaveShare {
+    uint32_t chunk, chunks, step, job, wpc;
+};
+__device__ __forceinline__ WaveShare wave_share(uint32_t items)
 {
-    const uint32_t block = eight / 4, unit = eight % 4 * blocks + block;
-    const float d = pk_scale(reinterpret_cast<const uint16_t *>(row + (q4 ? 16 : 32) * blocks)[block]);
-    if (q4) {
-        const uint32_t w = *reinterpret_cast<const u1_any *>(row + 4 * unit);
-        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int>((w >> (4 * (i / 2 + i % 2 * 4))) & 15u) - 8) * d;
-    } else {
-        const u2 w = *reinterpret_cast<const u2_any *>(row + 8 * unit);
-        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)))) * d;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), chunks = (items + kWave - 1) / kWave;
+    const uint32_t wpc = chunks == 1 ? 4 : chunks == 2 ? 2 : 1;
+    return {wave / wpc, chunks, 4 / wpc, wave % wpc, wpc};
+}
+
+// As k_pk_append for tokens of 64 items or more; UNIT: keys and values are read
+// with unit stride.
+template <uint32_t T, bool UNIT>
+__global__ __launch_bounds__(kBlock) void k_pk_append_wide(PagedAppendArgs a, FastDiv page, FastDiv head, uint32_t items)
+{
+    __shared__ uint32_t gone;
+    const uint32_t t0 = blockIdx.x * T;
+    int32_t mine[T];
+    const uint32_t drop = pa_dropped<T>(a, t0, mine, &gone);
+    constexpr uint32_t kBatch = T == 1 ? 1 : 4;
+    const WaveShare w = wave_share(items);
+    for (uint32_t c = w.chunk; c < w.chunks; c += w.step) {
+        const uint32_t r = c * kWave + threadIdx.x % kWave;
+        if (r >= items) continue;
+        const uint32_t h = head.div(r), eight = r - h * head.d;
+        for (uint32_t j0 = w.job; j0 < 2 * T; j0 += kBatch * w.wpc) {
+            float x[kBatch][8];
+            uint8_t *row[kBatch];
+#pragma unroll
+            for (uint32_t n = 0; n < kBatch; ++n) {
+                const uint32_t j = j0 + n * w.wpc, k = j % T;
+                row[n] = nullptr;
+                if (j >= 2 * T || ((drop >> k) & 1u)) continue;
+                const bool val = j >= T;
+                const int64_t *st = val ? a.v_st : a.k_st;
+                const PagePool &pool = val ? a.v_pool : a.k_pool;
+                const uint32_t slot = static_cast<uint32_t>(a.slots[static_cast<int64_t>(t0 + k) * a.slots_st]);
+                const uint32_t p = page.div(slot), at = slot - p * page.d;
+                row[n] = reinterpret_cast<uint8_t *>(pool.data + p * pool.st_page + at * pool.st_tok + h * pool.st_head);
+                const float *src = (val ? a.v : a.k) + static_cast<int64_t>(t0 + k) * st[2] + h * st[1] + static_cast<int64_t>(8 * eight) * st[0];
+                if constexpr (UNIT) {
+                    const v4f lo = *reinterpret_cast<const v4f_any *>(src), hi = *reinterpret_cast<const v4f_any *>(src + 4);
+                    for (int q = 0; q < 4; ++q) {
+                        x[n][q] = lo[q];
+                        x[n][4 + q] = hi[q];
+                    }
+                } else {
+                    for (int q = 0; q < 8; ++q) x[n][q] = src[q * st[0]];
+                }
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < kBatch; ++n)
+                if (row[n]) pack_eight((j0 + n * w.wpc >= T ? a.v_pool : a.k_pool).kind == PoolKind::Q4_0, x[n], row[n], head.d / 4, eight);
+        }
     }
 }
 
-// UNIT: keys and values are read with unit stride.
-template <uint32_t T, bool UNIT>
+template <uint32_t T>
 __global__ __launch_bounds__(kBlock) void k_pk_append(PagedAppendArgs a, FastDiv page, FastDiv head, FastDiv token)
 {
     __shared__ uint32_t gone;
@@ -169,15 +216,7 @@ __global__ __launch_bounds__(kBlock) void k_pk_append(PagedAppendArgs a, FastDiv
         const PagePool &pool = val ? a.v_pool : a.k_pool;
         const float *src = (val ? a.v : a.k) + static_cast<int64_t>(8 * eight) * st[0] + h * st[1] + static_cast<int64_t>(t0 + k) * st[2];
         float x[8];
-        if constexpr (UNIT) {
-            const v4f lo = *reinterpret_cast<const v4f_any *>(src), hi = *reinterpret_cast<const v4f_any *>(src + 4);
-            for (int q = 0; q < 4; ++q) {
-                x[q] = lo[q];
-                x[4 + q] = hi[q];
-            }
-        } else {
-            for (int q = 0; q < 8; ++q) x[q] = src[q * st[0]];
-        }
+        for (int q = 0; q < 8; ++q) x[q] = src[q * st[0]];
         uint16_t *row = pool.data + p * pool.st_page + h * pool.st_head + at * pool.st_tok;
         pack_eight(pool.kind == PoolKind::Q4_0, x, reinterpret_cast<uint8_t *>(row), head.d / 4, eight);
     }
@@ -185,17 +224,70 @@ __global__ __launch_bounds__(kBlock) void k_pk_append(PagedAppendArgs a, FastDiv
 
 // ---- tokens read back ------------------------------------------------------------------------
 //
-// Bound by the tokens' bytes, 4 written a value.  EIGHT: eight values a lane and
-// step, else one (rows of halves whose dim is no multiple of 8).
+// Bound by the tokens' bytes, 4 written a value.  An item is eight values, or one
+// of halves whose dim is no multiple of 8.
 
-constexpr uint32_t kPaRead = 8; // tokens of a workgroup
+constexpr uint32_t kPaRead = 8;              // tokens of a workgroup
+constexpr uint32_t kPaReadTokens = 1u << 25; // tokens of a launch: its threads are counted in 32 bits
+
+struct ReadItem {
+    u4 word;
+    uint16_t scale;
+};
+
+template <bool EIGHT>
+__device__ __forceinline__ ReadItem read_item(const PagePool &pool, const uint16_t *row, uint32_t blocks, uint32_t at)
+{
+    ReadItem x = {};
+    if constexpr (!EIGHT) {
+        x.word[0] = row[at];
+    } else if (!pool.packed()) {
+        x.word = *reinterpret_cast<const u4_any *>(row + 8 * at);
+    } else { // part at % 4 of block at / 4
+        const uint32_t unit = at % 4 * blocks + at / 4;
+        if (pool.kind == PoolKind::Q4_0) {
+            x.word[0] = *reinterpret_cast<const u1_any *>(row + 2 * unit);
+            x.scale = row[8 * blocks + at / 4];
+        } else {
+            const u2 w = *reinterpret_cast<const u2_any *>(row + 4 * unit);
+            x.word[0] = w[0];
+            x.word[1] = w[1];
+            x.scale = row[16 * blocks + at / 4];
+        }
+    }
+    return x;
+}
+
+template <bool EIGHT>
+__device__ __forceinline__ void write_item(PoolKind kind, const ReadItem &it, float *dst, int64_t st)
+{
+    constexpr int N = EIGHT ? 8 : 1;
+    float x[N];
+    if (EIGHT && kind == PoolKind::Q8_0) {
+        const float d = pk_scale(it.scale);
+        for (int q = 0; q < N; ++q) x[q] = static_cast<float>(static_cast<int8_t>(it.word[q / 4] >> (8 * (q % 4)))) * d;
+    } else if (EIGHT && kind == PoolKind::Q4_0) {
+        const float d = pk_scale(it.scale);
+        for (int q = 0; q < N; ++q) x[q] = static_cast<float>(static_cast<int>((it.word[0] >> (q % 2 * 16 + q / 2 * 4)) & 15u) - 8) * d;
+    } else {
+        for (int q = 0; q < N; ++q) {
+            const uint16_t b = static_cast<uint16_t>(it.word[q / 2] >> (16 * (q % 2)));
+            x[q] = kind == PoolKind::Bf16 ? from_half<true>(b) : from_half<false>(b);
+        }
+    }
+    if (EIGHT && st == 1) { // nothing here reads them again
+        for (int q = 0; q < N; q += 4)
+            __builtin_nontemporal_store((v4f{x[q], x[(q + 1) % N], x[(q + 2) % N], x[(q + 3) % N]}), reinterpret_cast<v4f_any *>(dst + q));
+        return;
+    }
+    for (int q = 0; q < N; ++q) dst[q * st] = x[q];
+}
 
 template <bool EIGHT>
 __global__ __launch_bounds__(kBlock) void k_pa_read(PagedReadArgs a, uint32_t per, FastDiv page, FastDiv head, FastDiv token)
 {
-    constexpr uint32_t N = EIGHT ? 8 : 1;
     const uint64_t slots = static_cast<uint64_t>(a.page) * a.pages;
-    const uint32_t t0 = blockIdx.x * per;
+    const uint32_t t0 = blockIdx.x * per, blocks = head.d / 4; // of a packed row
     for (uint32_t e = threadIdx.x; e < 2 * per * token.d; e += kBlock) {
         const uint32_t i = token.div(e), r = e - i * token.d;
         const bool val = i >= per;
@@ -206,26 +298,46 @@ __global__ __launch_bounds__(kBlock) void k_pa_read(PagedReadArgs a, uint32_t pe
         const uint32_t p = page.div(static_cast<uint32_t>(slot)), in = static_cast<uint32_t>(slot) - p * page.d;
         const PagePool &pool = val ? a.v_pool : a.k_pool;
         const int64_t *st = val ? a.v_st : a.k_st;
-        const uint16_t *row = pool.data + p * pool.st_page + h * pool.st_head + in * pool.st_tok;
-        float x[N];
-        if constexpr (EIGHT) {
-            if (pool.packed()) {
-                unpack_eight(pool.kind == PoolKind::Q4_0, reinterpret_cast<const uint8_t *>(row), head.d / 4, at, x);
-            } else {
-                const u4 w = *reinterpret_cast<const u4_any *>(row + 8 * at);
-                for (int q = 0; q < 8; ++q) {
-                    const uint16_t b = static_cast<uint16_t>(w[q / 2] >> (16 * (q % 2)));
-                    x[q] = pool.kind == PoolKind::Bf16 ? from_half<true>(b) : from_half<false>(b);
-                }
+        const ReadItem it = read_item<EIGHT>(pool, pool.data + p * pool.st_page + h * pool.st_head + in * pool.st_tok, blocks, at);
+        write_item<EIGHT>(pool.kind, it, (val ? a.v : a.k) + static_cast<int64_t>(EIGHT ? 8 * at : at) * st[0] + h * st[1] + static_cast<int64_t>(t) * st[2], st[0]);
+    }
+}
+
+// As k_pa_read by eights, for tokens of 64 items or more.
+__global__ __launch_bounds__(kBlock) void k_pa_read_wide(PagedReadArgs a, uint32_t per, FastDiv page, FastDiv head, uint32_t items)
+{
+    constexpr uint32_t kBatch = 2;
+    const uint64_t slots = static_cast<uint64_t>(a.page) * a.pages;
+    const uint32_t t0 = blockIdx.x * per, blocks = head.d / 4;
+    const WaveShare w = wave_share(items);
+    for (uint32_t c = w.chunk; c < w.chunks; c += w.step) {
+        const uint32_t r = c * kWave + threadIdx.x % kWave;
+        if (r >= items) continue;
+        const uint32_t h = head.div(r), at = r - h * head.d;
+        for (uint32_t j0 = w.job; j0 < 2 * per; j0 += kBatch * w.wpc) {
+            ReadItem it[kBatch];
+            int32_t slot[kBatch];
+#pragma unroll
+            for (uint32_t n = 0; n < kBatch; ++n) {
+                const uint32_t j = j0 + n * w.wpc, t = t0 + (j >= per ? j - per : j);
+                slot[n] = j < 2 * per && t < a.tokens ? a.slots[static_cast<int64_t>(t) * a.slots_st] : -1;
+                if (slot[n] >= 0 && static_cast<uint64_t>(slot[n]) >= slots) slot[n] = -1;
             }
-        } else {
-            x[0] = pool.kind == PoolKind::Bf16 ? from_half<true>(row[at]) : from_half<false>(row[at]);
-        }
-        float *dst = (val ? a.v : a.k) + static_cast<int64_t>(N * at) * st[0] + h * st[1] + static_cast<int64_t>(t) * st[2];
-        if (EIGHT && st[0] == 1) {
-            for (uint32_t q = 0; q < N; q += 4) *reinterpret_cast<v4f_any *>(dst + q) = v4f{x[q], x[(q + 1) % N], x[(q + 2) % N], x[(q + 3) % N]};
-        } else {
-            for (uint32_t q = 0; q < N; ++q) dst[q * st[0]] = x[q];
+#pragma unroll
+            for (uint32_t n = 0; n < kBatch; ++n) {
+                if (slot[n] < 0) continue;
+                const PagePool &pool = j0 + n * w.wpc >= per ? a.v_pool : a.k_pool;
+                const uint32_t p = page.div(static_cast<uint32_t>(slot[n])), in = static_cast<uint32_t>(slot[n]) - p * page.d;
+                it[n] = read_item<true>(pool, pool.data + p * pool.st_page + in * pool.st_tok + h * pool.st_head, blocks, at);
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < kBatch; ++n) {
+                if (slot[n] < 0) continue;
+                const uint32_t j = j0 + n * w.wpc, t = t0 + (j >= per ? j - per : j);
+                const bool val = j >= per;
+                const int64_t *st = val ? a.v_st : a.k_st;
+                write_item<true>((val ? a.v_pool : a.k_pool).kind, it[n], (val ? a.v : a.k) + static_cast<int64_t>(t) * st[2] + h * st[1] + static_cast<int64_t>(8 * at) * st[0], st[0]);
+            }
         }
     }
 }
@@ -246,10 +358,11 @@ static void pa_append(const PagedAppendArgs &a, hipStream_t stream)
 template <uint32_t T>
 static void pk_append(const PagedAppendArgs &a, hipStream_t stream)
 {
-    const uint32_t head = a.dim / 8, grid = (a.tokens + T - 1) / T;
-    const FastDiv page(a.page), per_head(head), per_token(head * a.kv_heads);
-    if (a.k_st[0] == 1 && a.v_st[0] == 1) k_pk_append<T, true><<<grid, kBlock, 0, stream>>>(a, page, per_head, per_token);
-    else k_pk_append<T, false><<<grid, kBlock, 0, stream>>>(a, page, per_head, per_token);
+    const uint32_t head = a.dim / 8, grid = (a.tokens + T - 1) / T, items = head * a.kv_heads;
+    const FastDiv page(a.page), per_head(head), per_token(items);
+    if (items < kWave) k_pk_append<T><<<grid, kBlock, 0, stream>>>(a, page, per_head, per_token);
+    else if (a.k_st[0] == 1 && a.v_st[0] == 1) k_pk_append_wide<T, true><<<grid, kBlock, 0, stream>>>(a, page, per_head, items);
+    else k_pk_append_wide<T, false><<<grid, kBlock, 0, stream>>>(a, page, per_head, items);
 }
 
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t stream)
@@ -273,12 +386,22 @@ hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t stream)
 hipError_t launch_paged_read(const PagedReadArgs &a, hipStream_t stream)
 {
     const bool eight = a.dim % 8 == 0;
-    const uint32_t head = eight ? a.dim / 8 : a.dim;
-    const uint32_t per = a.tokens >= 2048 ? kPaRead : 1, grid = (a.tokens + per - 1) / per;
-    const FastDiv page(a.page), per_head(head), per_token(head * a.kv_heads);
-    if (eight) k_pa_read<true><<<grid, kBlock, 0, stream>>>(a, per, page, per_head, per_token);
-    else k_pa_read<false><<<grid, kBlock, 0, stream>>>(a, per, page, per_head, per_token);
-    return hipGetLastError();
+    const uint32_t head = eight ? a.dim / 8 : a.dim, items = head * a.kv_heads;
+    const FastDiv page(a.page), per_head(head), per_token(items);
+    PagedReadArgs b = a;
+    for (uint64_t t = 0; t < a.tokens; t += kPaReadTokens) {
+        b.tokens = static_cast<uint32_t>(a.tokens - t < kPaReadTokens ? a.tokens - t : kPaReadTokens);
+        b.slots = a.slots + static_cast<int64_t>(t) * a.slots_st;
+        b.k = a.k + static_cast<int64_t>(t) * a.k_st[2];
+        b.v = a.v + static_cast<int64_t>(t) * a.v_st[2];
+        const uint32_t per = a.tokens >= 2048 ? kPaRead : 1, grid = (b.tokens + per - 1) / per;
+        if (eight && items >= kWave) k_pa_read_wide<<<grid, kBlock, 0, stream>>>(b, per, page, per_head, items);
+        else if (eight) k_pa_read<true><<<grid, kBlock, 0, stream>>>(b, per, page, per_head, per_token);
+        else k_pa_read<false><<<grid, kBlock, 0, stream>>>(b, per, page, per_head, per_token);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 namespace {

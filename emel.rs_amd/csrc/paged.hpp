@@ -30,7 +30,7 @@ __device__ __forceinline__ float from_half(uint16_t h)
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float v)
 {
-    return __builtin_bit_cast(float, dpp32<CTRL>(__builtin_bit_cast(uint32_t, v)));
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 
 // A block's scale: what is not finite stands for NaN.

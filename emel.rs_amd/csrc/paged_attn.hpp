@@ -376,6 +376,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
     constexpr bool K4 = PAGES >= PaPages::Q4Q8, V4 = PAGES == PaPages::Q8Q4 || PAGES == PaPages::Q4Q4;
     constexpr int KI = K4 ? 8 : 16, VI = V4 ? 8 : 16; // packed: halves of a block's whole numbers
     constexpr int kAcc = PACKED ? 2 * KS : VW;
+    constexpr bool kEarly = PACKED && KS <= 4 && FOLD >= KS;
     constexpr int F = PACKED ? FOLD : 1, kSets = PACKED ? (KS + F - 1) / F : 1;
     // packed: blocks of set e; words that a lane loads of a token's, and of those before
     constexpr auto blocks_of = [](int e) { return e < KS / F ? F : KS - e * F; };
@@ -493,8 +494,8 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         float m = -__builtin_inff(), l = 0.0f;
         v4f acc[kAcc];
         for (int j = 0; j < kAcc; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        float unit[PACKED ? KS : 1]; // packed: acc is in these parts of one
-        for (float &u : unit) u = 0x1p24f;
+        float unit[PACKED ? KS : 1]; // packed: what scales are taken by, 1 in the lanes of keys; acc is in these parts of one
+        for (float &u : unit) u = lane < 32 ? 1.0f : 0x1p24f;
         bool bad = sq.bad;
 
         const uint32_t t_end = sq.tokens < u1 * kPaUnit ? sq.tokens : u1 * kPaUnit;
@@ -616,7 +617,8 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         __syncthreads();
         // The packed loop runs ahead of itself: a step's keys are asked for when
         // the last one's scores are done with theirs, its values behind the last
-        // one's sums, so each load has half a step of instructions to come in.
+        // one's sums, so each load has half a step of instructions to come in (the
+        // last step asks for its own last token once more).
         uint32_t kw[2][PACKED ? (K4 ? 1 : 2) * KS : 1];
         uint32_t vw[8][kWords];              // the words of each token that hold the lane's values
         uint16_t bits[PACKED ? KS : 1];      // the scales of lane % 32's token, of keys or values
@@ -660,31 +662,29 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         };
         // the scales of this step into LDS; what is not a token counts for nothing
         auto place_scales = [&] {
-            float d[KS];
-            bool over = false;
+            float d[KS], most = 0.0f;
             for (int e = 0; e < KS; ++e) {
                 d[e] = t0 + lane % 32 < t_end || lane < 32 ? pk_scale(bits[e]) : 0.0f;
-                over |= __builtin_fabsf(d[e]) * unit[e] > 1.0f;
+                most = __builtin_fmaxf(most, __builtin_fabsf(d[e] * unit[e]));
             }
             // A value's scale larger than all before: acc goes by a power of two
             // that holds it, and eight times as large ones, so that few steps
             // come by here.
-            if (__any(over && lane >= 32)) {
+            if (__any(most > 1.0f && lane >= 32)) {
                 float f[kSets];
                 for (float &x : f) x = 1.0f;
                 for (int e = 0; e < KS; ++e) {
-                    const float top = wave_max_dpp(lane < 32 ? 0.0f : __builtin_fabsf(d[e]));
-                    if (top * unit[e] > 1.0f) {
+                    const float top = wave_max_dpp(lane < 32 ? 0.0f : __builtin_fabsf(d[e])), was = lane_f32(unit[e], 32);
+                    if (top * was > 1.0f) {
                         const uint32_t to = (250u << 23) - (__builtin_bit_cast(uint32_t, top) & 0x7f800000u);
-                        if (part == static_cast<uint32_t>(e % F))
-                            f[e / F] = __builtin_bit_cast(float, (127u << 23) + to - __builtin_bit_cast(uint32_t, unit[e]));
-                        unit[e] = __builtin_bit_cast(float, to);
+                        if (part == static_cast<uint32_t>(e % F)) f[e / F] = __builtin_bit_cast(float, (127u << 23) + to - __builtin_bit_cast(uint32_t, was));
+                        if (lane >= 32) unit[e] = __builtin_bit_cast(float, to);
                     }
                 }
                 for (int j = 0; j < kAcc; ++j) acc[j] *= f[j / (2 * F)];
             }
             __builtin_amdgcn_wave_barrier();
-            for (int e = 0; e < KS; ++e) scales[wave][lane / 32][e][lane % 32] = d[e] * (lane < 32 ? 1.0f : unit[e]);
+            for (int e = 0; e < KS; ++e) scales[wave][lane / 32][e][lane % 32] = d[e] * unit[e];
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         };
@@ -703,8 +703,12 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
             }
         }
         for (; PACKED && t0 < t_end; t0 += kPaUnit) {
-            const bool more = t0 + kPaUnit < t_end;
             float z[8];
+            u4 early[kEarly ? KS * P : 1]; // the operands, asked for ahead of the scales where registers hold them
+            if constexpr (kEarly) {
+                for (int i = 0; i < KS * P; ++i) early[i] = planes[(i / P / F * P + i % P) * kPlane + (part == static_cast<uint32_t>(i / P % F) ? lane : kWave)];
+                __builtin_amdgcn_sched_barrier(0);
+            }
             place_scales();
             v4f sum[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
             for (int e = 0; e < kSets; ++e) {
@@ -717,8 +721,9 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                         else x[b] = pk_halves8(kw[b][2 * i], kw[b][2 * i + 1], magic);
                     }
                     for (int p = P - 1; p >= 0; --p)
-                        for (int b = 0; b < 2; ++b) c[b] = mfma32<false>(x[b], planes[(e * P + p) * kPlane + at], c[b]);
+                        for (int b = 0; b < 2; ++b) c[b] = mfma32<false>(x[b], kEarly ? early[kEarly ? i * P + p : 0] : planes[(e * P + p) * kPlane + at], c[b]);
                 }
+                if (e == kSets - 1) ask_keys(t0 + kPaUnit);
                 for (int b = 0; b < 2; ++b) {
                     const v4f d = four(0, e, b);
                     for (int i = 0; i < 4; ++i)
@@ -730,17 +735,19 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                 if constexpr (F > 1) x += dpp_f32<kDppXor1>(x);
                 if constexpr (F > 2) x += dpp_f32<kDppXor2>(x);
                 if constexpr (F > 4) x += dpp_f32<kDppHalfMirror>(x);
-                z[i] = x * inv;
+                z[i] = x;
             }
-            if (more) ask_keys(t0 + kPaUnit);
-            if (__builtin_expect(a.soft_cap > 0.0f, 0))
-                for (int i = 0; i < 8; ++i) z[i] = pa_tanh(z[i]) * (a.soft_cap * 1.44269504088896340736f);
+            float by = inv; // what scores are to be multiplied by
+            if (__builtin_expect(a.soft_cap > 0.0f, 0)) {
+                for (int i = 0; i < 8; ++i) z[i] = pa_tanh(z[i] * inv) * (a.soft_cap * 1.44269504088896340736f);
+                by = 1.0f;
+            }
             if (t0 + 32 > t_end)
                 for (int b = 0; b < 8; ++b)
                     if (t0 + 16 * (b / 4) + 4 * g + b % 4 >= t_end) z[b] = -__builtin_inff();
             float top = z[0];
             for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, z[i]);
-            top = rows16(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+            top = rows16(top, [](float x, float y) { return __builtin_fmaxf(x, y); }) * by;
             if (__any(top > m)) {
                 const float m1 = __builtin_fmaxf(m, top);
                 const float f = m1 > m ? __builtin_amdgcn_exp2f(m - m1) : 1.0f; // m = -inf: 0
@@ -751,7 +758,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
             const float ref = (m == -__builtin_inff() ? 0.0f : m) - kLift;
             float w[8];
             for (int i = 0; i < 8; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(z[i] - ref);
+                w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], by, -ref));
                 l += w[i];
             }
             for (int e = 0; e < kSets; ++e) {
@@ -782,7 +789,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                     sum = mfma32<false>(x, hi, sum);
                 }
             }
-            if (more) ask_values();
+            ask_values();
         }
         for (; !PACKED && t0 < t_end; t0 += kPaUnit) {
             {
@@ -870,7 +877,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         float eight[kSets][8];
         for (int e = 0; PACKED && e < kSets; ++e) {
             const int n = blocks_of(e);
-            float u = unit[e * F];
+            float u = lane_f32(unit[e * F], 32);
             for (int i = 0; i < 8; ++i) {
                 constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7}; // Q4_0: the nibble of each value
                 const int at = V4 ? order[i] : i;
@@ -881,7 +888,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
                 eight[e][i] = of(0);
                 for (int b = 1; b < n; ++b) eight[e][i] = part == static_cast<uint32_t>(b) ? of(b) : eight[e][i];
             }
-            for (int b = 1; b < n; ++b) u = part == static_cast<uint32_t>(b) ? unit[e * F + b] : u;
+            for (int b = 1; b < n; ++b) u = part == static_cast<uint32_t>(b) ? lane_f32(unit[e * F + b], 32) : u;
             const float by = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, u)); // 1 / u
             for (float &x : eight[e]) x *= by;
         }

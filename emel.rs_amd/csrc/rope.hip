@@ -1,17 +1,22 @@
 // rope.hip -- rotary positions of several axes, turned into queries and keys.
+#include <utility>
+
 #include "common.hpp"
 #include "launch.hpp"
 
 namespace emel {
 namespace {
 
-// Pair i of a head turns by position * frequency.  A thread keeps its pairs'
-// frequencies, in quarter turns a position and in 64 bits, and walks tokens
-// and heads; a token's angles serve all of its heads.  In quarter turns the
-// reduction of far positions is exact: t - rint(t), whose rounding is 2^-53 of t,
-// so an angle is off by 2^-52 of itself and by f32's rounding of what is left.
+// Pair i of a head turns by position * frequency.  A workgroup works its pairs'
+// frequencies out, in quarter turns a position and in 64 bits, then the cos and
+// sin of a tile of tokens, one of each a thread, and walks the tile's heads with
+// them.  In quarter turns the reduction of far positions is exact: t - rint(t),
+// whose rounding is 2^-53 of t, so an angle is off by 2^-52 of itself and by
+// f32's rounding of what is left.
 //
-// Bound by the bytes, 4 read and 4 written a value.
+// Bound by the bytes, 4 read and 4 written a value: 8001 tokens of 40 heads of 128
+// 60 us (5.4 TB/s), 73 with every thread working out its own pairs' angles for all
+// heads over again.
 
 typedef v4f v4f_any __attribute__((aligned(4)));
 
@@ -39,12 +44,18 @@ __device__ __forceinline__ void quarter_turns(double t, float &c, float &s)
 
 struct RopePlan {
     FastDiv items;   // of a head in a workgroup
+    FastDiv turning; // pairs of a workgroup's items
     uint32_t rot;    // items of a head that turn; the others copy
     uint32_t all;    // items of a head
     uint32_t per;    // heads of a step
     uint32_t steps;  // of a token
-    uint64_t units, run; // token steps: all, and of a workgroup
+    uint32_t tile;   // tokens of a workgroup
+    uint32_t groups; // workgroups that share a tile's steps
+    bool stream;     // outputs that the dies' caches do not hold, stored past them (60 us, 64 through them)
 };
+
+constexpr uint32_t kRopeTurns = 1024;     // angles of a tile
+constexpr uint32_t kRopeGrid = 1u << 22;  // tiles of a launch, and its workgroups: threads are counted in 32 bits
 
 // An item: four pairs, or eight values behind the pairs that are copied; one
 // pair and two values where VEC is false.
@@ -52,98 +63,114 @@ template <bool VEC, bool ADJ>
 __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a, RopePlan pl)
 {
     constexpr uint32_t W = VEC ? 4 : 1;
-    const uint32_t slot = pl.items.div(threadIdx.x);
-    const uint32_t item = threadIdx.x - slot * pl.items.d + blockIdx.y * kBlock;
-    if (slot >= pl.per || item >= pl.all) return;
-    const bool turns = item < pl.rot;
+    __shared__ double freq[W * kBlock];
+    __shared__ uint8_t axis[W * kBlock];
+    __shared__ __attribute__((aligned(16))) float cosines[kRopeTurns], sines[kRopeTurns];
+    const uint32_t tid = threadIdx.x, first = blockIdx.y * kBlock; // the workgroup's items from `first` on
+    const uint32_t slot = pl.items.div(tid), local = tid - slot * pl.items.d, item = local + first;
+    const bool mine = slot < pl.per && item < pl.all, turns = item < pl.rot;
+    const uint32_t left = a.pairs > first * W ? a.pairs - first * W : 0, pairs = left < pl.items.d * W ? left : pl.items.d * W;
+    const uint32_t tile = blockIdx.x / pl.groups, group = blockIdx.x - tile * pl.groups;
+    const uint32_t token0 = tile * pl.tile, tokens = a.tokens - token0 < pl.tile ? a.tokens - token0 : pl.tile;
     const uint32_t heads = a.q.heads + a.k.heads;
 
-    double freq[W];
-    uint32_t axis[W];
-    if (turns) {
-        for (uint32_t w = 0; w < W; ++w) {
-            const uint32_t i = item * W + w;
-            RopeRun r = a.runs[0];
-            for (int n = 1; n < 4; ++n)
-                if (i >= a.runs[n].start) r = a.runs[n];
-            const uint32_t at = i - r.start, round = r.live == 1 ? at : r.live == 2 ? at / 2 : r.live == 3 ? at / 3 : at / 4;
-            axis[w] = (r.axes >> (2 * (at - round * r.live))) & 3u;
-            const double j = a.own ? r.round + round : i;
-            const double rate = axis[w] == 0 ? a.rate[0] : axis[w] == 1 ? a.rate[1] : axis[w] == 2 ? a.rate[2] : a.rate[3];
-            freq[w] = a.quarters * exp2(-j * rate);
-            if (a.factors) freq[w] /= static_cast<double>(a.factors[static_cast<int64_t>(i) * a.factors_st]);
-        }
-    }
-    uint64_t u = blockIdx.x * pl.run;
-    const uint64_t end = u + pl.run < pl.units ? u + pl.run : pl.units;
-    uint64_t token = u / pl.steps;
-    uint32_t step = static_cast<uint32_t>(u - token * pl.steps);
-    bool fresh = true;
-    float c[W], s[W];
-    for (; u < end; ++u) {
-        const uint32_t h = step * pl.per + slot;
-        const bool live = h < heads;
-        const bool is_k = h >= a.q.heads;
-        const RopeTensor &t = is_k ? a.k : a.q;
-        const int64_t head = is_k ? h - a.q.heads : h;
-        const float *x = t.x + head * t.x_st[1] + static_cast<int64_t>(token) * t.x_st[2];
-        float *y = t.y + head * t.y_st[1] + static_cast<int64_t>(token) * t.y_st[2];
-        // the first values of the item's pairs and their second ones
-        const uint32_t d0 = turns ? (ADJ ? 2 * W * item : W * item) : 2 * a.pairs + 2 * W * (item - pl.rot);
-        const uint32_t d1 = !turns || ADJ ? d0 + W : d0 + a.pairs;
+    // the first values of the item's pairs and their second ones
+    const uint32_t d0 = turns ? (ADJ ? 2 * W * item : W * item) : 2 * a.pairs + 2 * W * (item - pl.rot);
+    const uint32_t d1 = !turns || ADJ ? d0 + W : d0 + a.pairs;
+    struct Unit {
+        const float *x;
+        float *y;
+        int64_t st;
         float lo[W], hi[W];
-        if (live) {
-            if constexpr (VEC) {
-                const v4f p = *reinterpret_cast<const v4f_any *>(x + d0), r = *reinterpret_cast<const v4f_any *>(x + d1);
-                for (int w = 0; w < 4; ++w) {
-                    lo[w] = p[w];
-                    hi[w] = r[w];
-                }
+    };
+    auto ask = [&](uint32_t t, uint32_t step) {
+        Unit n = {};
+        const uint32_t h = step * pl.per + slot;
+        if (!mine || h >= heads) return n;
+        const RopeTensor &r = h >= a.q.heads ? a.k : a.q;
+        const int64_t head = h >= a.q.heads ? h - a.q.heads : h;
+        n.x = r.x + head * r.x_st[1] + static_cast<int64_t>(token0 + t) * r.x_st[2];
+        n.y = r.y + head * r.y_st[1] + static_cast<int64_t>(token0 + t) * r.y_st[2];
+        n.st = r.y_st[0];
+        if constexpr (VEC) {
+            const v4f p = *reinterpret_cast<const v4f_any *>(n.x + d0), q = *reinterpret_cast<const v4f_any *>(n.x + d1);
+            for (int w = 0; w < 4; ++w) {
+                n.lo[w] = p[w];
+                n.hi[w] = q[w];
+            }
+        } else {
+            n.lo[0] = n.x[d0 * r.x_st[0]];
+            n.hi[0] = d1 < a.dim ? n.x[d1 * r.x_st[0]] : 0.0f;
+        }
+        return n;
+    };
+    Unit next = ask(0, group);
+
+    for (uint32_t j = tid; j < pairs; j += kBlock) {
+        const uint32_t i = first * W + j;
+        RopeRun r = a.runs[0];
+        for (int n = 1; n < 4; ++n)
+            if (i >= a.runs[n].start) r = a.runs[n];
+        const uint32_t at = i - r.start, round = r.live == 1 ? at : r.live == 2 ? at / 2 : r.live == 3 ? at / 3 : at / 4;
+        const uint32_t x = (r.axes >> (2 * (at - round * r.live))) & 3u;
+        const double rate = x == 0 ? a.rate[0] : x == 1 ? a.rate[1] : x == 2 ? a.rate[2] : a.rate[3];
+        const double e = a.own ? r.round + round : i;
+        axis[j] = static_cast<uint8_t>(x);
+        freq[j] = a.quarters * exp2(-e * rate);
+        if (a.factors) freq[j] /= static_cast<double>(a.factors[static_cast<int64_t>(i) * a.factors_st]);
+    }
+    __syncthreads();
+    for (uint32_t e = tid; e < tokens * pairs; e += kBlock) {
+        const uint32_t t = pl.tile == 1 ? 0 : pl.turning.div(e), j = e - t * pairs;
+        const int32_t p = a.pos[static_cast<int64_t>(token0 + t) * a.pos_st[0] + axis[j] * a.pos_st[1]];
+        float c, s;
+        quarter_turns(p * freq[j], c, s);
+        cosines[e] = c * a.magnitude;
+        sines[e] = s * (a.back ? -a.magnitude : a.magnitude);
+    }
+    __syncthreads();
+    for (uint32_t t = 0, step = group; t < tokens;) {
+        const Unit n = next;
+        const uint32_t at = t * pairs + local * W; // of the item's angles
+        step += pl.groups;
+        if (step >= pl.steps) {
+            step = group;
+            ++t;
+        }
+        if (t < tokens) next = ask(t, step); // ahead of this one's stores
+        if (!n.y || (!turns && n.x == n.y)) continue;
+        float o0[W], o1[W], c[W], s[W];
+        for (uint32_t w = 0; w < W; ++w) {
+            c[w] = turns ? cosines[at + w] : 1.0f;
+            s[w] = turns ? sines[at + w] : 0.0f;
+        }
+        for (uint32_t w = 0; w < W; ++w) {
+            if (!turns) {
+                o0[w] = n.lo[w];
+                o1[w] = n.hi[w];
+            } else if constexpr (VEC && ADJ) { // pairs 0, 1 in lo, 2, 3 in hi
+                const float *v = w < 2 ? n.lo : n.hi;
+                const float e = v[2 * (w % 2)], f = v[2 * (w % 2) + 1];
+                float *o = w < 2 ? o0 : o1;
+                o[2 * (w % 2)] = __builtin_fmaf(e, c[w], -(f * s[w]));
+                o[2 * (w % 2) + 1] = __builtin_fmaf(e, s[w], f * c[w]);
             } else {
-                lo[0] = x[d0 * t.x_st[0]];
-                hi[0] = d1 < a.dim ? x[d1 * t.x_st[0]] : 0.0f;
+                o0[w] = __builtin_fmaf(n.lo[w], c[w], -(n.hi[w] * s[w]));
+                o1[w] = __builtin_fmaf(n.lo[w], s[w], n.hi[w] * c[w]);
             }
         }
-        if (turns && fresh) {
-            int32_t p[W];
-            for (uint32_t w = 0; w < W; ++w) p[w] = a.pos[static_cast<int64_t>(token) * a.pos_st[0] + axis[w] * a.pos_st[1]];
-            for (uint32_t w = 0; w < W; ++w) {
-                quarter_turns(p[w] * freq[w], c[w], s[w]);
-                c[w] *= a.magnitude;
-                s[w] *= a.back ? -a.magnitude : a.magnitude;
+        if constexpr (VEC) {
+            const v4f p = {o0[0], o0[1], o0[2], o0[3]}, q = {o1[0], o1[1], o1[2], o1[3]};
+            if (pl.stream) {
+                __builtin_nontemporal_store(p, reinterpret_cast<v4f_any *>(n.y + d0));
+                __builtin_nontemporal_store(q, reinterpret_cast<v4f_any *>(n.y + d1));
+            } else {
+                *reinterpret_cast<v4f_any *>(n.y + d0) = p;
+                *reinterpret_cast<v4f_any *>(n.y + d1) = q;
             }
-        }
-        if (live) {
-            float o0[W], o1[W];
-            for (uint32_t w = 0; w < W; ++w) {
-                if (!turns) {
-                    o0[w] = lo[w];
-                    o1[w] = hi[w];
-                } else if constexpr (VEC && ADJ) { // pairs 0, 1 in lo, 2, 3 in hi
-                    const float *v = w < 2 ? lo : hi;
-                    const float e = v[2 * (w % 2)], f = v[2 * (w % 2) + 1];
-                    float *o = w < 2 ? o0 : o1;
-                    o[2 * (w % 2)] = __builtin_fmaf(e, c[w], -(f * s[w]));
-                    o[2 * (w % 2) + 1] = __builtin_fmaf(e, s[w], f * c[w]);
-                } else {
-                    o0[w] = __builtin_fmaf(lo[w], c[w], -(hi[w] * s[w]));
-                    o1[w] = __builtin_fmaf(lo[w], s[w], hi[w] * c[w]);
-                }
-            }
-            if (turns || x != y) {
-                if constexpr (VEC) {
-                    *reinterpret_cast<v4f_any *>(y + d0) = v4f{o0[0], o0[1], o0[2], o0[3]};
-                    *reinterpret_cast<v4f_any *>(y + d1) = v4f{o1[0], o1[1], o1[2], o1[3]};
-                } else {
-                    y[d0 * t.y_st[0]] = o0[0];
-                    if (d1 < a.dim) y[d1 * t.y_st[0]] = o1[0];
-                }
-            }
-        }
-        fresh = ++step == pl.steps;
-        if (fresh) {
-            step = 0;
-            ++token;
+        } else {
+            n.y[d0 * n.st] = o0[0];
+            if (d1 < a.dim) n.y[d1 * n.st] = o1[0];
         }
     }
 }
@@ -156,15 +183,37 @@ hipError_t rope(const RopeArgs &a, hipStream_t stream)
     pl.rot = (a.pairs + W - 1) / W;
     pl.all = pl.rot + (a.dim - 2 * a.pairs + 2 * W - 1) / (2 * W);
     const uint32_t items = pl.all < kBlock ? pl.all : kBlock, chunks = (pl.all + kBlock - 1) / kBlock;
+    const uint32_t pairs = a.pairs < items * W ? a.pairs : items * W; // of a workgroup, at most
     pl.items = FastDiv(items);
     pl.per = kBlock / items;
     pl.steps = (a.q.heads + a.k.heads + pl.per - 1) / pl.per;
-    pl.units = static_cast<uint64_t>(a.tokens) * pl.steps;
-    const uint64_t most = 2048;
-    pl.run = (pl.units + most - 1) / most;
-    const uint32_t grid = static_cast<uint32_t>((pl.units + pl.run - 1) / pl.run);
-    k_rope<VEC, ADJ><<<dim3(grid, chunks), kBlock, 0, stream>>>(a, pl);
-    return hipGetLastError();
+    // Tiles for some 8000 workgroups (8001 tokens of 40 heads of 128 60.1 us, 71.7 with
+    // 2000), and no more angles than their places; heads of more items than a
+    // workgroup has threads take a token at a time, as their last workgroup has fewer
+    // pairs.  Few tokens' heads are shared out too.
+    const uint32_t most = chunks > 1 ? 1 : kRopeTurns / pairs, want = a.tokens / 8192 + 1;
+    pl.tile = want < most ? want : most;
+    uint32_t tiles = (a.tokens + pl.tile - 1) / pl.tile;
+    tiles = tiles < kRopeGrid ? tiles : kRopeGrid;
+    pl.groups = tiles < 512 ? pl.steps : 1;
+    if (pl.groups > kRopeGrid / tiles) pl.groups = kRopeGrid / tiles;
+    pl.stream = static_cast<uint64_t>(a.tokens) * (a.q.heads + a.k.heads) * a.dim * 4 > uint64_t{32} << 20;
+    pl.turning = FastDiv(pairs);
+    RopeArgs b = a;
+    const uint64_t part = static_cast<uint64_t>(tiles) * pl.tile;
+    for (uint64_t t = 0; t < a.tokens; t += part) {
+        b.tokens = static_cast<uint32_t>(a.tokens - t < part ? a.tokens - t : part);
+        b.pos = a.pos + static_cast<int64_t>(t) * a.pos_st[0];
+        for (auto [to, from] : {std::pair<RopeTensor *, const RopeTensor *>{&b.q, &a.q}, {&b.k, &a.k}}) {
+            to->x = from->x + static_cast<int64_t>(t) * from->x_st[2];
+            to->y = from->y + static_cast<int64_t>(t) * from->y_st[2];
+        }
+        const uint32_t grid = (b.tokens + pl.tile - 1) / pl.tile * pl.groups;
+        k_rope<VEC, ADJ><<<dim3(grid, chunks), kBlock, 0, stream>>>(b, pl);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 } // namespace

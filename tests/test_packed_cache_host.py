@@ -110,12 +110,30 @@ def test_attention_refusals(rec):
 
 
 def test_halves_are_read_too(rec):
-    for kind, dim in ((F16, 64), (BF16, 20)):
+    for kind, dim, kernel in ((F16, 64, "k_pa_read<true>"), (BF16, 20, "k_pa_read<false>"), (F16, 256, "k_pa_read_wide")):
         event = eh.OpPagedKvRead(v(3, [dim, P, H, N], kind), v(4, [dim, P, H, N], kind), v(2, [T, 1, 1, 1], I32), v(0, [dim, H, T, 1], mut=True), v(1, [dim, H, T, 1], mut=True))
         got, = rec.launches(event)
-        assert f"k_pa_read<{'true' if dim % 8 == 0 else 'false'}>" in got.name
+        assert kernel in got.name
     mixed = eh.OpPagedKvRead(pool(3, F16), pool(4, BF16), v(2, [T, 1, 1, 1], I32), v(0, [D, H, T, 1], mut=True), v(1, [D, H, T, 1], mut=True))
     assert status(rec, mixed) == S.SHAPE_MISMATCH
+
+
+@pytest.mark.parametrize("tokens,launches", [(1, 1), (1 << 17, 1), (1 << 25, 1), ((1 << 25) + 1, 2), ((1 << 31) - 1, 64)])
+def test_reads_of_many_tokens_run_in_parts(rec, tokens, launches):
+    """A launch counts its threads in 32 bits."""
+    event = eh.OpPagedKvRead(v(3, [32, 16, 1, 9000], Q4_0), v(4, [32, 16, 1, 9000], Q8_0), v(2, [tokens, 1, 1, 1], I32), v(0, [32, 1, tokens, 1], mut=True, size=1 << 50),
+                             eh.TensorViewMut(1 << 60, eh.Layout.dense(F32, [32, 1, tokens, 1]), 1 << 50))
+    got = rec.launches(event)
+    assert len(got) == launches and all(g.grid * g.block < 1 << 32 for g in got)
+
+
+@pytest.mark.parametrize("items", [1, 4, 16])
+def test_wide_tokens_share_a_workgroups_waves(rec, items):
+    for dim, kv, tokens in ((128, items, 5000), (256, items, 3)):
+        event = eh.OpPagedKvAppend(v(0, [dim, kv, tokens, 1]), v(1, [dim, kv, tokens, 1]), v(2, [tokens, 1, 1, 1], I32), v(3, [dim, 16, kv, 900], Q4_0, mut=True),
+                                   v(4, [dim, 16, kv, 900], Q8_0, mut=True))
+        got, = rec.launches(event)
+        assert ("wide" in got.name) == (dim // 8 * kv >= 64) and got.grid == (-(-tokens // 8) if tokens >= 2048 else tokens)
 
 
 @pytest.mark.parametrize("tokens,launches", [(1, 1), (1 << 17, 1), ((1 << 17) + 1, 2)])

@@ -109,3 +109,11 @@ def test_every_head_is_in_some_step(rec):
     for dim, heads, tokens in ((2, 1000, 3), (1024, 5, 1), (4096, 3, 7), (1 << 24, 1, 1), (6, 1, 100000)):
         got, = rec.launches(eh.OpRope(view(0, [dim, heads, tokens, 1]), view(1, [dim, heads, tokens, 1], mut=True), view(4, [tokens, 1, 1, 1], dtype=I32), [1]))
         assert got.block == 256 and got.grid > 0
+
+
+@pytest.mark.parametrize("dim,tokens,launches", [(64, 100000, 1), (64, (1 << 31) - 1, 16), (2048, (1 << 22) + 1, 2)])
+def test_very_many_tokens_run_in_parts(rec, dim, tokens, launches):
+    """A launch counts its threads in 32 bits."""
+    big = lambda at, mut=False: (eh.TensorViewMut if mut else eh.TensorView)(at << 58, eh.Layout.dense(eh.DType.F32, [dim, 1, tokens, 1]), 1 << 57)  # noqa: E731
+    got = rec.launches(eh.OpRope(big(1), big(2, True), view(4, [tokens, 1, 1, 1], dtype=I32), [dim // 2]))
+    assert len(got) == launches and all(g.grid * g.block < 1 << 32 for g in got)
