@@ -411,6 +411,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
     const uint32_t rows = PACKED ? pl.rows / pl.side : pl.rows;
     const uint32_t first_lane = thread % kWave;
     uint32_t total, run, cur, base; // base: the sequence's first unit
+    uint32_t more = 0; // packed: workgroups that take a unit above `run`, the first ones
     uint32_t s, setup;
     int32_t s_len;
     if (__builtin_expect(a.seqs <= kWave, 1)) { // every wave for itself: a sequence per first_lane
@@ -422,8 +423,12 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         setup = all * rows > share.d;
         total = (all + setup * a.seqs) * rows;
         pre += setup * (first_lane + 1);
-        run = share.div(total + share.d - 1);
+        run = share.div(PACKED ? total : total + share.d - 1);
         cur = block * run;
+        if constexpr (PACKED) {
+            more = total - run * share.d;
+            cur += block < more ? block : more;
+        }
         if (cur >= total) return;
         s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(__popcll(__ballot(first_lane < a.seqs && pre * rows <= cur))));
         base = lane_u32(pre - mine - setup, s) * rows;
@@ -447,8 +452,12 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         pre += setup * s0 - mine;
         mine += setup * (s1 - s0);
         total = (all + setup * a.seqs) * rows;
-        run = share.div(total + share.d - 1);
+        run = share.div(PACKED ? total : total + share.d - 1);
         cur = block * run;
+        if constexpr (PACKED) {
+            more = total - run * share.d;
+            cur += block < more ? block : more;
+        }
         if (cur >= total) return;
         if (mine && pre * rows <= cur && cur < (pre + mine) * rows) {
             uint32_t i = s0;
@@ -465,7 +474,13 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         base = found[1] * rows;
         s_len = pa_len(a, s);
     }
-    const uint32_t end = cur + run < total ? cur + run : total;
+    const uint32_t end = PACKED ? cur + run + (block < more) : cur + run < total ? cur + run : total;
+    // the block that has a unit
+    auto block_of = [&](uint32_t u) {
+        if (!PACKED) return u / run;
+        const uint32_t longer = more * (run + 1);
+        return u < longer ? u / (run + 1) : more + (u - longer) / run;
+    };
 
     PaSeq sq = pa_seq(a, s_len);
     uint32_t units = sq.units + setup;
@@ -979,7 +994,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         __syncthreads();
         const bool begins = PACKED ? u0 == 0 : n0 == 0;
         const bool whole = begins && n1 == units;
-        const uint32_t w0 = begins ? block : (row_at + (PACKED ? setup : 0)) / run; // the row's first workgroup
+        const uint32_t w0 = begins ? block : block_of(row_at + (PACKED ? setup : 0)); // the row's first workgroup
         const uint32_t own_block = PACKED ? block * pl.side + lane_row : block;
         float *slot = pl.parts + static_cast<size_t>(2 * own_block + (begins ? 1 : 0)) * pl.slot;
         // the waves' maximum and sum of a head, and each wave's weight
@@ -995,7 +1010,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedA
         };
         asm volatile("" : "+v"(tid));
         if constexpr (PACKED) {
-            pa_ends(a, pl, PaEnd{sq.tokens == 0 && !sq.bad, whole, heads, h0, s, w0, lane_row, (row_at + units - 1) / run - w0 + 1}, slot, joined,
+            pa_ends(a, pl, PaEnd{sq.tokens == 0 && !sq.bad, whole, heads, h0, s, w0, lane_row, whole ? 1 : block_of(row_at + units - 1) - w0 + 1}, slot, joined,
                     &wm[0][0], &wl[0][0], &last, tid);
             __syncthreads(); // the next segment reuses the shared arrays
             cur = row_at + n1;
