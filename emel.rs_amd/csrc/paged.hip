@@ -462,7 +462,7 @@ PaGrid pa_grid(const PagedAttnArgs &a)
     const uint32_t ks = (a.dim + 31) / 32, fixed = a.k_pool.packed() ? 4096 + ks * 1024 : 4096 + ks * 3 * 1024;
     const uint32_t sets = (ks + pa_fold(a) - 1) / pa_fold(a);
     const uint32_t planes = a.k_pool.packed() ? sets * 2 * (kWave + 1) * 4 : 0; // of score operands
-    uint32_t per = pa_per_cu(pa_pages(a), static_cast<int>(ks));
+    uint32_t per = pa_per_cu(static_cast<int>(ks), a.k_pool.packed() ? static_cast<int>(pa_fold(a)) : 0);
     for (;; --per) {
         const uint32_t side = pa_side(a, cus * per);
         const uint32_t joined = 4 * pa_heads(a) * (a.dim + 4), weights = (a.k_pool.packed() ? kPaLead : 0) + pa_heads(a) * (cus * per / side);

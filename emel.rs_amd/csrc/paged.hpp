@@ -51,8 +51,11 @@ constexpr uint32_t kPaLine = 64;   // words between arrival counters (a cache li
 enum class PaPages : int { F16 = 0, Bf16, Q8Q8, Q8Q4, Q4Q8, Q4Q4 };
 
 // Workgroups that a compute unit holds at once: the registers that their
-// launch bounds leave them.
-constexpr uint32_t pa_per_cu(PaPages, int ks) { return ks <= 2 ? 4 : ks <= 4 ? 3 : 2; }
+// launch bounds leave them.  `fold` is 0 for halves.  Packed heads of 96 and 128 with a
+// column each (more than 8 heads share their keys) scale and split a block's
+// weights at a time, which 168 registers do not hold: 64 sequences of 90 to 9000
+// tokens with 32/2 heads of 128 in Q4_0 35.4 us, 42.6 with three, in Q8_0 38.0 and 51.4.
+constexpr uint32_t pa_per_cu(int ks, int fold) { return ks <= 2 ? 4 : ks <= 4 && fold != 1 ? 3 : 2; }
 
 // What a launch derives on the host.
 struct PaPlan {

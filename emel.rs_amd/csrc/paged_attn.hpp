@@ -368,7 +368,7 @@ __device__ __forceinline__ void pa_ends(const PagedAttnArgs &a, const PaPlan &pl
 // blocks: it loads what lies side by side.  All of that costs as many matrix instructions
 // as FOLD 1 does.
 template <PaPages PAGES, int KS, int VW, int FOLD = 0>
-__global__ __launch_bounds__(kBlock, pa_per_cu(PAGES, KS)) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
+__global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAttnArgs a, PaPlan pl)
 {
     constexpr bool BF16 = PAGES == PaPages::Bf16, PACKED = PAGES > PaPages::Bf16;
     constexpr int P = kParts<BF16>;

@@ -102,7 +102,7 @@ def test_shapes_that_take_vectors(rec):
         return "k_rope<true" in got.name
 
     assert vec() and vec(80, (20, 20)) and vec(96, (16, 16, 8)) and vec(96, (20, 7, 17))
-    assert not vec(80, (33,)) and not vec(66, (32,)) and not vec(nb=[8, 512, 3072, 15360])
+    assert not vec(80, (33,)) and not vec(66, (32,)) and not vec(nb=[8, 544, 3264, 16320])
 
 
 def test_every_head_is_in_some_step(rec):
