@@ -1,5 +1,6 @@
 // paged_attn.hpp -- the attention of one new token per sequence over a paged
-// cache: the kernel that paged.hip builds for halves and packed.hip for packed rows.
+// cache: the kernel that paged.hip builds for halves, and a source for each pair of
+// types for packed rows.
 #pragma once
 
 #include "paged.hpp"
@@ -51,6 +52,24 @@ namespace {
 // the row's waves together are not.  The walk takes bf16 values by 2^-34, and a maximum
 // 34 above its own, which is what the joins weigh a part by.
 
+// Packed rows go the same way with their whole numbers as f16 halves, which are exact:
+//   scores   a block's products with q, two halves a value, times the block's
+//            scale in f32, added up over the blocks.
+//   values   out^T[dim, head] = N^T (w d)^T: a weight by the scale of its token's block
+//            is one f32 factor, taken by a power of two that keeps the largest
+//            such factor of a block of dims at 1 or below (`unit`: out is in parts of
+//            it until the end) and then cut into hi + lo: off by 2^-22 of
+//            itself, or 2^-35 of the block's largest where lo is subnormal.
+// A 32-token step of a head of 128 in Q4_0 is some 400 vector instructions, most of
+// them numbers made halves, and 32 matrix ones for 4.6 KB: what bounds short and middle
+// rows (64 sequences of 90 to 9000 tokens, 32/8 heads of 128: 55.6 us, 148 MB, 2.7
+// TB/s).  A token's rows are scattered over its page besides: 64 of 8000 take 178 us with
+// a token's heads in a row, 135 with a head's tokens in a row.  Long rows in
+// Q8_0 are bound by HBM (two of 40001 to 60001 with 32/32 heads: 169 us, 870 MB, 5.1
+// TB/s).  One sequence of 4001 takes 13 us, as with halves: latency.
+// A row's end runs once a workgroup, from cold: loops that were unrolled, 42 KB of code
+// with the rest, made the last workgroups of rows take 10 to 15 us longer than the 22 KB here.
+//
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
@@ -399,6 +418,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
     // Rows of a few units are mostly set-up, which more workgroups hide; long
     // ones stream best with two a compute unit (64 sequences of 90 to 9000
     // tokens 106 us, 113 with three; 640 of 100 tokens 90 us, 77 with three).
+    // Packed rows are unpacked as much as loaded, and take all.
     auto share_of = [&](uint32_t units) { return !PACKED && units > 4 * a.seqs ? pl.few : pl.grid; };
     // This workgroup's run of units, and the sequence it starts in.  A row's
     // set-up and end cost about a unit: it counts as one more, but where there

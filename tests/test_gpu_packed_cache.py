@@ -271,7 +271,7 @@ def test_attention_windows_caps_and_scales(gpu, kinds, window, cap, scale):
 
 
 @pytest.mark.parametrize("kinds", [KINDS[0], KINDS[3]])
-@pytest.mark.parametrize("seqs,low,high,heads,kv,dim", [(1, 9000, 9000, 8, 2, 128), (70, 1, 300, 4, 1, 64), (300, 3, 40, 8, 2, 64), (2, 3000, 5000, 8, 8, 256)])
+@pytest.mark.parametrize("seqs,low,high,heads,kv,dim", [(1, 9000, 9000, 8, 2, 128), (70, 1, 300, 4, 1, 64), (300, 3, 40, 8, 2, 64), (2, 3000, 5000, 8, 8, 256), (3, 500, 3000, 32, 32, 64), (2, 700, 1500, 48, 48, 128), (1, 1, 1, 64, 64, 32)])
 def test_attention_of_long_and_many_sequences(gpu, kinds, seqs, low, high, heads, kv, dim):
     lengths = rng(seqs).integers(low, high + 1, seqs).tolist()
     c = attend_case(gpu, kinds, heads, kv, dim, 16, lengths, "token", seqs)
