@@ -263,6 +263,15 @@ def test_attention_matches_the_formula(gpu, kinds, heads, kv, dim, page, order):
 
 
 @pytest.mark.parametrize("kinds", KINDS)
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 8, 9, 16])
+def test_attention_of_every_width_and_group(gpu, kinds, dim, group):
+    c = attend_case(gpu, kinds, 2 * group, 2, dim, 16, [1, 40, 300, 0, 515], "token", dim + group)
+    run(attend_event(c))
+    check_attention(c)
+
+
+@pytest.mark.parametrize("kinds", KINDS)
 @pytest.mark.parametrize("window,cap,scale", [(1, 0.0, 0.1), (33, 0.0, 0.2), (128, 30.0, 0.3), (1000, 5.0, -0.2), (10**9, 0.0, 0.0), (0, 50.0, 2.0)])
 def test_attention_windows_caps_and_scales(gpu, kinds, window, cap, scale):
     c = attend_case(gpu, kinds, 6, 2, 128, 16, [1, 5, 130, 1200, 0, 2049], "token", 7)
@@ -271,7 +280,7 @@ def test_attention_windows_caps_and_scales(gpu, kinds, window, cap, scale):
 
 
 @pytest.mark.parametrize("kinds", [KINDS[0], KINDS[3]])
-@pytest.mark.parametrize("seqs,low,high,heads,kv,dim", [(1, 9000, 9000, 8, 2, 128), (70, 1, 300, 4, 1, 64), (300, 3, 40, 8, 2, 64), (2, 3000, 5000, 8, 8, 256), (3, 500, 3000, 32, 32, 64), (2, 700, 1500, 48, 48, 128), (1, 1, 1, 64, 64, 32)])
+@pytest.mark.parametrize("seqs,low,high,heads,kv,dim", [(1, 9000, 9000, 8, 2, 128), (70, 1, 300, 4, 1, 64), (300, 3, 40, 8, 2, 64), (2, 3000, 5000, 8, 8, 256), (3, 500, 3000, 32, 32, 64), (2, 700, 1500, 48, 48, 128), (1, 1, 1, 64, 64, 32), (1, 60000, 60000, 4, 1, 64), (1, 50000, 50000, 16, 1, 96)])
 def test_attention_of_long_and_many_sequences(gpu, kinds, seqs, low, high, heads, kv, dim):
     lengths = rng(seqs).integers(low, high + 1, seqs).tolist()
     c = attend_case(gpu, kinds, heads, kv, dim, 16, lengths, "token", seqs)
@@ -540,5 +549,59 @@ def test_streams_do_not_share_scratch(gpu):
         for s, c in zip(streams, cases):
             assert eh.Kernel(s.cuda_stream, synchronous=False).process_event(attend_event(c)) == eh.Status.OK
     torch.cuda.synchronize()
+    for c in cases:
+        check_attention(c)
+
+
+def test_scratch_does_not_grow_under_capture(gpu):
+    """Refused where the call's scratch would grow; a reserve ahead lets it in."""
+    import ctypes
+
+    import torch
+
+    handle = ctypes.c_void_p()  # one of torch's streams may have scratch already
+    assert eh.load().emel_stream_create(ctypes.byref(handle)) == eh.Status.OK
+    stream = torch.cuda.ExternalStream(handle.value)
+    kernel = eh.Kernel(stream.cuda_stream, synchronous=False)
+    c = attend_case(gpu, KINDS[0], 8, 2, 128, 16, [900, 3], "token", 44)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        c["q"].mul_(1.0)
+        assert kernel.process_event(attend_event(c)) == eh.Status.STREAM_CAPTURE
+    assert eh.stream_reserve(32 << 20, 1 << 20, stream.cuda_stream) == eh.Status.OK
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        assert kernel.process_event(attend_event(c)) == eh.Status.OK
+    for _ in range(3):
+        c["y"].fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(c)
+    del graph
+    assert eh.load().emel_stream_destroy(handle) == eh.Status.OK
+
+
+def test_two_host_threads_on_one_stream(gpu):
+    import threading
+
+    import torch
+
+    stream = torch.cuda.Stream()
+    cases = [attend_case(gpu, KINDS[i], 8, 2, 64 * i, 16, [700, 40, 1500], "token", 50 + i) for i in (1, 2, 3)]
+    torch.cuda.synchronize()
+    got = []
+
+    def work(c):
+        kernel = eh.Kernel(stream.cuda_stream, synchronous=False)
+        got.append([kernel.process_event(attend_event(c)) for _ in range(20)])
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert got == [[eh.Status.OK] * 20] * 3
     for c in cases:
         check_attention(c)
