@@ -55,7 +55,13 @@ enum class PaPages : int { F16 = 0, Bf16, Q8Q8, Q8Q4, Q4Q8, Q4Q4 };
 // column each (more than 8 heads share their keys) scale and split a block's
 // weights at a time, which 168 registers do not hold: 64 sequences of 90 to 9000
 // tokens with 32/2 heads of 128 in Q4_0 35.4 us, 42.6 with three, in Q8_0 38.0 and 51.4.
-constexpr uint32_t pa_per_cu(int ks, int fold) { return ks <= 2 ? 4 : ks <= 4 && fold != 1 ? 3 : 2; }
+// Heads of 64 with a column each do not fit 128 registers: 24/2 heads in Q4_0 23.2 us, 24.9
+// with four, in Q8_0 25.1 and 30.1.
+constexpr uint32_t pa_per_cu(int ks, int fold)
+{
+    if (fold == 1 && ks > 1) return ks == 2 ? 3 : 2;
+    return ks <= 2 ? 4 : ks <= 4 ? 3 : 2;
+}
 
 // What a launch derives on the host.
 struct PaPlan {

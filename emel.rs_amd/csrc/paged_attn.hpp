@@ -56,10 +56,13 @@ namespace {
 //   scores   a block's products with q, two halves a value, times the block's
 //            scale in f32, added up over the blocks.
 //   values   out^T[dim, head] = N^T (w d)^T: a weight by the scale of its token's block
-//            is one f32 factor, taken by a power of two that keeps the largest
-//            such factor of a block of dims at 1 or below (`unit`: out is in parts of
-//            it until the end) and then cut into hi + lo: off by 2^-22 of
-//            itself, or 2^-35 of the block's largest where lo is subnormal.
+//            is one f32 factor, cut into hi + lo.  Each column has a power of two for
+//            each set of blocks (`raised`: its exponent, which out keeps until the end) that
+//            holds the largest such factor so far between 2^11 and 2^15: one is off by 2^-22
+//            of itself, or 2^-36 of that largest where lo is subnormal, whatever scales tokens
+//            of next to no weight have.  The power is 2^80 at most, so that sums stay in
+//            f32's range (2^14 the largest weight, 2^30 tokens): beside weights whose scales
+//            are 0 a factor is off by 2^-118 of the largest weight.
 // A 32-token step of a head of 128 in Q4_0 is some 400 vector instructions, most of
 // them numbers made halves, and 32 matrix ones for 4.6 KB: what bounds short and middle
 // rows (64 sequences of 90 to 9000 tokens, 32/8 heads of 128: 55.6 us, 148 MB, 2.7
@@ -402,6 +405,8 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
     constexpr auto words_of = [](int n) { return V4 ? (n + 3) / 4 : (n + 1) / 2; };
     constexpr int kWords = PACKED ? KS / F * words_of(F) + (KS % F ? words_of(KS % F) : 0) : 1;
     constexpr float kLift = BF16 ? 0.0f : 14.0f;
+    constexpr bool kOne = PACKED && kSets == 1; // the weights themselves are taken by the set's power
+    constexpr int kRaise = 80;
     // [wave][head of the group][dim]; packed: before that the score operands, by
     // planes of 64 lanes and a zero
     extern __shared__ __attribute__((aligned(16))) float joined[];
@@ -529,8 +534,11 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
         float m = -__builtin_inff(), l = 0.0f;
         v4f acc[kAcc];
         for (int j = 0; j < kAcc; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        float unit[PACKED ? KS : 1]; // packed: what scales are taken by, 1 in the lanes of keys; acc is in these parts of one
-        for (float &u : unit) u = lane < 32 ? 1.0f : 0x1p24f;
+        int raised[kSets]; // packed: acc of a set, and where there is one set l too, are taken by 2^raised
+        for (int &r : raised) r = kRaise;
+        float ref = 0.0f; // packed: what weights' exponents start from
+        auto refer = [&] { ref = (m == -__builtin_inff() ? 0.0f : m) - kLift - (kOne ? static_cast<float>(raised[0]) : 0.0f); };
+        if constexpr (PACKED) refer();
         bool bad = sq.bad;
 
         const uint32_t t_end = sq.tokens < u1 * kPaUnit ? sq.tokens : u1 * kPaUnit;
@@ -697,29 +705,8 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
         };
         // the scales of this step into LDS; what is not a token counts for nothing
         auto place_scales = [&] {
-            float d[KS], most = 0.0f;
-            for (int e = 0; e < KS; ++e) {
-                d[e] = t0 + lane % 32 < t_end || lane < 32 ? pk_scale(bits[e]) : 0.0f;
-                most = __builtin_fmaxf(most, __builtin_fabsf(d[e] * unit[e]));
-            }
-            // A value's scale larger than all before: acc goes by a power of two
-            // that holds it, and eight times as large ones, so that few steps
-            // come by here.
-            if (__any(most > 1.0f && lane >= 32)) {
-                float f[kSets];
-                for (float &x : f) x = 1.0f;
-                for (int e = 0; e < KS; ++e) {
-                    const float top = wave_max_dpp(lane < 32 ? 0.0f : __builtin_fabsf(d[e])), was = lane_f32(unit[e], 32);
-                    if (top * was > 1.0f) {
-                        const uint32_t to = (250u << 23) - (__builtin_bit_cast(uint32_t, top) & 0x7f800000u);
-                        if (part == static_cast<uint32_t>(e % F)) f[e / F] = __builtin_bit_cast(float, (127u << 23) + to - __builtin_bit_cast(uint32_t, was));
-                        if (lane >= 32) unit[e] = __builtin_bit_cast(float, to);
-                    }
-                }
-                for (int j = 0; j < kAcc; ++j) acc[j] *= f[j / (2 * F)];
-            }
             __builtin_amdgcn_wave_barrier();
-            for (int e = 0; e < KS; ++e) scales[wave][lane / 32][e][lane % 32] = d[e] * unit[e];
+            for (int e = 0; e < KS; ++e) scales[wave][lane / 32][e][lane % 32] = t0 + lane % 32 < t_end || lane < 32 ? pk_scale(bits[e]) : 0.0f;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         };
@@ -730,6 +717,8 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
         };
         uint32_t magic = 0x64006400u; // in a register: an instruction holds one constant
         asm volatile("" : "+v"(magic));
+        float one = 1.0f; // one that the compiler does not know: x * one - h takes a half as it is, x - h a conversion first
+        asm volatile("" : "+s"(one));
         if constexpr (PACKED) {
             if (t0 < t_end) {
                 ask_page(t0 + lane % 32);
@@ -783,14 +772,20 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
             float top = z[0];
             for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, z[i]);
             top = rows16(top, [](float x, float y) { return __builtin_fmaxf(x, y); }) * by;
+            int due[kSets] = {}; // what a set's power would be past its most: its sums are taken down by it
             if (__any(top > m)) {
-                const float m1 = __builtin_fmaxf(m, top);
-                const float f = m1 > m ? __builtin_amdgcn_exp2f(m - m1) : 1.0f; // m = -inf: 0
-                l *= f;
-                for (int j = 0; j < kAcc; ++j) acc[j] *= f;
+                // whole numbers, so that it moves by powers of two, which the sets' powers take up
+                const float m1 = __builtin_ceilf(__builtin_fmaxf(m, top));
+                const int down = static_cast<int>(__builtin_fmaxf(m - m1, -1000.0f)); // m = -inf: all of it
+                for (int e = 0; e < kSets; ++e) {
+                    const int to = raised[e] - down;
+                    raised[e] = to < kRaise ? to : kRaise;
+                    due[e] = raised[e] - to;
+                }
+                l *= __builtin_ldexpf(1.0f, kOne ? due[0] : down);
                 m = m1;
+                refer();
             }
-            const float ref = (m == -__builtin_inff() ? 0.0f : m) - kLift;
             float w[8];
             for (int i = 0; i < 8; ++i) {
                 w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], by, -ref));
@@ -798,16 +793,32 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
             }
             for (int e = 0; e < kSets; ++e) {
                 u4 hi, lo; // the weights by a block's scales, as halves that add up to 22 bits
+                float x[8], most = 0.0f;
+                const float up = kOne ? 1.0f : __builtin_ldexpf(1.0f, raised[e]);
                 for (int b = 0; b < 2; ++b) {
                     const v4f d = four(1, e, b);
-                    for (int i = 0; i < 2; ++i) {
-                        const float *x = w + 4 * b + 2 * i;
-                        const v2h h = __builtin_convertvector((v2f{x[0] * d[2 * i], x[1] * d[2 * i + 1]}), v2h);
-                        const v2f r = {__builtin_fmaf(x[0], d[2 * i], -static_cast<float>(h[0])),
-                                       __builtin_fmaf(x[1], d[2 * i + 1], -static_cast<float>(h[1]))};
-                        hi[2 * b + i] = __builtin_bit_cast(uint32_t, h);
-                        lo[2 * b + i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
+                    for (int i = 0; i < 4; ++i) x[4 * b + i] = w[4 * b + i] * up * d[i];
+                }
+                for (int i = 0; i < 8; ++i) most = __builtin_fmaxf(most, __builtin_fabsf(x[i]));
+                // A factor past what halves hold: eight times as large ones fit from
+                // here on, so that few steps come by.
+                if (__any(most >= 0x1p15f || due[e] < 0)) {
+                    most = rows16(most, [](float u, float v) { return __builtin_fmaxf(u, v); });
+                    const int down = most >= 0x1p15f ? static_cast<int>((__builtin_bit_cast(uint32_t, most) >> 23) & 255u) - 127 - 11 : 0;
+                    const float f = __builtin_ldexpf(1.0f, due[e] - down), fx = __builtin_ldexpf(1.0f, -down);
+                    raised[e] -= down;
+                    for (int j = 2 * F * e; j < 2 * F * e + 2 * blocks_of(e); ++j) acc[j] *= f;
+                    for (float &v : x) v *= fx;
+                    if constexpr (kOne) {
+                        l *= fx;
+                        refer();
                     }
+                }
+                for (int i = 0; i < 4; ++i) {
+                    const v2h h = __builtin_convertvector((v2f{x[2 * i], x[2 * i + 1]}), v2h);
+                    const v2f r = {__builtin_fmaf(x[2 * i], one, -static_cast<float>(h[0])), __builtin_fmaf(x[2 * i + 1], one, -static_cast<float>(h[1]))};
+                    hi[i] = __builtin_bit_cast(uint32_t, h);
+                    lo[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
                 }
                 const int n = blocks_of(e);
                 for (int j = 0; j < 2 * n; ++j) {
@@ -912,7 +923,6 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
         float eight[kSets][8];
         for (int e = 0; PACKED && e < kSets; ++e) {
             const int n = blocks_of(e);
-            float u = lane_f32(unit[e * F], 32);
             for (int i = 0; i < 8; ++i) {
                 constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7}; // Q4_0: the nibble of each value
                 const int at = V4 ? order[i] : i;
@@ -923,9 +933,9 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
                 eight[e][i] = of(0);
                 for (int b = 1; b < n; ++b) eight[e][i] = part == static_cast<uint32_t>(b) ? of(b) : eight[e][i];
             }
-            for (int b = 1; b < n; ++b) u = part == static_cast<uint32_t>(b) ? lane_f32(unit[e * F + b], 32) : u;
-            const float by = __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, u)); // 1 / u
-            for (float &x : eight[e]) x *= by;
+            const float down = __builtin_ldexpf(1.0f, -raised[e]);
+            for (float &x : eight[e]) x *= down;
+            if constexpr (kOne) l *= down;
         }
         // the wave's part: [head][dim], dims of lane row c = 4 g + i
         float *own = joined + wave * heads * pitch;

@@ -642,7 +642,8 @@ emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream);
  * largest weight, and 2^-39 of that below; and F16 halves below 2^-14, which are
  * subnormal, count to about 2^-38 of what they are multiplied by.  Packed rows'
  * numbers are exact in their products; q keeps 22 bits as with F16, and so does a weight
- * by its block's scale, relative to the largest such product of that block of dims.
+ * by its block's scale, down to 2^-14 of the largest such product of its head and block of
+ * dims, and 2^-36 of that (or 2^-118 of the head's largest weight, if more) below.
  * Wants the stream's workspace, which grows as the reductions' does: graphs
  * captured from one stream share it, and run one after the other, or are
  * captured from streams of their own.
