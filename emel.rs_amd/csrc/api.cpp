@@ -2771,7 +2771,9 @@ emel_status rope(const emel_rope_request *r, emel_stream stream)
     for (; n < 4; ++n) a.runs[n] = {UINT32_MAX, 0, 1, 0};
     for (int d = 0; d < 4; ++d) {
         const uint64_t count = a.own ? r->sections[d] : pairs;
-        a.rate[d] = count ? std::log2(static_cast<double>(r->base)) / static_cast<double>(count) : 0.0;
+        const long double rate = count ? std::log2(static_cast<long double>(r->base)) / static_cast<long double>(count) : 0.0L;
+        a.rate[d] = static_cast<double>(rate);
+        a.rest[d] = static_cast<double>(rate - a.rate[d]);
     }
     a.quarters = static_cast<double>(r->scale) * 0.6366197723675814; // 2 / pi
     a.magnitude = r->magnitude;

@@ -10,9 +10,12 @@ namespace {
 // Pair i of a head turns by position * frequency.  A workgroup works its pairs'
 // frequencies out, in quarter turns a position and in 64 bits, then the cos and
 // sin of a tile of tokens, one of each a thread, and walks the tile's heads with
-// them.  In quarter turns the reduction of far positions is exact: t - rint(t),
-// whose rounding is 2^-53 of t, so an angle is off by 2^-52 of itself and by
-// f32's rounding of what is left.
+// them.  In quarter turns the reduction of far positions is exact: t - rint(t).  An
+// exponent e rate is up to 128 and would lose a frequency 2^-47 of itself by its rounding: what
+// that and rate's own leave out goes in as a factor 1 - ln(2) rest.  With u = 2^-53 an angle is
+// then off by exp2's 2 u, 0.6 u of 2 / pi, u each of the products with scale, exp2, that
+// factor, the pair's factor and the position, and 0.2 u of rate + rest: 2^-50 of itself, and by
+// f32's rounding of what is left of it.
 //
 // Bound by the bytes, 4 read and 4 written a value: 8001 tokens of 40 heads of 128
 // 60 us (5.4 TB/s), 73 with every thread working out its own pairs' angles for all
@@ -114,9 +117,11 @@ __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a, RopePlan pl)
         const uint32_t at = i - r.start, round = r.live == 1 ? at : r.live == 2 ? at / 2 : r.live == 3 ? at / 3 : at / 4;
         const uint32_t x = (r.axes >> (2 * (at - round * r.live))) & 3u;
         const double rate = x == 0 ? a.rate[0] : x == 1 ? a.rate[1] : x == 2 ? a.rate[2] : a.rate[3];
-        const double e = a.own ? r.round + round : i;
+        const double rest = x == 0 ? a.rest[0] : x == 1 ? a.rest[1] : x == 2 ? a.rest[2] : a.rest[3];
+        const double e = a.own ? r.round + round : i, by = e * rate, left = __builtin_fma(e, rate, -by) + e * rest;
+        const double f = a.quarters * exp2(-by);
         axis[j] = static_cast<uint8_t>(x);
-        freq[j] = a.quarters * exp2(-e * rate);
+        freq[j] = __builtin_fma(f, -0.6931471805599453 * left, f);
         if (a.factors) freq[j] /= static_cast<double>(a.factors[static_cast<int64_t>(i) * a.factors_st]);
     }
     __syncthreads();

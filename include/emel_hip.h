@@ -554,7 +554,7 @@ emel_status emel_op_mul_mat_q4_k(const emel_tensor_view *weights, const emel_ten
  * pair's number in the head (NULL: 1).  EMEL_ROPE_BACKWARD takes the angle's opposite: from
  * the gradient of a result it makes that of its input.
  * Angles are worked out in 64 bits (off by 2^-50 of themselves at most), cos
- * and sin rounded to f32.  Positions and factors are device memory, read when the kernel
+ * and sin in f32 (off by 2^-23).  Positions and factors are device memory, read when the kernel
  * runs.
  *
  * Guards: a NULL request, view or data, or a misaligned pointer, is

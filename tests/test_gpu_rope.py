@@ -1,4 +1,6 @@
 """GPU: rotary positions of several axes against their formula in 64 bits."""
+from decimal import Decimal, localcontext
+
 import numpy as np
 import pytest
 
@@ -164,3 +166,44 @@ def test_more_values_than_32_bits_count(gpu):
     run(eh.OpRope(view(x), out(x), view(torch.from_numpy(pos).to(gpu)), [32]))
     within(store[rows].cpu().numpy(), *rope(q, pos, [32]), "far rows")
     assert int((store != 0).sum()) <= 2 * dim
+
+
+def reduced_angles(positions, pairs, base, scale, factors):
+    """(angles [tokens, pairs], reduced to a turn, what they were), from 90 digits."""
+    with localcontext() as ctx:
+        ctx.prec = 90
+        pi = 4 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239))
+        rate = -Decimal(float(np.float32(base))).ln() / pairs
+        out, size = np.zeros((len(positions), pairs)), np.zeros((len(positions), pairs))
+        for i in range(pairs):
+            freq = (i * rate).exp() * Decimal(float(np.float32(scale))) / Decimal(float(factors[i]))
+            for t, p in enumerate(positions):
+                angle = int(p) * freq
+                out[t, i], size[t, i] = float(angle % (2 * pi)), abs(float(angle))
+    return out, size
+
+
+def arctan_of_inverse(n):
+    power, total, k = Decimal(1) / n, Decimal(0), 0
+    while abs(power) > Decimal(10) ** -95:
+        total += (power if k % 2 == 0 else -power) / (2 * k + 1)
+        power, k = power / (n * n), k + 1
+    return total
+
+
+@pytest.mark.parametrize("base,scale", [(1e4, 2.0**12), (5e6, 2.0**20), (5e6, 2.0**30), (3e38, 2.0**115), (1e-30, 2.0**-100)])
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_angles_keep_50_bits(gpu, base, scale, adjacent):
+    """An angle is off by 2^-50 of itself: as cos and sin count turns of 2^30 and more, f32's roundings hide no more than that.
+    They are off by 2^-23 each, and the products and the sum round by 2^-24 each: 2^-22 of |x| + |y|."""
+    pairs = 32
+    q, _, pos = arrays(14, 40, 1, 1, 2 * pairs, 1, 2**31 - 1)
+    pos[0, :3] = 2**31 - 1, -2**31, 1
+    factors = rng(15).uniform(0.5, 8.0, pairs).astype(np.float32)
+    got, _ = turned(gpu, q, q, pos, [pairs], base=base, scale=scale, factors=factors, adjacent=adjacent)
+    angle, size = reduced_angles(pos[0], pairs, base, scale, factors)
+    first, second = (slice(0, None, 2), slice(1, None, 2)) if adjacent else (slice(0, pairs), slice(pairs, None))
+    x, y = q[:, 0, first].astype(np.float64), q[:, 0, second].astype(np.float64)
+    tol = (np.abs(x) + np.abs(y)) * (2.0**-22 + size * 2.0**-50)
+    within(got[:, 0, first], x * np.cos(angle) - y * np.sin(angle), tol, "first")
+    within(got[:, 0, second], x * np.sin(angle) + y * np.cos(angle), tol, "second")
