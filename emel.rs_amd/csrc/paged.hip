@@ -448,17 +448,6 @@ uint32_t pa_side(const PagedAttnArgs &a, uint32_t workgroups)
     return side;
 }
 
-// Columns of a packed row's head: as many as 16 columns and its blocks allow (64
-// sequences of 90 to 9000 tokens with 32/8 heads of 128 in Q4_0 50.1 us with four,
-// 66.6 with one; one of 4001 13.2 and 16.2).
-uint32_t pa_fold(const PagedAttnArgs &a)
-{
-    const uint32_t group = a.heads / a.kv_heads;
-    uint32_t f = 8;
-    while (f > 1 && (f / 2 >= a.dim / 32 || group * f > 16)) f /= 2;
-    return f;
-}
-
 // Floats of a workspace slot.
 uint32_t pa_slot(const PagedAttnArgs &a)
 {
@@ -474,9 +463,9 @@ PaGrid pa_grid(const PagedAttnArgs &a)
         return static_cast<uint32_t>(n);
     }();
     const uint32_t ks = (a.dim + 31) / 32, fixed = a.k_pool.packed() ? 4096 + ks * 1024 : 4096 + ks * 3 * 1024;
-    const uint32_t sets = (ks + pa_fold(a) - 1) / pa_fold(a);
-    const uint32_t planes = a.k_pool.packed() ? sets * 2 * (kWave + 1) * 4 : 0; // of score operands
-    uint32_t per = pa_per_cu(static_cast<int>(ks), a.k_pool.packed() ? static_cast<int>(pa_fold(a)) : 0);
+    const int fold = a.k_pool.packed() ? pa_fold(static_cast<int>(ks), a.heads / a.kv_heads) : 0;
+    const uint32_t planes = fold ? (ks + fold - 1) / fold * 2 * (kWave + 1) * 4 : 0; // of score operands
+    uint32_t per = pa_per_cu(static_cast<int>(ks), fold);
     for (;; --per) {
         const uint32_t side = pa_side(a, cus * per);
         const uint32_t joined = 4 * pa_heads(a) * (a.dim + 4), weights = (a.k_pool.packed() ? kPaLead : 0) + pa_heads(a) * (cus * per / side);

@@ -50,6 +50,17 @@ constexpr uint32_t kPaLine = 64;   // words between arrival counters (a cache li
 // What the pages of keys and of values hold.
 enum class PaPages : int { F16 = 0, Bf16, Q8Q8, Q8Q4, Q4Q8, Q4Q4 };
 
+// Columns of a packed row's head of ks blocks, whose keys `group` heads share: as
+// many as 16 columns and its blocks allow (64 sequences of 90 to 9000 tokens with
+// 32/8 heads of 128 in Q4_0 50 us with four, 66.6 with one, over one set of inputs; one
+// of 4001 13.2 and 16.2).
+constexpr int pa_fold(int ks, uint32_t group)
+{
+    int f = 8;
+    while (f > 1 && (f / 2 >= ks || group * f > 16)) f /= 2;
+    return f;
+}
+
 // Workgroups that a compute unit holds at once: the registers that their
 // launch bounds leave them.  `fold` is 0 for halves.  Packed heads of 96 and 128 with a
 // column each (more than 8 heads share their keys) scale and split a block's

@@ -1,5 +1,6 @@
 """CPU: what a packed paged cache refuses, what it launches, and the definition of its rows."""
 import ctypes
+import re
 
 import numpy as np
 import pytest
@@ -173,3 +174,22 @@ def test_rows_come_back_as_they_were(kind):
     rows[:, -4:] = np.where(d < 0.002, np.float16(0.002), d).view(np.uint8)
     want = decode(kind, rows)
     assert np.array_equal(decode(kind, encode(kind, want.astype(np.float32))), want)
+
+
+@pytest.mark.parametrize("kd,vd", [(Q8_0, Q8_0), (Q8_0, Q4_0), (Q4_0, Q8_0), (Q4_0, Q4_0)])
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+def test_attentions_lds_is_its_kernels(rec, kd, vd, dim):
+    """The launch's LDS holds what the kernel that it picks lays out there, by the columns a head that its name gives: score
+    operands of each set of blocks, the waves' parts of a head's values, and a weight for each part of a row."""
+    for group in list(range(1, 18)) + [31, 32, 33, 48]:
+        for kv, s in ((1, 3), (8, 70)):
+            heads = group * kv
+            event = eh.OpPagedAttention(v(0, [dim, heads, s, 1]), v(1, [dim, 16, kv, 900], kd), v(2, [dim, 16, kv, 900], vd), v(3, [7, s, 1, 1], I32), v(4, [s, 1, 1, 1], I32),
+                                        v(5, [dim, heads, s, 1], mut=True), scale=0.1)
+            got, = rec.launches(event)
+            blocks, values, fold = (int(n) for n in re.search(r"k_pa_attn<.*, (\d+), (\d+), (\d+)>", got.name).groups())
+            assert 32 * blocks == dim and values == 2 * blocks
+            shared = min(group, 16)
+            assert shared * fold <= 16 and (fold == 1 or fold < 2 * blocks)
+            operands, parts = -(-blocks // fold) * 2 * 65 * 16, 4 * 4 * shared * (dim + 4)
+            assert got.lds >= max(operands, parts) and got.lds + 4096 + 1024 * blocks <= 160 * 1024 and got.grid % 256 == 0
