@@ -57,7 +57,7 @@ enum class PaPages : int { F16 = 0, Bf16, Q8Q8, Q8Q4, Q4Q8, Q4Q4 };
 constexpr int pa_fold(int ks, uint32_t group)
 {
     int f = 8;
-    while (f > 1 && (f / 2 >= ks || group * f > 16)) f /= 2;
+    while (f > 1 && (f / 2 >= ks || group > 16u / f)) f /= 2; // group * f may pass 32 bits
     return f;
 }
 

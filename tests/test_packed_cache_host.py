@@ -193,3 +193,12 @@ def test_attentions_lds_is_its_kernels(rec, kd, vd, dim):
             assert shared * fold <= 16 and (fold == 1 or fold < 2 * blocks)
             operands, parts = -(-blocks // fold) * 2 * 65 * 16, 4 * 4 * shared * (dim + 4)
             assert got.lds >= max(operands, parts) and got.lds + 4096 + 1024 * blocks <= 160 * 1024 and got.grid % 256 == 0
+
+
+@pytest.mark.parametrize("group", [1 << 28, (1 << 28) + 1, 1 << 29, (1 << 29) + 2, 3 << 29, (1 << 31) - 1])
+def test_any_number_of_heads_to_a_cache_head(rec, group):
+    """Sixteen heads of a row leave each one column, however many groups of sixteen there are."""
+    event = eh.OpPagedAttention(v(0, [256, group, 1, 1]), v(1, [256, 16, 1, 9], Q8_0), v(2, [256, 16, 1, 9], Q4_0), v(3, [1, 1, 1, 1], I32), v(4, [1, 1, 1, 1], I32),
+                                v(5, [256, group, 1, 1], mut=True), scale=0.1)
+    got, = rec.launches(event)
+    assert re.search(r"k_pa_attn<.*, 8, 16, 1>", got.name), got.name
