@@ -60,9 +60,9 @@ namespace {
 //            each set of blocks (`raised`: its exponent, which out keeps until the end) that
 //            holds the largest such factor so far between 2^11 and 2^15: one is off by 2^-22
 //            of itself, or 2^-36 of that largest where lo is subnormal, whatever scales tokens
-//            of next to no weight have.  The power is 2^80 at most, so that sums stay in
-//            f32's range (2^14 the largest weight, 2^30 tokens): beside weights whose scales
-//            are 0 a factor is off by 2^-118 of the largest weight.
+//            of next to no weight have.  The power is 2^94 at most, so that factors stay in
+//            f32's range: beside weights whose scales are 0 one is off by 2^-118 of the
+//            largest weight.
 // A 32-token step of a head of 128 in Q4_0 is some 400 vector instructions, most of
 // them numbers made halves, and 32 matrix ones for 4.6 KB: what bounds short and middle
 // rows (64 sequences of 90 to 9000 tokens, 32/8 heads of 128: 55.6 us, 148 MB, 2.7
@@ -405,8 +405,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
     constexpr auto words_of = [](int n) { return V4 ? (n + 3) / 4 : (n + 1) / 2; };
     constexpr int kWords = PACKED ? KS / F * words_of(F) + (KS % F ? words_of(KS % F) : 0) : 1;
     constexpr float kLift = BF16 ? 0.0f : 14.0f;
-    constexpr bool kOne = PACKED && kSets == 1; // the weights themselves are taken by the set's power
-    constexpr int kRaise = 80;
+    constexpr int kRaise = 94;
     // [wave][head of the group][dim]; packed: before that the score operands, by
     // planes of 64 lanes and a zero
     extern __shared__ __attribute__((aligned(16))) float joined[];
@@ -534,11 +533,8 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
         float m = -__builtin_inff(), l = 0.0f;
         v4f acc[kAcc];
         for (int j = 0; j < kAcc; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        int raised[kSets]; // packed: acc of a set, and where there is one set l too, are taken by 2^raised
+        int raised[kSets]; // packed: acc of a set is taken by 2^raised
         for (int &r : raised) r = kRaise;
-        float ref = 0.0f; // packed: what weights' exponents start from
-        auto refer = [&] { ref = (m == -__builtin_inff() ? 0.0f : m) - kLift - (kOne ? static_cast<float>(raised[0]) : 0.0f); };
-        if constexpr (PACKED) refer();
         bool bad = sq.bad;
 
         const uint32_t t_end = sq.tokens < u1 * kPaUnit ? sq.tokens : u1 * kPaUnit;
@@ -782,10 +778,11 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
                     raised[e] = to < kRaise ? to : kRaise;
                     due[e] = raised[e] - to;
                 }
-                l *= __builtin_ldexpf(1.0f, kOne ? due[0] : down);
+                l *= __builtin_ldexpf(1.0f, down);
                 m = m1;
-                refer();
             }
+            // 1 for the largest weight: a power of two within the exponent would cost it bits
+            const float ref = m == -__builtin_inff() ? 0.0f : m;
             float w[8];
             for (int i = 0; i < 8; ++i) {
                 w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], by, -ref));
@@ -794,7 +791,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
             for (int e = 0; e < kSets; ++e) {
                 u4 hi, lo; // the weights by a block's scales, as halves that add up to 22 bits
                 float x[8], most = 0.0f;
-                const float up = kOne ? 1.0f : __builtin_ldexpf(1.0f, raised[e]);
+                const float up = __builtin_ldexpf(1.0f, raised[e]);
                 for (int b = 0; b < 2; ++b) {
                     const v4f d = four(1, e, b);
                     for (int i = 0; i < 4; ++i) x[4 * b + i] = w[4 * b + i] * up * d[i];
@@ -809,10 +806,6 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
                     raised[e] -= down;
                     for (int j = 2 * F * e; j < 2 * F * e + 2 * blocks_of(e); ++j) acc[j] *= f;
                     for (float &v : x) v *= fx;
-                    if constexpr (kOne) {
-                        l *= fx;
-                        refer();
-                    }
                 }
                 for (int i = 0; i < 4; ++i) {
                     const v2h h = __builtin_convertvector((v2f{x[2 * i], x[2 * i + 1]}), v2h);
@@ -935,7 +928,6 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
             }
             const float down = __builtin_ldexpf(1.0f, -raised[e]);
             for (float &x : eight[e]) x *= down;
-            if constexpr (kOne) l *= down;
         }
         // the wave's part: [head][dim], dims of lane row c = 4 g + i
         float *own = joined + wave * heads * pitch;
@@ -987,7 +979,7 @@ __global__ __launch_bounds__(kBlock, pa_per_cu(KS, FOLD)) void k_pa_attn(PagedAt
                         mm = m1;
                     }
                 }
-                const float lift = BF16 ? 1.0f : 16384.0f; // as the parts of waves that do not walk
+                const float lift = BF16 || PACKED ? 1.0f : 16384.0f; // as the parts of waves that do not walk
                 for (uint32_t i = 0; i < 4; ++i)
                     if (4 * lane + i < dim) own[h * pitch + 4 * lane + i] = av[i] * lift;
                 if (lane == 0) {

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from helpers import rng
+from packed_cache_reference import decode
 from test_gpu_packed_cache import KINDS, attend_case, attend_event, cached, run, up, within
 
 pytestmark = pytest.mark.gpu
@@ -28,17 +29,19 @@ def even(gpu, kinds, heads, kv, dim, lengths, seed, small):
 
 def special(gpu, c, s, j, score, scale):
     """Token j of sequence s gets this score (scale dim^-0.5) under every head, and values with this scale."""
-    dim, kind = c["dim"], c["kinds"][0]
-    blocks = dim // 32
     page, tok = int(c["table"][s, j // 16]), j % 16
-    top = TOP[kind]
-    d = np.float16(score * dim**0.5 / 8.0 / -top)  # the lowest number
+    c["kp"][page, :, tok] = key(gpu, c, score)
+    c["vp"][page, :, tok, -c["dim"] // 16:] = up(gpu, np.full(c["dim"] // 32, scale, np.float16).view(np.uint8))
+
+
+def key(gpu, c, score):
+    """A key's row: the lowest number in front of the queries' 8, nothing else."""
+    blocks, kind = c["dim"] // 32, c["kinds"][0]
     row = np.full(c["kp"].shape[-1] - 2 * blocks, 0x88 if kind == "q4_0" else 0, np.uint8)
-    row[0] = 0x80 if kind == "q4_0" else 256 - top
+    row[0] = 0x80 if kind == "q4_0" else 256 - TOP[kind]
     scales = np.zeros(blocks, np.float16)
-    scales[0] = d
-    c["kp"][page, :, tok] = up(gpu, np.concatenate([row, scales.view(np.uint8)]))
-    c["vp"][page, :, tok, -2 * blocks:] = up(gpu, np.full(blocks, scale, np.float16).view(np.uint8))
+    scales[0] = score * c["dim"]**0.5 / 8.0 / -TOP[kind]
+    return up(gpu, np.concatenate([row, scales.view(np.uint8)]))
 
 
 def formula(q, k, v, rows, kind, dim):
@@ -111,3 +114,29 @@ def test_weight_moves_from_large_scales_to_small_ones(gpu, kinds, heads, kv, dim
         special(gpu, c, s, later, 80.0, 2e-5)
     run(attend_event(c))
     check(c)
+
+
+@pytest.mark.parametrize("kinds", [KINDS[0], KINDS[3]])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 4, 128), (4, 1, 128), (2, 1, 224), (16, 1, 256)])
+@pytest.mark.parametrize("empty", [False, True])
+def test_a_token_with_all_the_weight_is_its_values(gpu, kinds, heads, kv, dim, empty):
+    """Far into sequences of several steps a wave, where the others have e^-45 of its weight each: a result is the value but for the
+    rounding of the weight's product (2^-24), of its halves (2^-23), of their sum, of the sum's inverse and of the last
+    product (2^-24 each), so within 2^-21, whether or not the first block has values."""
+    lengths = [7000] * 40
+    c = even(gpu, kinds, heads, kv, dim, lengths, heads + dim + 3, 0.5)
+    g = rng(heads + dim + 4)
+    at = g.integers(1000, 7000, 40).tolist()
+    places = [int(c["table"][s, j // 16]) for s, j in enumerate(at)], slice(None), [j % 16 for j in at]
+    kept = c["kp"][places].clone()  # scores within 5 of 0
+    c["kp"][:] = key(gpu, c, -50.0)
+    c["kp"][places] = kept
+    if empty:
+        c["vp"][..., -dim // 16: 2 - dim // 16] = 0
+    run(attend_event(c))
+    got = c["y"].cpu().numpy().astype(np.float64)
+    for s, j in enumerate(at):
+        v = decode(kinds[1], c["vp"][int(c["table"][s, j // 16]), :, j % 16].cpu().numpy())
+        want = np.repeat(v, heads // kv, 0)
+        # the others' values: 127 at most
+        within(got[s], want, np.abs(want) * 2.0**-21 + 7000 * 128 * 2.0**-57, f"sequence {s}")
