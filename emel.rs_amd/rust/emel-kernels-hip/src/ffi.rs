@@ -95,12 +95,13 @@ pub const EMEL_BINARY_SUB: u32 = 1;
 pub const EMEL_BINARY_MUL: u32 = 2;
 pub const EMEL_BINARY_DIV: u32 = 3;
 
-// ---- emel_generic_op ----
+// ---- emel_rope_flag ----
 pub const EMEL_ROPE_ADJACENT: u32 = 1;
 pub const EMEL_ROPE_IN_TURN: u32 = 2;
 pub const EMEL_ROPE_OWN_FREQUENCIES: u32 = 4;
 pub const EMEL_ROPE_BACKWARD: u32 = 8;
 
+// ---- emel_generic_op ----
 pub const EMEL_GENERIC_DUP: u32 = 0;
 pub const EMEL_GENERIC_ADD: u32 = 1;
 pub const EMEL_GENERIC_ADD_ID: u32 = 2;

@@ -288,6 +288,19 @@ def test_enum_constants_have_gcc_values(c_facts):
     assert consts["EMEL_GET_ROWS_INLINE_INDICES"][1] == int(inline)
 
 
+def test_constants_stand_under_their_enums_heading():
+    """A run of constants of ffi.rs has a heading with its enum's name."""
+    heading = {}
+    at = ""
+    for line in FFI.read_text().splitlines():
+        at = m.group(1) if (m := re.match(r"// -+ (\w+)", line)) else at
+        heading |= {m.group(1): at} if (m := re.match(r"pub const (\w+):", line)) else {}
+    for m in re.finditer(r"typedef enum (\w+)\s*\{(.*?)\}\s*\w+\s*;", strip_comments(HEADER.read_text()), flags=re.S):
+        for entry in filter(None, (e.strip() for e in m.group(2).split(","))):
+            name = re.match(r"\w+", entry).group(0)
+            assert heading[name] == m.group(1), name
+
+
 def test_safe_layer_calls_only_declared_functions_and_all_of_them():
     declared = set(rust_externs())
     used = set()
