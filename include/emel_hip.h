@@ -70,7 +70,9 @@ typedef enum emel_status {
 
 /* Wire dtype codes, DType::from_code (crates/emel-kernels/src/any/
  * tensor_view.rs:111-158): the codes some entry point of this library reads.
- * Views of any other code (0..255) are carried and validated, never read. */
+ * Views of any other code (0..255) are carried and validated, never read.
+ * Q4_0 and Q8_0 are blocks one after the other, but in pages of the key-value
+ * cache, whose rows have the same bytes in an order of their own (see there). */
 typedef enum emel_dtype {
     EMEL_DTYPE_F32 = 0,
     EMEL_DTYPE_F16 = 1,
@@ -592,7 +594,7 @@ emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream);
  * No counterpart in the pinned path.  The cache is two pools of pages, one for
  * keys and one for values, of the same extents: views [dim, page, kv_heads, pages]
  * of halves (F16 or BF16, the same for both, nb[0] == 2) or of packed rows
- * (each Q8_0 or Q4_0, nb[0] == 1, dim a multiple of 32), with any other strides
+ * (each Q8_0 or Q4_0, nb[0] == 1, dim a multiple of 32, else INVALID_VIEW), with any other strides
  * that are multiples of 2 (a token's heads side by side, or a head's tokens, or
  * both pools interleaved in one allocation).  Slot p * page + t is token t of page p.
  *
@@ -630,7 +632,7 @@ emel_status emel_op_rope(const emel_rope_request *request, emel_stream stream);
  * dst are F32 [dim, heads, seqs, 1]; heads is a multiple of kv_heads, and
  * head h reads cache head h / (heads / kv_heads).  Position j of sequence s
  * is token j % page of page page_table[j / page, s] (I32 [max pages, seqs, 1,
- * 1]); lengths is I32 [seqs, 1, 1, 1].  dim is a multiple of 8 (of 32 for packed rows), at
+ * 1]); lengths is I32 [seqs, 1, 1, 1].  dim is a multiple of 8, at
  * most 256 (else UNSUPPORTED_OPERATION).  Both index tensors are device memory, read
  * when the kernel runs, so a captured call follows them.  A sequence of
  * length 0 gets zeros.  One whose length is negative or past max pages * page, or that
