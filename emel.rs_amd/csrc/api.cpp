@@ -2773,7 +2773,7 @@ emel_status rope(const emel_rope_request *r, emel_stream stream)
         const uint64_t count = a.own ? r->sections[d] : pairs;
         const long double rate = count ? std::log2(static_cast<long double>(r->base)) / static_cast<long double>(count) : 0.0L;
         a.rate[d] = static_cast<double>(rate);
-        a.rest[d] = static_cast<double>(rate - a.rate[d]);
+        a.rest[d] = static_cast<float>(rate - a.rate[d]);
     }
     a.quarters = static_cast<double>(r->scale) * 0.6366197723675814; // 2 / pi
     a.magnitude = r->magnitude;

@@ -273,7 +273,7 @@ struct RopeArgs {
     int64_t factors_st;
     RopeRun runs[4];      // by start; unused ones start past the pairs
     double rate[4];       // log2 of the base by the exponent's count, of each axis,
-    double rest[4];       // and what its rounding left
+    float rest[4];        // and what its rounding left
     double quarters;      // quarter turns of a position at exponent 0
     float magnitude;
     bool own, adjacent, back;

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kBlock) void k_rope(RopeArgs a, RopePlan pl)
         const uint32_t at = i - r.start, round = r.live == 1 ? at : r.live == 2 ? at / 2 : r.live == 3 ? at / 3 : at / 4;
         const uint32_t x = (r.axes >> (2 * (at - round * r.live))) & 3u;
         const double rate = x == 0 ? a.rate[0] : x == 1 ? a.rate[1] : x == 2 ? a.rate[2] : a.rate[3];
-        const double rest = x == 0 ? a.rest[0] : x == 1 ? a.rest[1] : x == 2 ? a.rest[2] : a.rest[3];
+        const float rest = x == 0 ? a.rest[0] : x == 1 ? a.rest[1] : x == 2 ? a.rest[2] : a.rest[3];
         const double e = a.own ? r.round + round : i, by = e * rate, left = __builtin_fma(e, rate, -by) + e * rest;
         const double f = a.quarters * exp2(-by);
         axis[j] = static_cast<uint8_t>(x);
