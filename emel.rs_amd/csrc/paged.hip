@@ -74,8 +74,8 @@ __global__ __launch_bounds__(kBlock) void k_pa_append(PagedAppendArgs a, FastDiv
 // x - n d, which is exact in f32 (x is a multiple of 2^-25 d or below d / 2), says so.
 //
 // Bound by the bytes, 4 read a value and 1.0625 or 0.5625 written: 8001 tokens of 1024
-// keys in Q8_0 and values in Q4_0 26 us (79 MB, 3.0 TB/s), with the latest slots' look-up
-// as for halves; a few tokens by the launch.
+// keys in Q8_0 and values in Q4_0 25.5 us (79 MB, 3.1 TB/s), of which the look through
+// the later slots, as for halves, is 4.4; a few tokens by the launch.
 
 // What is to be added to n so that it is the nearest whole number of scales in
 // x, ties to even, for an n that is off by one at most.
@@ -435,10 +435,10 @@ struct PaGrid {
 };
 
 // Packed rows side by side: as many as the rows and a die's workgroups divide by
-// (64 sequences of 90 to 9000 tokens, a token's 8 heads in a row, 55.6 us, 74.3 with each
+// (64 sequences of 90 to 9000 tokens, a token's 8 heads in a row, 54.8 us, 72.9 with each
 // row by itself; two of 40001 to 60001 tokens with 32 heads in Q8_0 212 us, 218 with
-// 8 side by side, 266 with each by itself; pages of a head's tokens in a row the same
-// within 2%).
+// 8 side by side, 269 with each by itself, in Q4_0 143, 156 and 211; pages of a head's
+// tokens in a row the same within 3%).
 uint32_t pa_side(const PagedAttnArgs &a, uint32_t workgroups)
 {
     if (!a.k_pool.packed()) return 1;

@@ -52,8 +52,7 @@ enum class PaPages : int { F16 = 0, Bf16, Q8Q8, Q8Q4, Q4Q8, Q4Q4 };
 
 // Columns of a packed row's head of ks blocks, whose keys `group` heads share: as
 // many as 16 columns and its blocks allow (64 sequences of 90 to 9000 tokens with
-// 32/8 heads of 128 in Q4_0 50 us with four, 66.6 with one, over one set of inputs; one
-// of 4001 13.2 and 16.2).
+// 32/8 heads of 128 in Q4_0 54.8 us with four, 68.8 with one; one of 4001 12.4 and 14.8).
 constexpr int pa_fold(int ks, uint32_t group)
 {
     int f = 8;
@@ -65,9 +64,10 @@ constexpr int pa_fold(int ks, uint32_t group)
 // launch bounds leave them.  `fold` is 0 for halves.  Packed heads of 96 and 128 with a
 // column each (more than 8 heads share their keys) scale and split a block's
 // weights at a time, which 168 registers do not hold: 64 sequences of 90 to 9000
-// tokens with 32/2 heads of 128 in Q4_0 35.4 us, 42.6 with three, in Q8_0 38.0 and 51.4.
-// Heads of 64 with a column each do not fit 128 registers: 24/2 heads in Q4_0 23.2 us, 24.9
-// with four, in Q8_0 25.1 and 30.1.
+// tokens with 32/2 heads of 128 in Q4_0 35.0 us, 44.9 with three, in Q8_0 38.9 and 60.3.
+// Heads of 64 with a column each do not fit 128 registers: 24/2 heads in Q4_0 23.2 us, 24.7
+// with four, in Q8_0 25.2 and 40.1.  Three kernels (Q8_0 with 4 blocks and 4 columns, Q8_0 keys
+// with 8 blocks and one) keep two to four registers of a segment in scratch, none of a step.
 constexpr uint32_t pa_per_cu(int ks, int fold)
 {
     if (fold == 1 && ks > 1) return ks == 2 ? 3 : 2;

@@ -65,14 +65,15 @@ namespace {
 //            largest weight.
 // A 32-token step of a head of 128 in Q4_0 is some 400 vector instructions, most of
 // them numbers made halves, and 32 matrix ones for 4.6 KB: what bounds short and middle
-// rows (64 sequences of 90 to 9000 tokens, 32/8 heads of 128: 55.6 us, 148 MB, 2.7
-// TB/s).  A token's rows are scattered over its page besides: 64 of 8000 take 178 us with
-// a token's heads in a row, 135 with a head's tokens in a row.  Long rows in
-// Q8_0 are bound by HBM (two of 40001 to 60001 with 32/32 heads: 169 us, 870 MB, 5.1
-// TB/s).  One sequence of 4001 takes 13 us, as with halves: latency.
+// rows (64 sequences of 90 to 9000 tokens, 32/8 heads of 128: 54.8 us, 148 MB, 2.7
+// TB/s).  A token's rows are scattered over its page besides: 64 of 8000 take 175 us with
+// a token's heads in a row, 133 with a head's tokens in a row; over the same pages for
+// all, which the caches hold, 120 and 112.  Long rows in
+// Q8_0 are bound by HBM (two of 40001 to 60001 with 32/32 heads: 164 us, 870 MB, 5.3
+// TB/s).  One sequence of 4001 takes 12.4 us, as with halves: latency.
 // A row's end runs once a workgroup, from cold: loops that were unrolled, 42 KB of code
 // with the rest, made the last workgroups of rows take 10 to 15 us longer than the 22 KB here.
-//
+
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
